@@ -19,7 +19,7 @@ class Config(C.Structure):
                 ("device", C.c_int), ("rms_eps", C.c_float)]
 
 
-_vp, _i, _sz, _u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
+_vp, _i, _sz, _u64, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float
 _ip = C.POINTER(C.c_int)
 _llp = C.POINTER(C.c_longlong)
 
@@ -55,6 +55,11 @@ PROTOTYPES = {
     "hy3a_import_kv": (_i, [_vp, _i, _i, _i, _i, _vp, _vp]),
     "hy3a_slot_bytes": (_i, [_i]),
     "hy3a_fill_random": (_i, [_vp, _i, _i, _i, _i, _u64]),
+    "hy3a_route": (_i, [_vp, _i, _i, _i, _vp, _sz, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "hy3a_experts_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "hy3a_experts": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz]),
+    "hy3a_adapters_workspace": (_sz, [_i, _i, _i]),
+    "hy3a_adapters": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz]),
     "hy3a_launch_count": (_u64, [_vp]),
     "hy3a_decode_schedule_kv": (_i, [_i, _i, _ip, _i, _i, _i, _llp, _llp, _llp]),
     "hy3a_decode_schedule": (_i, [_i, _ip, _i, _i, _i, _llp, _llp, _llp]),
@@ -85,6 +90,7 @@ def load_library():
 
 
 _bound = None
+BOUND = ("batch_set", "append", "decode_step", "prefill", "route", "experts_workspace", "experts", "adapters_workspace", "adapters")
 
 
 def load_native():
@@ -101,6 +107,6 @@ def load_native():
     from ._build import torch_key
     if _native.torch_key != torch_key():
         raise Hy3AttnError(-3, "the native binding was built for torch %s, this is %s: build it again with `python -m hy3_b200._build`" % (_native.torch_key, torch_key()))
-    _native.bind(*(C.cast(getattr(lib, "hy3a_" + f), _vp).value for f in ("batch_set", "append", "decode_step", "prefill")))
+    _native.bind(*(C.cast(getattr(lib, "hy3a_" + f), _vp).value for f in BOUND))
     _bound = _native
     return _bound

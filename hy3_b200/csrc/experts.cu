@@ -1,0 +1,259 @@
+/*
+ * experts.cu -- gated feed-forward networks of routed experts (hy3a_experts):
+ *
+ *      y[t] = sum_j w[t][j] * down_e (silu(gate_e x[t]) * (up_e x[t])),   e = ids[t][j]
+ *
+ * A slot is a (row, choice) pair, t * top_k + j.  Four launches, all on the stream, nothing read back:
+ *   1. plan      counts the slots of each held expert, and lists them expert by expert;
+ *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand);
+ *   3. down      y of every listed slot, fp32;
+ *   4. combine   sums a row's slots in the order of j, fp32, and rounds once.
+ * Slots whose id is outside [first_expert, first_expert + held) are left out everywhere.  The place of a slot within its expert's list
+ * comes from an atomic and may differ from run to run; no sum depends on it, so results do not.
+ */
+#include <math.h>
+
+#include "layer.h"
+
+namespace {
+
+using namespace hy3a_layer;
+
+/* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
+struct workspace {
+    size_t off, active, slot, h, y, total;
+};
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+workspace layout(long long slots, int hidden, int inter, int held) {
+    workspace w;
+    w.off = 0;
+    w.active = w.off + up256(((size_t)held + 1) * 4);
+    w.slot = w.active + up256(((size_t)held + 1) * 4);
+    w.h = w.slot + up256((size_t)slots * 4);
+    w.y = w.h + up256((size_t)slots * inter * 2);
+    w.total = w.y + up256((size_t)slots * hidden * 4);
+    return w;
+}
+
+struct expert_args {
+    const void *x;
+    size_t x_stride;
+    const int *ids;
+    const float *weights;
+    const void *gate, *up, *down;
+    void *out;
+    size_t out_stride;
+    int rows, top_k, hidden, inter, held, first, slots;
+    int *off;           /* [held + 1] first listed slot of each expert */
+    int *active;        /* [0] number of experts with slots, [1..] which */
+    int *slot;          /* [slots] listed slots, expert by expert */
+    void *h;            /* [slots][inter], in the order of the list */
+    float *y;           /* [slots][hidden], in the order of the slots */
+};
+
+__device__ __forceinline__ int local_expert(const expert_args &a, int id) {
+    const int e = id - a.first;
+    return id >= 0 && e >= 0 && e < a.held ? e : -1;
+}
+
+/* ---- 1. plan: one block ------------------------------------------------------------------------------------------------ */
+constexpr int kPlanThreads = 1024, kMaxHeld = 1024;
+__global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const expert_args a) {
+    __shared__ int s_count[kMaxHeld], s_warp[32], s_warp_active[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_release();
+    for (int e = tid; e < a.held; e += kPlanThreads) s_count[e] = 0;
+    __syncthreads();
+    pdl_wait();
+    for (int i = tid; i < a.slots; i += kPlanThreads) {
+        const int e = local_expert(a, a.ids[i]);
+        if (e >= 0) atomicAdd(&s_count[e], 1);
+    }
+    __syncthreads();
+    /* a thread per expert: exclusive sums of the counts and of the experts with any */
+    const int n = tid < a.held ? s_count[tid] : 0;
+    int sum = n;
+    const unsigned has = __ballot_sync(0xffffffffu, n > 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) { s_warp[warp] = sum; s_warp_active[warp] = __popc(has); }
+    __syncthreads();
+    if (warp == 0) {
+        int v = s_warp[lane], u = s_warp_active[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v2 = __shfl_up_sync(0xffffffffu, v, o), u2 = __shfl_up_sync(0xffffffffu, u, o);
+            if (lane >= o) { v += v2; u += u2; }
+        }
+        s_warp[lane] = v;
+        s_warp_active[lane] = u;
+    }
+    __syncthreads();
+    const int before = sum - n + (warp ? s_warp[warp - 1] : 0), at = __popc(has & ((1u << lane) - 1)) + (warp ? s_warp_active[warp - 1] : 0);
+    if (tid < a.held) {
+        a.off[tid] = before;
+        s_count[tid] = before;          /* from here on: where the expert's next slot goes */
+        if (n > 0) a.active[1 + at] = tid;
+    }
+    if (tid == 0) { a.off[a.held] = s_warp[31]; a.active[0] = s_warp_active[31]; }
+    __syncthreads();
+    for (int i = tid; i < a.slots; i += kPlanThreads) {
+        const int e = local_expert(a, a.ids[i]);
+        if (e >= 0) a.slot[atomicAdd(&s_count[e], 1)] = i;
+    }
+}
+
+/* ---- 2. and 3.: few slots per expert ------------------------------------------------------------------------------------
+ * A block takes one expert and 16 of its weight rows, 8 warps share the k's, fragments come straight from global memory (layer.h), and
+ * the warps' sums meet in shared memory in a fixed order.  Up to 32 slots go through together.  Rows 0-7 of the gate / up product's A
+ * are gate rows, rows 8-15 the up rows of the same index, so that both halves of a pair lie in one lane. */
+constexpr int kFewWarps = 8, kFewSlots = 32, kUnroll = 4;
+template <class T, bool DOWN>
+__global__ void __launch_bounds__(32 * kFewWarps) hy3a_experts_few_kernel(const expert_args a) {
+    __shared__ float s_sum[kFewWarps][kFewSlots / 8][4][32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_release();
+    pdl_wait();
+    if (blockIdx.y >= a.active[0]) return;
+    const int e = a.active[1 + blockIdx.y], p0 = a.off[e], count = a.off[e + 1] - p0;
+    const int K = DOWN ? a.inter : a.hidden, M = DOWN ? a.hidden : a.inter;
+    const int m0 = blockIdx.x * (DOWN ? 16 : 8), r_lo = m0 + g, r_hi = DOWN ? m0 + 8 + g : r_lo;
+    const T *w_lo = reinterpret_cast<const T *>(DOWN ? a.down : a.gate) + ((size_t)e * M + r_lo) * K;
+    const T *w_hi = reinterpret_cast<const T *>(DOWN ? a.down : a.up) + ((size_t)e * M + r_hi) * K;
+    const bool has_lo = r_lo < M, has_hi = r_hi < M;
+    for (int base = 0; base < count; base += kFewSlots) {
+        const int groups = min(kFewSlots / 8, (count - base + 7) >> 3);
+        const T *row[kFewSlots / 8];
+#pragma unroll
+        for (int i = 0; i < kFewSlots / 8; i++) {
+            const int p = p0 + base + 8 * i + g;
+            row[i] = nullptr;
+            if (base + 8 * i + g < count) row[i] = DOWN ? reinterpret_cast<const T *>(a.h) + (size_t)p * a.inter : reinterpret_cast<const T *>(a.x) + (size_t)(a.slot[p] / a.top_k) * a.x_stride;
+        }
+        float acc[kFewSlots / 8][4] = {};
+        for (int kb = warp * 32; kb < K; kb += 32 * kFewWarps * kUnroll) {
+            const int k0 = kb + t * 8;
+            uint4 lo[kUnroll], hi[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; u++) {
+                const int k = k0 + u * 32 * kFewWarps;
+                lo[u] = has_lo && k < K ? load_once(w_lo + k) : zero16();
+                hi[u] = has_hi && k < K ? load_once(w_hi + k) : zero16();
+            }
+#pragma unroll
+            for (int i = 0; i < kFewSlots / 8; i++) {
+                if (i < groups) {
+#pragma unroll
+                    for (int u = 0; u < kUnroll; u++) {
+                        const int k = k0 + u * 32 * kFewWarps;
+                        mma32<T>(acc[i], lo[u], hi[u], row[i] && k < K ? load_row(row[i] + k) : zero16());
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kFewSlots / 8; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s_sum[warp][i][c][lane] = acc[i][c];
+        __syncthreads();
+        /* accumulator c of lane (g, t): row g (c < 2) or g + 8, column 2t + (c & 1) */
+        const int m = tid & 7, col = tid >> 3, from = m * 4 + ((col & 7) >> 1), c0 = col & 1, i = col >> 3;
+        if (base + col < count) {
+            float lo = 0.f, hi = 0.f;
+#pragma unroll
+            for (int w = 0; w < kFewWarps; w++) { lo += s_sum[w][i][c0][from]; hi += s_sum[w][i][2 + c0][from]; }
+            const int p = p0 + base + col;
+            if (DOWN) {
+                float *y = a.y + (size_t)a.slot[p] * a.hidden + m0;
+                if (m0 + m < M) y[m] = lo;
+                if (m0 + 8 + m < M) y[8 + m] = hi;
+            } else if (m0 + m < M) {
+                reinterpret_cast<T *>(a.h)[(size_t)p * a.inter + m0 + m] = type<T>::down(__fdividef(lo, 1.f + __expf(-lo)) * hi);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+/* ---- 4. combine: a thread per 4 columns of a row ------------------------------------------------------------------------ */
+template <class T>
+__global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
+    pdl_release();
+    pdl_wait();
+    const int row = blockIdx.x, d = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (d >= a.hidden) return;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < a.top_k; j++) {
+        const size_t s = (size_t)row * a.top_k + j;
+        if (local_expert(a, a.ids[s]) < 0) continue;
+        const float w = a.weights[s];
+        const float4 v = *reinterpret_cast<const float4 *>(a.y + s * a.hidden + d);
+        sum.x += w * v.x; sum.y += w * v.y; sum.z += w * v.z; sum.w += w * v.w;
+    }
+    T o[4] = {type<T>::down(sum.x), type<T>::down(sum.y), type<T>::down(sum.z), type<T>::down(sum.w)};
+    *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + (size_t)row * a.out_stride + d) = *reinterpret_cast<const uint2 *>(o);
+}
+
+template <class T>
+cudaError_t launch(const expert_args &a, void *stream) {
+    cudaError_t e;
+    {   hy3a_launch l(dim3(1), dim3(kPlanThreads), 0, stream);
+        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel, a)) != cudaSuccess) return e; }
+    const int most = a.slots < a.held ? a.slots : a.held;       /* experts that can have slots */
+    {   hy3a_launch l(dim3((a.inter + 7) / 8, most), dim3(32 * kFewWarps), 0, stream);
+        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, false>, a)) != cudaSuccess) return e; }
+    {   hy3a_launch l(dim3((a.hidden + 15) / 16, most), dim3(32 * kFewWarps), 0, stream);
+        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, true>, a)) != cudaSuccess) return e; }
+    hy3a_launch l(dim3(a.rows, (a.hidden / 4 + 255) / 256), dim3(256), 0, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T>, a);
+}
+
+int check_sizes(const char *who, int rows, int top_k, int hidden, int inter, int held) {
+    if (rows < 0) return hy3a_fail(NULL, HY3A_EINVAL, "%s: rows %d < 0", who, rows);
+    if (top_k < 1 || top_k > 32) return hy3a_fail(NULL, HY3A_EINVAL, "%s: top_k %d not in [1,32]", who, top_k);
+    if (hidden < 8 || hidden % 8 || inter < 8 || inter % 8) return hy3a_fail(NULL, HY3A_EINVAL, "%s: hidden %d and inter %d have to be multiples of 8", who, hidden, inter);
+    if (held < 1 || held > kMaxHeld) return hy3a_fail(NULL, HY3A_EINVAL, "%s: %d experts held, not in [1,%d]", who, held, kMaxHeld);
+    if ((long long)rows * top_k > 0x7fffffffll / 2) return hy3a_fail(NULL, HY3A_EINVAL, "%s: %d rows of %d slots are too many", who, rows, top_k);
+    return 0;
+}
+
+} /* namespace */
+
+extern "C" {
+
+size_t hy3a_experts_workspace(int rows, int top_k, int hidden, int inter, int held) {
+    if (check_sizes("experts_workspace", rows, top_k, hidden, inter, held)) return 0;
+    return layout((long long)rows * top_k, hidden, inter, held).total;
+}
+
+int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int inter, int held, int first_expert, const void *x, size_t x_stride,
+                 const int *ids, const float *weights, const void *gate, const void *up, const void *down, void *out, size_t out_stride,
+                 void *work, size_t work_bytes) {
+    if (dtype != HY3A_F16 && dtype != HY3A_BF16) return hy3a_fail(NULL, HY3A_EINVAL, "experts: dtype %d not in {1,2}", dtype);
+    int rc = check_sizes("experts", rows, top_k, hidden, inter, held);
+    if (rc) return rc;
+    if (first_expert < 0 || first_expert > 0x7fffffff - held) return hy3a_fail(NULL, HY3A_EINVAL, "experts: first_expert %d", first_expert);
+    if (rows == 0) return HY3A_OK;
+    if (!x || !ids || !weights || !gate || !up || !down || !out || !work) return hy3a_fail(NULL, HY3A_EINVAL, "experts: NULL argument");
+    if (((uintptr_t)x | (uintptr_t)gate | (uintptr_t)up | (uintptr_t)down | (uintptr_t)out) & 15) return hy3a_fail(NULL, HY3A_EINVAL, "experts: pointers must be 16-byte aligned");
+    if (((uintptr_t)ids | (uintptr_t)weights) & 3) return hy3a_fail(NULL, HY3A_EINVAL, "experts: ids and weights must be 4-byte aligned");
+    if ((uintptr_t)work & 255) return hy3a_fail(NULL, HY3A_EINVAL, "experts: the workspace must be 256-byte aligned");
+    if ((x_stride & 7) || (out_stride & 7)) return hy3a_fail(NULL, HY3A_EINVAL, "experts: row strides must be multiples of 8");
+    if (x_stride < (size_t)hidden && rows > 1) return hy3a_fail(NULL, HY3A_EINVAL, "experts: x rows of %d overlap at a stride of %zu", hidden, x_stride);
+    if (out_stride < (size_t)hidden && rows > 1) return hy3a_fail(NULL, HY3A_EINVAL, "experts: out rows of %d overlap at a stride of %zu", hidden, out_stride);
+    const workspace w = layout((long long)rows * top_k, hidden, inter, held);
+    if (work_bytes < w.total) return hy3a_fail(NULL, HY3A_EINVAL, "experts: the workspace has %zu bytes, %zu are needed (hy3a_experts_workspace)", work_bytes, w.total);
+    int dev, sms;
+    if ((rc = hy3a_layer_device("experts", &dev, &sms))) return rc;
+    char *b = (char *)work;
+    expert_args a = {x, x_stride, ids, weights, gate, up, down, out, out_stride, rows, top_k, hidden, inter, held, first_expert, rows * top_k,
+                     (int *)(b + w.off), (int *)(b + w.active), (int *)(b + w.slot), b + w.h, (float *)(b + w.y)};
+    const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, stream) : launch<__nv_bfloat16>(a, stream);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", cudaGetErrorString(e));
+    return HY3A_OK;
+}
+
+} /* extern "C" */

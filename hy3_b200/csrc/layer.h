@@ -1,0 +1,79 @@
+/*
+ * layer.h -- what the operators beside the attention share (route.cu, experts.cu, adapters.cu): the device check and launch attributes on
+ * the host; 16-byte loads, conversions and the warp-level matrix product on the device.
+ *
+ * The warp-level product takes its fragments straight from global memory.  mma.m16n8k16 wants of lane (g = lane / 4, t = lane % 4) the
+ * k's {2t, 2t+1, 2t+8, 2t+9} of rows g and g + 8 of A and of column g of B.  A sum does not mind the order of its terms, so k is
+ * renamed: lane t loads k = 8t .. 8t+7 of a 32-k block as 16 bytes, and the first and second half of them are two steps.  Both operands
+ * use the same names, four lanes read 64 contiguous bytes of a row, and no shared memory is touched.
+ */
+#ifndef HY3A_LAYER_H
+#define HY3A_LAYER_H
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ctx.h"
+
+/* The current device's number and SM count; refuses devices that sm_100a code cannot run on. */
+int hy3a_layer_device(const char *who, int *device, int *sms);
+
+/* launch configuration with programmatic stream serialisation: the kernels wait (pdl_wait) before they touch memory */
+struct hy3a_launch {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    hy3a_launch(dim3 grid, dim3 block, size_t smem, void *stream) : cfg(), attr() {
+        cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+    }
+};
+
+namespace hy3a_layer {
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class T> struct type;
+template <> struct type<__nv_bfloat16> {
+    static constexpr int code = HY3A_BF16;
+    static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+};
+template <> struct type<__half> {
+    static constexpr int code = HY3A_F16;
+    static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+};
+template <> struct type<float> {
+    static constexpr int code = HY3A_F32;
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+
+/* 16 bytes that are read once (weights) / again and again (rows) */
+__device__ __forceinline__ uint4 load_once(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_row(const void *p) { return *reinterpret_cast<const uint4 *>(p); }
+__device__ __forceinline__ uint4 zero16() { return make_uint4(0, 0, 0, 0); }
+
+/* two k-steps of 16: rows g (lo) and g + 8 (hi) of A, column g of B, 8 k's each */
+template <class T> __device__ __forceinline__ void mma32(float (&d)[4], const uint4 &lo, const uint4 &hi, const uint4 &b) {
+    type<T>::mma(d, lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+    type<T>::mma(d, lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+}
+
+} /* namespace hy3a_layer */
+#endif

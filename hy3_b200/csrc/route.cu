@@ -1,0 +1,207 @@
+/*
+ * route.cu -- routing of rows to experts (hy3a_route), and the device check of the operators beside the attention.
+ *
+ * s = sigmoid(l) or softmax(l); c = s + bias picks; w = s (renormalised, scaled) weighs.  The selection is a matter of exact values: c
+ * is computed with IEEE division and CUDA's expf, the softmax's denominator is summed in 64 bits and rounded once (its value then
+ * does not hang on the order of the sum), and ties go to the lowest index.
+ */
+#include <atomic>
+
+#include "layer.h"
+
+int hy3a_layer_device(const char *who, int *device, int *sms) {
+    static std::atomic<int> known[64];      /* per device: 0 not asked yet, -1 another architecture, else its SM count */
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "%s: no CUDA device (%s): this library has no CPU path", who, cudaGetErrorString(e));
+    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        int major = 0, minor = 0;
+        if ((e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev)) != cudaSuccess ||
+            (e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev)) != cudaSuccess ||
+            (e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+            return hy3a_fail(NULL, HY3A_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+        if (major != 10 || minor != 0) n = -1;
+        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    }
+    if (n < 0) return hy3a_fail(NULL, HY3A_EDEVICE, "%s: device %d is not of compute capability 10.0; the kernels are built for sm_100a only", who, dev);
+    *device = dev;
+    *sms = n;
+    return 0;
+}
+
+namespace {
+
+using namespace hy3a_layer;
+
+constexpr int kWarps = 4;             /* rows per block, a warp each */
+constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
+
+/* order of floats as unsigned numbers; no c is -0 (s >= +0, and x + -x rounds to +0) */
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned u = __float_as_uint(v);
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+
+struct route_args {
+    const void *logits;
+    size_t stride;
+    const float *bias;
+    int rows, experts, top_k, softmax, groups, top_groups, renormalize;
+    float scale;
+    int *ids;
+    float *weights;
+};
+
+/* the two best of two pairs */
+__device__ __forceinline__ void two_best(float &a, float &b, float c, float d) {
+    const float lo = fminf(a, c);
+    a = fmaxf(a, c);
+    b = fmaxf(lo, fmaxf(b, d));
+}
+
+/* One warp per row; lane i holds experts i, i + 32, ... (coalesced), VPL of them. */
+template <class T, int VPL, bool GROUPED>
+__global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_args a) {
+    __shared__ float s_pick[GROUPED ? kWarps : 1][GROUPED ? 32 * VPL : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kWarps + warp;
+    pdl_release();
+    pdl_wait();
+    if (row >= a.rows) return;
+    const T *l = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.stride;
+    float s[VPL];
+    unsigned key[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; j++) s[j] = lane + 32 * j < a.experts ? type<T>::up(l[lane + 32 * j]) : -INFINITY;
+    unsigned open = 0;                /* bit j: not closed by a logit of -inf (and there) */
+#pragma unroll
+    for (int j = 0; j < VPL; j++) open |= s[j] == -INFINITY ? 0u : 1u << j;
+    if (a.softmax) {
+        float m = s[0];
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < VPL; j++) { m = fmaxf(m, s[j]); nan |= isnan(s[j]); }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (__any_sync(0xffffffffu, nan)) m = NAN;       /* fmaxf drops a NaN: a row with one has no softmax */
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < VPL; j++) {
+            s[j] = lane + 32 * j < a.experts ? expf(__fsub_rn(s[j], m)) : 0.f;
+            sum += (double)s[j];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float d = (float)sum;
+#pragma unroll
+        for (int j = 0; j < VPL; j++) s[j] = __fdiv_rn(s[j], d);
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPL; j++) s[j] = __fdiv_rn(1.f, __fadd_rn(1.f, expf(-s[j])));
+    }
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        const int e = lane + 32 * j;
+        float c = a.bias && e < a.experts ? __fadd_rn(s[j], a.bias[e]) : s[j];
+        if (isnan(c)) c = -3.402823466e38f;      /* below everything that is open, so that a row of NaN keeps ids in range and shows NaN weights */
+        if (!((open >> j) & 1)) c = -INFINITY;
+        key[j] = c == -INFINITY ? 0u : ordered(c);
+        if (GROUPED) s_pick[warp][e] = c;
+    }
+    if (GROUPED) {
+        /* a group stands with the sum of its two best open experts: `per` lanes scan each group, and meet */
+        const int size = a.experts / a.groups;
+        int per = 32;
+        while (per * a.groups > 32) per >>= 1;
+        const int grp = lane / per, sub = lane % per;
+        float b1 = -INFINITY, b2 = -INFINITY;
+        __syncwarp();
+        if (grp < a.groups) for (int i = sub; i < size; i += per) two_best(b1, b2, s_pick[warp][grp * size + i], -INFINITY);
+        for (int o = 1; o < per; o <<= 1) {
+            const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+            two_best(b1, b2, c1, c2);
+        }
+        const float stands = b2 == -INFINITY ? b1 : __fadd_rn(b1, b2);
+        /* groups that come before this one: better, or as good with a lower index */
+        int before = 0;
+        for (int g = 0; g < a.groups; g++) {
+            const float o = __shfl_sync(0xffffffffu, stands, g * per);
+            before += o > stands || (o == stands && g < grp);
+        }
+        const unsigned kept = __ballot_sync(0xffffffffu, before < a.top_groups);
+#pragma unroll
+        for (int j = 0; j < VPL; j++) {
+            const int g = min((lane + 32 * j) / size, a.groups - 1);
+            if (!((kept >> (g * per)) & 1)) key[j] = 0u;
+        }
+    }
+    int my_id = -1;
+    float my_w = 0.f;
+    for (int r = 0; r < a.top_k; r++) {
+        unsigned m = key[0];
+#pragma unroll
+        for (int j = 1; j < VPL; j++) m = max(m, key[j]);
+        const unsigned best = __reduce_max_sync(0xffffffffu, m);
+        if (best == 0u) break;                  /* only closed experts are left */
+        int e = 0x7fffffff;
+#pragma unroll
+        for (int j = VPL - 1; j >= 0; j--) if (key[j] == best) e = lane + 32 * j;
+        const int id = __reduce_min_sync(0xffffffffu, e);
+        float w = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPL; j++) if (lane + 32 * j == id) { key[j] = 0u; w = s[j]; }
+        w = __shfl_sync(0xffffffffu, w, id & 31);
+        if (lane == r) { my_id = id; my_w = w; }
+    }
+    if (a.renormalize) {
+        float sum = my_w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        my_w = __fdiv_rn(my_w, __fadd_rn(sum, 1e-20f));
+    }
+    if (lane < a.top_k) {
+        a.ids[(size_t)row * a.top_k + lane] = my_id;
+        a.weights[(size_t)row * a.top_k + lane] = my_w * a.scale;
+    }
+}
+
+template <class T, int VPL>
+cudaError_t launch_vpl(const route_args &a, void *stream) {
+    hy3a_launch l(dim3((a.rows + kWarps - 1) / kWarps), dim3(32 * kWarps), 0, stream);
+    return a.groups > 1 ? cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, false>, a);
+}
+template <class T>
+cudaError_t launch_type(const route_args &a, void *stream) {
+    const int n = (a.experts + 31) / 32;
+    if (n <= 1) return launch_vpl<T, 1>(a, stream);
+    if (n <= 2) return launch_vpl<T, 2>(a, stream);
+    if (n <= 4) return launch_vpl<T, 4>(a, stream);
+    if (n <= 6) return launch_vpl<T, 6>(a, stream);
+    if (n <= 8) return launch_vpl<T, 8>(a, stream);
+    if (n <= 16) return launch_vpl<T, 16>(a, stream);
+    return launch_vpl<T, 32>(a, stream);
+}
+
+} /* namespace */
+
+extern "C" int hy3a_route(void *stream, int dtype, int rows, int experts, const void *logits, size_t stride, const float *bias, int top_k, int score,
+                          int groups, int top_groups, int renormalize, float scale, int *ids, float *weights) {
+    if (dtype != HY3A_F32 && dtype != HY3A_F16 && dtype != HY3A_BF16) return hy3a_fail(NULL, HY3A_EINVAL, "route: dtype %d not in {0,1,2}", dtype);
+    if (rows < 0) return hy3a_fail(NULL, HY3A_EINVAL, "route: rows %d < 0", rows);
+    if (experts < 1 || experts > kMaxExperts) return hy3a_fail(NULL, HY3A_EINVAL, "route: experts %d not in [1,%d]", experts, kMaxExperts);
+    if (top_k < 1 || top_k > kMaxTopK || top_k > experts) return hy3a_fail(NULL, HY3A_EINVAL, "route: top_k %d not in [1,%d]", top_k, experts < kMaxTopK ? experts : kMaxTopK);
+    if (score != HY3A_SCORE_SIGMOID && score != HY3A_SCORE_SOFTMAX) return hy3a_fail(NULL, HY3A_EINVAL, "route: score %d not in {0,1}", score);
+    if (groups < 1 || groups > kMaxGroups || experts % groups) return hy3a_fail(NULL, HY3A_EINVAL, "route: groups %d: a divisor of %d experts up to %d", groups, experts, kMaxGroups);
+    if (top_groups < 1 || top_groups > groups) return hy3a_fail(NULL, HY3A_EINVAL, "route: top_groups %d not in [1,%d]", top_groups, groups);
+    if (top_k > experts / groups * top_groups) return hy3a_fail(NULL, HY3A_EINVAL, "route: top_k %d, but %d groups of %d experts stay", top_k, top_groups, experts / groups);
+    if (rows == 0) return HY3A_OK;
+    if (!logits || !ids || !weights) return hy3a_fail(NULL, HY3A_EINVAL, "route: NULL argument");
+    const size_t el = dtype == HY3A_F32 ? 4 : 2;
+    if (((uintptr_t)logits & (el - 1)) || (((uintptr_t)bias | (uintptr_t)ids | (uintptr_t)weights) & 3)) return hy3a_fail(NULL, HY3A_EINVAL, "route: a pointer is not aligned to its type");
+    int dev, sms, rc = hy3a_layer_device("route", &dev, &sms);
+    if (rc) return rc;
+    const route_args a = {logits, stride, bias, rows, experts, top_k, score == HY3A_SCORE_SOFTMAX, groups, top_groups, renormalize != 0, scale, ids, weights};
+    const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "route: %s", cudaGetErrorString(e));
+    return HY3A_OK;
+}

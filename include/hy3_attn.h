@@ -76,7 +76,7 @@ void hy3a_default_config(hy3a_config *cfg);
 int hy3a_create(const hy3a_config *cfg, hy3a_ctx **out);
 /* Replaces the KV part of hy3_gpu_free (hy3_gpu.cu:632-642). */
 void hy3a_destroy(hy3a_ctx *ctx);
-/* Message of the last failure on ctx (or of the last failed hy3a_create when ctx is NULL). */
+/* Message of the last failure on ctx; ctx NULL: of the calling thread's last failed hy3a_create, or operator beside the attention. */
 const char *hy3a_last_error(const hy3a_ctx *ctx);
 /* Bytes of device memory one 128-token block occupies for this configuration. */
 size_t hy3a_block_bytes(const hy3a_config *cfg);
@@ -241,6 +241,51 @@ int hy3a_slot_bytes(int kv_dtype);
 /* Fill slots [t0, t0+n) of (layer, seq) on the device with seeded N(0,1) K and V passed
  * through this cache's quantiser (benchmark set-up; no host traffic).                 */
 int hy3a_fill_random(hy3a_ctx *ctx, int layer, int seq, int t0, int n, uint64_t seed);
+
+/* ---- operators beside the attention -------------------------------------------------------
+ * What else a layer does with rows that are chosen one by one: the experts that a row is routed to, and the low-rank adapter
+ * of its request.  (The reference routes and multiplies on the CPU or with a warp per weight row, hy3.c:1266-1303, hy3_gpu.cu:75-130; it
+ * has no adapters.)  They need no context: the stream (a cudaStream_t) and the workspace are arguments, work is enqueued on the
+ * current device, which has to be the stream's, nothing is allocated, copied to the host or kept between calls, and all of
+ * them can be captured in a graph.  Messages: hy3a_last_error(NULL) of the calling thread.  A workspace may be used again by the
+ * next call on the same stream; its contents do not matter.  rows may be 0.                                                  */
+enum { HY3A_F32 = 0, HY3A_F16 = 1, HY3A_BF16 = 2 };                 /* types of rows */
+enum { HY3A_SCORE_SIGMOID = 0, HY3A_SCORE_SOFTMAX = 1 };
+
+/* Routes rows to experts.  Scores s = sigmoid(l) or softmax(l) of a row's logits (dtype HY3A_F32 / F16 / BF16, `stride` elements from row to
+ * row), in 32 bits; c = s + bias (bias fp32 [experts], may be NULL) picks and s weighs:
+ *   - a logit or a bias of -inf closes its expert for the row;
+ *   - groups > 1: the experts form that many groups of neighbours (a divisor, at most 32), a group stands with the sum of its two
+ *     largest c, and only the experts of the best top_groups groups stay open;
+ *   - the top_k (at most 32) largest c are taken, in descending order, ties to the lowest index; ids [rows][top_k], -1 with weight 0 where no
+ *     open expert is left;
+ *   - weights [rows][top_k]: s, divided by (their sum + 1e-20) if renormalize, times scale (the architecture: sigmoid, bias, 8 of 192,
+ *     renormalised, 2.826).
+ * A NaN ranks below every number, so ids stay in range, and shows in the weights where it is taken.  experts: at most 1024.  */
+int hy3a_route(void *stream, int dtype, int rows, int experts, const void *logits, size_t stride, const float *bias, int top_k, int score,
+               int groups, int top_groups, int renormalize, float scale, int *ids, float *weights);
+
+/* Gated feed-forward networks of routed experts: out[t] = sum over j of weights[t][j] * down_e (silu(gate_e x[t]) * (up_e x[t])) with
+ * e = ids[t][j], sums in fp32.  The experts [first_expert, first_expert + held) are held here; slots with another id (-1 among them) are
+ * left out, and a row without any is 0: ranks that split the experts add their outputs up.  dtype HY3A_F16 or HY3A_BF16 is that of x
+ * [rows][hidden], out and the weights gate, up [held][inter][hidden] and down [held][hidden][inter] (dense); the gated products are
+ * rounded to it once between the two.  hidden and inter are multiples of 8, row strides too, held and top_k at most 1024 and 32;
+ * pointers 16-byte aligned, the workspace (hy3a_experts_workspace bytes, 0 on bad sizes) 256.  out must not overlap x.
+ * The result depends on the inputs alone, not on how slots are ordered within an expert.                                     */
+size_t hy3a_experts_workspace(int rows, int top_k, int hidden, int inter, int held);
+int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int inter, int held, int first_expert, const void *x, size_t x_stride,
+                 const int *ids, const float *weights, const void *gate, const void *up, const void *down, void *out, size_t out_stride,
+                 void *work, size_t work_bytes);
+
+/* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scales[i] * b_i (a_i x[t]) with i = ids[t], sums in
+ * fp32.  Rows with an id outside [0, adapters) (-1: no adapter) are base.  x [rows][width], a [adapters][rank][width] and b
+ * [adapters][out_width][rank] (dense) are of dtype HY3A_F16 or HY3A_BF16; base and out [rows][out_width] of the same type or fp32 (the
+ * rows that hy3a_decode_step takes); out may be base.  width, out_width and rank (at most 256) are multiples of 8: adapters of smaller
+ * ranks are filled up with zeros.  Pointers 16-byte aligned; rows start on 16-byte boundaries.                               */
+size_t hy3a_adapters_workspace(int rows, int width, int rank);
+int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, int adapters, int rank, const void *x, size_t x_stride, int base_dtype,
+                  const void *base, size_t base_stride, const void *a, const void *b, const int *ids, const float *scales, void *out,
+                  size_t out_stride, void *work, size_t work_bytes);
 
 /* ---- introspection ------------------------------------------------------------------*/
 /* Number of kernels this library has launched on ctx since creation. */
