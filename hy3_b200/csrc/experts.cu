@@ -4,7 +4,7 @@
  *      y[t] = sum_j w[t][j] * down_e (silu(gate_e x[t]) * (up_e x[t])),   e = ids[t][j]
  *
  * A slot is a (row, choice) pair, t * top_k + j.  Four launches, all on the stream, nothing read back:
- *   1. plan      counts the slots of each held expert, and lists them expert by expert;
+ *   1. plan      counts the slots of each held expert, lists them expert by expert, and cuts the lists into tiles;
  *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand);
  *   3. down      y of every listed slot, fp32;
  *   4. combine   sums a row's slots in the order of j, fp32, and rounds once.
@@ -13,7 +13,7 @@
  */
 #include <math.h>
 
-#include "layer.h"
+#include "experts.h"
 
 namespace {
 
@@ -21,7 +21,7 @@ using namespace hy3a_layer;
 
 /* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
 struct workspace {
-    size_t off, active, slot, h, y, total;
+    size_t off, active, slot, row, tiles, h, y, total;
 };
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 workspace layout(long long slots, int hidden, int inter, int held) {
@@ -29,27 +29,13 @@ workspace layout(long long slots, int hidden, int inter, int held) {
     w.off = 0;
     w.active = w.off + up256(((size_t)held + 1) * 4);
     w.slot = w.active + up256(((size_t)held + 1) * 4);
-    w.h = w.slot + up256((size_t)slots * 4);
+    w.row = w.slot + up256((size_t)slots * 4);
+    w.tiles = w.row + up256((size_t)slots * 4);
+    w.h = w.tiles + 256 + up256(((size_t)slots / kTileSlots + (slots < held ? slots : held)) * sizeof(expert_tile));     /* their number, then the table */
     w.y = w.h + up256((size_t)slots * inter * 2);
     w.total = w.y + up256((size_t)slots * hidden * 4);
     return w;
 }
-
-struct expert_args {
-    const void *x;
-    size_t x_stride;
-    const int *ids;
-    const float *weights;
-    const void *gate, *up, *down;
-    void *out;
-    size_t out_stride;
-    int rows, top_k, hidden, inter, held, first, slots;
-    int *off;           /* [held + 1] first listed slot of each expert */
-    int *active;        /* [0] number of experts with slots, [1..] which */
-    int *slot;          /* [slots] listed slots, expert by expert */
-    void *h;            /* [slots][inter], in the order of the list */
-    float *y;           /* [slots][hidden], in the order of the slots */
-};
 
 __device__ __forceinline__ int local_expert(const expert_args &a, int id) {
     const int e = id - a.first;
@@ -58,9 +44,30 @@ __device__ __forceinline__ int local_expert(const expert_args &a, int id) {
 
 /* ---- 1. plan: one block ------------------------------------------------------------------------------------------------ */
 constexpr int kPlanThreads = 1024, kMaxHeld = 1024;
+/* exclusive sum over the block's threads; `total` gets the whole */
+__device__ __forceinline__ int block_sum(int n, int *s_warp /* [32] */, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int v = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();                  /* (the array may still be read from the sum before) */
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int w = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += u;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    return v - n + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
+}
 __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const expert_args a) {
-    __shared__ int s_count[kMaxHeld], s_warp[32], s_warp_active[32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ int s_count[kMaxHeld], s_warp[32];
+    const int tid = threadIdx.x;
     pdl_release();
     for (int e = tid; e < a.held; e += kPlanThreads) s_count[e] = 0;
     __syncthreads();
@@ -70,46 +77,33 @@ __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const e
         if (e >= 0) atomicAdd(&s_count[e], 1);
     }
     __syncthreads();
-    /* a thread per expert: exclusive sums of the counts and of the experts with any */
-    const int n = tid < a.held ? s_count[tid] : 0;
-    int sum = n;
-    const unsigned has = __ballot_sync(0xffffffffu, n > 0);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-    }
-    if (lane == 31) { s_warp[warp] = sum; s_warp_active[warp] = __popc(has); }
-    __syncthreads();
-    if (warp == 0) {
-        int v = s_warp[lane], u = s_warp_active[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v2 = __shfl_up_sync(0xffffffffu, v, o), u2 = __shfl_up_sync(0xffffffffu, u, o);
-            if (lane >= o) { v += v2; u += u2; }
-        }
-        s_warp[lane] = v;
-        s_warp_active[lane] = u;
-    }
-    __syncthreads();
-    const int before = sum - n + (warp ? s_warp[warp - 1] : 0), at = __popc(has & ((1u << lane) - 1)) + (warp ? s_warp_active[warp - 1] : 0);
+    /* a thread per expert */
+    const int n = tid < a.held ? s_count[tid] : 0, c = (n + kTileSlots - 1) / kTileSlots;
+    int slots, actives, tiles;
+    const int p0 = block_sum(n, s_warp, slots), at = block_sum(n > 0, s_warp, actives), first = block_sum(c, s_warp, tiles);
     if (tid < a.held) {
-        a.off[tid] = before;
-        s_count[tid] = before;          /* from here on: where the expert's next slot goes */
+        a.off[tid] = p0;
+        s_count[tid] = p0;              /* from here on: where the expert's next slot goes */
         if (n > 0) a.active[1 + at] = tid;
+        for (int j = 0; j < c; j++) a.tiles[first + j] = {tid, first, c, p0, n};
     }
-    if (tid == 0) { a.off[a.held] = s_warp[31]; a.active[0] = s_warp_active[31]; }
+    if (tid == 0) { a.off[a.held] = slots; a.active[0] = actives; *a.n_tiles = tiles; }
     __syncthreads();
     for (int i = tid; i < a.slots; i += kPlanThreads) {
         const int e = local_expert(a, a.ids[i]);
-        if (e >= 0) a.slot[atomicAdd(&s_count[e], 1)] = i;
+        if (e >= 0) {
+            const int p = atomicAdd(&s_count[e], 1);
+            a.slot[p] = i;
+            a.row[p] = i / a.top_k;
+        }
     }
 }
 
-/* ---- 2. and 3.: few slots per expert ------------------------------------------------------------------------------------
+/* ---- 2. and 3. of calls with few slots (the others: experts_umma.cu) ------------------------------------------------------------------------------------
  * A block takes one expert and 16 of its weight rows, 8 warps share the k's, fragments come straight from global memory (layer.h), and
  * the warps' sums meet in shared memory in a fixed order.  Up to 32 slots go through together.  Rows 0-7 of the gate / up product's A
  * are gate rows, rows 8-15 the up rows of the same index, so that both halves of a pair lie in one lane. */
+constexpr int kFewMost = 32;           /* slots of a call below which its products run here */
 constexpr int kFewWarps = 8, kFewSlots = 32, kUnroll = 4;
 template <class T, bool DOWN>
 __global__ void __launch_bounds__(32 * kFewWarps) hy3a_experts_few_kernel(const expert_args a) {
@@ -131,7 +125,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) hy3a_experts_few_kernel(const 
         for (int i = 0; i < kFewSlots / 8; i++) {
             const int p = p0 + base + 8 * i + g;
             row[i] = nullptr;
-            if (base + 8 * i + g < count) row[i] = DOWN ? reinterpret_cast<const T *>(a.h) + (size_t)p * a.inter : reinterpret_cast<const T *>(a.x) + (size_t)(a.slot[p] / a.top_k) * a.x_stride;
+            if (base + 8 * i + g < count) row[i] = DOWN ? reinterpret_cast<const T *>(a.h) + (size_t)p * a.inter : reinterpret_cast<const T *>(a.x) + (size_t)a.row[p] * a.x_stride;
         }
         float acc[kFewSlots / 8][4] = {};
         for (int kb = warp * 32; kb < K; kb += 32 * kFewWarps * kUnroll) {
@@ -198,15 +192,23 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
 }
 
 template <class T>
-cudaError_t launch(const expert_args &a, void *stream) {
+cudaError_t launch_few(const expert_args &a, void *stream) {
     cudaError_t e;
-    {   hy3a_launch l(dim3(1), dim3(kPlanThreads), 0, stream);
-        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel, a)) != cudaSuccess) return e; }
     const int most = a.slots < a.held ? a.slots : a.held;       /* experts that can have slots */
     {   hy3a_launch l(dim3((a.inter + 7) / 8, most), dim3(32 * kFewWarps), 0, stream);
         if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, false>, a)) != cudaSuccess) return e; }
-    {   hy3a_launch l(dim3((a.hidden + 15) / 16, most), dim3(32 * kFewWarps), 0, stream);
-        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, true>, a)) != cudaSuccess) return e; }
+    hy3a_launch l(dim3((a.hidden + 15) / 16, most), dim3(32 * kFewWarps), 0, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, true>, a);
+}
+template <class T>
+cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
+    cudaError_t e;
+    {   hy3a_launch l(dim3(1), dim3(kPlanThreads), 0, stream);
+        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel, a)) != cudaSuccess) return e; }
+    /* a handful of slots (bf16, 192 experts of 4096 x 1536; us a pass, few / umma): 8 slots 74 / 83, 64 slots 390 / 343 */
+    if (a.slots < kFewMost) e = launch_few<T>(a, stream);
+    else e = hy3a_experts_launch_umma(a, type<T>::code, device, sms, stream, what);
+    if (e != cudaSuccess) return e;
     hy3a_launch l(dim3(a.rows, (a.hidden / 4 + 255) / 256), dim3(256), 0, stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T>, a);
 }
@@ -250,9 +252,11 @@ int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int i
     if ((rc = hy3a_layer_device("experts", &dev, &sms))) return rc;
     char *b = (char *)work;
     expert_args a = {x, x_stride, ids, weights, gate, up, down, out, out_stride, rows, top_k, hidden, inter, held, first_expert, rows * top_k,
-                     (int *)(b + w.off), (int *)(b + w.active), (int *)(b + w.slot), b + w.h, (float *)(b + w.y)};
-    const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, stream) : launch<__nv_bfloat16>(a, stream);
-    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", cudaGetErrorString(e));
+                     (int *)(b + w.off), (int *)(b + w.active), (int *)(b + w.slot), (int *)(b + w.row), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles),
+                     b + w.h, (float *)(b + w.y)};
+    const char *what = NULL;
+    const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, dev, sms, stream, &what) : launch<__nv_bfloat16>(a, dev, sms, stream, &what);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;
 }
 

@@ -1,0 +1,328 @@
+/*
+ * experts_umma.cu -- the experts' two products on 5th-generation tensor cores (tcgen05 + TMEM + TMA).
+ *
+ * The weights are the M side of a product and the slots its N side: an expert has few or many slots, N takes any multiple of 16 up to 256, and
+ * no rows are padded to 128.  A pair of CTAs (cta_group::2) works on 256 weight rows x up to 256 slots: each CTA holds its 128 weight
+ * rows and half of the slots' rows in shared memory, and all slots of its weight rows in tensor memory (two accumulators of 256 columns, so that
+ * one is stored while the next is computed).  Per CTA:
+ *   warps 4-7 TMA producers: 64 k's a step into a ring of 6 stages; weight rows as boxes, slot rows gathered four at a time by row number
+ *             (tile::gather4), both with 128-byte swizzle; the byte counts of both CTAs go to the leader's barriers;
+ *   warp 8    MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
+ *   warps 0-3 epilogue: tcgen05.ld, then h or y.
+ * Gate / up: 16 gate rows and the 16 up rows of the same index alternate in the tile, so that a pair's halves lie 16 lanes apart in one
+ * warp and meet in a shuffle.
+ *
+ * Pairs take tiles in turn: (slots' tile, 256 weight rows), the tiles of an expert's slots innermost, so that pairs that work on the same weights
+ * at the same time find them in L2.
+ *
+ * Every wait is bounded; one that runs out raises the CTA's abort flag and a code in the error word (hy3a_layer_sync), lets all warps fall
+ * through, and TMEM is always released.
+ */
+#include <cuda.h>
+
+#include <atomic>
+
+#include "experts.h"
+
+namespace {
+
+using namespace hy3a_layer;
+
+constexpr int kStages = 6, kProducer = 4, kProducers = 4, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
+constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;      /* 128 rows of 64 k's, 2 bytes each */
+constexpr int kOffBar = kStages * (kABytes + kBBytes), kSmem = kOffBar + 256 + 1024;
+enum { B_FULL = 0, B_EMPTY = kStages, B_TFULL = 2 * kStages, B_TEMPTY = 2 * kStages + 2, B_COUNT = 2 * kStages + 4 };
+static_assert(8 * B_COUNT + 16 <= 256, "barriers");
+
+__device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
+
+__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity, unsigned hint_ns) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(hint_ns) : "memory");
+    return ok != 0;
+}
+/* Waits until the phase of that parity is over; false once anything in the CTA has given up.  A wait gives up after half a second and many polls. */
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int *abort_flag, unsigned where) {
+    if (mbar_try(bar, parity, 2000u)) return true;
+    unsigned long long t0, t1;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (unsigned i = 0; i < (1u << 22); i++) {
+        if (mbar_try(bar, parity, 20000u)) return true;
+        if (*abort_flag) return false;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+        if (i >= (1u << 13) && t1 - t0 > 500000000ull) break;
+    }
+    *abort_flag = 1;
+    if (atomicCAS(&g_err[0], 0u, 2u) == 0u) g_err[1] = where;
+    return false;
+}
+__device__ __forceinline__ unsigned cluster_addr(unsigned addr, unsigned rank) {
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+/* Copies are issued in uniform control flow by one elected lane (lead), so that their operands are computed in the uniform data path; both CTAs
+ * count their bytes at the leader's barrier. */
+__device__ __forceinline__ void tma_box(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %6, 0;\n"
+                 " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap *map, unsigned bar, int x, const int4 &row, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %8, 0;\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w), "r"(lead) : "memory");
+}
+/* K-major operand, 128-byte swizzle: 8-row groups 1024 B apart, descriptor version 1, layout 2 */
+__device__ __forceinline__ unsigned long long make_desc(unsigned saddr) {
+    return (unsigned long long)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned elect_one() {
+    unsigned p;
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ void umma_lead(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate, unsigned lead) {
+    asm volatile("{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n @e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(unsigned bar, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}"
+                 ::"r"(bar), "r"(lead), "h"((unsigned short)3) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+
+/* what a tile is: its expert, weight rows from m0 (gate / up: pairs) and n of the listed slots from p0 */
+struct where { int e, m0, p0, n; };
+template <bool DOWN>
+__device__ __forceinline__ where tile_of(const expert_args &a, int t, int m_tiles) {
+    const expert_tile &d = a.tiles[t / m_tiles];
+    const int in = t - d.first * m_tiles, m = in / d.tiles, j = in - m * d.tiles;
+    const int width = ((d.count + d.tiles - 1) / d.tiles + 15) & ~15;       /* even, in the hardware's steps; at most 256, so no tile is empty */
+    where w;
+    w.e = d.expert; w.m0 = m * (DOWN ? 256 : 128); w.p0 = d.p0 + j * width; w.n = min(width, d.count - j * width);
+    return w;
+}
+
+template <class T, bool DOWN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_rows, const expert_args a) {
+    extern __shared__ uint8_t s_raw[];
+    uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
+    const unsigned sbase = smem_u32(sm), bar0 = sbase + kOffBar;
+    volatile unsigned *s_tmem = reinterpret_cast<volatile unsigned *>(sm + kOffBar + 8 * B_COUNT);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT + 4);
+#define BAR(i) (bar0 + 8u * (unsigned)(i))
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned rank = blockIdx.x & 1u;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int K = DOWN ? a.inter : a.hidden, steps = (K + 63) >> 6, m_tiles = DOWN ? (a.hidden + 255) >> 8 : (a.inter + 127) >> 7;
+
+    if (tid == 0) {
+        *s_abort = 0;
+        for (int i = 0; i < kStages; i++) { mbar_init(BAR(B_FULL + i), 1); mbar_init(BAR(B_EMPTY + i), 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_TFULL + i), 1); mbar_init(BAR(B_TEMPTY + i), 8); }      /* empty: the epilogue warps of both CTAs */
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kProducer && lane < 3) {
+        const CUtensorMap *m = lane == 0 ? &tm_w0 : (lane == 1 ? &tm_w1 : &tm_rows);
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar0 + 8u * B_COUNT), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = *s_tmem;
+    pdl_release();
+    pdl_wait();
+    const int total = *a.n_tiles * m_tiles;
+
+    if (warp >= kProducer && warp < kProducer + kProducers) {
+        /* ===================== producers: each a quarter of the weight boxes and of the slot rows' gathers ===================== */
+        const int part = warp - kProducer;
+        const unsigned lead = elect_one();
+        unsigned st = 0, ph = 0;
+        for (int t = pair; t < total; t += pairs) {
+            const where w = tile_of<DOWN>(a, t, m_tiles);
+            const int N = (w.n + 15) & ~15, half = N >> 1, last = w.p0 + w.n - 1;
+            int4 row[32 / kProducers];
+#pragma unroll
+            for (int i = 0; i < 32 / kProducers; i++) {
+                const int p = w.p0 + (int)rank * half + 4 * (part + kProducers * i);       /* rows past the last are copies of it, and are not stored */
+                row[i] = make_int4(min(p, last), min(p + 1, last), min(p + 2, last), min(p + 3, last));
+                if (!DOWN && 4 * (part + kProducers * i) < half) row[i] = make_int4(a.row[row[i].x], a.row[row[i].y], a.row[row[i].z], a.row[row[i].w]);
+            }
+            bool ok = true;
+            for (int s = 0; s < steps; s++) {
+                if (!(ok = mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, 20u))) break;
+                const unsigned full = cluster_addr(BAR(B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
+                if (part == 0 && rank == 0 && lead) mbar_expect_tx(BAR(B_FULL + st), 2 * kABytes + N * 128);
+                if (DOWN) {
+                    if (part == 0) tma_box(sa, &tm_w0, full, s * 64, w.m0 + (int)rank * 128, w.e, lead);
+                } else {
+                    const int m = w.m0 + (int)rank * 64 + part * 16;
+                    tma_box(sa + part * 4096, &tm_w0, full, s * 64, m, w.e, lead);
+                    tma_box(sa + part * 4096 + 2048, &tm_w1, full, s * 64, m, w.e, lead);
+                }
+#pragma unroll
+                for (int i = 0; i < 32 / kProducers; i++)
+                    if (4 * (part + kProducers * i) < half) tma_gather4(sb + (part + kProducers * i) * 512, &tm_rows, full, s * 64, row[i], lead);
+                if (++st == kStages) { st = 0; ph ^= 1u; }
+            }
+            if (!ok) break;
+        }
+        /* the last commits reach the barriers of both CTAs before either leaves */
+        for (int i = 0; i < kStages && !*s_abort; i++) {
+            if (!mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, 24u)) break;
+            if (++st == kStages) { st = 0; ph ^= 1u; }
+        }
+    } else if (warp == kIssuer) {
+        if (rank == 0) {
+            /* ===================== MMA issuer: uniform control flow, one elected lane issues ===================== */
+            const unsigned lead = elect_one();
+            constexpr unsigned kType = type<T>::code == HY3A_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            unsigned st = 0, ph = 0, buf = 0, tph = 0;
+            for (int t = pair; t < total; t += pairs) {
+                const where w = tile_of<DOWN>(a, t, m_tiles);
+                const unsigned idesc = (1u << 4) | kType | (((unsigned)(w.n + 15) >> 4) << 18) | ((256u >> 4) << 24);
+                if (!mbar_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, 21u)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                bool ok = true;
+                for (int s = 0; s < steps; s++) {
+                    if (!(ok = mbar_wait(BAR(B_FULL + st), ph, s_abort, 22u))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned sa = sbase + st * (kABytes + kBBytes);
+                    const unsigned long long da = make_desc(sa), db = make_desc(sa + kABytes);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) umma_lead(tmem + buf * 256u, da + 2 * k, db + 2 * k, idesc, s + k > 0, lead);
+                    umma_commit_lead(BAR(B_EMPTY + st), lead);
+                    if (++st == kStages) { st = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                umma_commit_lead(BAR(B_TFULL + buf), lead);
+                if (++buf == 2) { buf = 0; tph ^= 1u; }
+            }
+        }
+    } else {
+        /* ===================== epilogue: warp w has weight rows 32w .. 32w + 31 of the CTA ===================== */
+        unsigned buf = 0, tph = 0;
+        for (int t = pair; t < total; t += pairs) {
+            const where w = tile_of<DOWN>(a, t, m_tiles);
+            if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, 23u)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int m = DOWN ? w.m0 + (int)rank * 128 + warp * 32 + lane : w.m0 + (int)rank * 64 + warp * 16 + (lane & 15);
+            const bool has = m < (DOWN ? a.hidden : a.inter);
+            for (int c0 = 0; c0 < w.n; c0 += 32) {
+                unsigned v[32];
+                tmem_ld32(tmem + ((unsigned)(warp * 32) << 16) + buf * 256u + c0, v);
+                if (DOWN) {
+                    const int mine = c0 + lane < w.n ? a.slot[w.p0 + c0 + lane] : 0;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const int slot = __shfl_sync(0xffffffffu, mine, j);
+                        if (has && c0 + j < w.n) a.y[(size_t)slot * a.hidden + m] = __uint_as_float(v[j]);
+                    }
+                } else {
+                    /* lanes below 16 have the gate, the others the up of one pair; of two slots each half finishes one */
+                    const bool second = lane >= 16;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(second ? v[j] : v[j + 1]), 16);
+                        const float g = second ? other : __uint_as_float(v[j]), u = second ? __uint_as_float(v[j + 1]) : other;
+                        const int n = c0 + j + second;
+                        if (has && n < w.n) reinterpret_cast<T *>(a.h)[(size_t)(w.p0 + n) * a.inter + m] = type<T>::down(__fdividef(g, 1.f + __expf(-g)) * u);
+                    }
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_TEMPTY + buf), 0));
+            if (++buf == 2) { buf = 0; tph ^= 1u; }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the step that was given up are still on their way */
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+#undef BAR
+}
+
+typedef CUresult (*encode_tiled_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+encode_tiled_fn find_encode_tiled() {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+    return (encode_tiled_fn)p;
+}
+
+struct maps { CUtensorMap gate, up, down, x, h; };
+/* 16-bit rows of `inner`, boxes of 64 of them: [depth][rows][inner], or [rows][inner] with a stride to gather from */
+bool encode(encode_tiled_fn enc, CUtensorMap *m, int rank, const void *base, size_t inner, size_t rows, size_t depth, size_t stride, int box_rows) {
+    const cuuint64_t dims[3] = {inner, rows, depth}, strides[2] = {stride * 2, stride * rows * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T>
+cudaError_t launch(const expert_args &a, const maps &m, int device, int sms, void *stream) {
+    static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
+    cudaError_t e;
+    if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
+        if ((e = cudaFuncSetAttribute(hy3a_experts_umma_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(hy3a_experts_umma_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if (device < 64) ready[device].store(true, std::memory_order_release);
+    }
+    const dim3 grid(sms & ~1);
+    {   hy3a_launch l(grid, dim3(kThreads), kSmem, stream);
+        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_umma_kernel<T, false>, m.gate, m.up, m.x, a)) != cudaSuccess) return e; }
+    hy3a_launch l(grid, dim3(kThreads), kSmem, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_experts_umma_kernel<T, true>, m.down, m.down, m.h, a);
+}
+
+} /* namespace */
+
+cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device, int sms, void *stream, const char **what) {
+    static const encode_tiled_fn enc = find_encode_tiled();
+    *what = nullptr;
+    if (!enc) { *what = "cuTensorMapEncodeTiled is not available from the driver"; return cudaErrorNotSupported; }
+    maps m;
+    /* (the two 16-bit types are moved alike) */
+    const bool ok = encode(enc, &m.gate, 3, a.gate, a.hidden, a.inter, a.held, a.hidden, 16) && encode(enc, &m.up, 3, a.up, a.hidden, a.inter, a.held, a.hidden, 16) &&
+                    encode(enc, &m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 128) && encode(enc, &m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 1) &&
+                    encode(enc, &m.h, 2, a.h, a.inter, a.slots, 1, a.inter, 1);
+    if (!ok) { *what = "cuTensorMapEncodeTiled failed"; return cudaErrorInvalidValue; }
+    return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
+}
+
+extern "C" int hy3a_layer_sync(void *stream) {
+    unsigned err[2] = {0, 0}, none[2] = {0, 0};
+    cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(err, g_err, sizeof(err));
+    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_sync: %s", cudaGetErrorString(e));
+    if (err[0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", err[0], err[1]);
+    return HY3A_OK;
+}

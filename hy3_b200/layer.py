@@ -56,3 +56,13 @@ def adapters(x, base, a, b, ids, scales, out=None):
     x [rows, width], a [adapters, rank, width], b [adapters, out_width, rank] fp16 or bf16, base [rows, out_width] of the same type or
     fp32 (row strides of x, base and out free), ids int32 [rows] (-1: none), scales fp32 [adapters].  Returns out (may be base), of base's type."""
     return _out(load_native().adapters(_stream(x), x, base, a, b, ids, scales, out))
+
+
+def layer_sync(device=None):
+    """Waits for torch's current stream on `device` (default: the current one), and raises `Hy3AttnError` if a bounded device-side wait of
+    `experts` ran out there since the last call."""
+    import torch
+    with torch.cuda.device(device):
+        rc = load_library().hy3a_layer_sync(torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _out(rc)

@@ -287,6 +287,10 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
                   const void *base, size_t base_stride, const void *a, const void *b, const int *ids, const float *scales, void *out,
                   size_t out_stride, void *work, size_t work_bytes);
 
+/* cudaStreamSynchronize on the stream + read of the operators' device error words: HY3A_ETIMEOUT if a bounded device-side wait of
+ * hy3a_experts ran out on the current device since the last call (it then returned early, and outputs since are not valid).  */
+int hy3a_layer_sync(void *stream);
+
 /* ---- introspection ------------------------------------------------------------------*/
 /* Number of kernels this library has launched on ctx since creation. */
 uint64_t hy3a_launch_count(const hy3a_ctx *ctx);
