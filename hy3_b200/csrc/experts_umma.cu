@@ -5,9 +5,10 @@
  * no rows are padded to 128.  A pair of CTAs (cta_group::2) works on 256 weight rows x up to 256 slots: each CTA holds its 128 weight
  * rows and half of the slots' rows in shared memory, and all slots of its weight rows in tensor memory (two accumulators of 256 columns, so that
  * one is stored while the next is computed).  Per CTA:
- *   warps 4-7 TMA producers: 64 k's a step into a ring of 6 stages; weight rows as boxes, slot rows gathered four at a time by row number
- *             (tile::gather4), both with 128-byte swizzle; the byte counts of both CTAs go to the leader's barriers;
- *   warp 8    MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
+ *   warps 4-11 TMA producers: 64 k's a step into a ring of 6 stages; weight rows as boxes, rows of x gathered four at a time by row number
+ *             (tile::gather4), rows of h, which lie in the order of the list, as boxes of 8, all with 128-byte swizzle; the byte counts of
+ *             both CTAs go to the leader's barriers;
+ *   warp 12   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
  *   warps 0-3 epilogue: tcgen05.ld, then h or y.
  * Gate / up: 16 gate rows and the 16 up rows of the same index alternate in the tile, so that a pair's halves lie 16 lanes apart in one
  * warp and meet in a shuffle.
@@ -28,7 +29,7 @@ namespace {
 
 using namespace hy3a_layer;
 
-constexpr int kStages = 6, kProducer = 4, kProducers = 4, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
+constexpr int kStages = 6, kProducer = 4, kProducers = 8, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
 constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;      /* 128 rows of 64 k's, 2 bytes each */
 constexpr int kOffBar = kStages * (kABytes + kBBytes), kSmem = kOffBar + 256 + 1024;
 enum { B_FULL = 0, B_EMPTY = kStages, B_TFULL = 2 * kStages, B_TEMPTY = 2 * kStages + 2, B_COUNT = 2 * kStages + 4 };
@@ -118,6 +119,30 @@ __device__ __forceinline__ where tile_of(const expert_args &a, int t, int m_tile
     return w;
 }
 
+/* The steps of one tile for one producer warp: its weight box, and MINE of the tile's slot rows (gathers of 4, or boxes of 8), whose number is a
+ * constant here so that the row numbers stay where the copy instruction reads them from: looked up in every step, a gather cost 52 clocks. */
+struct ring_state { unsigned st, ph; };
+template <bool DOWN, int MINE>
+__device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, const CUtensorMap *tm_rows, unsigned sbase, unsigned bar0, volatile int *s_abort, int steps, unsigned bytes /* 0: not the one that counts */,
+                                        int part, int m, int e, const int4 (&row)[4], unsigned lead) {
+    unsigned st = q.st, ph = q.ph;
+    for (int s = 0; s < steps; s++) {
+        if (!mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, 20u)) return false;
+        const unsigned full = cluster_addr(bar0 + 8u * (B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
+        if (bytes && lead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
+        if (!DOWN) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
+        else if (part == 0) tma_box(sa, tm_w, full, s * 64, m, e, lead);
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            if (DOWN) tma_box(sb + (part + kProducers * i) * 1024, tm_rows, full, s * 64, row[i].x, 0, lead);
+            else tma_gather4(sb + (part + kProducers * i) * 512, tm_rows, full, s * 64, row[i], lead);
+        }
+        if (++st == kStages) { st = 0; ph ^= 1u; }
+    }
+    q.st = st; q.ph = ph;
+    return true;
+}
+
 template <class T, bool DOWN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1, const __grid_constant__ CUtensorMap tm_rows, const expert_args a) {
@@ -127,7 +152,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     volatile unsigned *s_tmem = reinterpret_cast<volatile unsigned *>(sm + kOffBar + 8 * B_COUNT);
     volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT + 4);
 #define BAR(i) (bar0 + 8u * (unsigned)(i))
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31;
     const unsigned rank = blockIdx.x & 1u;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int K = DOWN ? a.inter : a.hidden, steps = (K + 63) >> 6, m_tiles = DOWN ? (a.hidden + 255) >> 8 : (a.inter + 127) >> 7;
@@ -156,39 +181,37 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     const int total = *a.n_tiles * m_tiles;
 
     if (warp >= kProducer && warp < kProducer + kProducers) {
-        /* ===================== producers: each a quarter of the weight boxes and of the slot rows' gathers ===================== */
+        /* ===================== producers: each an eighth of the weight boxes and of the slot rows ===================== */
         const int part = warp - kProducer;
         const unsigned lead = elect_one();
-        unsigned st = 0, ph = 0;
+        ring_state q = {0, 0};
         for (int t = pair; t < total; t += pairs) {
             const where w = tile_of<DOWN>(a, t, m_tiles);
-            const int N = (w.n + 15) & ~15, half = N >> 1, last = w.p0 + w.n - 1;
-            int4 row[32 / kProducers];
+            constexpr int kRows = DOWN ? 8 : 4;                                 /* of one copy */
+            const int N = (w.n + 15) & ~15, half = N >> 1, first = w.p0 + (int)rank * half, last = w.p0 + w.n - 1;
+            const int mine = (half / kRows - part + kProducers - 1) / kProducers;       /* (half is a multiple of 8) */
+            int4 row[4];
 #pragma unroll
-            for (int i = 0; i < 32 / kProducers; i++) {
-                const int p = w.p0 + (int)rank * half + 4 * (part + kProducers * i);       /* rows past the last are copies of it, and are not stored */
-                row[i] = make_int4(min(p, last), min(p + 1, last), min(p + 2, last), min(p + 3, last));
-                if (!DOWN && 4 * (part + kProducers * i) < half) row[i] = make_int4(a.row[row[i].x], a.row[row[i].y], a.row[row[i].z], a.row[row[i].w]);
+            for (int i = 0; i < 4; i++) {
+                const int p = first + kRows * (part + kProducers * i);
+                /* rows past the last are copies of it (gathered), or whatever lies behind: they are not stored */
+                row[i] = make_int4(p, min(p + 1, last), min(p + 2, last), min(p + 3, last));
+                if (!DOWN && i < mine) row[i] = make_int4(a.row[min(p, last)], a.row[row[i].y], a.row[row[i].z], a.row[row[i].w]);
             }
-            bool ok = true;
-            for (int s = 0; s < steps; s++) {
-                if (!(ok = mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, 20u))) break;
-                const unsigned full = cluster_addr(BAR(B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
-                if (part == 0 && rank == 0 && lead) mbar_expect_tx(BAR(B_FULL + st), 2 * kABytes + N * 128);
-                if (DOWN) {
-                    if (part == 0) tma_box(sa, &tm_w0, full, s * 64, w.m0 + (int)rank * 128, w.e, lead);
-                } else {
-                    const int m = w.m0 + (int)rank * 64 + part * 16;
-                    tma_box(sa + part * 4096, &tm_w0, full, s * 64, m, w.e, lead);
-                    tma_box(sa + part * 4096 + 2048, &tm_w1, full, s * 64, m, w.e, lead);
-                }
-#pragma unroll
-                for (int i = 0; i < 32 / kProducers; i++)
-                    if (4 * (part + kProducers * i) < half) tma_gather4(sb + (part + kProducers * i) * 512, &tm_rows, full, s * 64, row[i], lead);
-                if (++st == kStages) { st = 0; ph ^= 1u; }
+            const unsigned bytes = part == 0 && rank == 0 ? 2 * kABytes + N * 128 : 0;
+            const CUtensorMap *tm = !DOWN && (part & 1) ? &tm_w1 : &tm_w0;
+            const int m = DOWN ? w.m0 + (int)rank * 128 : w.m0 + (int)rank * 64 + (part >> 1) * 16;
+            bool ok;
+            switch (mine) {
+                case 4: ok = produce<DOWN, 4>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
+                case 3: ok = produce<DOWN, 3>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
+                case 2: ok = produce<DOWN, 2>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
+                case 1: ok = produce<DOWN, 1>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
+                default: ok = produce<DOWN, 0>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead);
             }
             if (!ok) break;
         }
+        unsigned st = q.st, ph = q.ph;
         /* the last commits reach the barriers of both CTAs before either leaves */
         for (int i = 0; i < kStages && !*s_abort; i++) {
             if (!mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, 24u)) break;
@@ -312,7 +335,7 @@ cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device
     /* (the two 16-bit types are moved alike) */
     const bool ok = encode(enc, &m.gate, 3, a.gate, a.hidden, a.inter, a.held, a.hidden, 16) && encode(enc, &m.up, 3, a.up, a.hidden, a.inter, a.held, a.hidden, 16) &&
                     encode(enc, &m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 128) && encode(enc, &m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 1) &&
-                    encode(enc, &m.h, 2, a.h, a.inter, a.slots, 1, a.inter, 1);
+                    encode(enc, &m.h, 3, a.h, a.inter, a.slots, 1, a.inter, 8);
     if (!ok) { *what = "cuTensorMapEncodeTiled failed"; return cudaErrorInvalidValue; }
     return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
 }
