@@ -21,12 +21,18 @@ struct expert_args {
     int rows, top_k, hidden, inter, held, first, slots;
     int *off;           /* [held + 1] first listed slot of each expert */
     int *active;        /* [0] number of experts with slots, [1..] which */
-    int *slot, *row;    /* [slots] listed slots, expert by expert, and the rows that they belong to */
+    int *row, *place;   /* [slots] rows of the listed slots, expert by expert; where each slot is in that list */
     expert_tile *tiles; /* [*n_tiles] */
     int *n_tiles;
     void *h;            /* [slots][inter], in the order of the list */
-    float *y;           /* [slots][hidden], in the order of the slots */
+    float *y;           /* [slots][hidden], in the order of the list: calls with few slots */
+    short *q;           /* the same of the others, in 16 bits: with 2^e the power of two below the largest magnitude of 32 neighbours, multiples of 2^(e - 14) */
+    float *q_scale;     /* [slots][hidden / 32, rounded up] that scale */
 };
+/* y is written and read once between two launches, and at many slots that is what these take: 8192 slots of 4096 are 134 MB in fp32.  16 bits of
+ * fixed point leave at most 2^-15 of the largest neighbour, a hundredth of what the rounding of a bf16 result leaves and a tenth of an fp16
+ * one's.  Neighbours that are not all finite are kept as bf16 instead (scale -1), so that infinities and NaN stay where they are; a largest
+ * magnitude below 2^-100 counts as 0. */
 
 /* Both products on tcgen05 (many slots per expert). */
 cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device, int sms, void *stream, const char **what);

@@ -5,11 +5,11 @@
  * no rows are padded to 128.  A pair of CTAs (cta_group::2) works on 256 weight rows x up to 256 slots: each CTA holds its 128 weight
  * rows and half of the slots' rows in shared memory, and all slots of its weight rows in tensor memory (two accumulators of 256 columns, so that
  * one is stored while the next is computed).  Per CTA:
- *   warps 4-11 TMA producers: 64 k's a step into a ring of 6 stages; weight rows as boxes, rows of x gathered four at a time by row number
+ *   warps 8-15 TMA producers: 64 k's a step into a ring of 6 stages; weight rows as boxes, rows of x gathered four at a time by row number
  *             (tile::gather4), rows of h, which lie in the order of the list, as boxes of 8, all with 128-byte swizzle; the byte counts of
  *             both CTAs go to the leader's barriers;
- *   warp 12   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
- *   warps 0-3 epilogue: tcgen05.ld, then h or y.
+ *   warp 16   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
+ *   warps 0-7 epilogue: tcgen05.ld, then h or y.
  * Gate / up: 16 gate rows and the 16 up rows of the same index alternate in the tile, so that a pair's halves lie 16 lanes apart in one
  * warp and meet in a shuffle.
  *
@@ -29,9 +29,10 @@ namespace {
 
 using namespace hy3a_layer;
 
-constexpr int kStages = 6, kProducer = 4, kProducers = 8, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
+constexpr int kStages = 6, kEpilogues = 8, kProducer = kEpilogues, kProducers = 8, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
 constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;      /* 128 rows of 64 k's, 2 bytes each */
-constexpr int kOffBar = kStages * (kABytes + kBBytes), kSmem = kOffBar + 256 + 1024;
+constexpr int kPitch = 144, kPatch = 16 * kPitch;              /* an epilogue warp's patch: 16 slots of 32 fp32 values, rows 16 bytes apart in the banks */
+constexpr int kOffPatch = kStages * (kABytes + kBBytes), kOffBar = kOffPatch + kEpilogues * kPatch, kSmem = kOffBar + 256 + 1024;
 enum { B_FULL = 0, B_EMPTY = kStages, B_TFULL = 2 * kStages, B_TEMPTY = 2 * kStages + 2, B_COUNT = 2 * kStages + 4 };
 static_assert(8 * B_COUNT + 16 <= 256, "barriers");
 
@@ -99,13 +100,18 @@ __device__ __forceinline__ void umma_commit_lead(unsigned bar, unsigned lead) {
     asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}"
                  ::"r"(bar), "r"(lead), "h"((unsigned short)3) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
                  "tcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+/* 32 bytes */
+__device__ __forceinline__ void store32(void *p, const unsigned (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+__device__ __forceinline__ short to_short(float v) { short r; asm("cvt.rni.sat.s16.f32 %0, %1;" : "=h"(r) : "f"(v)); return r; }
 
 /* what a tile is: its expert, weight rows from m0 (gate / up: pairs) and n of the listed slots from p0 */
 struct where { int e, m0, p0, n; };
@@ -160,7 +166,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     if (tid == 0) {
         *s_abort = 0;
         for (int i = 0; i < kStages; i++) { mbar_init(BAR(B_FULL + i), 1); mbar_init(BAR(B_EMPTY + i), 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_TFULL + i), 1); mbar_init(BAR(B_TEMPTY + i), 8); }      /* empty: the epilogue warps of both CTAs */
+        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_TFULL + i), 1); mbar_init(BAR(B_TEMPTY + i), 2 * kEpilogues); }      /* empty: the epilogue warps of both CTAs */
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kProducer && lane < 3) {
@@ -245,35 +251,71 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             }
         }
     } else {
-        /* ===================== epilogue: warp w has weight rows 32w .. 32w + 31 of the CTA ===================== */
+        /* ===================== epilogue: warp w has weight rows 32 (w % 4) .. + 31 of the CTA, and every other 16 slots =====================
+         * A lane has a weight row, and what is stored is a slot's row: 16 slots at a time turn in a patch of shared memory, and leave as 16 or
+         * 32 bytes a lane (a store for each slot, of 32 neighbouring values, takes the warp 90 clocks beside the copies and products). */
         unsigned buf = 0, tph = 0;
+        const int quarter = warp & 3, sl = lane & 15, half = lane >> 4;
+        uint8_t *patch = sm + kOffPatch + warp * kPatch;
+        const int scales = (a.hidden + 31) >> 5;
+        const bool whole = !(a.hidden & 15);
         for (int t = pair; t < total; t += pairs) {
             const where w = tile_of<DOWN>(a, t, m_tiles);
             if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, 23u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int m = DOWN ? w.m0 + (int)rank * 128 + warp * 32 + lane : w.m0 + (int)rank * 64 + warp * 16 + (lane & 15);
-            const bool has = m < (DOWN ? a.hidden : a.inter);
-            for (int c0 = 0; c0 < w.n; c0 += 32) {
-                unsigned v[32];
-                tmem_ld32(tmem + ((unsigned)(warp * 32) << 16) + buf * 256u + c0, v);
+            const int m0 = DOWN ? w.m0 + (int)rank * 128 + quarter * 32 : w.m0 + (int)rank * 64 + quarter * 16;
+            for (int c0 = (warp >> 2) * 16; c0 < w.n; c0 += 32) {
+                unsigned v[16];
+                tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * 256u + c0, v);
+                const int p = w.p0 + c0 + sl;
                 if (DOWN) {
-                    const int mine = c0 + lane < w.n ? a.slot[w.p0 + c0 + lane] : 0;
+                    const bool has = m0 + lane < a.hidden;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int slot = __shfl_sync(0xffffffffu, mine, j);
-                        if (has && c0 + j < w.n) a.y[(size_t)slot * a.hidden + m] = __uint_as_float(v[j]);
+                    for (int j = 0; j < 16; j++) *reinterpret_cast<float *>(patch + j * kPitch + lane * 4) = has ? __uint_as_float(v[j]) : 0.f;
+                    __syncwarp();
+                    /* half a slot's 32 values */
+                    float f[16], top = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float4 x = *reinterpret_cast<const float4 *>(patch + sl * kPitch + half * 64 + j * 16);
+                        f[4 * j] = x.x; f[4 * j + 1] = x.y; f[4 * j + 2] = x.z; f[4 * j + 3] = x.w;
+                        top = max_nan(max_nan(top, max_nan(fabsf(x.x), fabsf(x.y))), max_nan(fabsf(x.z), fabsf(x.w)));
+                    }
+                    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const unsigned ex = __float_as_uint(top) >> 23;                  /* 2^(ex - 127) <= it */
+                    const bool nil = ex < 27, odd = ex >= 255;
+                    const float times = __uint_as_float((nil || odd ? 0u : 268u - ex) << 23);
+                    unsigned o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[j] = (unsigned)(unsigned short)to_short(f[2 * j] * times) | ((unsigned)(unsigned short)to_short(f[2 * j + 1] * times) << 16);
+                    if (__any_sync(0xffffffffu, odd)) {
+                        if (odd) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) o[j] = (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * j])) | ((unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * j + 1])) << 16);
+                        }
+                    }
+                    if (c0 + sl < w.n && m0 < a.hidden) {
+                        short *q = a.q + (size_t)p * a.hidden + m0 + half * 16;
+                        if (whole && m0 + half * 16 + 16 <= a.hidden) store32(q, o);
+                        else {                                                      /* rows of 16 bytes only, or the last of them */
+                            if (m0 + half * 16 + 8 <= a.hidden) *reinterpret_cast<uint4 *>(q) = make_uint4(o[0], o[1], o[2], o[3]);
+                            if (m0 + half * 16 + 16 <= a.hidden) *reinterpret_cast<uint4 *>(q + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+                        }
+                        if (half == 0) a.q_scale[(size_t)p * scales + (m0 >> 5)] = odd ? -1.f : __uint_as_float((nil ? 0u : ex - 14u) << 23);
                     }
                 } else {
                     /* lanes below 16 have the gate, the others the up of one pair; of two slots each half finishes one */
-                    const bool second = lane >= 16;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(second ? v[j] : v[j + 1]), 16);
-                        const float g = second ? other : __uint_as_float(v[j]), u = second ? __uint_as_float(v[j + 1]) : other;
-                        const int n = c0 + j + second;
-                        if (has && n < w.n) reinterpret_cast<T *>(a.h)[(size_t)(w.p0 + n) * a.inter + m] = type<T>::down(__fdividef(g, 1.f + __expf(-g)) * u);
+                    for (int j = 0; j < 16; j += 2) {
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(half ? v[j] : v[j + 1]), 16);
+                        const float g = half ? other : __uint_as_float(v[j]), u = half ? __uint_as_float(v[j + 1]) : other;
+                        *reinterpret_cast<T *>(patch + (j + half) * 48 + sl * 2) = type<T>::down(__fdividef(g, 1.f + __expf(-g)) * u);
                     }
+                    __syncwarp();
+                    const uint4 o = *reinterpret_cast<const uint4 *>(patch + sl * 48 + half * 16);
+                    if (c0 + sl < w.n && m0 + half * 8 < a.inter) *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.h) + (size_t)p * a.inter + m0 + half * 8) = o;
                 }
+                __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
