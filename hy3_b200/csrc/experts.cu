@@ -6,8 +6,9 @@
  * A slot is a (row, choice) pair, t * top_k + j.  Four launches, all on the stream, nothing read back:
  *   1. plan      counts the slots of each held expert, lists them expert by expert, and cuts the lists into tiles;
  *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand);
- *   3. down      y of every listed slot, fp32 (few slots) or in fixed point (experts.h);
+ *   3. down      y of every listed slot, in fixed point (experts.h);
  *   4. combine   sums a row's slots in the order of j, fp32, and rounds once.
+ * Fewer than 32 slots take two, gate / up and down with the sum.
  * Slots whose id is outside [first_expert, first_expert + held) are left out everywhere.  The place of a slot within its expert's list
  * comes from an atomic and may differ from run to run; no sum depends on it, so results do not.
  */
@@ -23,21 +24,18 @@ constexpr int kFewMost = 32;           /* slots of a call below which its produc
 
 /* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
 struct workspace {
-    size_t off, active, row, place, tiles, h, y, scale, total;
+    size_t row, place, tiles, h, q, scale, total;
 };
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 workspace layout(long long slots, int hidden, int inter, int held) {
     workspace w;
-    w.off = 0;
-    w.active = w.off + up256(((size_t)held + 1) * 4);
-    w.row = w.active + up256(((size_t)held + 1) * 4);
+    w.row = 0;
     w.place = w.row + up256((size_t)slots * 4);
     w.tiles = w.place + up256((size_t)slots * 4);
     w.h = w.tiles + 256 + up256(((size_t)slots / kTileSlots + (slots < held ? slots : held)) * sizeof(expert_tile));     /* their number, then the table */
-    w.y = w.h + up256((size_t)slots * inter * 2);
-    const bool few = slots < kFewMost;
-    w.scale = w.y + up256((size_t)slots * hidden * (few ? 4 : 2));
-    w.total = w.scale + (few ? 0 : up256((size_t)slots * ((hidden + 31) / 32) * 4));
+    w.q = w.h + up256((size_t)slots * inter * 2);
+    w.scale = w.q + up256((size_t)slots * hidden * 2);
+    w.total = w.scale + up256((size_t)slots * ((hidden + 31) / 32) * 4);
     return w;
 }
 
@@ -63,7 +61,7 @@ __device__ __forceinline__ int peer_value(const int *p, unsigned rank) {
 }
 template <int BLOCKS>
 __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const expert_args a) {
-    __shared__ int s_count[kMaxHeld], s_next[kMaxHeld], s_warp[3][32];
+    __shared__ int s_count[kMaxHeld], s_next[kMaxHeld], s_warp[2][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned me = BLOCKS > 1 ? cluster_rank() : 0;
     const int per = (a.slots + BLOCKS - 1) / BLOCKS, begin = min(a.slots, (int)me * per), end = min(a.slots, begin + per);
@@ -91,40 +89,38 @@ __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const e
         }
     }
     const int tiles = (n + kTileSlots - 1) / kTileSlots;
-    int sum[3] = {n, tiles, n > 0};
+    int sum[2] = {n, tiles};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
+        for (int i = 0; i < 2; i++) {
             const int u = __shfl_up_sync(0xffffffffu, sum[i], o);
             if (lane >= o) sum[i] += u;
         }
 #pragma unroll
-    for (int i = 0; i < 3; i++) if (lane == 31) s_warp[i][warp] = sum[i];
+    for (int i = 0; i < 2; i++) if (lane == 31) s_warp[i][warp] = sum[i];
     __syncthreads();
-    int total[3];
+    int total = 0;
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
+    for (int i = 0; i < 2; i++) {
         int w = s_warp[i][lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += u;
         }
-        total[i] = __shfl_sync(0xffffffffu, w, 31);
+        if (i == 1) total = __shfl_sync(0xffffffffu, w, 31);
         const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
         sum[i] += warp ? before : 0;
     }
-    const int p0 = sum[0] - n, first = sum[1] - tiles, at = sum[2] - (n > 0);
+    const int p0 = sum[0] - n, first = sum[1] - tiles;
     if (tid < a.held) {
         s_next[tid] = p0 + earlier;           /* where the block's next slot of the expert goes */
         if (me == 0) {
-            a.off[tid] = p0;
-            if (n > 0) a.active[1 + at] = tid;
             for (int j = 0; j < tiles; j++) a.tiles[first + j] = {tid, first, tiles, p0, n};
         }
     }
-    if (tid == 0 && me == 0) { a.off[a.held] = total[0]; a.active[0] = total[2]; *a.n_tiles = total[1]; }
+    if (tid == 0 && me == 0) *a.n_tiles = total;
     __syncthreads();
 #pragma unroll 4
     for (int i = begin + tid; i < end; i += kPlanThreads) {
@@ -138,80 +134,129 @@ __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const e
     if (BLOCKS > 1) cluster_sync();           /* nobody leaves while its counts are read */
 }
 
-/* ---- 2. and 3. of calls with few slots (the others: experts_umma.cu) ------------------------------------------------------------------------------------
- * A block takes one expert and 16 of its weight rows, 8 warps share the k's, fragments come straight from global memory (layer.h), and
- * the warps' sums meet in shared memory in a fixed order.  Up to 32 slots go through together.  Rows 0-7 of the gate / up product's A
- * are gate rows, rows 8-15 the up rows of the same index, so that both halves of a pair lie in one lane. */
-constexpr int kFewWarps = 8, kFewSlots = 32, kUnroll = 4;
-template <class T, bool DOWN>
-__global__ void __launch_bounds__(32 * kFewWarps) hy3a_experts_few_kernel(const expert_args a) {
-    __shared__ float s_sum[kFewWarps][kFewSlots / 8][4][32];
+/* ---- calls with few slots (at most 31; the others: experts_umma.cu) -----------------------------------------------------
+ * Two launches, without a plan: every warp sees all slots.  The first slot of an expert leads, and takes the expert's other slots along, 8 at a
+ * time (more than 8 read the weights again, from L2).  Fragments come straight from global memory (layer.h), 16 loads of 16 bytes in
+ * flight a lane. */
+constexpr int kFewWarps = 8, kFewLoads = 8 /* k blocks of 32 in flight */;
+/* lane s: expert of slot s (-1: none), the slots of the same expert */
+__device__ __forceinline__ int few_slots(const expert_args &a, unsigned &same) {
+    const int lane = threadIdx.x & 31, e = lane < a.slots ? local_expert(a, a.ids[lane]) : -1;
+    same = __match_any_sync(0xffffffffu, e);
+    return e;
+}
+/* position of the n-th set bit, -1 if there are fewer */
+__device__ __forceinline__ int nth_bit(unsigned bits, int n) {
+    for (; n > 0; n--) bits &= bits - 1;
+    return bits ? __ffs(bits) - 1 : -1;
+}
+template <class T> __device__ __forceinline__ void few_load(uint4 (&lo)[kFewLoads], uint4 (&hi)[kFewLoads], const T *w_lo, const T *w_hi, bool has_lo, bool has_hi, int k, int step, int K) {
+#pragma unroll
+    for (int u = 0; u < kFewLoads; u++) {
+        lo[u] = has_lo && k + u * step < K ? load_once(w_lo + k + u * step) : zero16();
+        hi[u] = has_hi && k + u * step < K ? load_once(w_hi + k + u * step) : zero16();
+    }
+}
+template <class T> __device__ __forceinline__ void few_multiply(float (&acc)[4], const uint4 (&lo)[kFewLoads], const uint4 (&hi)[kFewLoads], const T *row, int k, int step, int K) {
+#pragma unroll
+    for (int u = 0; u < kFewLoads; u++) mma32<T>(acc, lo[u], hi[u], row && k + u * step < K ? load_row(row + k + u * step) : zero16());
+}
+
+/* h of one expert's slots, 8 of its rows: block = (8 pairs of gate and up rows, slot that may lead); the warps share the k's, and their sums
+ * meet in shared memory in a fixed order.  Rows 0-7 of A are gate rows, rows 8-15 the up rows of the same index: both halves of a pair lie in
+ * one lane. */
+template <class T>
+__global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(const expert_args a) {
+    __shared__ float s_sum[kFewWarps][4][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    pdl_release();
     pdl_wait();
-    if (blockIdx.y >= a.active[0]) return;
-    const int e = a.active[1 + blockIdx.y], p0 = a.off[e], count = a.off[e + 1] - p0;
-    const int K = DOWN ? a.inter : a.hidden, M = DOWN ? a.hidden : a.inter;
-    const int m0 = blockIdx.x * (DOWN ? 16 : 8), r_lo = m0 + g, r_hi = DOWN ? m0 + 8 + g : r_lo;
-    const T *w_lo = reinterpret_cast<const T *>(DOWN ? a.down : a.gate) + ((size_t)e * M + r_lo) * K;
-    const T *w_hi = reinterpret_cast<const T *>(DOWN ? a.down : a.up) + ((size_t)e * M + r_hi) * K;
-    const bool has_lo = r_lo < M, has_hi = r_hi < M;
-    for (int base = 0; base < count; base += kFewSlots) {
-        const int groups = min(kFewSlots / 8, (count - base + 7) >> 3);
-        const T *row[kFewSlots / 8];
-#pragma unroll
-        for (int i = 0; i < kFewSlots / 8; i++) {
-            const int p = p0 + base + 8 * i + g;
-            row[i] = nullptr;
-            if (base + 8 * i + g < count) row[i] = DOWN ? reinterpret_cast<const T *>(a.h) + (size_t)p * a.inter : reinterpret_cast<const T *>(a.x) + (size_t)a.row[p] * a.x_stride;
+    pdl_release();                          /* behind the wait: what the next kernel reads before its own is complete */
+    unsigned same;
+    const int mine = few_slots(a, same), e = __shfl_sync(0xffffffffu, mine, blockIdx.y);
+    const unsigned slots = __shfl_sync(0xffffffffu, same, blockIdx.y);
+    if (e < 0 || (int)blockIdx.y != __ffs(slots) - 1) return;
+    const int K = a.hidden, M = a.inter, m0 = blockIdx.x * 8, step = 32 * kFewWarps;
+    const bool has = m0 + g < M;
+    const T *gate = reinterpret_cast<const T *>(a.gate) + ((size_t)e * M + m0 + g) * K, *up = reinterpret_cast<const T *>(a.up) + ((size_t)e * M + m0 + g) * K;
+    for (int base = 0; base < __popc(slots); base += 8) {
+        const int s = nth_bit(slots, base + g);
+        const T *x = s >= 0 ? reinterpret_cast<const T *>(a.x) + (size_t)(s / a.top_k) * a.x_stride : nullptr;
+        float acc[4] = {};
+        for (int kb = warp * 32; kb < K; kb += step * kFewLoads) {
+            uint4 lo[kFewLoads], hi[kFewLoads];
+            few_load(lo, hi, gate, up, has, has, kb + t * 8, step, K);
+            few_multiply(acc, lo, hi, x, kb + t * 8, step, K);
         }
-        float acc[kFewSlots / 8][4] = {};
-        for (int kb = warp * 32; kb < K; kb += 32 * kFewWarps * kUnroll) {
-            const int k0 = kb + t * 8;
-            uint4 lo[kUnroll], hi[kUnroll];
+        if (base) __syncthreads();
 #pragma unroll
-            for (int u = 0; u < kUnroll; u++) {
-                const int k = k0 + u * 32 * kFewWarps;
-                lo[u] = has_lo && k < K ? load_once(w_lo + k) : zero16();
-                hi[u] = has_hi && k < K ? load_once(w_hi + k) : zero16();
-            }
-#pragma unroll
-            for (int i = 0; i < kFewSlots / 8; i++) {
-                if (i < groups) {
-#pragma unroll
-                    for (int u = 0; u < kUnroll; u++) {
-                        const int k = k0 + u * 32 * kFewWarps;
-                        mma32<T>(acc[i], lo[u], hi[u], row[i] && k < K ? load_row(row[i] + k) : zero16());
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kFewSlots / 8; i++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s_sum[warp][i][c][lane] = acc[i][c];
+        for (int c = 0; c < 4; c++) s_sum[warp][c][lane] = acc[c];
         __syncthreads();
         /* accumulator c of lane (g, t): row g (c < 2) or g + 8, column 2t + (c & 1) */
-        const int m = tid & 7, col = tid >> 3, from = m * 4 + ((col & 7) >> 1), c0 = col & 1, i = col >> 3;
-        if (base + col < count) {
+        if (tid < 64) {
+            const int m = tid & 7, col = tid >> 3, from = m * 4 + (col >> 1), c = col & 1, to = nth_bit(slots, base + col);
             float lo = 0.f, hi = 0.f;
 #pragma unroll
-            for (int w = 0; w < kFewWarps; w++) { lo += s_sum[w][i][c0][from]; hi += s_sum[w][i][2 + c0][from]; }
-            const int p = p0 + base + col;
-            if (DOWN) {
-                float *y = a.y + (size_t)p * a.hidden + m0;
-                if (m0 + m < M) y[m] = lo;
-                if (m0 + 8 + m < M) y[8 + m] = hi;
-            } else if (m0 + m < M) {
-                reinterpret_cast<T *>(a.h)[(size_t)p * a.inter + m0 + m] = type<T>::down(__fdividef(lo, 1.f + __expf(-lo)) * hi);
-            }
+            for (int w = 0; w < kFewWarps; w++) { lo += s_sum[w][c][from]; hi += s_sum[w][2 + c][from]; }
+            if (to >= 0 && m0 + m < M) reinterpret_cast<T *>(a.h)[(size_t)to * M + m0 + m] = type<T>::down(__fdividef(lo, 1.f + __expf(-lo)) * hi);
         }
-        __syncthreads();
     }
 }
 
-/* ---- 4. combine: a thread per 8 columns of a row; FIXED: y is a.q and a.q_scale (experts.h) ------------------------------ */
-template <class T, bool FIXED>
+/* out: block = 16 columns; its warps take the experts in turn, or shares of their k's where there are fewer experts than warps, and the slots'
+ * sums are weighed and added up in shared memory, in the order of the choices.  The first weights are on their way before the wait for h. */
+template <class T>
+__global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kernel(const expert_args a) {
+    __shared__ float s_y[kFewWarps][kFewMost][16];                         /* [share of the k's][slot][column] */
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    unsigned same;
+    const int mine = few_slots(a, same);
+    const unsigned any = __ballot_sync(0xffffffffu, mine >= 0), leaders = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(same) - 1);
+    const int n = __popc(leaders), shares = n ? max(1, kFewWarps / n) : 1;
+    const int K = a.inter, M = a.hidden, m0 = blockIdx.x * 16, step = shares * 32;
+    bool waited = false;
+    for (int unit = warp; unit < n * shares; unit += kFewWarps) {
+        const int which = unit / shares, share = unit - which * shares, lead = nth_bit(leaders, which);
+        const int e = __shfl_sync(0xffffffffu, mine, lead);
+        const unsigned slots = __shfl_sync(0xffffffffu, same, lead);
+        const T *w_lo = reinterpret_cast<const T *>(a.down) + ((size_t)e * M + m0 + g) * K, *w_hi = w_lo + (size_t)8 * K;
+        const bool has_lo = m0 + g < M, has_hi = m0 + 8 + g < M;
+        for (int base = 0; base < __popc(slots); base += 8) {
+            const int s = nth_bit(slots, base + g);
+            const T *h = s >= 0 ? reinterpret_cast<const T *>(a.h) + (size_t)s * K : nullptr;
+            float acc[4] = {};
+            for (int kb = share * 32; kb < K; kb += step * kFewLoads) {
+                uint4 lo[kFewLoads], hi[kFewLoads];
+                few_load(lo, hi, w_lo, w_hi, has_lo, has_hi, kb + t * 8, step, K);
+                if (!waited) { pdl_wait(); waited = true; }
+                few_multiply(acc, lo, hi, h, kb + t * 8, step, K);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int to = nth_bit(slots, base + 2 * t + (c & 1));
+                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = acc[c];
+            }
+        }
+    }
+    if (!waited) pdl_wait();
+    pdl_release();
+    __syncthreads();
+    const int m = tid & 15;
+    if (m0 + m >= M) return;
+    for (int row = tid >> 4; row < a.rows; row += 2 * kFewWarps) {
+        float sum = 0.f;
+        for (int j = 0; j < a.top_k; j++) {
+            const int s = row * a.top_k + j;
+            if (!((any >> s) & 1)) continue;
+            float y = 0.f;
+            for (int i = 0; i < shares; i++) y += s_y[i][s][m];
+            sum += a.weights[s] * y;
+        }
+        reinterpret_cast<T *>(a.out)[(size_t)row * a.out_stride + m0 + m] = type<T>::down(sum);
+    }
+}
+
+/* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------ */
+template <class T>
 __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
     pdl_release();
     pdl_wait();
@@ -230,23 +275,16 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
         const float w = __shfl_sync(0xffffffffu, w_lane, j);
         const size_t p = (size_t)__shfl_sync(0xffffffffu, place, j);
         if (!in) continue;
-        if (FIXED) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(a.q + p * a.hidden + d);
-            const float scale = a.q_scale[p * ((a.hidden + 31) >> 5) + (d >> 5)];
-            const unsigned u[4] = {v.x, v.y, v.z, v.w};
-            if (scale >= 0.f) {
-                const float ws = w * scale;
+        const uint4 v = *reinterpret_cast<const uint4 *>(a.q + p * a.hidden + d);
+        const float scale = a.q_scale[p * ((a.hidden + 31) >> 5) + (d >> 5)];
+        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+        if (scale >= 0.f) {
+            const float ws = w * scale;
 #pragma unroll
-                for (int i = 0; i < 4; i++) { sum[2 * i] += ws * (float)(short)(u[i] & 0xffff); sum[2 * i + 1] += ws * (float)(short)(u[i] >> 16); }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) { sum[2 * i] += w * __uint_as_float(u[i] << 16); sum[2 * i + 1] += w * __uint_as_float(u[i] & 0xffff0000u); }
-            }
+            for (int i = 0; i < 4; i++) { sum[2 * i] += ws * (float)(short)(u[i] & 0xffff); sum[2 * i + 1] += ws * (float)(short)(u[i] >> 16); }
         } else {
-            const float4 *y = reinterpret_cast<const float4 *>(a.y + p * a.hidden + d);
-            const float4 v0 = y[0], v1 = y[1];
-            sum[0] += w * v0.x; sum[1] += w * v0.y; sum[2] += w * v0.z; sum[3] += w * v0.w;
-            sum[4] += w * v1.x; sum[5] += w * v1.y; sum[6] += w * v1.z; sum[7] += w * v1.w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) { sum[2 * i] += w * __uint_as_float(u[i] << 16); sum[2 * i + 1] += w * __uint_as_float(u[i] & 0xffff0000u); }
         }
     }
     if (!in) return;
@@ -258,26 +296,25 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
 
 template <class T>
 cudaError_t launch_few(const expert_args &a, void *stream) {
-    cudaError_t e;
-    const int most = a.slots < a.held ? a.slots : a.held;       /* experts that can have slots */
-    {   hy3a_launch l(dim3((a.inter + 7) / 8, most), dim3(32 * kFewWarps), 0, stream);
-        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, false>, a)) != cudaSuccess) return e; }
-    hy3a_launch l(dim3((a.hidden + 15) / 16, most), dim3(32 * kFewWarps), 0, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_kernel<T, true>, a);
+    hy3a_launch l(dim3((a.inter + 7) / 8, a.slots), dim3(32 * kFewWarps), 0, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T>, a);
+    if (e != cudaSuccess) return e;
+    hy3a_launch d(dim3((a.hidden + 15) / 16), dim3(32 * kFewWarps), 0, stream);
+    return cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T>, a);
 }
 template <class T>
 cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
+    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 57.7 / 70.5, 107 / 113, 155 / 154; fp16, 3 of 10 of
+     * 1032 x 200 for 1, 10 rows 7 / 17, 9.4 / 17.8 */
+    if (a.slots < kFewMost) return launch_few<T>(a, stream);
     cudaError_t e;
-    const bool shared = a.slots >= kPlanShared, few = a.slots < kFewMost;
+    const bool shared = a.slots >= kPlanShared;
     {   hy3a_launch l(dim3(shared ? kPlanCluster : 1), dim3(kPlanThreads), 0, stream);
         if (shared) l.cluster(kPlanCluster);
         if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<kPlanCluster>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<1>, a)) != cudaSuccess) return e; }
-    /* a handful of slots (bf16, 192 experts of 4096 x 1536; us a pass, few / umma): 8 slots 74 / 83, 64 slots 390 / 343 */
-    if (few) e = launch_few<T>(a, stream);
-    else e = hy3a_experts_launch_umma(a, type<T>::code, device, sms, stream, what);
-    if (e != cudaSuccess) return e;
+    if ((e = hy3a_experts_launch_umma(a, type<T>::code, device, sms, stream, what)) != cudaSuccess) return e;
     hy3a_launch l(dim3(a.rows, (a.hidden / 8 + 255) / 256), dim3(256), 0, stream);
-    return few ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T, false>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T, true>, a);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T>, a);
 }
 
 int check_sizes(const char *who, int rows, int top_k, int hidden, int inter, int held) {
@@ -319,8 +356,7 @@ int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int i
     if ((rc = hy3a_layer_device("experts", &dev, &sms))) return rc;
     char *b = (char *)work;
     expert_args a = {x, x_stride, ids, weights, gate, up, down, out, out_stride, rows, top_k, hidden, inter, held, first_expert, rows * top_k,
-                     (int *)(b + w.off), (int *)(b + w.active), (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles),
-                     b + w.h, (float *)(b + w.y), (short *)(b + w.y), (float *)(b + w.scale)};
+                     (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles), b + w.h, (short *)(b + w.q), (float *)(b + w.scale)};
     const char *what = NULL;
     const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, dev, sms, stream, &what) : launch<__nv_bfloat16>(a, dev, sms, stream, &what);
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", what ? what : cudaGetErrorString(e));

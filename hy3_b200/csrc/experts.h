@@ -19,14 +19,11 @@ struct expert_args {
     void *out;
     size_t out_stride;
     int rows, top_k, hidden, inter, held, first, slots;
-    int *off;           /* [held + 1] first listed slot of each expert */
-    int *active;        /* [0] number of experts with slots, [1..] which */
     int *row, *place;   /* [slots] rows of the listed slots, expert by expert; where each slot is in that list */
     expert_tile *tiles; /* [*n_tiles] */
     int *n_tiles;
-    void *h;            /* [slots][inter], in the order of the list */
-    float *y;           /* [slots][hidden], in the order of the list: calls with few slots */
-    short *q;           /* the same of the others, in 16 bits: with 2^e the power of two below the largest magnitude of 32 neighbours, multiples of 2^(e - 14) */
+    void *h;            /* [slots][inter], in the order of the list (few slots: of the slots) */
+    short *q;           /* [slots][hidden], in the order of the list: y in 16 bits; with 2^e the power of two below the largest magnitude of 32 neighbours, multiples of 2^(e - 14) */
     float *q_scale;     /* [slots][hidden / 32, rounded up] that scale */
 };
 /* y is written and read once between two launches, and at many slots that is what these take: 8192 slots of 4096 are 134 MB in fp32.  16 bits of
