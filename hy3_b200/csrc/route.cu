@@ -4,6 +4,12 @@
  * s = sigmoid(l) or softmax(l); c = s + bias picks; w = s (renormalised, scaled) weighs.  The selection is a matter of exact values: c
  * is computed with IEEE division and CUDA's expf, the softmax's denominator is summed in 64 bits and rounded once (its value then
  * does not hang on the order of the sum), and ties go to the lowest index.
+ *
+ * A warp takes a row, a lane every 32nd expert.  What bounds it is the number of instructions (a row of 256 logits is 512 to 1024 bytes), so the top
+ * k are not looked for k times over all values: the k-th largest of the 32 lanes' maxima is no larger than the k-th largest value, and the
+ * few values (10 or so of 192) that reach it are packed into a lane each and ranked.  A softmax without bias is selected by exp(l - max), and
+ * only what reaches the threshold is divided: the quotients are in the same order, except that neighbours may round to one, so the threshold
+ * is lowered by more than a rounding.  Rows where more than 32 values reach it (many equal ones) take k searches.
  */
 #include <atomic>
 
@@ -47,7 +53,8 @@ struct route_args {
     const void *logits;
     size_t stride;
     const float *bias;
-    int rows, experts, top_k, softmax, groups, top_groups, renormalize;
+    int rows, experts, top_k, softmax, groups, top_groups, renormalize, group_size;
+    unsigned group_magic;            /* 2^32 / group_size, rounded up: x / group_size is the upper half of x * group_magic for x < 1024 and group_size > 1 */
     float scale;
     int *ids;
     float *weights;
@@ -60,23 +67,30 @@ __device__ __forceinline__ void two_best(float &a, float &b, float c, float d) {
     b = fmaxf(lo, fmaxf(b, d));
 }
 
-/* One warp per row; lane i holds experts i, i + 32, ... (coalesced), VPL of them. */
-template <class T, int VPL, bool GROUPED>
+constexpr float kLowest = -3.402823466e38f;
+/* what a pick counts for: below everything that is open, but open, if it is NaN, so that a row of NaN keeps ids in range and shows NaN weights */
+__device__ __forceinline__ unsigned key_of(float c, bool open) { return !open || c == -INFINITY ? 0u : ordered(isnan(c) ? kLowest : c); }
+
+/* One warp per row; lane i holds experts i, i + 32, ... (coalesced), VPL of them.  QUOTIENT: softmax without bias. */
+template <class T, int VPL, bool GROUPED, bool QUOTIENT>
 __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_args a) {
     __shared__ float s_pick[GROUPED ? kWarps : 1][GROUPED ? 32 * VPL : 1];
+    __shared__ uint4 s_few[kWarps][32];                  /* {key, score, expert} of what reaches the threshold */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kWarps + warp;
     pdl_release();
     pdl_wait();
     if (row >= a.rows) return;
     const T *l = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.stride;
-    float s[VPL];
-    unsigned key[VPL];
+    float s[VPL];                                       /* scores; QUOTIENT: numerators */
+    unsigned key[VPL];                                  /* order of picks, 0: closed */
 #pragma unroll
     for (int j = 0; j < VPL; j++) s[j] = lane + 32 * j < a.experts ? type<T>::up(l[lane + 32 * j]) : -INFINITY;
     unsigned open = 0;                /* bit j: not closed by a logit of -inf (and there) */
 #pragma unroll
     for (int j = 0; j < VPL; j++) open |= s[j] == -INFINITY ? 0u : 1u << j;
-    if (a.softmax) {
+    float d = 1.f;                    /* denominator */
+    bool row_nan = false;
+    if (QUOTIENT || a.softmax) {
         float m = s[0];
         bool nan = false;
 #pragma unroll
@@ -92,9 +106,12 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float d = (float)sum;
+        d = (float)sum;
+        row_nan = isnan(d);           /* also of a row without open experts, and of one with +inf */
+        if (!QUOTIENT) {
 #pragma unroll
-        for (int j = 0; j < VPL; j++) s[j] = __fdiv_rn(s[j], d);
+            for (int j = 0; j < VPL; j++) s[j] = __fdiv_rn(s[j], d);
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < VPL; j++) s[j] = __fdiv_rn(1.f, __fadd_rn(1.f, expf(-s[j])));
@@ -102,24 +119,36 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
 #pragma unroll
     for (int j = 0; j < VPL; j++) {
         const int e = lane + 32 * j;
-        float c = a.bias && e < a.experts ? __fadd_rn(s[j], a.bias[e]) : s[j];
-        if (isnan(c)) c = -3.402823466e38f;      /* below everything that is open, so that a row of NaN keeps ids in range and shows NaN weights */
-        if (!((open >> j) & 1)) c = -INFINITY;
-        key[j] = c == -INFINITY ? 0u : ordered(c);
-        if (GROUPED) s_pick[warp][e] = c;
+        if (QUOTIENT) {
+            const float v = row_nan ? 0.f : s[j];       /* numerators of a NaN row count alike: its quotients all are NaN */
+            key[j] = (open >> j) & 1 ? __float_as_uint(v) + 1u : 0u;
+            if (GROUPED) s_pick[warp][e] = (open >> j) & 1 ? v : -INFINITY;
+        } else {
+            const float c = a.bias && e < a.experts ? __fadd_rn(s[j], a.bias[e]) : s[j];
+            key[j] = key_of(c, (open >> j) & 1);
+            if (GROUPED) s_pick[warp][e] = !((open >> j) & 1) ? -INFINITY : (isnan(c) ? kLowest : c);
+        }
     }
     if (GROUPED) {
         /* a group stands with the sum of its two best open experts: `per` lanes scan each group, and meet */
-        const int size = a.experts / a.groups;
+        const int size = a.group_size;
         int per = 32;
         while (per * a.groups > 32) per >>= 1;
         const int grp = lane / per, sub = lane % per;
         float b1 = -INFINITY, b2 = -INFINITY;
         __syncwarp();
-        if (grp < a.groups) for (int i = sub; i < size; i += per) two_best(b1, b2, s_pick[warp][grp * size + i], -INFINITY);
+        if (grp < a.groups) for (int i = sub; i < size; i += per) {
+            const float v = s_pick[warp][grp * size + i];
+            b2 = fmaxf(b2, fminf(b1, v));
+            b1 = fmaxf(b1, v);
+        }
         for (int o = 1; o < per; o <<= 1) {
             const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
             two_best(b1, b2, c1, c2);
+        }
+        if (QUOTIENT) {
+            b1 = b1 == -INFINITY ? b1 : (row_nan ? kLowest : __fdiv_rn(b1, d));
+            b2 = b2 == -INFINITY ? b2 : (row_nan ? kLowest : __fdiv_rn(b2, d));
         }
         const float stands = b2 == -INFINITY ? b1 : __fadd_rn(b1, b2);
         /* groups that come before this one: better, or as good with a lower index */
@@ -131,44 +160,96 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
         const unsigned kept = __ballot_sync(0xffffffffu, before < a.top_groups);
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
-            const int g = min((lane + 32 * j) / size, a.groups - 1);
-            if (!((kept >> (g * per)) & 1)) key[j] = 0u;
+            const int g = size == 1 ? lane + 32 * j : (int)__umulhi((unsigned)(lane + 32 * j), a.group_magic);      /* (past the last expert: any, it is closed) */
+            if (!((kept >> ((g * per) & 31)) & 1)) key[j] = 0u;
         }
     }
-    int my_id = -1;
-    float my_w = 0.f;
+    /* the k-th largest of the lanes' maxima (equal ones leave together: then of more than k) */
+    unsigned m = key[0], least = 0;
+#pragma unroll
+    for (int j = 1; j < VPL; j++) m = max(m, key[j]);
     for (int r = 0; r < a.top_k; r++) {
-        unsigned m = key[0];
-#pragma unroll
-        for (int j = 1; j < VPL; j++) m = max(m, key[j]);
-        const unsigned best = __reduce_max_sync(0xffffffffu, m);
-        if (best == 0u) break;                  /* only closed experts are left */
-        int e = 0x7fffffff;
-#pragma unroll
-        for (int j = VPL - 1; j >= 0; j--) if (key[j] == best) e = lane + 32 * j;
-        const int id = __reduce_min_sync(0xffffffffu, e);
-        float w = 0.f;
-#pragma unroll
-        for (int j = 0; j < VPL; j++) if (lane + 32 * j == id) { key[j] = 0u; w = s[j]; }
-        w = __shfl_sync(0xffffffffu, w, id & 31);
-        if (lane == r) { my_id = id; my_w = w; }
+        least = __reduce_max_sync(0xffffffffu, m);
+        if (m == least) m = 0u;
     }
+    if (QUOTIENT && least) {
+        /* quotients of numerators that differ by less than 2^-22 may be equal; near the subnormal numbers by more: then everything counts */
+        const float t = __uint_as_float(least - 1u);
+        least = t > 1e-30f ? __float_as_uint(t * (1.f - 9.5367e-7f)) + 1u : 1u;
+    }
+    least = max(least, 1u);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+        const bool in = key[j] >= least;
+        const unsigned all = __ballot_sync(0xffffffffu, in);
+        const int at = n + __popc(all & ((1u << lane) - 1u));
+        if (in && at < 32) s_few[warp][at] = make_uint4(key[j], __float_as_uint(s[j]), lane + 32 * j, 0u);
+        n += __popc(all);
+    }
+    int my_id = -1, rank = lane;                        /* the rank-th choice: expert and weight */
+    float my_w = 0.f;
+    if (n <= 32) {
+        __syncwarp();
+        const uint4 few = s_few[warp][lane];
+        unsigned k = lane < n ? few.x : 0u;
+        float w = __uint_as_float(few.y);
+        if (QUOTIENT) {
+            w = __fdiv_rn(w, d);
+            if (k) k = key_of(w, true);
+        }
+        /* (the list is in the order of the experts) */
+        rank = 0;
+        for (int i = 0; i < n; i++) {
+            const unsigned o = __shfl_sync(0xffffffffu, k, i);
+            rank += o > k || (o == k && i < lane);
+        }
+        if (lane < n) { my_id = (int)few.z; my_w = w; }
+        else rank = lane;                               /* (lanes past the list: the choices that are left) */
+    } else {
+        if (QUOTIENT) {
+#pragma unroll
+            for (int j = 0; j < VPL; j++) {
+                s[j] = __fdiv_rn(s[j], d);
+                if (key[j]) key[j] = key_of(s[j], true);
+            }
+        }
+        for (int r = 0; r < a.top_k; r++) {
+            unsigned top = key[0];
+#pragma unroll
+            for (int j = 1; j < VPL; j++) top = max(top, key[j]);
+            const unsigned best = __reduce_max_sync(0xffffffffu, top);
+            if (best == 0u) break;                      /* only closed experts are left */
+            int e = 0x7fffffff;
+#pragma unroll
+            for (int j = VPL - 1; j >= 0; j--) if (key[j] == best) e = lane + 32 * j;
+            const int id = __reduce_min_sync(0xffffffffu, e);
+            float w = 0.f;
+#pragma unroll
+            for (int j = 0; j < VPL; j++) if (lane + 32 * j == id) { key[j] = 0u; w = s[j]; }
+            w = __shfl_sync(0xffffffffu, w, id & 31);
+            if (lane == r) { my_id = id; my_w = w; }
+        }
+    }
+    if (rank >= a.top_k) my_w = 0.f;
     if (a.renormalize) {
         float sum = my_w;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         my_w = __fdiv_rn(my_w, __fadd_rn(sum, 1e-20f));
     }
-    if (lane < a.top_k) {
-        a.ids[(size_t)row * a.top_k + lane] = my_id;
-        a.weights[(size_t)row * a.top_k + lane] = my_w * a.scale;
+    if (rank < a.top_k) {
+        a.ids[(size_t)row * a.top_k + rank] = my_id;
+        a.weights[(size_t)row * a.top_k + rank] = my_w * a.scale;
     }
 }
 
 template <class T, int VPL>
 cudaError_t launch_vpl(const route_args &a, void *stream) {
     hy3a_launch l(dim3((a.rows + kWarps - 1) / kWarps), dim3(32 * kWarps), 0, stream);
-    return a.groups > 1 ? cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, false>, a);
+    const bool quotient = a.softmax && !a.bias;
+    if (a.groups > 1) return quotient ? cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, true, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, true, false>, a);
+    return quotient ? cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, false, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_route_kernel<T, VPL, false, false>, a);
 }
 template <class T>
 cudaError_t launch_type(const route_args &a, void *stream) {
@@ -200,7 +281,8 @@ extern "C" int hy3a_route(void *stream, int dtype, int rows, int experts, const 
     if (((uintptr_t)logits & (el - 1)) || (((uintptr_t)bias | (uintptr_t)ids | (uintptr_t)weights) & 3)) return hy3a_fail(NULL, HY3A_EINVAL, "route: a pointer is not aligned to its type");
     int dev, sms, rc = hy3a_layer_device("route", &dev, &sms);
     if (rc) return rc;
-    const route_args a = {logits, stride, bias, rows, experts, top_k, score == HY3A_SCORE_SOFTMAX, groups, top_groups, renormalize != 0, scale, ids, weights};
+    const route_args a = {logits, stride, bias, rows, experts, top_k, score == HY3A_SCORE_SOFTMAX, groups, top_groups, renormalize != 0,
+                          experts / groups, (unsigned)(((1ull << 32) + experts / groups - 1) / (experts / groups)), scale, ids, weights};
     const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "route: %s", cudaGetErrorString(e));
     return HY3A_OK;
