@@ -53,12 +53,14 @@ struct route_args {
     const void *logits;
     size_t stride;
     const float *bias;
-    int rows, experts, top_k, softmax, groups, top_groups, renormalize, group_size;
+    int rows, experts, top_k, softmax, groups, top_groups, renormalize, group_size, group_shift /* 2^shift lanes scan a group */, group_skew;
     unsigned group_magic;            /* 2^32 / group_size, rounded up: x / group_size is the upper half of x * group_magic for x < 1024 and group_size > 1 */
     float scale;
     int *ids;
     float *weights;
 };
+
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
 /* the two best of two pairs */
 __device__ __forceinline__ void two_best(float &a, float &b, float c, float d) {
@@ -92,12 +94,10 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
     bool row_nan = false;
     if (QUOTIENT || a.softmax) {
         float m = s[0];
-        bool nan = false;
 #pragma unroll
-        for (int j = 0; j < VPL; j++) { m = fmaxf(m, s[j]); nan |= isnan(s[j]); }
+        for (int j = 1; j < VPL; j++) m = max_nan(m, s[j]);       /* a row with a NaN has no softmax */
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (__any_sync(0xffffffffu, nan)) m = NAN;       /* fmaxf drops a NaN: a row with one has no softmax */
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
@@ -131,16 +131,19 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
     }
     if (GROUPED) {
         /* a group stands with the sum of its two best open experts: `per` lanes scan each group, and meet */
-        const int size = a.group_size;
-        int per = 32;
-        while (per * a.groups > 32) per >>= 1;
-        const int grp = lane / per, sub = lane % per;
+        const int size = a.group_size, shift = a.group_shift, per = 1 << shift, grp = lane >> shift, sub = lane & (per - 1);
         float b1 = -INFINITY, b2 = -INFINITY;
         __syncwarp();
-        if (grp < a.groups) for (int i = sub; i < size; i += per) {
-            const float v = s_pick[warp][grp * size + i];
-            b2 = fmaxf(b2, fminf(b1, v));
-            b1 = fmaxf(b1, v);
+        if (grp < a.groups) {
+            const float *p = s_pick[warp] + grp * size;
+            int i = sub + (a.group_skew ? lane - sub : 0);       /* groups of 32 would all start in the same bank */
+            for (int q = sub; q < size; q += per) {
+                const float v = p[i];
+                b2 = fmaxf(b2, fminf(b1, v));
+                b1 = fmaxf(b1, v);
+                i += per;
+                if (i >= size) i -= size;
+            }
         }
         for (int o = 1; o < per; o <<= 1) {
             const float c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
@@ -151,17 +154,15 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
             b2 = b2 == -INFINITY ? b2 : (row_nan ? kLowest : __fdiv_rn(b2, d));
         }
         const float stands = b2 == -INFINITY ? b1 : __fadd_rn(b1, b2);
-        /* groups that come before this one: better, or as good with a lower index */
+        /* groups that come before this one: better, or as good with a lower index (o > mine, or o >= mine: a key is at least 1) */
+        const unsigned mine = ordered(stands);
         int before = 0;
-        for (int g = 0; g < a.groups; g++) {
-            const float o = __shfl_sync(0xffffffffu, stands, g * per);
-            before += o > stands || (o == stands && g < grp);
-        }
+        for (int g = 0; g < a.groups; g++) before += __shfl_sync(0xffffffffu, mine, g << shift) > mine - (g < grp);
         const unsigned kept = __ballot_sync(0xffffffffu, before < a.top_groups);
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
             const int g = size == 1 ? lane + 32 * j : (int)__umulhi((unsigned)(lane + 32 * j), a.group_magic);      /* (past the last expert: any, it is closed) */
-            if (!((kept >> ((g * per) & 31)) & 1)) key[j] = 0u;
+            if (!((kept >> ((g << shift) & 31)) & 1)) key[j] = 0u;
         }
     }
     /* the k-th largest of the lanes' maxima (equal ones leave together: then of more than k) */
@@ -200,10 +201,8 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
         }
         /* (the list is in the order of the experts) */
         rank = 0;
-        for (int i = 0; i < n; i++) {
-            const unsigned o = __shfl_sync(0xffffffffu, k, i);
-            rank += o > k || (o == k && i < lane);
-        }
+#pragma unroll 4
+        for (int i = 0; i < n; i++) rank += __shfl_sync(0xffffffffu, k, i) > k - (k && i < lane);      /* larger, or as large and before it */
         if (lane < n) { my_id = (int)few.z; my_w = w; }
         else rank = lane;                               /* (lanes past the list: the choices that are left) */
     } else {
@@ -281,8 +280,11 @@ extern "C" int hy3a_route(void *stream, int dtype, int rows, int experts, const 
     if (((uintptr_t)logits & (el - 1)) || (((uintptr_t)bias | (uintptr_t)ids | (uintptr_t)weights) & 3)) return hy3a_fail(NULL, HY3A_EINVAL, "route: a pointer is not aligned to its type");
     int dev, sms, rc = hy3a_layer_device("route", &dev, &sms);
     if (rc) return rc;
+    const int size = experts / groups;
+    int shift = 5;
+    while ((groups << shift) > 32) shift--;
     const route_args a = {logits, stride, bias, rows, experts, top_k, score == HY3A_SCORE_SOFTMAX, groups, top_groups, renormalize != 0,
-                          experts / groups, (unsigned)(((1ull << 32) + experts / groups - 1) / (experts / groups)), scale, ids, weights};
+                          experts / groups, shift, size >= 32 && size % (1 << shift) == 0, (unsigned)(((1ull << 32) + experts / groups - 1) / (experts / groups)), scale, ids, weights};
     const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "route: %s", cudaGetErrorString(e));
     return HY3A_OK;
