@@ -17,11 +17,12 @@
 #include <algorithm>
 #include <atomic>
 
-#include "layer.h"
+#include "ring.cuh"
 
 namespace {
 
 using namespace hy3a_layer;
+using namespace hy3a_ring;
 
 constexpr int kMaxRank = 256;
 constexpr int kCut = 1024;           /* k's of a reduce block: 128 of each of its 8 warps */
@@ -50,6 +51,9 @@ __device__ __forceinline__ int nth_adapter(int id, unsigned todo, int n) {
         todo &= ~__ballot_sync(0xffffffffu, id == ad);
     }
 }
+
+/* the lanes (rows) of an adapter, none for -1 */
+__device__ __forceinline__ unsigned rows_of(int id, int ad) { return __ballot_sync(0xffffffffu, id >= 0 && id == ad); }
 
 /* ---- 1. reduce: block = (8 G rows, 16 RB ranks, a cut); SPLIT: and one of the tile's adapters -------------------------------- */
 template <class T, int G, int RB, bool SPLIT>
@@ -113,9 +117,9 @@ __global__ void __launch_bounds__(32 * kReduceWarps) hy3a_adapters_reduce_kernel
 
 /* Puts a tile's u into shared memory: the cuts' sum, the scale, the split into two numbers; neighbouring threads share a row, four ranks each
  * at a time.  `any`: the rows that have an adapter (the others get zeros). */
-template <class T, int TOK, int THREADS>
-__device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
-    constexpr int PT = THREADS / TOK, NQ = kMaxRank / 4 / PT;
+template <class T, int TOK, int THREADS, int NQ>
+__device__ __forceinline__ void put_u_of(const adapter_args &a, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+    constexpr int PT = THREADS / TOK;
     const int i = threadIdx.x / PT, sub = threadIdx.x % PT;
     const bool on = (any >> i) & 1;
     const float scale = on ? a.scales[a.ids[t0 + i]] : 0.f;
@@ -123,17 +127,20 @@ __device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t
     float4 v[NQ];
     float m = 0.f;
 #pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const int r = 4 * (sub + PT * q);
-        v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on && r < a.rank) {
-#pragma unroll 4
-            for (int c = 0; c < a.cuts; c++) {
-                const float4 w = *reinterpret_cast<const float4 *>(u + (size_t)c * a.rows * a.rank + r);
-                v[q].x += w.x; v[q].y += w.y; v[q].z += w.z; v[q].w += w.w;
-            }
-            v[q].x *= scale; v[q].y *= scale; v[q].z *= scale; v[q].w *= scale;
+    for (int q = 0; q < NQ; q++) v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const size_t step = (size_t)a.rows * a.rank;
+#pragma unroll 2
+    for (int c = 0; c < a.cuts; c++, u += step) {
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            const int r = 4 * (sub + PT * q);
+            const float4 w = on && r < a.rank ? *reinterpret_cast<const float4 *>(u + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[q].x += w.x; v[q].y += w.y; v[q].z += w.z; v[q].w += w.w;
         }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        v[q].x *= scale; v[q].y *= scale; v[q].z *= scale; v[q].w *= scale;
         const float big = 3.402823466e38f, x[4] = {fabsf(v[q].x), fabsf(v[q].y), fabsf(v[q].z), fabsf(v[q].w)};
 #pragma unroll
         for (int z = 0; z < 4; z++) if (x[z] <= big) m = fmaxf(m, x[z]);
@@ -157,6 +164,13 @@ __device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t
             *reinterpret_cast<uint2 *>(s_lo + i * pitch + r) = *reinterpret_cast<const uint2 *>(lo);
         }
     }
+}
+template <class T, int TOK, int THREADS>
+__device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+    constexpr int MOST = kMaxRank * TOK / 4 / THREADS;             /* four ranks at a time of a thread, at the largest rank */
+    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, any, t0, pitch, s_hi, s_lo, s_back);
+    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, any, t0, pitch, s_hi, s_lo, s_back);
+    else put_u_of<T, TOK, THREADS, MOST>(a, any, t0, pitch, s_hi, s_lo, s_back);
 }
 
 /* The columns of the output are the M side of the second product; which of a warp's 64 is which row of it is free, and chosen so that a
@@ -183,7 +197,7 @@ __global__ void __launch_bounds__(32 * kExpandWarps) hy3a_adapters_expand_kernel
     const unsigned none = __ballot_sync(0xffffffffu, lane < 8 && t0 + lane < a.rows && my < 0);
     const int ad = nth_adapter(my, any, blockIdx.z);
     if (ad < 0 && blockIdx.z > 0) return;
-    any = __ballot_sync(0xffffffffu, my >= 0 && my == ad);
+    any = rows_of(my, ad);
     const unsigned rows = any | (blockIdx.z == 0 ? none : 0u);       /* rows without an adapter go with the first */
     uint4 held[2][NB];
 #pragma unroll
@@ -226,151 +240,200 @@ __global__ void __launch_bounds__(32 * kExpandWarps) hy3a_adapters_expand_kernel
     }
 }
 
-/* ---- 2. expand, long inputs: block = (32 rows, `span` columns in tiles of 128) --------------------------------------------
- * Units (column tile, adapter of the row tile, 32 ranks) go through a ring of 4 stages filled by cp.async: 128 rows of B of 32 ranks, and with
- * the last unit of a column tile the tile of base.  A warp has 16 rows x 32 columns; a lane 4 neighbouring columns of each of its rows. */
-constexpr int kLongRows = 32, kLongCols = 128, kLongStages = 4, kLongThreads = 256, kLongSpan = 512;
+/* ---- 2. expand, long inputs: block = (32 rows, 4 column tiles of 128) --------------------------------------------
+ * Units (column tile, adapter of the row tile, 32 ranks) go through a ring of 4 stages that TMA fills: 128 rows of B of 32 ranks, and with
+ * the last unit of a column tile the tile of base, which becomes the tile of the output where it lies and leaves by TMA.  Bounds are the tensor
+ * maps'.  Warps 0-3 multiply (32 rows x 32 columns each), warp 4 fetches, warp 5 stores.  Base and output are what this kernel has to move (168 MB for 2048
+ * rows of 10240 in fp32); written with loads and stores of the multiplying warps, their addresses took more issue slots than the products. */
+constexpr int kLongRows = 32, kLongCols = 128, kLongStages = 4, kLongThreads = 192, kLongTiles = 4;
 template <class O> struct long_stage {
-    static constexpr int pitch = kLongCols * sizeof(O) + 16, b_bytes = kLongCols * 64, bytes = b_bytes + kLongRows * pitch;
+    static constexpr int box = 128 / sizeof(O) /* columns of a box: 128 bytes */, base_bytes = kLongRows * kLongCols * sizeof(O), b_bytes = kLongCols * 64, bytes = b_bytes + base_bytes;
 };
-__device__ __forceinline__ void copy_async(void *dst, const void *src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+enum { A_FULL = 0, A_DONE = kLongStages, A_EMPTY = 2 * kLongStages };
+__device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
+
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-/* 16-byte chunk c of row n of a stage's 32 ranks of B: pairs of rows share 128 bytes, and trade places so that rows 4 apart do not meet in a bank */
-__device__ __forceinline__ int chunk_of(int n, int c) { return (n >> 1) * 128 + (((n ^ (n >> 2)) & 1) << 6) + c * 16; }
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, unsigned src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+}
+
 template <class T, class O>
-__global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_kernel(const adapter_args a) {
-    extern __shared__ uint4 s_raw[];
+__global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_base,
+                                                                                const __grid_constant__ CUtensorMap tm_out, const adapter_args a) {
+    extern __shared__ uint8_t s_bytes[];
     using stage = long_stage<O>;
-    uint8_t *ring = reinterpret_cast<uint8_t *>(s_raw);
+    uint8_t *ring = s_bytes + ((1024u - (smem_u32(s_bytes) & 1023u)) & 1023u);
     const int chunks = (a.rank + 31) >> 5, pitch = chunks * 32 + 8;      /* elements of a row of u: 16 bytes more than a multiple of 64 */
     T *s_hi = reinterpret_cast<T *>(ring + kLongStages * stage::bytes), *s_lo = s_hi + kLongRows * pitch;
     __shared__ float s_back[kLongRows];
-    __shared__ int s_adapter[kLongRows];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int t0 = blockIdx.x * kLongRows, c_begin = blockIdx.y * a.span, c_end = min(a.out_width, c_begin + a.span);
-    const int tok = (warp & 1) * 16, col = (warp >> 1) * 32;             /* the warp's part of a tile */
-    pdl_release();
-    pdl_wait();
-    const int my = id_of(a, t0 + lane);
-    const unsigned any = __ballot_sync(0xffffffffu, my >= 0);
-    int n_ad = 0;                                                        /* adapters of the tile */
-    for (unsigned todo = any; todo; n_ad++) {
-        const int ad = __shfl_sync(0xffffffffu, my, __ffs(todo) - 1);
-        todo &= ~__ballot_sync(0xffffffffu, my == ad);
-        if (tid == 0) s_adapter[n_ad] = ad;
+    __shared__ alignas(8) unsigned long long s_bar[3 * kLongStages];
+    __shared__ int s_abort_flag;
+    volatile int *s_abort = &s_abort_flag;
+    const unsigned bar0 = smem_u32(s_bar);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int across = (a.out_width + kLongCols - 1) / kLongCols;
+    const int t0 = blockIdx.x * kLongRows, first = blockIdx.y * kLongTiles, count = min(kLongTiles, across - first);      /* column tiles */
+    if (tid == 0) {
+        s_abort_flag = 0;
+        for (int i = 0; i < kLongStages; i++) { mbar_init(bar0 + 8 * (A_FULL + i), 1); mbar_init(bar0 + 8 * (A_DONE + i), 4); mbar_init(bar0 + 8 * (A_EMPTY + i), 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    const int tiles = (c_end - c_begin + kLongCols - 1) / kLongCols, per = max(1, n_ad * chunks);
-    /* the thread's 16-byte pieces of a stage, as far as they do not depend on the unit */
-    constexpr int PER = 16 / sizeof(O), QR = kLongCols / PER /* pieces of a row of base */, NBASE = kLongRows * QR / kLongThreads, STEP = kLongThreads / QR;
-    const int bn = tid >> 2, br = (tid & 3) * 8, row0 = tid / QR, c_in = (tid % QR) * PER;
-    const T *b_at = reinterpret_cast<const T *>(a.b) + (size_t)(c_begin + bn) * a.rank + br;
-    const O *base_at = reinterpret_cast<const O *>(a.base) + (size_t)(t0 + row0) * a.base_stride + c_begin + c_in;
-    const size_t ad_size = (size_t)a.out_width * a.rank;
-    int f_c0 = c_begin, f_k = 0, f_r0 = 0;              /* the next unit to fetch: column, adapter of the tile, rank */
-    const T *f_b = b_at + (n_ad ? s_adapter[0] : 0) * ad_size;
-    auto fetch = [&](int slot) {
-        uint8_t *st = ring + slot * stage::bytes;
-        if (f_c0 < c_end) {
-            if (n_ad) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const bool on = f_c0 + bn + 64 * i < c_end && f_r0 + br < a.rank;
-                    copy_async(st + chunk_of(bn + 64 * i, tid & 3), on ? f_b + 64 * i * a.rank : reinterpret_cast<const T *>(a.b), on);
-                }
-                f_b += 32;
-                f_r0 += 32;
-            }
-            if (f_r0 >= a.rank || !n_ad) {
-                f_r0 = 0;
-                if (++f_k >= n_ad) {
-                    f_k = 0;
-#pragma unroll
-                    for (int i = 0; i < NBASE; i++) {
-                        const bool on = t0 + row0 + STEP * i < a.rows && f_c0 + c_in < c_end;
-                        copy_async(st + stage::b_bytes + (row0 + STEP * i) * stage::pitch + c_in * sizeof(O), on ? base_at + (size_t)(STEP * i) * a.base_stride : reinterpret_cast<const O *>(a.base), on);
+    pdl_release();
+    pdl_wait();
+    const int my = id_of(a, t0 + lane);                                  /* lane i: the id of row i of the tile */
+    const unsigned any = __ballot_sync(0xffffffffu, my >= 0);
+    int n_ad = 0;                                                        /* adapters of the tile */
+    for (unsigned todo = any; todo; n_ad++) todo &= ~rows_of(my, __shfl_sync(0xffffffffu, my, __ffs(todo) - 1));
+    const int per = max(1, n_ad * chunks);                               /* units of a column tile */
+    unsigned st = 0, ph = 0;
+    if (warp == 5) {
+        /* gives the stages back, those with output when it has been read */
+        int pending = -1;
+        bool ok = true;
+        for (int tile = 0; tile < count && ok; tile++) {
+            const int c0 = (first + tile) * kLongCols;
+            if (lane == 0) {
+                for (int in = 0; in < per; in++) {
+                    if (!(ok = mbar_wait(bar0 + 8 * (A_DONE + st), ph, s_abort, g_err, 32u))) break;
+                    const bool last = in == per - 1;
+                    if (last) {
+                        for (int i = 0; i < kLongCols / stage::box; i++) {
+                            const int c = c0 + i * stage::box;
+                            if (c < a.out_width) tma_store(&tm_out, smem_u32(ring) + st * stage::bytes + stage::b_bytes + i * kLongRows * 128, c, t0);
+                        }
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
-                    f_c0 += kLongCols;
-                    base_at += kLongCols;
-                    b_at += (size_t)kLongCols * a.rank;
+                    if (pending >= 0) {                 /* the output before this unit's */
+                        if (last) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        mbar_arrive(bar0 + 8 * (A_EMPTY + pending));
+                    }
+                    pending = last ? (int)st : -1;
+                    if (!last) mbar_arrive(bar0 + 8 * (A_EMPTY + st));
+                    if (++st == kLongStages) { st = 0; ph ^= 1u; }
                 }
-                f_b = b_at + (n_ad ? s_adapter[f_k] : 0) * ad_size;
+            }
+            __syncwarp();
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else if (warp == 4) {
+        const unsigned lead = elect_one();
+        bool ok = true;
+        for (int tile = 0; tile < count && ok; tile++) {
+            const int c0 = (first + tile) * kLongCols;
+            int k = 0, r0 = 0, ad = nth_adapter(my, any, 0);
+            for (int in = 0; in < per; in++) {
+                if (!(ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 30u))) break;
+                const unsigned full = bar0 + 8 * (A_FULL + st), dst = smem_u32(ring) + st * stage::bytes;
+                const bool last = in == per - 1;
+                if (lead) {
+                    mbar_expect_tx(full, (n_ad ? stage::b_bytes : 0) + (last ? stage::base_bytes : 0));
+                    if (n_ad) tma_load(dst, &tm_b, full, r0, c0, ad);
+                    if (last)
+                        for (int i = 0; i < kLongCols / stage::box; i++) tma_load(dst + stage::b_bytes + i * kLongRows * 128, &tm_base, full, c0 + i * stage::box, t0);
+                }
+                __syncwarp();
+                if ((r0 += 32) >= a.rank) { r0 = 0; ad = nth_adapter(my, any, ++k); }
+                if (++st == kLongStages) { st = 0; ph ^= 1u; }
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    } else {
+        put_u<T, kLongRows, 128>(a, any, t0, pitch, s_hi, s_lo, s_back);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const T *u_hi = s_hi + g * pitch + t * 8, *u_lo = s_lo + g * pitch + t * 8;
+        const int col = warp * 32;
+        bool ok = true;
+        for (int tile = 0; tile < count && ok; tile++) {
+            float acc[2][4][4] = {};
+            int k = 0, r = 0;
+            unsigned mine = any;                                         /* rows of the unit's adapter */
+            if (n_ad > 1) mine = rows_of(my, nth_adapter(my, any, 0));
+            for (int in = 0; in < per; in++) {
+                if (!(ok = mbar_wait(bar0 + 8 * (A_FULL + st), ph, s_abort, g_err, 31u))) break;
+                uint8_t *const at = ring + st * stage::bytes;
+                if (n_ad) {
+                    /* product m of the warp's two: its row g is column 4g + 2m, row g + 8 the one behind it */
+                    uint4 f[4];
 #pragma unroll
-    for (int u = 0; u < kLongStages - 1; u++) fetch(u);
-    put_u<T, kLongRows, kLongThreads>(a, any, t0, pitch, s_hi, s_lo, s_back);
-    const T *u_hi = s_hi + (tok + g) * pitch + t * 8, *u_lo = s_lo + (tok + g) * pitch + t * 8;
-    O *out = reinterpret_cast<O *>(a.out) + (size_t)(t0 + tok + 2 * t) * a.out_stride + c_begin + col + 4 * g;
-    int slot = 0;
-    for (int tile = 0; tile < tiles; tile++) {
-        float acc[2][2][4] = {};
-        const uint8_t *st = ring;
-        int k = 0, r = 0;
-        for (int in = 0; in < per; in++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kLongStages - 2) : "memory");
-            __syncthreads();                   /* the unit is there for all, and the one before it has been read by all */
-            fetch((slot + kLongStages - 1) % kLongStages);
-            st = ring + slot * stage::bytes;
-            slot = (slot + 1) % kLongStages;
-            if (!n_ad) break;
-            const unsigned mine = n_ad == 1 ? any : __ballot_sync(0xffffffffu, my == s_adapter[k]);
-            if ((mine >> tok) & 0xffff) {
-                /* product m of the warp's two: its row g is column 4g + 2m, row g + 8 the one behind it */
-                uint4 f[4];
+                    for (int j = 0; j < 4; j++) {
+                        const int n = col + 4 * g + j;
+                        f[j] = *reinterpret_cast<const uint4 *>(at + n * 64 + ((t ^ ((n >> 1) & 3)) << 4));
+                    }
 #pragma unroll
-                for (int j = 0; j < 4; j++) f[j] = *reinterpret_cast<const uint4 *>(st + chunk_of(col + 4 * g + j, t));
+                    for (int i = 0; i < 4; i++) {
+                        if (!((mine >> (8 * i)) & 0xff)) continue;
+                        const uint4 hi = *reinterpret_cast<const uint4 *>(u_hi + 8 * i * pitch + r), lo = *reinterpret_cast<const uint4 *>(u_lo + 8 * i * pitch + r);
+                        if (n_ad == 1) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint4 hi = *reinterpret_cast<const uint4 *>(u_hi + 8 * i * pitch + r), lo = *reinterpret_cast<const uint4 *>(u_lo + 8 * i * pitch + r);
-                    if (n_ad == 1) {
+                            for (int m = 0; m < 2; m++) { mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], lo); mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], hi); }
+                        } else {
+                            /* an adapter that is not finite must not reach the others' rows: only its own columns are taken */
+                            const bool c0 = (mine >> (8 * i + 2 * t)) & 1, c1 = (mine >> (8 * i + 2 * t + 1)) & 1;
 #pragma unroll
-                        for (int m = 0; m < 2; m++) { mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], lo); mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], hi); }
-                    } else {
-                        /* an adapter that is not finite must not reach the others' rows: only its own columns are taken */
-                        const bool c0 = (mine >> (tok + 8 * i + 2 * t)) & 1, c1 = (mine >> (tok + 8 * i + 2 * t + 1)) & 1;
-#pragma unroll
-                        for (int m = 0; m < 2; m++) {
-                            float d[4] = {acc[m][i][0], acc[m][i][1], acc[m][i][2], acc[m][i][3]};
-                            mma32<T>(d, f[2 * m], f[2 * m + 1], lo);
-                            mma32<T>(d, f[2 * m], f[2 * m + 1], hi);
-                            if (c0) { acc[m][i][0] = d[0]; acc[m][i][2] = d[2]; }
-                            if (c1) { acc[m][i][1] = d[1]; acc[m][i][3] = d[3]; }
+                            for (int m = 0; m < 2; m++) {
+                                float d[4] = {acc[m][i][0], acc[m][i][1], acc[m][i][2], acc[m][i][3]};
+                                mma32<T>(d, f[2 * m], f[2 * m + 1], lo);
+                                mma32<T>(d, f[2 * m], f[2 * m + 1], hi);
+                                if (c0) { acc[m][i][0] = d[0]; acc[m][i][2] = d[2]; }
+                                if (c1) { acc[m][i][1] = d[1]; acc[m][i][3] = d[3]; }
+                            }
                         }
                     }
+                    if ((r += 32) >= a.rank) {
+                        r = 0;
+                        if (n_ad > 1) mine = rows_of(my, nth_adapter(my, any, ++k));
+                    }
                 }
+                if (in == per - 1) {
+                    struct alignas(4 * sizeof(O)) four { O v[4]; };
+                    four o[4][2];
+                    /* columns 4g .. 4g + 3 of row 8i + 2t + c */
+                    auto place = [&](int i, int c) {
+                        const int row = 8 * i + 2 * t + c, b = (col + 4 * g) * (int)sizeof(O);           /* byte of the tile's row */
+                        return reinterpret_cast<four *>(at + stage::b_bytes + (b >> 7) * kLongRows * 128 + row * 128 + ((((b >> 4) & 7) ^ (row & 7)) << 4) + (b & 15));
+                    };
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) o[i][c] = *place(i, c);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const int row = 8 * i + 2 * t + c;
+                            const float back = s_back[row];
+                            const bool with = (any >> row) & 1;
+#pragma unroll
+                            for (int z = 0; z < 4; z++) {
+                                const O v = type<O>::down(type<O>::up(o[i][c].v[z]) + back * acc[z >> 1][i][(z & 1) * 2 + c]);
+                                if (with) o[i][c].v[z] = v;
+                            }
+                            *place(i, c) = o[i][c];
+                        }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar0 + 8 * (A_DONE + st));
+                if (++st == kLongStages) { st = 0; ph ^= 1u; }
             }
-            if ((r += 32) >= a.rank) { r = 0; k++; }
         }
-        const bool in_columns = c_begin + tile * kLongCols + col + 4 * g < c_end;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int row = tok + 8 * i + 2 * t + c;
-                struct alignas(4 * sizeof(O)) four { O v[4]; };
-                four o = *reinterpret_cast<const four *>(st + stage::b_bytes + row * stage::pitch + (col + 4 * g) * sizeof(O));
-                if ((any >> row) & 1) {
-                    const float back = s_back[row];
-#pragma unroll
-                    for (int z = 0; z < 4; z++) o.v[z] = type<O>::down(type<O>::up(o.v[z]) + back * acc[z >> 1][i][(z & 1) * 2 + c]);
-                }
-                if (t0 + row < a.rows && in_columns) *reinterpret_cast<four *>(out + (size_t)(8 * i + c) * a.out_stride) = o;
-            }
-        out += kLongCols;
     }
+    if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the unit that was given up are still on their way */
 }
 
 constexpr int kShort = 256;           /* rows up to which a tile's adapters are blocks of their own */
 
 template <class T, class O>
-cudaError_t launch(adapter_args a, int device, int sms, void *stream) {
+cudaError_t launch(adapter_args a, int device, void *stream, const char **what) {
     cudaError_t e;
     const int pitch = (a.rank + 31) / 32 * 32 + 8, rank_blocks = (a.rank + 15) / 16;
-    if (a.rows <= kShort) {
+    if (a.rows <= kShort || a.base_stride < (size_t)a.out_width) {      /* (rows of base that overlap, as of one that is expanded, have no tensor map) */
         const int tiles = (a.rows + 7) / 8, z = std::min({8, a.rows, a.adapters});
         {   hy3a_launch l(dim3(tiles, a.cuts * rank_blocks, z), dim3(32 * kReduceWarps), 0, stream);
             if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true>, a)) != cudaSuccess) return e; }
@@ -378,18 +441,25 @@ cudaError_t launch(adapter_args a, int device, int sms, void *stream) {
         hy3a_launch l(dim3(tiles, (a.out_width + a.span - 1) / a.span, z), dim3(32 * kExpandWarps), (size_t)2 * 8 * pitch * sizeof(T), stream);
         return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_kernel<T, O>, a);
     }
-    constexpr int kMostSmem = kLongStages * long_stage<O>::bytes + 2 * kLongRows * (kMaxRank + 8) * sizeof(T);
+    constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kMostSmem = kRing + 2 * kLongRows * (kMaxRank + 8) * sizeof(T);
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
         if ((e = cudaFuncSetAttribute(hy3a_adapters_expand_long_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
+    CUtensorMap tm_b, tm_base, tm_out;
+    constexpr int box = long_stage<O>::box;
+    if (!encode(&tm_b, 3, a.b, 2, a.rank, a.out_width, a.adapters, a.rank, 32, kLongCols) || !encode(&tm_base, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, kLongRows) ||
+        !encode(&tm_out, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, kLongRows)) {
+        *what = "no tensor map (cuTensorMapEncodeTiled)";
+        return cudaErrorInvalidValue;
+    }
     const int tiles = (a.rows + kLongRows - 1) / kLongRows;
     {   hy3a_launch l(dim3(tiles, a.cuts * ((rank_blocks + 1) / 2)), dim3(32 * kReduceWarps), 0, stream);
         if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, kLongRows / 8, 2, false>, a)) != cudaSuccess) return e; }
-    a.span = kLongSpan;
-    hy3a_launch l(dim3(tiles, (a.out_width + a.span - 1) / a.span), dim3(kLongThreads), kLongStages * long_stage<O>::bytes + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, a);
+    const int across = (a.out_width + kLongCols - 1) / kLongCols;
+    hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, a);
 }
 
 int check_sizes(const char *who, int rows, int width, int rank) {
@@ -401,6 +471,13 @@ int check_sizes(const char *who, int rows, int width, int rank) {
 int cuts_of(int width) { return (width + kCut - 1) / kCut; }
 
 } /* namespace */
+
+cudaError_t hy3a_adapters_error(unsigned *err) {
+    const unsigned none[2] = {0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
+    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
+    return e;
+}
 
 extern "C" {
 
@@ -430,9 +507,10 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
     if (work_bytes < need) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: the workspace has %zu bytes, %zu are needed (hy3a_adapters_workspace)", work_bytes, need);
     const adapter_args a = {x, base, a_, b_, x_stride, base_stride, out_stride, ids, scales, out, (float *)work, rows, width, out_width, adapters, rank, cuts_of(width), 0};
     cudaError_t e;
-    if (dtype == HY3A_F16) e = base_dtype == HY3A_F32 ? launch<__half, float>(a, dev, sms, stream) : launch<__half, __half>(a, dev, sms, stream);
-    else e = base_dtype == HY3A_F32 ? launch<__nv_bfloat16, float>(a, dev, sms, stream) : launch<__nv_bfloat16, __nv_bfloat16>(a, dev, sms, stream);
-    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "adapters: %s", cudaGetErrorString(e));
+    const char *what = NULL;
+    if (dtype == HY3A_F16) e = base_dtype == HY3A_F32 ? launch<__half, float>(a, dev, stream, &what) : launch<__half, __half>(a, dev, stream, &what);
+    else e = base_dtype == HY3A_F32 ? launch<__nv_bfloat16, float>(a, dev, stream, &what) : launch<__nv_bfloat16, __nv_bfloat16>(a, dev, stream, &what);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "adapters: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;
 }
 

@@ -19,15 +19,15 @@
  * Every wait is bounded; one that runs out raises the CTA's abort flag and a code in the error word (hy3a_layer_sync), lets all warps fall
  * through, and TMEM is always released.
  */
-#include <cuda.h>
-
 #include <atomic>
 
 #include "experts.h"
+#include "ring.cuh"
 
 namespace {
 
 using namespace hy3a_layer;
+using namespace hy3a_ring;
 
 constexpr int kStages = 6, kEpilogues = 8, kProducer = kEpilogues, kProducers = 8, kIssuer = kProducer + kProducers, kThreads = 32 * (kIssuer + 1);
 constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;      /* 128 rows of 64 k's, 2 bytes each */
@@ -38,30 +38,7 @@ static_assert(8 * B_COUNT + 16 <= 256, "barriers");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
-__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
-__device__ __forceinline__ void mbar_expect_tx(unsigned bar, unsigned bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity, unsigned hint_ns) {
-    unsigned ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(hint_ns) : "memory");
-    return ok != 0;
-}
-/* Waits until the phase of that parity is over; false once anything in the CTA has given up.  A wait gives up after half a second and many polls. */
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int *abort_flag, unsigned where) {
-    if (mbar_try(bar, parity, 2000u)) return true;
-    unsigned long long t0, t1;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-    for (unsigned i = 0; i < (1u << 22); i++) {
-        if (mbar_try(bar, parity, 20000u)) return true;
-        if (*abort_flag) return false;
-        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-        if (i >= (1u << 13) && t1 - t0 > 500000000ull) break;
-    }
-    *abort_flag = 1;
-    if (atomicCAS(&g_err[0], 0u, 2u) == 0u) g_err[1] = where;
-    return false;
-}
 __device__ __forceinline__ unsigned cluster_addr(unsigned addr, unsigned rank) {
     unsigned r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -86,11 +63,6 @@ __device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap *map
 /* K-major operand, 128-byte swizzle: 8-row groups 1024 B apart, descriptor version 1, layout 2 */
 __device__ __forceinline__ unsigned long long make_desc(unsigned saddr) {
     return (unsigned long long)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ unsigned elect_one() {
-    unsigned p;
-    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));
-    return p;
 }
 __device__ __forceinline__ void umma_lead(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate, unsigned lead) {
     asm volatile("{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n @e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
@@ -133,7 +105,7 @@ __device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, 
                                         int part, int m, int e, const int4 (&row)[4], unsigned lead) {
     unsigned st = q.st, ph = q.ph;
     for (int s = 0; s < steps; s++) {
-        if (!mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, 20u)) return false;
+        if (!mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
         const unsigned full = cluster_addr(bar0 + 8u * (B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
         if (bytes && lead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
         if (!DOWN) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
@@ -220,7 +192,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         unsigned st = q.st, ph = q.ph;
         /* the last commits reach the barriers of both CTAs before either leaves */
         for (int i = 0; i < kStages && !*s_abort; i++) {
-            if (!mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, 24u)) break;
+            if (!mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, g_err, 24u)) break;
             if (++st == kStages) { st = 0; ph ^= 1u; }
         }
     } else if (warp == kIssuer) {
@@ -232,11 +204,11 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             for (int t = pair; t < total; t += pairs) {
                 const where w = tile_of<DOWN>(a, t, m_tiles);
                 const unsigned idesc = (1u << 4) | kType | (((unsigned)(w.n + 15) >> 4) << 18) | ((256u >> 4) << 24);
-                if (!mbar_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, 21u)) break;
+                if (!mbar_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, g_err, 21u)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 bool ok = true;
                 for (int s = 0; s < steps; s++) {
-                    if (!(ok = mbar_wait(BAR(B_FULL + st), ph, s_abort, 22u))) break;
+                    if (!(ok = mbar_wait(BAR(B_FULL + st), ph, s_abort, g_err, 22u))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned sa = sbase + st * (kABytes + kBBytes);
                     const unsigned long long da = make_desc(sa), db = make_desc(sa + kABytes);
@@ -261,7 +233,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         const bool whole = !(a.hidden & 15);
         for (int t = pair; t < total; t += pairs) {
             const where w = tile_of<DOWN>(a, t, m_tiles);
-            if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, 23u)) break;
+            if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, g_err, 23u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int m0 = DOWN ? w.m0 + (int)rank * 128 + quarter * 32 : w.m0 + (int)rank * 64 + quarter * 16;
             for (int c0 = (warp >> 2) * 16; c0 < w.n; c0 += 32) {
@@ -333,24 +305,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
 #undef BAR
 }
 
-typedef CUresult (*encode_tiled_fn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
-                                    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-encode_tiled_fn find_encode_tiled() {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
-    return (encode_tiled_fn)p;
-}
-
 struct maps { CUtensorMap gate, up, down, x, h; };
-/* 16-bit rows of `inner`, boxes of 64 of them: [depth][rows][inner], or [rows][inner] with a stride to gather from */
-bool encode(encode_tiled_fn enc, CUtensorMap *m, int rank, const void *base, size_t inner, size_t rows, size_t depth, size_t stride, int box_rows) {
-    const cuuint64_t dims[3] = {inner, rows, depth}, strides[2] = {stride * 2, stride * rows * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
-    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <class T>
 cudaError_t launch(const expert_args &a, const maps &m, int device, int sms, void *stream) {
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
@@ -370,24 +325,18 @@ cudaError_t launch(const expert_args &a, const maps &m, int device, int sms, voi
 } /* namespace */
 
 cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device, int sms, void *stream, const char **what) {
-    static const encode_tiled_fn enc = find_encode_tiled();
     *what = nullptr;
-    if (!enc) { *what = "cuTensorMapEncodeTiled is not available from the driver"; return cudaErrorNotSupported; }
     maps m;
-    /* (the two 16-bit types are moved alike) */
-    const bool ok = encode(enc, &m.gate, 3, a.gate, a.hidden, a.inter, a.held, a.hidden, 16) && encode(enc, &m.up, 3, a.up, a.hidden, a.inter, a.held, a.hidden, 16) &&
-                    encode(enc, &m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 128) && encode(enc, &m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 1) &&
-                    encode(enc, &m.h, 3, a.h, a.inter, a.slots, 1, a.inter, 8);
-    if (!ok) { *what = "cuTensorMapEncodeTiled failed"; return cudaErrorInvalidValue; }
+    const bool ok = encode(&m.gate, 3, a.gate, 2, a.hidden, a.inter, a.held, a.hidden, 64, 16) && encode(&m.up, 3, a.up, 2, a.hidden, a.inter, a.held, a.hidden, 64, 16) &&
+                    encode(&m.down, 3, a.down, 2, a.inter, a.hidden, a.held, a.inter, 64, 128) && encode(&m.x, 2, a.x, 2, a.hidden, a.rows, 1, a.x_stride, 64, 1) &&
+                    encode(&m.h, 3, a.h, 2, a.inter, a.slots, 1, a.inter, 64, 8);
+    if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
     return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
 }
 
-extern "C" int hy3a_layer_sync(void *stream) {
-    unsigned err[2] = {0, 0}, none[2] = {0, 0};
-    cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(err, g_err, sizeof(err));
+cudaError_t hy3a_experts_error(unsigned *err) {
+    const unsigned none[2] = {0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
     if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
-    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_sync: %s", cudaGetErrorString(e));
-    if (err[0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", err[0], err[1]);
-    return HY3A_OK;
+    return e;
 }

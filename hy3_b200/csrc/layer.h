@@ -18,6 +18,10 @@
 /* The current device's number and SM count; refuses devices that sm_100a code cannot run on. */
 int hy3a_layer_device(const char *who, int *device, int *sms);
 
+/* The files' error words {code, where} of the first wait that ran out on the current device; read and cleared. */
+cudaError_t hy3a_experts_error(unsigned *err);
+cudaError_t hy3a_adapters_error(unsigned *err);
+
 /* launch configuration with programmatic stream serialisation: the kernels wait (pdl_wait) before they touch memory */
 struct hy3a_launch {
     cudaLaunchConfig_t cfg;

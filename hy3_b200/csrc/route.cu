@@ -289,3 +289,14 @@ extern "C" int hy3a_route(void *stream, int dtype, int rows, int experts, const 
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "route: %s", cudaGetErrorString(e));
     return HY3A_OK;
 }
+
+extern "C" int hy3a_layer_sync(void *stream) {
+    unsigned err[2][2] = {{0, 0}, {0, 0}};
+    cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e == cudaSuccess) e = hy3a_experts_error(err[0]);
+    if (e == cudaSuccess) e = hy3a_adapters_error(err[1]);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_sync: %s", cudaGetErrorString(e));
+    for (int i = 0; i < 2; i++)
+        if (err[i][0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "%s: a device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", i ? "adapters" : "experts", err[i][0], err[i][1]);
+    return HY3A_OK;
+}
