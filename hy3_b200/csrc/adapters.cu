@@ -56,8 +56,8 @@ __device__ __forceinline__ int nth_adapter(int id, unsigned todo, int n) {
 __device__ __forceinline__ unsigned rows_of(int id, int ad) { return __ballot_sync(0xffffffffu, id >= 0 && id == ad); }
 
 /* ---- 1. reduce: block = (8 G rows, 16 RB ranks, a cut); SPLIT: and one of the tile's adapters -------------------------------- */
-template <class T, int G, int RB, bool SPLIT>
-__global__ void __launch_bounds__(32 * kReduceWarps) hy3a_adapters_reduce_kernel(const adapter_args a) {
+template <class T, int G, int RB, bool SPLIT, bool WIDE>
+__global__ void __launch_bounds__(32 * kReduceWarps, G > 1 ? 2 : 4) hy3a_adapters_reduce_kernel(const adapter_args a) {
     __shared__ float s_sum[kReduceWarps][RB][G][4][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rank_blocks = (a.rank + 16 * RB - 1) / (16 * RB), cut = blockIdx.y / rank_blocks, r0 = (blockIdx.y - cut * rank_blocks) * 16 * RB, t0 = blockIdx.x * 8 * G;
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(32 * kReduceWarps) hy3a_adapters_reduce_kernel
         if (ad < 0) return;
         todo = __ballot_sync(0xffffffffu, id == ad);
     }
-    const int k0 = cut * kCut + warp * (kCut / kReduceWarps) + t * 8;
+    const int k0 = cut * kCut + warp * (kCut / kReduceWarps) + t * 16;
     while (todo) {
         const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
         const unsigned mine = __ballot_sync(0xffffffffu, id == ad);
@@ -78,20 +78,19 @@ __global__ void __launch_bounds__(32 * kReduceWarps) hy3a_adapters_reduce_kernel
         const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)ad * a.rank + r0 + g) * a.width;
         float acc[RB][G][4] = {};
 #pragma unroll
-        for (int i = 0; i < kCut / kReduceWarps / 32; i++) {
-            const int k = k0 + 32 * i;
-            uint4 lo[RB], hi[RB];
+        for (int i = 0; i < kCut / kReduceWarps / 64; i++) {
+            const int k = k0 + 64 * i;
+            k16 lo[RB], hi[RB];
 #pragma unroll
             for (int b = 0; b < RB; b++) {
-                lo[b] = r0 + 16 * b + g < a.rank && k < a.width ? load_row(w + (size_t)16 * b * a.width + k) : zero16();
-                hi[b] = r0 + 16 * b + 8 + g < a.rank && k < a.width ? load_row(w + (size_t)(16 * b + 8) * a.width + k) : zero16();
+                lo[b] = load16<WIDE, false>(w + (size_t)16 * b * a.width + k, r0 + 16 * b + g < a.rank ? a.width - k : 0);
+                hi[b] = load16<WIDE, false>(w + (size_t)(16 * b + 8) * a.width + k, r0 + 16 * b + 8 + g < a.rank ? a.width - k : 0);
             }
 #pragma unroll
             for (int j = 0; j < G; j++) {
-                const bool on = (mine >> (8 * j + g)) & 1;
-                const uint4 x = on && k < a.width ? load_row(reinterpret_cast<const T *>(a.x) + (size_t)(t0 + 8 * j + g) * a.x_stride + k) : zero16();
+                const k16 x = load16<WIDE, false>(reinterpret_cast<const T *>(a.x) + (size_t)(t0 + 8 * j + g) * a.x_stride + k, (mine >> (8 * j + g)) & 1 ? a.width - k : 0);
 #pragma unroll
-                for (int b = 0; b < RB; b++) mma32<T>(acc[b][j], lo[b], hi[b], x);
+                for (int b = 0; b < RB; b++) mma64<T>(acc[b][j], lo[b], hi[b], x);
             }
         }
 #pragma unroll
@@ -433,10 +432,11 @@ template <class T, class O>
 cudaError_t launch(adapter_args a, int device, void *stream, const char **what) {
     cudaError_t e;
     const int pitch = (a.rank + 31) / 32 * 32 + 8, rank_blocks = (a.rank + 15) / 16;
+    const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
     if (a.rows <= kShort || a.base_stride < (size_t)a.out_width) {      /* (rows of base that overlap, as of one that is expanded, have no tensor map) */
         const int tiles = (a.rows + 7) / 8, z = std::min({8, a.rows, a.adapters});
         {   hy3a_launch l(dim3(tiles, a.cuts * rank_blocks, z), dim3(32 * kReduceWarps), 0, stream);
-            if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true>, a)) != cudaSuccess) return e; }
+            if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true, false>, a)) != cudaSuccess) return e; }
         a.span = kExpandWarps * kExpandCols;
         hy3a_launch l(dim3(tiles, (a.out_width + a.span - 1) / a.span, z), dim3(32 * kExpandWarps), (size_t)2 * 8 * pitch * sizeof(T), stream);
         return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_kernel<T, O>, a);
@@ -455,8 +455,8 @@ cudaError_t launch(adapter_args a, int device, void *stream, const char **what) 
         return cudaErrorInvalidValue;
     }
     const int tiles = (a.rows + kLongRows - 1) / kLongRows;
-    {   hy3a_launch l(dim3(tiles, a.cuts * ((rank_blocks + 1) / 2)), dim3(32 * kReduceWarps), 0, stream);
-        if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, kLongRows / 8, 2, false>, a)) != cudaSuccess) return e; }
+    {   hy3a_launch l(dim3((a.rows + 15) / 16, a.cuts * ((rank_blocks + 1) / 2)), dim3(32 * kReduceWarps), 0, stream);
+        if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false, false>, a)) != cudaSuccess) return e; }
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
     hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, a);

@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const e
 
 /* ---- calls with few slots (at most 31; the others: experts_umma.cu) -----------------------------------------------------
  * Two launches, without a plan: every warp sees all slots.  The first slot of an expert leads, and takes the expert's other slots along, 8 at a
- * time (more than 8 read the weights again, from L2).  Fragments come straight from global memory (layer.h), 16 loads of 16 bytes in
+ * time (more than 8 read the weights again, from L2).  Fragments come straight from global memory (layer.h), 8 loads of 32 bytes in
  * flight a lane. */
-constexpr int kFewWarps = 8, kFewLoads = 8 /* k blocks of 32 in flight */;
+constexpr int kFewWarps = 8, kFewLoads = 4 /* k blocks of 64 in flight */;
 /* lane s: expert of slot s (-1: none), the slots of the same expert */
 __device__ __forceinline__ int few_slots(const expert_args &a, unsigned &same) {
     const int lane = threadIdx.x & 31, e = lane < a.slots ? local_expert(a, a.ids[lane]) : -1;
@@ -150,22 +150,22 @@ __device__ __forceinline__ int nth_bit(unsigned bits, int n) {
     for (; n > 0; n--) bits &= bits - 1;
     return bits ? __ffs(bits) - 1 : -1;
 }
-template <class T> __device__ __forceinline__ void few_load(uint4 (&lo)[kFewLoads], uint4 (&hi)[kFewLoads], const T *w_lo, const T *w_hi, bool has_lo, bool has_hi, int k, int step, int K) {
+template <class T, bool WIDE> __device__ __forceinline__ void few_load(k16 (&lo)[kFewLoads], k16 (&hi)[kFewLoads], const T *w_lo, const T *w_hi, bool has_lo, bool has_hi, int k, int step, int K) {
 #pragma unroll
     for (int u = 0; u < kFewLoads; u++) {
-        lo[u] = has_lo && k + u * step < K ? load_once(w_lo + k + u * step) : zero16();
-        hi[u] = has_hi && k + u * step < K ? load_once(w_hi + k + u * step) : zero16();
+        lo[u] = load16<WIDE, true>(w_lo + k + u * step, has_lo ? K - k - u * step : 0);
+        hi[u] = load16<WIDE, true>(w_hi + k + u * step, has_hi ? K - k - u * step : 0);
     }
 }
-template <class T> __device__ __forceinline__ void few_multiply(float (&acc)[4], const uint4 (&lo)[kFewLoads], const uint4 (&hi)[kFewLoads], const T *row, int k, int step, int K) {
+template <class T, bool WIDE> __device__ __forceinline__ void few_multiply(float (&acc)[4], const k16 (&lo)[kFewLoads], const k16 (&hi)[kFewLoads], const T *row, int k, int step, int K) {
 #pragma unroll
-    for (int u = 0; u < kFewLoads; u++) mma32<T>(acc, lo[u], hi[u], row && k + u * step < K ? load_row(row + k + u * step) : zero16());
+    for (int u = 0; u < kFewLoads; u++) mma64<T>(acc, lo[u], hi[u], load16<WIDE, false>(row + k + u * step, row ? K - k - u * step : 0));
 }
 
 /* h of one expert's slots, 8 of its rows: block = (8 pairs of gate and up rows, slot that may lead); the warps share the k's, and their sums
  * meet in shared memory in a fixed order.  Rows 0-7 of A are gate rows, rows 8-15 the up rows of the same index: both halves of a pair lie in
  * one lane. */
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(const expert_args a) {
     __shared__ float s_sum[kFewWarps][4][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -175,17 +175,17 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(
     const int mine = few_slots(a, same), e = __shfl_sync(0xffffffffu, mine, blockIdx.y);
     const unsigned slots = __shfl_sync(0xffffffffu, same, blockIdx.y);
     if (e < 0 || (int)blockIdx.y != __ffs(slots) - 1) return;
-    const int K = a.hidden, M = a.inter, m0 = blockIdx.x * 8, step = 32 * kFewWarps;
+    const int K = a.hidden, M = a.inter, m0 = blockIdx.x * 8, step = 64 * kFewWarps;
     const bool has = m0 + g < M;
     const T *gate = reinterpret_cast<const T *>(a.gate) + ((size_t)e * M + m0 + g) * K, *up = reinterpret_cast<const T *>(a.up) + ((size_t)e * M + m0 + g) * K;
     for (int base = 0; base < __popc(slots); base += 8) {
         const int s = nth_bit(slots, base + g);
         const T *x = s >= 0 ? reinterpret_cast<const T *>(a.x) + (size_t)(s / a.top_k) * a.x_stride : nullptr;
         float acc[4] = {};
-        for (int kb = warp * 32; kb < K; kb += step * kFewLoads) {
-            uint4 lo[kFewLoads], hi[kFewLoads];
-            few_load(lo, hi, gate, up, has, has, kb + t * 8, step, K);
-            few_multiply(acc, lo, hi, x, kb + t * 8, step, K);
+        for (int kb = warp * 64; kb < K; kb += step * kFewLoads) {
+            k16 lo[kFewLoads], hi[kFewLoads];
+            few_load<T, WIDE>(lo, hi, gate, up, has, has, kb + t * 16, step, K);
+            few_multiply<T, WIDE>(acc, lo, hi, x, kb + t * 16, step, K);
         }
         if (base) __syncthreads();
 #pragma unroll
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(
 
 /* out: block = 16 columns; its warps take the experts in turn, or shares of their k's where there are fewer experts than warps, and the slots'
  * sums are weighed and added up in shared memory, in the order of the choices.  The first weights are on their way before the wait for h. */
-template <class T>
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kernel(const expert_args a) {
     __shared__ float s_y[kFewWarps][kFewMost][16];                         /* [share of the k's][slot][column] */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
     const int mine = few_slots(a, same);
     const unsigned any = __ballot_sync(0xffffffffu, mine >= 0), leaders = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(same) - 1);
     const int n = __popc(leaders), shares = n ? max(1, kFewWarps / n) : 1;
-    const int K = a.inter, M = a.hidden, m0 = blockIdx.x * 16, step = shares * 32;
+    const int K = a.inter, M = a.hidden, m0 = blockIdx.x * 16, step = shares * 64;
     bool waited = false;
     for (int unit = warp; unit < n * shares; unit += kFewWarps) {
         const int which = unit / shares, share = unit - which * shares, lead = nth_bit(leaders, which);
@@ -224,11 +224,11 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
             const int s = nth_bit(slots, base + g);
             const T *h = s >= 0 ? reinterpret_cast<const T *>(a.h) + (size_t)s * K : nullptr;
             float acc[4] = {};
-            for (int kb = share * 32; kb < K; kb += step * kFewLoads) {
-                uint4 lo[kFewLoads], hi[kFewLoads];
-                few_load(lo, hi, w_lo, w_hi, has_lo, has_hi, kb + t * 8, step, K);
+            for (int kb = share * 64; kb < K; kb += step * kFewLoads) {
+                k16 lo[kFewLoads], hi[kFewLoads];
+                few_load<T, WIDE>(lo, hi, w_lo, w_hi, has_lo, has_hi, kb + t * 16, step, K);
                 if (!waited) { pdl_wait(); waited = true; }
-                few_multiply(acc, lo, hi, h, kb + t * 8, step, K);
+                few_multiply<T, WIDE>(acc, lo, hi, h, kb + t * 16, step, K);
             }
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -297,10 +297,11 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
 template <class T>
 cudaError_t launch_few(const expert_args &a, void *stream) {
     hy3a_launch l(dim3((a.inter + 7) / 8, a.slots), dim3(32 * kFewWarps), 0, stream);
-    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T>, a);
+    const bool wide_up = wide_rows({a.x, a.gate, a.up}, {a.x_stride, (size_t)a.hidden}), wide_down = wide_rows({a.down}, {(size_t)a.inter});
+    const cudaError_t e = wide_up ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T, false>, a);
     if (e != cudaSuccess) return e;
     hy3a_launch d(dim3((a.hidden + 15) / 16), dim3(32 * kFewWarps), 0, stream);
-    return cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T>, a);
+    return wide_down ? cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T, true>, a) : cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T, false>, a);
 }
 template <class T>
 cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
