@@ -24,7 +24,7 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kMaxRank = 256;
+constexpr int kMaxRank = 256, kMaxWidth = 1 << 20;
 constexpr int kCut = 1024;           /* k's of a reduce block: 128 of each of its 8 warps */
 constexpr int kReduceWarps = 8, kExpandWarps = 4, kExpandCols = 64 /* columns of a warp at a time */;
 
@@ -465,6 +465,7 @@ cudaError_t launch(adapter_args a, int device, void *stream, const char **what) 
 int check_sizes(const char *who, int rows, int width, int rank) {
     if (rows < 0) return hy3a_fail(NULL, HY3A_EINVAL, "%s: rows %d < 0", who, rows);
     if (width < 8 || width % 8) return hy3a_fail(NULL, HY3A_EINVAL, "%s: width %d is no multiple of 8", who, width);
+    if (width > kMaxWidth) return hy3a_fail(NULL, HY3A_EINVAL, "%s: width %d is over %d", who, width, kMaxWidth);
     if (rank < 8 || rank % 8 || rank > kMaxRank) return hy3a_fail(NULL, HY3A_EINVAL, "%s: rank %d is no multiple of 8 up to %d (fill smaller ones up with zeros)", who, rank, kMaxRank);
     return 0;
 }
@@ -493,6 +494,7 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
     if (base_dtype != dtype && base_dtype != HY3A_F32) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: base_dtype %d is neither the rows' (%d) nor fp32", base_dtype, dtype);
     int rc = check_sizes("adapters", rows, width, rank);
     if (rc) return rc;
+    if (out_width > kMaxWidth) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: out_width %d is over %d", out_width, kMaxWidth);
     if (out_width < 8 || out_width % 8) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: out_width %d is no multiple of 8", out_width);
     if (adapters < 1) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: %d adapters", adapters);
     if (rows == 0) return HY3A_OK;

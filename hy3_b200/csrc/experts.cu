@@ -318,12 +318,15 @@ cudaError_t launch(const expert_args &a, int device, int sms, void *stream, cons
     return cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T>, a);
 }
 
+/* tiles are counted in 32 bits: 2^28 slots in tiles of 256, times 2^16 weight rows in tiles of 128 (pairs) */
+constexpr int kMaxWidth = 65536;
 int check_sizes(const char *who, int rows, int top_k, int hidden, int inter, int held) {
     if (rows < 0) return hy3a_fail(NULL, HY3A_EINVAL, "%s: rows %d < 0", who, rows);
     if (top_k < 1 || top_k > 32) return hy3a_fail(NULL, HY3A_EINVAL, "%s: top_k %d not in [1,32]", who, top_k);
     if (hidden < 8 || hidden % 8 || inter < 8 || inter % 8) return hy3a_fail(NULL, HY3A_EINVAL, "%s: hidden %d and inter %d have to be multiples of 8", who, hidden, inter);
     if (held < 1 || held > kMaxHeld) return hy3a_fail(NULL, HY3A_EINVAL, "%s: %d experts held, not in [1,%d]", who, held, kMaxHeld);
-    if ((long long)rows * top_k > 0x7fffffffll / 2) return hy3a_fail(NULL, HY3A_EINVAL, "%s: %d rows of %d slots are too many", who, rows, top_k);
+    if (hidden > kMaxWidth || inter > kMaxWidth) return hy3a_fail(NULL, HY3A_EINVAL, "%s: hidden %d or inter %d is over %d", who, hidden, inter, kMaxWidth);
+    if ((long long)rows * top_k >= 1ll << 28) return hy3a_fail(NULL, HY3A_EINVAL, "%s: %d rows of %d slots are too many", who, rows, top_k);
     return 0;
 }
 

@@ -269,7 +269,7 @@ int hy3a_route(void *stream, int dtype, int rows, int experts, const void *logit
  * e = ids[t][j], sums in fp32.  The experts [first_expert, first_expert + held) are held here; slots with another id (-1 among them) are
  * left out, and a row without any is 0: ranks that split the experts add their outputs up.  dtype HY3A_F16 or HY3A_BF16 is that of x
  * [rows][hidden], out and the weights gate, up [held][inter][hidden] and down [held][hidden][inter] (dense); the gated products are
- * rounded to it once between the two.  hidden and inter are multiples of 8, row strides too, held and top_k at most 1024 and 32;
+ * rounded to it once between the two.  hidden and inter are multiples of 8 up to 65536, row strides multiples of 8, held and top_k at most 1024 and 32;
  * pointers 16-byte aligned, the workspace (hy3a_experts_workspace bytes, 0 on bad sizes) 256.  out must not overlap x.
  * The result depends on the inputs alone, not on how slots are ordered within an expert.                                     */
 size_t hy3a_experts_workspace(int rows, int top_k, int hidden, int inter, int held);
@@ -280,7 +280,7 @@ int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int i
 /* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scales[i] * b_i (a_i x[t]) with i = ids[t], sums in
  * fp32.  Rows with an id outside [0, adapters) (-1: no adapter) are base.  x [rows][width], a [adapters][rank][width] and b
  * [adapters][out_width][rank] (dense) are of dtype HY3A_F16 or HY3A_BF16; base and out [rows][out_width] of the same type or fp32 (the
- * rows that hy3a_decode_step takes); out may be base.  width, out_width and rank (at most 256) are multiples of 8: adapters of smaller
+ * rows that hy3a_decode_step takes); out may be base.  width, out_width (at most 2^20) and rank (at most 256) are multiples of 8: adapters of smaller
  * ranks are filled up with zeros.  Pointers 16-byte aligned; rows start on 16-byte boundaries.                               */
 size_t hy3a_adapters_workspace(int rows, int width, int rank);
 int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, int adapters, int rank, const void *x, size_t x_stride, int base_dtype,

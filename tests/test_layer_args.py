@@ -36,7 +36,7 @@ def test_experts(lib):
 
     def call(dtype=2, rows=5, top_k=2, hidden=64, inter=32, held=3, first=0, x=P, xs=64, ids=P, w=P, gate=P, up=P, down=P, out=P, os_=64, work=P, bytes_=need):
         return lib.hy3a_experts(None, dtype, rows, top_k, hidden, inter, held, first, x, xs, ids, w, gate, up, down, out, os_, work, bytes_)
-    for kw, text in (({"dtype": 0}, "dtype"), ({"rows": -1}, "rows"), ({"top_k": 0}, "top_k"), ({"top_k": 33}, "top_k"), ({"hidden": 60}, "multiples"), ({"inter": 12}, "multiples"),
+    for kw, text in (({"dtype": 0}, "dtype"), ({"rows": -1}, "rows"), ({"top_k": 0}, "top_k"), ({"top_k": 33}, "top_k"), ({"hidden": 60}, "multiples"), ({"inter": 12}, "multiples"), ({"hidden": 65544, "xs": 65544}, "over"), ({"inter": 65544}, "over"), ({"rows": 1 << 27}, "many"),
                      ({"held": 0}, "held"), ({"held": 1025}, "held"), ({"first": -1}, "first_expert"), ({"first": 2 ** 31 - 2}, "first_expert"), ({"x": None}, "NULL"), ({"work": None}, "NULL"),
                      ({"x": P + 8}, "16-byte"), ({"gate": P + 2}, "16-byte"), ({"out": P + 4}, "16-byte"), ({"ids": P + 2}, "4-byte"), ({"work": P + 16}, "256-byte"), ({"xs": 68}, "strides"),
                      ({"xs": 56}, "overlap"), ({"os_": 56}, "overlap"), ({"bytes_": need - 1}, "workspace")):
@@ -51,7 +51,7 @@ def test_adapters(lib):
 
     def call(dtype=2, rows=5, width=64, out_width=72, n=3, rank=16, x=P, xs=64, bt=0, base=P, bs=72, a=P, b=P, ids=P, scales=P, out=P, os_=72, work=P, bytes_=need):
         return lib.hy3a_adapters(None, dtype, rows, width, out_width, n, rank, x, xs, bt, base, bs, a, b, ids, scales, out, os_, work, bytes_)
-    for kw, text in (({"dtype": 0}, "dtype"), ({"bt": 1}, "base_dtype"), ({"rows": -1}, "rows"), ({"width": 60}, "width"), ({"out_width": 12}, "out_width"), ({"n": 0}, "adapters"),
+    for kw, text in (({"dtype": 0}, "dtype"), ({"bt": 1}, "base_dtype"), ({"rows": -1}, "rows"), ({"width": 60}, "width"), ({"out_width": 12}, "out_width"), ({"width": (1 << 20) + 8}, "over"), ({"out_width": (1 << 20) + 8}, "over"), ({"n": 0}, "adapters"),
                      ({"rank": 0}, "rank"), ({"rank": 12}, "rank"), ({"rank": 264}, "rank"), ({"x": None}, "NULL"), ({"scales": None}, "NULL"), ({"x": P + 8}, "16-byte"), ({"out": P + 4}, "16-byte"),
                      ({"ids": P + 2}, "4-byte"), ({"xs": 68}, "16-byte boundaries"), ({"bs": 74}, "16-byte boundaries"), ({"os_": 64}, "overlap")):
         refused(lib, call(**kw), text)
