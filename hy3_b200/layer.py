@@ -60,7 +60,7 @@ def adapters(x, base, a, b, ids, scales, out=None):
 
 def layer_sync(device=None):
     """Waits for torch's current stream on `device` (default: the current one), and raises `Hy3AttnError` if a bounded device-side wait of
-    `experts` ran out there since the last call."""
+    `experts` or `adapters` ran out there since the last call."""
     import torch
     with torch.cuda.device(device):
         rc = load_library().hy3a_layer_sync(torch.cuda.current_stream().cuda_stream)

@@ -288,7 +288,8 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
                   size_t out_stride, void *work, size_t work_bytes);
 
 /* cudaStreamSynchronize on the stream + read of the operators' device error words: HY3A_ETIMEOUT if a bounded device-side wait of
- * hy3a_experts ran out on the current device since the last call (it then returned early, and outputs since are not valid).  */
+ * hy3a_experts or hy3a_adapters ran out on the current device since the last call (it then returned early, and outputs since are
+ * not valid).  */
 int hy3a_layer_sync(void *stream);
 
 /* ---- introspection ------------------------------------------------------------------*/
