@@ -14,6 +14,8 @@
  */
 #include <math.h>
 
+#include <algorithm>
+
 #include "experts.h"
 
 namespace {
@@ -255,11 +257,12 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
     }
 }
 
-/* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------ */
+/* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------
+ * (The ids, weights and places come from launches that are complete before `down` lets this one begin.)  A warp for a whole row, 32 columns a
+ * lane in flight, takes 45 us instead of 41 for 8192 rows of 4096. */
 template <class T>
 __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
     pdl_release();
-    pdl_wait();
     const int row = blockIdx.x, d = (blockIdx.y * 256 + threadIdx.x) * 8, lane = threadIdx.x & 31;
     const size_t s0 = (size_t)row * a.top_k;
     const bool mine = lane < a.top_k && local_expert(a, a.ids[s0 + lane]) >= 0;
@@ -267,6 +270,7 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
     const int place = mine ? a.place[s0 + lane] : 0;
     unsigned todo = __ballot_sync(0xffffffffu, mine);
     const bool in = d < a.hidden;
+    pdl_wait();
     float sum[8] = {};
 #pragma unroll 4
     while (todo) {                            /* (in the order of the choices) */

@@ -88,28 +88,44 @@ __device__ __forceinline__ short to_short(float v) { short r; asm("cvt.rni.sat.s
 /* what a tile is: its expert, weight rows from m0 (gate / up: pairs) and n of the listed slots from p0 */
 struct where { int e, m0, p0, n; };
 template <bool DOWN>
-__device__ __forceinline__ where tile_of(const expert_args &a, int t, int m_tiles) {
-    const expert_tile &d = a.tiles[t / m_tiles];
+__device__ __forceinline__ where tile_of(const expert_tile &d, int t, int m_tiles) {
     const int in = t - d.first * m_tiles, m = in / d.tiles, j = in - m * d.tiles;
     const int width = ((d.count + d.tiles - 1) / d.tiles + 15) & ~15;       /* even, in the hardware's steps; at most 256, so no tile is empty */
     where w;
     w.e = d.expert; w.m0 = m * (DOWN ? 256 : 128); w.p0 = d.p0 + j * width; w.n = min(width, d.count - j * width);
     return w;
 }
+/* a warp's walk over the pair's tiles; the next one's line of the table is on its way while a tile is worked on */
+template <bool DOWN>
+struct tile_walk {
+    const expert_args &a;
+    const int step, m_tiles, total;
+    int t;
+    expert_tile next;
+    __device__ __forceinline__ tile_walk(const expert_args &a_, int first, int step_, int m_tiles_, int total_) : a(a_), step(step_), m_tiles(m_tiles_), total(total_), t(first - step_) { fetch(); }
+    __device__ __forceinline__ void fetch() { if (t + step < total) next = a.tiles[(t + step) / m_tiles]; }
+    __device__ __forceinline__ bool take(where &w) {
+        t += step;
+        if (t >= total) return false;
+        w = tile_of<DOWN>(next, t, m_tiles);
+        fetch();
+        return true;
+    }
+};
 
 /* The steps of one tile for one producer warp: its weight box, and MINE of the tile's slot rows (gathers of 4, or boxes of 8), whose number is a
  * constant here so that the row numbers stay where the copy instruction reads them from: looked up in every step, a gather cost 52 clocks. */
 struct ring_state { unsigned st, ph; };
 template <bool DOWN, int MINE>
-__device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, const CUtensorMap *tm_rows, unsigned sbase, unsigned bar0, volatile int *s_abort, int steps, unsigned bytes /* 0: not the one that counts */,
+__device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, const CUtensorMap *tm_rows, unsigned sbase, unsigned bar0, volatile int *s_abort, int steps, int ahead /* steps whose weights are under way */, unsigned bytes /* 0: not the one that counts */,
                                         int part, int m, int e, const int4 (&row)[4], unsigned lead) {
     unsigned st = q.st, ph = q.ph;
     for (int s = 0; s < steps; s++) {
         if (!mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
         const unsigned full = cluster_addr(bar0 + 8u * (B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
-        if (bytes && lead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
+        if (bytes && lead && s >= ahead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
         if (!DOWN) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
-        else if (part == 0) tma_box(sa, tm_w, full, s * 64, m, e, lead);
+        else if (part == 0 && s >= ahead) tma_box(sa, tm_w, full, s * 64, m, e, lead);
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
             if (DOWN) tma_box(sb + (part + kProducers * i) * 1024, tm_rows, full, s * 64, row[i].x, 0, lead);
@@ -154,17 +170,21 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *s_tmem;
+    /* Gate / up lets the next launch begin behind its own wait: that one finds the plan complete, and fetches its first weights before it waits
+     * for h. */
+    if (!DOWN) pdl_wait();
     pdl_release();
-    pdl_wait();
     const int total = *a.n_tiles * m_tiles;
+    if (DOWN && !(warp >= kProducer && warp < kProducer + kProducers)) pdl_wait();
 
     if (warp >= kProducer && warp < kProducer + kProducers) {
         /* ===================== producers: each an eighth of the weight boxes and of the slot rows ===================== */
         const int part = warp - kProducer;
         const unsigned lead = elect_one();
         ring_state q = {0, 0};
-        for (int t = pair; t < total; t += pairs) {
-            const where w = tile_of<DOWN>(a, t, m_tiles);
+        tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
+        int ahead = 0;                  /* steps whose weights are under way */
+        for (where w; walk.take(w);) {
             constexpr int kRows = DOWN ? 8 : 4;                                 /* of one copy */
             const int N = (w.n + 15) & ~15, half = N >> 1, first = w.p0 + (int)rank * half, last = w.p0 + w.n - 1;
             const int mine = (half / kRows - part + kProducers - 1) / kProducers;       /* (half is a multiple of 8) */
@@ -179,16 +199,28 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             const unsigned bytes = part == 0 && rank == 0 ? 2 * kABytes + N * 128 : 0;
             const CUtensorMap *tm = !DOWN && (part & 1) ? &tm_w1 : &tm_w0;
             const int m = DOWN ? w.m0 + (int)rank * 128 : w.m0 + (int)rank * 64 + (part >> 1) * 16;
+            if (DOWN && walk.t == pair) {
+                ahead = min(steps, kStages);
+                if (part == 0)
+                    for (int s = 0; s < ahead; s++) {
+                        const unsigned full = cluster_addr(BAR(B_FULL + s), 0);
+                        if (bytes && lead) mbar_expect_tx(BAR(B_FULL + s), bytes);
+                        tma_box(sbase + s * (kABytes + kBBytes), tm, full, s * 64, m, w.e, lead);
+                    }
+                pdl_wait();
+            }
             bool ok;
             switch (mine) {
-                case 4: ok = produce<DOWN, 4>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
-                case 3: ok = produce<DOWN, 3>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
-                case 2: ok = produce<DOWN, 2>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
-                case 1: ok = produce<DOWN, 1>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead); break;
-                default: ok = produce<DOWN, 0>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, bytes, part, m, w.e, row, lead);
+                case 4: ok = produce<DOWN, 4>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, ahead, bytes, part, m, w.e, row, lead); break;
+                case 3: ok = produce<DOWN, 3>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, ahead, bytes, part, m, w.e, row, lead); break;
+                case 2: ok = produce<DOWN, 2>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, ahead, bytes, part, m, w.e, row, lead); break;
+                case 1: ok = produce<DOWN, 1>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, ahead, bytes, part, m, w.e, row, lead); break;
+                default: ok = produce<DOWN, 0>(q, tm, &tm_rows, sbase, bar0, s_abort, steps, ahead, bytes, part, m, w.e, row, lead);
             }
             if (!ok) break;
+            ahead = 0;
         }
+        if (DOWN && pair >= total) pdl_wait();
         unsigned st = q.st, ph = q.ph;
         /* the last commits reach the barriers of both CTAs before either leaves */
         for (int i = 0; i < kStages && !*s_abort; i++) {
@@ -201,8 +233,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             const unsigned lead = elect_one();
             constexpr unsigned kType = type<T>::code == HY3A_BF16 ? (1u << 7) | (1u << 10) : 0u;
             unsigned st = 0, ph = 0, buf = 0, tph = 0;
-            for (int t = pair; t < total; t += pairs) {
-                const where w = tile_of<DOWN>(a, t, m_tiles);
+            tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
+            for (where w; walk.take(w);) {
                 const unsigned idesc = (1u << 4) | kType | (((unsigned)(w.n + 15) >> 4) << 18) | ((256u >> 4) << 24);
                 if (!mbar_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, g_err, 21u)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -231,8 +263,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         uint8_t *patch = sm + kOffPatch + warp * kPatch;
         const int scales = (a.hidden + 31) >> 5;
         const bool whole = !(a.hidden & 15);
-        for (int t = pair; t < total; t += pairs) {
-            const where w = tile_of<DOWN>(a, t, m_tiles);
+        tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
+        for (where w; walk.take(w);) {
             if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, g_err, 23u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int m0 = DOWN ? w.m0 + (int)rank * 128 + quarter * 32 : w.m0 + (int)rank * 64 + quarter * 16;
