@@ -26,7 +26,7 @@ using namespace hy3a_ring;
 
 constexpr int kMaxRank = 256, kMaxWidth = 1 << 20;
 constexpr int kCut = 1024;           /* k's of a reduce block: 128 of each of its 8 warps */
-constexpr int kReduceWarps = 8, kExpandWarps = 4, kExpandCols = 64 /* columns of a warp at a time */;
+constexpr int kReduceWarps = 8, kExpandCols = 64 /* columns of a warp at a time */;
 
 struct adapter_args {
     const void *x, *base, *a, *b;
@@ -52,12 +52,21 @@ __device__ __forceinline__ int nth_adapter(int id, unsigned todo, int n) {
     }
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 peer_value(unsigned addr, unsigned rank) {
+    unsigned p;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+    return v;
+}
 /* the lanes (rows) of an adapter, none for -1 */
 __device__ __forceinline__ unsigned rows_of(int id, int ad) { return __ballot_sync(0xffffffffu, id >= 0 && id == ad); }
 
-/* ---- 1. reduce: block = (8 G rows, 16 RB ranks, a cut); SPLIT: and one of the tile's adapters -------------------------------- */
-template <class T, int G, int RB, bool SPLIT, bool WIDE>
-__global__ void __launch_bounds__(32 * kReduceWarps, G > 1 ? 2 : 4) hy3a_adapters_reduce_kernel(const adapter_args a) {
+/* ---- long inputs, 1. reduce: block = (8 G rows, 16 RB ranks, a cut) ------------------------------------------------------- */
+template <class T, int G, int RB, bool WIDE>
+__global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_kernel(const adapter_args a) {
     __shared__ float s_sum[kReduceWarps][RB][G][4][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rank_blocks = (a.rank + 16 * RB - 1) / (16 * RB), cut = blockIdx.y / rank_blocks, r0 = (blockIdx.y - cut * rank_blocks) * 16 * RB, t0 = blockIdx.x * 8 * G;
@@ -65,11 +74,6 @@ __global__ void __launch_bounds__(32 * kReduceWarps, G > 1 ? 2 : 4) hy3a_adapter
     pdl_wait();
     const int id = lane < 8 * G ? id_of(a, t0 + lane) : -1;
     unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
-    if (SPLIT) {
-        const int ad = nth_adapter(id, todo, blockIdx.z);
-        if (ad < 0) return;
-        todo = __ballot_sync(0xffffffffu, id == ad);
-    }
     const int k0 = cut * kCut + warp * (kCut / kReduceWarps) + t * 16;
     while (todo) {
         const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
@@ -110,30 +114,28 @@ __global__ void __launch_bounds__(32 * kReduceWarps, G > 1 ? 2 : 4) hy3a_adapter
             for (int v = 0; v < kReduceWarps; v++) sum += s_sum[v][r >> 4][tt >> 3][c][from];
             a.u[((size_t)cut * a.rows + t0 + tt) * a.rank + r0 + r] = sum;
         }
-        if (!SPLIT) __syncthreads();
+        __syncthreads();
     }
 }
 
-/* Puts a tile's u into shared memory: the cuts' sum, the scale, the split into two numbers; neighbouring threads share a row, four ranks each
+/* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers; neighbouring threads share a row, four ranks each
  * at a time.  `any`: the rows that have an adapter (the others get zeros). */
-template <class T, int TOK, int THREADS, int NQ>
-__device__ __forceinline__ void put_u_of(const adapter_args &a, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+template <class T, int TOK, int THREADS, int NQ, class U>
+__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
     constexpr int PT = THREADS / TOK;
     const int i = threadIdx.x / PT, sub = threadIdx.x % PT;
     const bool on = (any >> i) & 1;
     const float scale = on ? a.scales[a.ids[t0 + i]] : 0.f;
-    const float *u = a.u + (size_t)(t0 + i) * a.rank;
     float4 v[NQ];
     float m = 0.f;
 #pragma unroll
     for (int q = 0; q < NQ; q++) v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const size_t step = (size_t)a.rows * a.rank;
 #pragma unroll 2
-    for (int c = 0; c < a.cuts; c++, u += step) {
+    for (int c = 0; c < parts; c++) {
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
             const int r = 4 * (sub + PT * q);
-            const float4 w = on && r < a.rank ? *reinterpret_cast<const float4 *>(u + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 w = on && r < a.rank ? u(c, i, r) : make_float4(0.f, 0.f, 0.f, 0.f);
             v[q].x += w.x; v[q].y += w.y; v[q].z += w.z; v[q].w += w.w;
         }
     }
@@ -164,12 +166,12 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, unsigned any, in
         }
     }
 }
-template <class T, int TOK, int THREADS>
-__device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+template <class T, int TOK, int THREADS, class U>
+__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
     constexpr int MOST = kMaxRank * TOK / 4 / THREADS;             /* four ranks at a time of a thread, at the largest rank */
-    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, any, t0, pitch, s_hi, s_lo, s_back);
-    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, any, t0, pitch, s_hi, s_lo, s_back);
-    else put_u_of<T, TOK, THREADS, MOST>(a, any, t0, pitch, s_hi, s_lo, s_back);
+    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
+    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
+    else put_u_of<T, TOK, THREADS, MOST>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
 }
 
 /* The columns of the output are the M side of the second product; which of a warp's 64 is which row of it is free, and chosen so that a
@@ -177,17 +179,21 @@ __device__ __forceinline__ void put_u(const adapter_args &a, unsigned any, int t
  * instruction of the warp then moves 128 contiguous bytes of each of four rows: fp32 two runs of 4 columns a lane, 16-bit types one of 8. */
 template <class O> __device__ __forceinline__ int column(int g, int col) { return sizeof(O) == 4 ? (col & 4) * 8 + g * 4 + (col & 3) : g * 8 + col; }
 
-/* ---- 2. expand, short inputs: block = (8 rows, 256 columns, one of the tile's adapters) -----------------------------------
- * A warp's part of base is on its way before u is put together. */
-template <class T, class O>
-__global__ void __launch_bounds__(32 * kExpandWarps) hy3a_adapters_expand_kernel(const adapter_args a) {
-    extern __shared__ uint4 s_raw[];
-    constexpr int PER = 16 / sizeof(O), NB = 8 / PER;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int pitch = (a.rank + 31) / 32 * 32 + 8;               /* elements of a row of u: 16 bytes more than a multiple of 64 */
-    T *s_hi = reinterpret_cast<T *>(s_raw), *s_lo = s_hi + 8 * pitch;
+/* ---- short inputs: cluster of 8 blocks = (8 rows, one of the tile's adapters, 8 x `span` columns) ---------------------------
+ * Each block multiplies the rows by an eighth of A's width, the blocks meet in shared memory, and each adds its columns: one launch, u never
+ * leaves the chip, and A is read once for 8 x span columns.  B is asked of L2 and base of memory before the first product begins. */
+constexpr int kShortBlocks = 8, kShortWarps = 8;
+template <class T, class O, bool WIDE>
+__global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kernel(const adapter_args a) {
+    constexpr int PER = 16 / sizeof(O), NB = 8 / PER, RB = 4;            /* blocks of 16 ranks at a time */
+    __shared__ float s_sum[kShortWarps][RB][4][32];
+    __shared__ alignas(16) float s_part[8 * kMaxRank];                   /* [row][rank] of the block's share of the width */
+    __shared__ alignas(16) uint8_t s_u[2 * 8 * (kMaxRank + 8) * sizeof(T)];
     __shared__ float s_back[8];
-    const int t0 = blockIdx.x * 8, n0 = blockIdx.y * a.span + warp * kExpandCols, n_end = a.out_width;
+    const int pitch = (a.rank + 31) / 32 * 32 + 8;                       /* elements of a row of u: 16 bytes more than a multiple of 64 */
+    T *s_hi = reinterpret_cast<T *>(s_u), *s_lo = s_hi + 8 * pitch;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int share = blockIdx.y % kShortBlocks, t0 = blockIdx.x * 8, c_begin = blockIdx.y * a.span, n_end = min(a.out_width, c_begin + a.span);
     pdl_release();
     pdl_wait();
     /* lane i keeps the id of row i of the tile */
@@ -195,48 +201,102 @@ __global__ void __launch_bounds__(32 * kExpandWarps) hy3a_adapters_expand_kernel
     unsigned any = __ballot_sync(0xffffffffu, my >= 0);
     const unsigned none = __ballot_sync(0xffffffffu, lane < 8 && t0 + lane < a.rows && my < 0);
     const int ad = nth_adapter(my, any, blockIdx.z);
-    if (ad < 0 && blockIdx.z > 0) return;
+    if (ad < 0 && blockIdx.z > 0) return;                                /* (so do the cluster's others) */
     any = rows_of(my, ad);
-    const unsigned rows = any | (blockIdx.z == 0 ? none : 0u);       /* rows without an adapter go with the first */
+    const unsigned rows = any | (blockIdx.z == 0 ? none : 0u);           /* rows without an adapter go with the first */
+    const T *const b = reinterpret_cast<const T *>(a.b) + (size_t)(ad < 0 ? 0 : ad) * a.out_width * a.rank;
+    if (any && c_begin < n_end)
+        for (size_t i = (size_t)tid * 64, n = (size_t)(n_end - c_begin) * a.rank; i < n; i += 32 * kShortWarps * 64)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(b + (size_t)c_begin * a.rank + i));
     uint4 held[2][NB];
+    auto fetch_base = [&](int n0) {
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-        for (int q = 0; q < NB; q++) {
-            const int n = n0 + column<O>(g, q * PER);
-            held[c][q] = ((rows >> (2 * t + c)) & 1) && n < n_end ? load_row(reinterpret_cast<const O *>(a.base) + (size_t)(t0 + 2 * t + c) * a.base_stride + n) : zero16();
-        }
-    put_u<T, 8, 32 * kExpandWarps>(a, any, t0, pitch, s_hi, s_lo, s_back);
-    __syncthreads();
-    float acc[4][4] = {};
+            for (int q = 0; q < NB; q++) {
+                const int n = n0 + column<O>(g, q * PER);
+                held[c][q] = ((rows >> (2 * t + c)) & 1) && n < n_end ? load_row(reinterpret_cast<const O *>(a.base) + (size_t)(t0 + 2 * t + c) * a.base_stride + n) : zero16();
+            }
+    };
+    int n0 = c_begin + warp * kExpandCols;
+    fetch_base(n0);
     if (any) {
-        const T *w = reinterpret_cast<const T *>(a.b) + ((size_t)ad * a.out_width + n0) * a.rank;
-        for (int r = t * 8; r < (a.rank + 31) / 32 * 32; r += 32) {
-            uint4 f[8];
+        const int slice = ((a.width + kShortBlocks - 1) / kShortBlocks + 63) / 64 * 64, k_begin = share * slice, k_end = min(a.width, k_begin + slice);
+        const T *x = reinterpret_cast<const T *>(a.x) + (size_t)(t0 + g) * a.x_stride;
+        const bool on = (any >> g) & 1;
+        for (int r0 = 0; r0 < a.rank; r0 += 16 * RB) {
+            const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)ad * a.rank + r0 + g) * a.width;
+            float acc[RB][4] = {};
+            for (int kb = k_begin + warp * 64; kb < k_end; kb += 64 * kShortWarps) {
+                const int k = kb + t * 16, left = k_end - k;
+                k16 lo[RB], hi[RB];
 #pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = r < a.rank && n0 + column<O>(g, j) < n_end ? load_row(w + (size_t)column<O>(g, j) * a.rank + r) : zero16();
-            const uint4 hi = *reinterpret_cast<const uint4 *>(s_hi + g * pitch + r), lo = *reinterpret_cast<const uint4 *>(s_lo + g * pitch + r);
+                for (int i = 0; i < RB; i++) {
+                    lo[i] = load16<WIDE, false>(w + (size_t)16 * i * a.width + k, r0 + 16 * i + g < a.rank ? left : 0);
+                    hi[i] = load16<WIDE, false>(w + (size_t)(16 * i + 8) * a.width + k, r0 + 16 * i + 8 + g < a.rank ? left : 0);
+                }
+                const k16 v = load16<WIDE, false>(x + k, on ? left : 0);
 #pragma unroll
-            for (int j = 0; j < 4; j++) { mma32<T>(acc[j], f[2 * j], f[2 * j + 1], lo); mma32<T>(acc[j], f[2 * j], f[2 * j + 1], hi); }
+                for (int i = 0; i < RB; i++) mma64<T>(acc[i], lo[i], hi[i], v);
+            }
+            if (r0) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < RB; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s_sum[warp][i][c][lane] = acc[i][c];
+            __syncthreads();
+            /* accumulator c of lane (g, t): rank g or g + 8 (c >= 2), row 2t + (c & 1) */
+            for (int i = tid; i < 8 * 16 * RB; i += 32 * kShortWarps) {
+                const int tt = i / (16 * RB), r = i % (16 * RB), c = ((r >> 3) & 1) * 2 + (tt & 1), from = (r & 7) * 4 + (tt >> 1);
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < kShortWarps; v++) sum += s_sum[v][r >> 4][c][from];
+                if (r0 + r < a.rank) s_part[tt * a.rank + r0 + r] = sum;
+            }
         }
     }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const unsigned part = (unsigned)__cvta_generic_to_shared(s_part);
+    put_u<T, 8, 32 * kShortWarps>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, any, t0, pitch, s_hi, s_lo, s_back);
+    __syncwarp();
+    cluster_arrive();                        /* the others' shares have been read */
+    __syncthreads();
+    for (; n0 < n_end; n0 += kShortWarps * kExpandCols) {
+        float acc[4][4] = {};
+        if (any) {
+            const T *w = b + (size_t)n0 * a.rank;
+            for (int r = t * 8; r < (a.rank + 31) / 32 * 32; r += 32) {
+                uint4 f[8];
 #pragma unroll
-    for (int c = 0; c < 2; c++) {
-        const int tt = 2 * t + c;
-        if (!((rows >> tt) & 1)) continue;
-        O *out = reinterpret_cast<O *>(a.out) + (size_t)(t0 + tt) * a.out_stride;
-        const float back = s_back[tt];
-        const bool with = (any >> tt) & 1;
+                for (int j = 0; j < 8; j++) f[j] = r < a.rank && n0 + column<O>(g, j) < n_end ? load_row(w + (size_t)column<O>(g, j) * a.rank + r) : zero16();
+                const uint4 hi = *reinterpret_cast<const uint4 *>(s_hi + g * pitch + r), lo = *reinterpret_cast<const uint4 *>(s_lo + g * pitch + r);
 #pragma unroll
-        for (int q = 0; q < NB; q++) {
-            const int n = n0 + column<O>(g, q * PER);
-            O *o = reinterpret_cast<O *>(&held[c][q]);
-#pragma unroll
-            for (int z = 0; z < PER; z++)
-                if (with) o[z] = type<O>::down(type<O>::up(o[z]) + back * acc[(q * PER + z) >> 1][(z & 1) * 2 + c]);
-            if (n < n_end) *reinterpret_cast<uint4 *>(out + n) = held[c][q];
+                for (int j = 0; j < 4; j++) { mma32<T>(acc[j], f[2 * j], f[2 * j + 1], lo); mma32<T>(acc[j], f[2 * j], f[2 * j + 1], hi); }
+            }
         }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int tt = 2 * t + c;
+            if (!((rows >> tt) & 1)) continue;
+            O *out = reinterpret_cast<O *>(a.out) + (size_t)(t0 + tt) * a.out_stride;
+            const float back = s_back[tt];
+            const bool with = (any >> tt) & 1;
+#pragma unroll
+            for (int q = 0; q < NB; q++) {
+                const int n = n0 + column<O>(g, q * PER);
+                O *o = reinterpret_cast<O *>(&held[c][q]);
+#pragma unroll
+                for (int z = 0; z < PER; z++)
+                    if (with) o[z] = type<O>::down(type<O>::up(o[z]) + back * acc[(q * PER + z) >> 1][(z & 1) * 2 + c]);
+                if (n < n_end) *reinterpret_cast<uint4 *>(out + n) = held[c][q];
+            }
+        }
+        if (n0 + kShortWarps * kExpandCols < n_end) fetch_base(n0 + kShortWarps * kExpandCols);
     }
+    __syncwarp();
+    cluster_wait();
 }
 
 /* ---- 2. expand, long inputs: block = (32 rows, 4 column tiles of 128) --------------------------------------------
@@ -343,7 +403,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
             }
         }
     } else {
-        put_u<T, kLongRows, 128>(a, any, t0, pitch, s_hi, s_lo, s_back);
+        put_u<T, kLongRows, 128>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + t0 + i) * a.rank + r); }, a.cuts, any, t0, pitch, s_hi, s_lo, s_back);
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const T *u_hi = s_hi + g * pitch + t * 8, *u_lo = s_lo + g * pitch + t * 8;
         const int col = warp * 32;
@@ -434,12 +494,11 @@ cudaError_t launch(adapter_args a, int device, void *stream, const char **what) 
     const int pitch = (a.rank + 31) / 32 * 32 + 8, rank_blocks = (a.rank + 15) / 16;
     const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
     if (a.rows <= kShort || a.base_stride < (size_t)a.out_width) {      /* (rows of base that overlap, as of one that is expanded, have no tensor map) */
-        const int tiles = (a.rows + 7) / 8, z = std::min({8, a.rows, a.adapters});
-        {   hy3a_launch l(dim3(tiles, a.cuts * rank_blocks, z), dim3(32 * kReduceWarps), 0, stream);
-            if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 1, 1, true, false>, a)) != cudaSuccess) return e; }
-        a.span = kExpandWarps * kExpandCols;
-        hy3a_launch l(dim3(tiles, (a.out_width + a.span - 1) / a.span, z), dim3(32 * kExpandWarps), (size_t)2 * 8 * pitch * sizeof(T), stream);
-        return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_kernel<T, O>, a);
+        a.span = a.rows <= 8 ? 256 : 512;
+        const int groups = (a.out_width + kShortBlocks * a.span - 1) / (kShortBlocks * a.span);
+        hy3a_launch l(dim3((a.rows + 7) / 8, kShortBlocks * groups, std::min({8, a.rows, a.adapters})), dim3(32 * kShortWarps), 0, stream);
+        l.cluster(1, kShortBlocks);
+        return wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, false>, a);
     }
     constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kMostSmem = kRing + 2 * kLongRows * (kMaxRank + 8) * sizeof(T);
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
@@ -456,7 +515,7 @@ cudaError_t launch(adapter_args a, int device, void *stream, const char **what) 
     }
     const int tiles = (a.rows + kLongRows - 1) / kLongRows;
     {   hy3a_launch l(dim3((a.rows + 15) / 16, a.cuts * ((rank_blocks + 1) / 2)), dim3(32 * kReduceWarps), 0, stream);
-        if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false, false>, a)) != cudaSuccess) return e; }
+        if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
     hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, a);

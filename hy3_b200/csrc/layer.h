@@ -35,9 +35,9 @@ struct hy3a_launch {
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr; cfg.numAttrs = 1;
     }
-    void cluster(int n) {
+    void cluster(int x, int y = 1) {
         attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = n; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        attr[1].val.clusterDim.x = x; attr[1].val.clusterDim.y = y; attr[1].val.clusterDim.z = 1;
         cfg.numAttrs = 2;
     }
 };
