@@ -3,20 +3,21 @@
  *
  *      out[t] = base[t] + scales[a] * B_a (A_a x[t]),   a = ids[t]
  *
- * Two launches:
- *   1. reduce   u[s][t] = A_a x[t] over the s-th 1024 of the width, fp32;
- *   2. expand   sums the cuts in their order, and adds B_a (scales[a] u[t]) to base.  u enters the product as two numbers of the rows'
- *               type, a rounded value and the rest, so that an fp32 result keeps about 17 (bf16) or 22 (fp16) bits of it; each row of u is
- *               brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.
- * Both walk tiles of rows and need no sorting.  Long inputs (prompts: neighbouring rows share an adapter) take tiles of 32 rows and go
- * through the adapters that occur in one; short ones (a row per request) tiles of 8, and each adapter of a tile is a block of its own, so
- * that no block waits for one adapter's weights after another's.
+ * u = A_a x enters the second product as two numbers of the rows' type, a rounded value and the rest, so that an fp32 result keeps about 17 (bf16)
+ * or 22 (fp16) bits of it; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.
+ *
+ * Rows are worked on in tiles of one adapter, so that its weights are read once for all of a tile, whatever the order of the rows:
+ *   up to 8 rows        one launch: a cluster of blocks for each adapter that occurs (short kernel);
+ *   up to kShort rows   the rows are listed by adapter (grouping.cuh) in tiles of 8, and each tile is a cluster's;
+ *   more                listed in tiles of 32; 1. reduce: u[s][t] = A_a x[t] over the s-th 1024 of the width, fp32; 2. expand.
+ * Parts of u are added in their order wherever they meet.
  */
 #include <math.h>
 
 #include <algorithm>
 #include <atomic>
 
+#include "grouping.cuh"
 #include "ring.cuh"
 
 namespace {
@@ -27,6 +28,10 @@ using namespace hy3a_ring;
 constexpr int kMaxRank = 256, kMaxWidth = 1 << 20;
 constexpr int kCut = 1024;           /* k's of a reduce block: 128 of each of its 8 warps */
 constexpr int kReduceWarps = 8, kExpandCols = 64 /* columns of a warp at a time */;
+constexpr int kLongRows = 32, kLongCols = 128, kLongStages = 4, kLongThreads = 192, kLongTiles = 5;
+
+/* `count` listed rows from `first` on, all of one adapter (-1: none) */
+struct adapter_tile { int adapter, first, count, unused; };
 
 struct adapter_args {
     const void *x, *base, *a, *b;
@@ -34,7 +39,10 @@ struct adapter_args {
     const int *ids;
     const float *scales;
     void *out;
-    float *u;            /* [cuts][rows][rank] */
+    float *u;            /* [cuts][rows][rank], in the order of the list */
+    int *list;           /* [rows] rows, adapter by adapter (those without one behind the others) */
+    adapter_tile *tiles; /* [*n_tiles] */
+    int *n_tiles;
     int rows, width, out_width, adapters, rank, cuts, span /* columns of an expand block */;
 };
 
@@ -52,8 +60,6 @@ __device__ __forceinline__ int nth_adapter(int id, unsigned todo, int n) {
     }
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ float4 peer_value(unsigned addr, unsigned rank) {
     unsigned p;
     float4 v;
@@ -64,68 +70,79 @@ __device__ __forceinline__ float4 peer_value(unsigned addr, unsigned rank) {
 /* the lanes (rows) of an adapter, none for -1 */
 __device__ __forceinline__ unsigned rows_of(int id, int ad) { return __ballot_sync(0xffffffffu, id >= 0 && id == ad); }
 
-/* ---- long inputs, 1. reduce: block = (8 G rows, 16 RB ranks, a cut) ------------------------------------------------------- */
+/* ---- plan ---------------------------------------------------------------------------------------------------------------- */
+constexpr int kPlanShared = 512;                          /* rows from which the blocks of a cluster share them: their warps take turns (2048 rows 11.5 us with one block) */
+constexpr int kMaxListed = 2 * kGroupThreads - 1;       /* adapters whose rows can be listed */
+template <int BLOCKS>
+__global__ void __launch_bounds__(kGroupThreads) hy3a_adapters_plan_kernel(const adapter_args a, int tile_rows) {
+    pdl_release();
+    const int tiles = group_items<BLOCKS, 2, true>(
+        a.rows, a.adapters + 1, tile_rows, [&](int i) { const int id = a.ids[i]; return id >= 0 && id < a.adapters ? id : a.adapters; },
+        [&](int ad, int p0, int n, int first, int count) { for (int j = 0; j < count; j++) a.tiles[first + j] = {ad < a.adapters ? ad : -1, p0 + j * tile_rows, min(tile_rows, n - j * tile_rows), 0}; },
+        [&](int i, int p) { a.list[p] = i; });
+    if (threadIdx.x == 0 && (BLOCKS == 1 || cluster_rank() == 0)) *a.n_tiles = tiles;
+}
+
+/* ---- long inputs, 1. reduce: block = (8 G rows of a tile, 16 RB ranks, a cut) ---------------------------------------------- */
 template <class T, int G, int RB, bool WIDE>
 __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_kernel(const adapter_args a) {
     __shared__ float s_sum[kReduceWarps][RB][G][4][32];
+    constexpr int PARTS = kLongRows / (8 * G);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int rank_blocks = (a.rank + 16 * RB - 1) / (16 * RB), cut = blockIdx.y / rank_blocks, r0 = (blockIdx.y - cut * rank_blocks) * 16 * RB, t0 = blockIdx.x * 8 * G;
+    const int rank_blocks = (a.rank + 16 * RB - 1) / (16 * RB), cut = blockIdx.y / rank_blocks, r0 = (blockIdx.y - cut * rank_blocks) * 16 * RB, tile = blockIdx.x / PARTS;
     pdl_release();
     pdl_wait();
-    const int id = lane < 8 * G ? id_of(a, t0 + lane) : -1;
-    unsigned todo = __ballot_sync(0xffffffffu, id >= 0);
+    const adapter_tile d = a.tiles[tile];        /* (the table has a line for each block that is launched; asked for together) */
+    if (tile >= *a.n_tiles) return;
+    const int p0 = d.first + ((int)blockIdx.x - tile * PARTS) * 8 * G, count = d.first + d.count - p0;
+    if (d.adapter < 0 || count <= 0) return;
     const int k0 = cut * kCut + warp * (kCut / kReduceWarps) + t * 16;
-    while (todo) {
-        const int ad = __shfl_sync(0xffffffffu, id, __ffs(todo) - 1);
-        const unsigned mine = __ballot_sync(0xffffffffu, id == ad);
-        todo &= ~mine;
-        const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)ad * a.rank + r0 + g) * a.width;
-        float acc[RB][G][4] = {};
+    const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)d.adapter * a.rank + r0 + g) * a.width, *x[G];
 #pragma unroll
-        for (int i = 0; i < kCut / kReduceWarps / 64; i++) {
-            const int k = k0 + 64 * i;
-            k16 lo[RB], hi[RB];
+    for (int j = 0; j < G; j++) x[j] = reinterpret_cast<const T *>(a.x) + (size_t)a.list[p0 + min(8 * j + g, count - 1)] * a.x_stride;
+    float acc[RB][G][4] = {};
 #pragma unroll
-            for (int b = 0; b < RB; b++) {
-                lo[b] = load16<WIDE, false>(w + (size_t)16 * b * a.width + k, r0 + 16 * b + g < a.rank ? a.width - k : 0);
-                hi[b] = load16<WIDE, false>(w + (size_t)(16 * b + 8) * a.width + k, r0 + 16 * b + 8 + g < a.rank ? a.width - k : 0);
-            }
+    for (int i = 0; i < kCut / kReduceWarps / 64; i++) {
+        const int k = k0 + 64 * i;
+        k16 lo[RB], hi[RB];
 #pragma unroll
-            for (int j = 0; j < G; j++) {
-                const k16 x = load16<WIDE, false>(reinterpret_cast<const T *>(a.x) + (size_t)(t0 + 8 * j + g) * a.x_stride + k, (mine >> (8 * j + g)) & 1 ? a.width - k : 0);
-#pragma unroll
-                for (int b = 0; b < RB; b++) mma64<T>(acc[b][j], lo[b], hi[b], x);
-            }
+        for (int b = 0; b < RB; b++) {
+            lo[b] = load16<WIDE, false>(w + (size_t)16 * b * a.width + k, r0 + 16 * b + g < a.rank ? a.width - k : 0);
+            hi[b] = load16<WIDE, false>(w + (size_t)(16 * b + 8) * a.width + k, r0 + 16 * b + 8 + g < a.rank ? a.width - k : 0);
         }
 #pragma unroll
-        for (int b = 0; b < RB; b++)
+        for (int j = 0; j < G; j++) {
+            const k16 v = load16<WIDE, false>(x[j] + k, a.width - k);
 #pragma unroll
-            for (int j = 0; j < G; j++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) s_sum[warp][b][j][c][lane] = acc[b][j][c];
-        __syncthreads();
-        /* accumulator c of lane (g, t): rank g or g + 8 (c >= 2), row 2t + (c & 1) */
-        for (int i = tid; i < 8 * G * 16 * RB; i += 32 * kReduceWarps) {
-            const int tt = i / (16 * RB), r = i % (16 * RB);
-            if (!((mine >> tt) & 1) || r0 + r >= a.rank) continue;
-            const int c = ((r >> 3) & 1) * 2 + (tt & 1), from = (r & 7) * 4 + ((tt & 7) >> 1);
-            float sum = 0.f;
-#pragma unroll
-            for (int v = 0; v < kReduceWarps; v++) sum += s_sum[v][r >> 4][tt >> 3][c][from];
-            a.u[((size_t)cut * a.rows + t0 + tt) * a.rank + r0 + r] = sum;
+            for (int b = 0; b < RB; b++) mma64<T>(acc[b][j], lo[b], hi[b], v);
         }
-        __syncthreads();
+    }
+#pragma unroll
+    for (int b = 0; b < RB; b++)
+#pragma unroll
+        for (int j = 0; j < G; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s_sum[warp][b][j][c][lane] = acc[b][j][c];
+    __syncthreads();
+    /* accumulator c of lane (g, t): rank g or g + 8 (c >= 2), row 2t + (c & 1) */
+    for (int i = tid; i < 8 * G * 16 * RB; i += 32 * kReduceWarps) {
+        const int tt = i / (16 * RB), r = i % (16 * RB);
+        if (tt >= count || r0 + r >= a.rank) continue;
+        const int c = ((r >> 3) & 1) * 2 + (tt & 1), from = (r & 7) * 4 + ((tt & 7) >> 1);
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < kReduceWarps; v++) sum += s_sum[v][r >> 4][tt >> 3][c][from];
+        a.u[((size_t)cut * a.rows + p0 + tt) * a.rank + r0 + r] = sum;
     }
 }
 
-/* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers; neighbouring threads share a row, four ranks each
- * at a time.  `any`: the rows that have an adapter (the others get zeros). */
+/* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers;
+ * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros). */
 template <class T, int TOK, int THREADS, int NQ, class U>
-__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_hi, T *s_lo, float *s_back) {
     constexpr int PT = THREADS / TOK;
     const int i = threadIdx.x / PT, sub = threadIdx.x % PT;
     const bool on = (any >> i) & 1;
-    const float scale = on ? a.scales[a.ids[t0 + i]] : 0.f;
     float4 v[NQ];
     float m = 0.f;
 #pragma unroll
@@ -167,11 +184,11 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
     }
 }
 template <class T, int TOK, int THREADS, class U>
-__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, unsigned any, int t0, int pitch, T *s_hi, T *s_lo, float *s_back) {
+__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_hi, T *s_lo, float *s_back) {
     constexpr int MOST = kMaxRank * TOK / 4 / THREADS;             /* four ranks at a time of a thread, at the largest rank */
-    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
-    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
-    else put_u_of<T, TOK, THREADS, MOST>(a, u, parts, any, t0, pitch, s_hi, s_lo, s_back);
+    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
+    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
+    else put_u_of<T, TOK, THREADS, MOST>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
 }
 
 /* The columns of the output are the M side of the second product; which of a warp's 64 is which row of it is free, and chosen so that a
@@ -179,11 +196,12 @@ __device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int par
  * instruction of the warp then moves 128 contiguous bytes of each of four rows: fp32 two runs of 4 columns a lane, 16-bit types one of 8. */
 template <class O> __device__ __forceinline__ int column(int g, int col) { return sizeof(O) == 4 ? (col & 4) * 8 + g * 4 + (col & 3) : g * 8 + col; }
 
-/* ---- short inputs: cluster of 8 blocks = (8 rows, one of the tile's adapters, 8 x `span` columns) ---------------------------
+/* ---- short inputs: cluster of 8 blocks = (a tile of 8 rows, 8 x `span` columns) --------------------------------------------------
+ * LISTED: the tile is one of the table's, whose rows are listed; otherwise 8 rows in their order, and one of the adapters among them (blockIdx.z).
  * Each block multiplies the rows by an eighth of A's width, the blocks meet in shared memory, and each adds its columns: one launch, u never
  * leaves the chip, and A is read once for 8 x span columns.  B is asked of L2 and base of memory before the first product begins. */
 constexpr int kShortBlocks = 8, kShortWarps = 8;
-template <class T, class O, bool WIDE>
+template <class T, class O, bool WIDE, bool LISTED>
 __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kernel(const adapter_args a) {
     constexpr int PER = 16 / sizeof(O), NB = 8 / PER, RB = 4;            /* blocks of 16 ranks at a time */
     __shared__ float s_sum[kShortWarps][RB][4][32];
@@ -193,17 +211,29 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     const int pitch = (a.rank + 31) / 32 * 32 + 8;                       /* elements of a row of u: 16 bytes more than a multiple of 64 */
     T *s_hi = reinterpret_cast<T *>(s_u), *s_lo = s_hi + 8 * pitch;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int share = blockIdx.y % kShortBlocks, t0 = blockIdx.x * 8, c_begin = blockIdx.y * a.span, n_end = min(a.out_width, c_begin + a.span);
+    const int share = blockIdx.y % kShortBlocks, c_begin = blockIdx.y * a.span, n_end = min(a.out_width, c_begin + a.span);
     pdl_release();
     pdl_wait();
-    /* lane i keeps the id of row i of the tile */
-    const int my = lane < 8 ? id_of(a, t0 + lane) : -1;
-    unsigned any = __ballot_sync(0xffffffffu, my >= 0);
-    const unsigned none = __ballot_sync(0xffffffffu, lane < 8 && t0 + lane < a.rows && my < 0);
-    const int ad = nth_adapter(my, any, blockIdx.z);
-    if (ad < 0 && blockIdx.z > 0) return;                                /* (so do the cluster's others) */
-    any = rows_of(my, ad);
-    const unsigned rows = any | (blockIdx.z == 0 ? none : 0u);           /* rows without an adapter go with the first */
+    /* lane i (and i + 8, ...) keeps row i of the tile */
+    int row, ad;
+    unsigned rows, any;                                                  /* the block's rows, and those with an adapter */
+    if (LISTED) {
+        const adapter_tile d = a.tiles[blockIdx.x];                      /* (the table has a line for each block that is launched; asked for together) */
+        if ((int)blockIdx.x >= *a.n_tiles) return;                       /* (so do the cluster's others) */
+        row = a.list[d.first + min(lane & 7, d.count - 1)];
+        ad = d.adapter;
+        rows = (1u << d.count) - 1u;
+        any = ad < 0 ? 0u : rows;
+    } else {
+        row = min((int)blockIdx.x * 8 + (lane & 7), a.rows - 1);
+        const int my = lane < 8 ? id_of(a, blockIdx.x * 8 + lane) : -1;
+        const unsigned with = __ballot_sync(0xffffffffu, my >= 0), none = __ballot_sync(0xffffffffu, lane < 8 && (int)blockIdx.x * 8 + lane < a.rows && my < 0);
+        ad = nth_adapter(my, with, blockIdx.z);
+        if (ad < 0 && blockIdx.z > 0) return;
+        any = rows_of(my, ad);
+        rows = any | (blockIdx.z == 0 ? none : 0u);                      /* rows without an adapter go with the first */
+    }
+    const int row_g = __shfl_sync(0xffffffffu, row, g), row_t[2] = {__shfl_sync(0xffffffffu, row, 2 * t), __shfl_sync(0xffffffffu, row, 2 * t + 1)};
     const T *const b = reinterpret_cast<const T *>(a.b) + (size_t)(ad < 0 ? 0 : ad) * a.out_width * a.rank;
     if (any && c_begin < n_end)
         for (size_t i = (size_t)tid * 64, n = (size_t)(n_end - c_begin) * a.rank; i < n; i += 32 * kShortWarps * 64)
@@ -215,14 +245,14 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
 #pragma unroll
             for (int q = 0; q < NB; q++) {
                 const int n = n0 + column<O>(g, q * PER);
-                held[c][q] = ((rows >> (2 * t + c)) & 1) && n < n_end ? load_row(reinterpret_cast<const O *>(a.base) + (size_t)(t0 + 2 * t + c) * a.base_stride + n) : zero16();
+                held[c][q] = ((rows >> (2 * t + c)) & 1) && n < n_end ? load_row(reinterpret_cast<const O *>(a.base) + (size_t)row_t[c] * a.base_stride + n) : zero16();
             }
     };
     int n0 = c_begin + warp * kExpandCols;
     fetch_base(n0);
     if (any) {
         const int slice = ((a.width + kShortBlocks - 1) / kShortBlocks + 63) / 64 * 64, k_begin = share * slice, k_end = min(a.width, k_begin + slice);
-        const T *x = reinterpret_cast<const T *>(a.x) + (size_t)(t0 + g) * a.x_stride;
+        const T *x = reinterpret_cast<const T *>(a.x) + (size_t)row_g * a.x_stride;
         const bool on = (any >> g) & 1;
         for (int r0 = 0; r0 < a.rank; r0 += 16 * RB) {
             const T *w = reinterpret_cast<const T *>(a.a) + ((size_t)ad * a.rank + r0 + g) * a.width;
@@ -259,7 +289,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     cluster_arrive();
     cluster_wait();
     const unsigned part = (unsigned)__cvta_generic_to_shared(s_part);
-    put_u<T, 8, 32 * kShortWarps>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, any, t0, pitch, s_hi, s_lo, s_back);
+    put_u<T, 8, 32 * kShortWarps>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, ad < 0 ? 0.f : a.scales[ad], any, pitch, s_hi, s_lo, s_back);
     __syncwarp();
     cluster_arrive();                        /* the others' shares have been read */
     __syncthreads();
@@ -280,7 +310,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
         for (int c = 0; c < 2; c++) {
             const int tt = 2 * t + c;
             if (!((rows >> tt) & 1)) continue;
-            O *out = reinterpret_cast<O *>(a.out) + (size_t)(t0 + tt) * a.out_stride;
+            O *out = reinterpret_cast<O *>(a.out) + (size_t)row_t[c] * a.out_stride;
             const float back = s_back[tt];
             const bool with = (any >> tt) & 1;
 #pragma unroll
@@ -299,73 +329,86 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     cluster_wait();
 }
 
-/* ---- 2. expand, long inputs: block = (32 rows, 4 column tiles of 128) --------------------------------------------
- * Units (column tile, adapter of the row tile, 32 ranks) go through a ring of 4 stages that TMA fills: 128 rows of B of 32 ranks, and with
- * the last unit of a column tile the tile of base, which becomes the tile of the output where it lies and leaves by TMA.  Bounds are the tensor
- * maps'.  Warps 0-3 multiply (32 rows x 32 columns each), warp 4 fetches, warp 5 stores.  Base and output are what this kernel has to move (168 MB for 2048
- * rows of 10240 in fp32); written with loads and stores of the multiplying warps, their addresses took more issue slots than the products. */
-constexpr int kLongRows = 32, kLongCols = 128, kLongStages = 4, kLongThreads = 192, kLongTiles = 4;
+/* ---- 2. expand, long inputs: block = (a tile of 32 rows, 4 column tiles of 128) -------------------------------------------
+ * Units (column tile, 32 ranks) go through a ring of 4 stages that TMA fills: 128 rows of B of 32 ranks, and with the last unit of a column tile the
+ * tile of base, as one box where the rows are neighbours (a prompt's), four rows at a time by their numbers otherwise (tile::gather4, tile::scatter4:
+ * 54 us of 2048 rows on 4096 -> 10240 become 76); it becomes the tile of the output where it lies and leaves the same way.  Bounds are the tensor maps'.  Warps 0-3 multiply (32 rows x 32 columns each), warp 4 fetches, warp 5 stores.  Base and output are
+ * what this kernel has to move (168 MB for 2048 rows of 10240 in fp32); written with loads and stores of the multiplying warps, their addresses took
+ * more issue slots than the products. */
 template <class O> struct long_stage {
     static constexpr int box = 128 / sizeof(O) /* columns of a box: 128 bytes */, base_bytes = kLongRows * kLongCols * sizeof(O), b_bytes = kLongCols * 64, bytes = b_bytes + base_bytes;
 };
 enum { A_FULL = 0, A_DONE = kLongStages, A_EMPTY = 2 * kLongStages };
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
-__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap *map, unsigned bar, int x, const int4 &row) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w) : "memory");
 }
 __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void tma_store(const CUtensorMap *map, unsigned src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_scatter4(const CUtensorMap *map, unsigned src, int x, const int4 &row) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile::scatter4.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
+                 ::"l"(map), "r"(src), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w) : "memory");
 }
 
 template <class T, class O>
 __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_base,
-                                                                                const __grid_constant__ CUtensorMap tm_out, const adapter_args a) {
+                                                                                const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_base32, const __grid_constant__ CUtensorMap tm_out32,
+                                                                                const adapter_args a) {
     extern __shared__ uint8_t s_bytes[];
     using stage = long_stage<O>;
     uint8_t *ring = s_bytes + ((1024u - (smem_u32(s_bytes) & 1023u)) & 1023u);
     const int chunks = (a.rank + 31) >> 5, pitch = chunks * 32 + 8;      /* elements of a row of u: 16 bytes more than a multiple of 64 */
     T *s_hi = reinterpret_cast<T *>(ring + kLongStages * stage::bytes), *s_lo = s_hi + kLongRows * pitch;
     __shared__ float s_back[kLongRows];
+    __shared__ alignas(16) int s_rows[kLongRows];
     __shared__ alignas(8) unsigned long long s_bar[3 * kLongStages];
     __shared__ int s_abort_flag;
     volatile int *s_abort = &s_abort_flag;
     const unsigned bar0 = smem_u32(s_bar);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
-    const int t0 = blockIdx.x * kLongRows, first = blockIdx.y * kLongTiles, count = min(kLongTiles, across - first);      /* column tiles */
+    const int c_first = blockIdx.y * kLongTiles, columns = min(kLongTiles, across - c_first);      /* column tiles */
     if (tid == 0) {
         s_abort_flag = 0;
         for (int i = 0; i < kLongStages; i++) { mbar_init(bar0 + 8 * (A_FULL + i), 1); mbar_init(bar0 + 8 * (A_DONE + i), 4); mbar_init(bar0 + 8 * (A_EMPTY + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
     pdl_release();
     pdl_wait();
-    const int my = id_of(a, t0 + lane);                                  /* lane i: the id of row i of the tile */
-    const unsigned any = __ballot_sync(0xffffffffu, my >= 0);
-    int n_ad = 0;                                                        /* adapters of the tile */
-    for (unsigned todo = any; todo; n_ad++) todo &= ~rows_of(my, __shfl_sync(0xffffffffu, my, __ffs(todo) - 1));
-    const int per = max(1, n_ad * chunks);                               /* units of a column tile */
+    const adapter_tile d = a.tiles[blockIdx.x];
+    if ((int)blockIdx.x >= *a.n_tiles) return;
+    const int ad = d.adapter, last_row = d.count - 1;
+    if (warp == 0) s_rows[lane] = a.list[d.first + min(lane, last_row)];     /* places past the last row stand for it: what is stored there twice is the same */
+    __syncthreads();
+    const int per = ad < 0 ? 1 : chunks;                                 /* units of a column tile */
+    const bool run = last_row == kLongRows - 1 && s_rows[last_row] - s_rows[0] == last_row;      /* the listed rows ascend: 32 neighbours are one box */
     unsigned st = 0, ph = 0;
     if (warp == 5) {
         /* gives the stages back, those with output when it has been read */
-        int pending = -1;
-        bool ok = true;
-        for (int tile = 0; tile < count && ok; tile++) {
-            const int c0 = (first + tile) * kLongCols;
-            if (lane == 0) {
+        if (lane == 0) {
+            int pending = -1;
+            bool ok = true;
+            for (int tile = 0; tile < columns && ok; tile++) {
+                const int c0 = (c_first + tile) * kLongCols;
                 for (int in = 0; in < per; in++) {
                     if (!(ok = mbar_wait(bar0 + 8 * (A_DONE + st), ph, s_abort, g_err, 32u))) break;
                     const bool last = in == per - 1;
                     if (last) {
-                        for (int i = 0; i < kLongCols / stage::box; i++) {
-                            const int c = c0 + i * stage::box;
-                            if (c < a.out_width) tma_store(&tm_out, smem_u32(ring) + st * stage::bytes + stage::b_bytes + i * kLongRows * 128, c, t0);
-                        }
+                        const unsigned src = smem_u32(ring) + st * stage::bytes + stage::b_bytes;
+                        for (int i = 0; i < kLongCols / stage::box; i++)
+                            if (c0 + i * stage::box >= a.out_width) break;
+                            else if (run) tma_store(&tm_out32, src + i * kLongRows * 128, c0 + i * stage::box, s_rows[0]);
+                            else
+                                for (int q = 0; q <= last_row >> 2; q++) tma_scatter4(&tm_out, src + i * kLongRows * 128 + q * 512, c0 + i * stage::box, *reinterpret_cast<const int4 *>(s_rows + 4 * q));
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                     if (pending >= 0) {                 /* the output before this unit's */
@@ -378,45 +421,39 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
                     if (++st == kLongStages) { st = 0; ph ^= 1u; }
                 }
             }
-            __syncwarp();
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (warp == 4) {
-        const unsigned lead = elect_one();
-        bool ok = true;
-        for (int tile = 0; tile < count && ok; tile++) {
-            const int c0 = (first + tile) * kLongCols;
-            int k = 0, r0 = 0, ad = nth_adapter(my, any, 0);
-            for (int in = 0; in < per; in++) {
-                if (!(ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 30u))) break;
-                const unsigned full = bar0 + 8 * (A_FULL + st), dst = smem_u32(ring) + st * stage::bytes;
-                const bool last = in == per - 1;
-                if (lead) {
-                    mbar_expect_tx(full, (n_ad ? stage::b_bytes : 0) + (last ? stage::base_bytes : 0));
-                    if (n_ad) tma_load(dst, &tm_b, full, r0, c0, ad);
+        if (lane == 0) {
+            bool ok = true;
+            for (int tile = 0; tile < columns && ok; tile++) {
+                const int c0 = (c_first + tile) * kLongCols, boxes = min(kLongCols / stage::box, (a.out_width - c0 + stage::box - 1) / stage::box), fours = (last_row >> 2) + 1;
+                for (int in = 0; in < per; in++) {
+                    if (!(ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 30u))) break;
+                    const unsigned full = bar0 + 8 * (A_FULL + st), dst = smem_u32(ring) + st * stage::bytes;
+                    const bool last = in == per - 1;
+                    mbar_expect_tx(full, (ad < 0 ? 0 : stage::b_bytes) + (last ? boxes * fours * 512 : 0));
+                    if (ad >= 0) tma_load(dst, &tm_b, full, in * 32, c0, ad);
                     if (last)
-                        for (int i = 0; i < kLongCols / stage::box; i++) tma_load(dst + stage::b_bytes + i * kLongRows * 128, &tm_base, full, c0 + i * stage::box, t0);
+                        for (int i = 0; i < boxes; i++)
+                            if (run) tma_load(dst + stage::b_bytes + i * kLongRows * 128, &tm_base32, full, c0 + i * stage::box, s_rows[0]);
+                            else for (int q = 0; q < fours; q++) tma_gather4(dst + stage::b_bytes + i * kLongRows * 128 + q * 512, &tm_base, full, c0 + i * stage::box, *reinterpret_cast<const int4 *>(s_rows + 4 * q));
+                    if (++st == kLongStages) { st = 0; ph ^= 1u; }
                 }
-                __syncwarp();
-                if ((r0 += 32) >= a.rank) { r0 = 0; ad = nth_adapter(my, any, ++k); }
-                if (++st == kLongStages) { st = 0; ph ^= 1u; }
             }
         }
     } else {
-        put_u<T, kLongRows, 128>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + t0 + i) * a.rank + r); }, a.cuts, any, t0, pitch, s_hi, s_lo, s_back);
+        if (ad >= 0) put_u<T, kLongRows, 128>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_hi, s_lo, s_back);
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const T *u_hi = s_hi + g * pitch + t * 8, *u_lo = s_lo + g * pitch + t * 8;
-        const int col = warp * 32;
+        const int col = warp * 32, groups = (d.count + 7) >> 3;
         bool ok = true;
-        for (int tile = 0; tile < count && ok; tile++) {
+        for (int tile = 0; tile < columns && ok; tile++) {
             float acc[2][4][4] = {};
-            int k = 0, r = 0;
-            unsigned mine = any;                                         /* rows of the unit's adapter */
-            if (n_ad > 1) mine = rows_of(my, nth_adapter(my, any, 0));
             for (int in = 0; in < per; in++) {
                 if (!(ok = mbar_wait(bar0 + 8 * (A_FULL + st), ph, s_abort, g_err, 31u))) break;
                 uint8_t *const at = ring + st * stage::bytes;
-                if (n_ad) {
+                if (ad >= 0) {
                     /* product m of the warp's two: its row g is column 4g + 2m, row g + 8 the one behind it */
                     uint4 f[4];
 #pragma unroll
@@ -426,55 +463,36 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        if (!((mine >> (8 * i)) & 0xff)) continue;
-                        const uint4 hi = *reinterpret_cast<const uint4 *>(u_hi + 8 * i * pitch + r), lo = *reinterpret_cast<const uint4 *>(u_lo + 8 * i * pitch + r);
-                        if (n_ad == 1) {
+                        if (i >= groups) continue;
+                        const uint4 hi = *reinterpret_cast<const uint4 *>(u_hi + 8 * i * pitch + in * 32), lo = *reinterpret_cast<const uint4 *>(u_lo + 8 * i * pitch + in * 32);
 #pragma unroll
-                            for (int m = 0; m < 2; m++) { mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], lo); mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], hi); }
-                        } else {
-                            /* an adapter that is not finite must not reach the others' rows: only its own columns are taken */
-                            const bool c0 = (mine >> (8 * i + 2 * t)) & 1, c1 = (mine >> (8 * i + 2 * t + 1)) & 1;
-#pragma unroll
-                            for (int m = 0; m < 2; m++) {
-                                float d[4] = {acc[m][i][0], acc[m][i][1], acc[m][i][2], acc[m][i][3]};
-                                mma32<T>(d, f[2 * m], f[2 * m + 1], lo);
-                                mma32<T>(d, f[2 * m], f[2 * m + 1], hi);
-                                if (c0) { acc[m][i][0] = d[0]; acc[m][i][2] = d[2]; }
-                                if (c1) { acc[m][i][1] = d[1]; acc[m][i][3] = d[3]; }
-                            }
-                        }
-                    }
-                    if ((r += 32) >= a.rank) {
-                        r = 0;
-                        if (n_ad > 1) mine = rows_of(my, nth_adapter(my, any, ++k));
+                        for (int m = 0; m < 2; m++) { mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], lo); mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], hi); }
                     }
                 }
                 if (in == per - 1) {
-                    struct alignas(4 * sizeof(O)) four { O v[4]; };
-                    four o[4][2];
-                    /* columns 4g .. 4g + 3 of row 8i + 2t + c */
-                    auto place = [&](int i, int c) {
-                        const int row = 8 * i + 2 * t + c, b = (col + 4 * g) * (int)sizeof(O);           /* byte of the tile's row */
-                        return reinterpret_cast<four *>(at + stage::b_bytes + (b >> 7) * kLongRows * 128 + row * 128 + ((((b >> 4) & 7) ^ (row & 7)) << 4) + (b & 15));
-                    };
+                    if (ad >= 0) {
+                        struct alignas(4 * sizeof(O)) four { O v[4]; };
+                        four o[4][2];
+                        /* columns 4g .. 4g + 3 of row 8i + 2t + c */
+                        auto place = [&](int i, int c) {
+                            const int row = 8 * i + 2 * t + c, b = (col + 4 * g) * (int)sizeof(O);           /* byte of the tile's row */
+                            return reinterpret_cast<four *>(at + stage::b_bytes + (b >> 7) * kLongRows * 128 + row * 128 + ((((b >> 4) & 7) ^ (row & 7)) << 4) + (b & 15));
+                        };
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                        for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) o[i][c] = *place(i, c);
+                            for (int c = 0; c < 2; c++) if (i < groups) o[i][c] = *place(i, c);
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                        for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const int row = 8 * i + 2 * t + c;
-                            const float back = s_back[row];
-                            const bool with = (any >> row) & 1;
+                            for (int c = 0; c < 2; c++) {
+                                if (i >= groups) continue;
+                                const float back = s_back[8 * i + 2 * t + c];
 #pragma unroll
-                            for (int z = 0; z < 4; z++) {
-                                const O v = type<O>::down(type<O>::up(o[i][c].v[z]) + back * acc[z >> 1][i][(z & 1) * 2 + c]);
-                                if (with) o[i][c].v[z] = v;
+                                for (int z = 0; z < 4; z++) o[i][c].v[z] = type<O>::down(type<O>::up(o[i][c].v[z]) + back * acc[z >> 1][i][(z & 1) * 2 + c]);
+                                *place(i, c) = o[i][c];
                             }
-                            *place(i, c) = o[i][c];
-                        }
+                    }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
@@ -486,39 +504,50 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the unit that was given up are still on their way */
 }
 
-constexpr int kShort = 256;           /* rows up to which a tile's adapters are blocks of their own */
+/* Rows up to which tiles of 8 are taken (us a pass, tiles of 8 / of 32): 64, 128 and 256 rows of as many requests on 8192 -> 4096 20.1 / 21.5, 28.6 / 30.0,
+ * 30.4 / 32.0; of a few prompts on 4096 -> 10240 11.9 / 18.5, 17.2 / 19.9, 26.7 / 23.8. */
+constexpr int kShort = 128;
+int most_tiles(const adapter_args &a, int tile_rows) { return a.rows / tile_rows + std::min(a.rows, a.adapters + 1); }
 
+template <class T, class O, bool LISTED>
+cudaError_t launch_short(adapter_args a, bool wide, void *stream) {
+    a.span = a.rows <= 8 ? 256 : 512;
+    const int groups = (a.out_width + kShortBlocks * a.span - 1) / (kShortBlocks * a.span);
+    hy3a_launch l(LISTED ? dim3(most_tiles(a, 8), kShortBlocks * groups) : dim3((a.rows + 7) / 8, kShortBlocks * groups, std::min({8, a.rows, a.adapters})), dim3(32 * kShortWarps), 0, stream);
+    l.cluster(1, kShortBlocks);
+    return wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, true, LISTED>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, false, LISTED>, a);
+}
 template <class T, class O>
-cudaError_t launch(adapter_args a, int device, void *stream, const char **what) {
+cudaError_t launch(const adapter_args &a, int device, void *stream, const char **what) {
     cudaError_t e;
-    const int pitch = (a.rank + 31) / 32 * 32 + 8, rank_blocks = (a.rank + 15) / 16;
     const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
-    if (a.rows <= kShort || a.base_stride < (size_t)a.out_width) {      /* (rows of base that overlap, as of one that is expanded, have no tensor map) */
-        a.span = a.rows <= 8 ? 256 : 512;
-        const int groups = (a.out_width + kShortBlocks * a.span - 1) / (kShortBlocks * a.span);
-        hy3a_launch l(dim3((a.rows + 7) / 8, kShortBlocks * groups, std::min({8, a.rows, a.adapters})), dim3(32 * kShortWarps), 0, stream);
-        l.cluster(1, kShortBlocks);
-        return wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, false>, a);
-    }
+    if (a.rows <= 8 || a.adapters > kMaxListed) return launch_short<T, O, false>(a, wide, stream);
+    const bool shared = a.rows >= kPlanShared, shorts = a.rows <= kShort || a.base_stride < (size_t)a.out_width;      /* (rows of base that overlap have no tensor map) */
+    const int tile_rows = shorts ? 8 : kLongRows;
+    {   hy3a_launch l(dim3(shared ? kGroupCluster : 1), dim3(kGroupThreads), 0, stream);
+        if (shared) l.cluster(kGroupCluster);
+        if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<kGroupCluster>, a, tile_rows) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<1>, a, tile_rows)) != cudaSuccess) return e; }
+    if (shorts) return launch_short<T, O, true>(a, wide, stream);
     constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kMostSmem = kRing + 2 * kLongRows * (kMaxRank + 8) * sizeof(T);
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
         if ((e = cudaFuncSetAttribute(hy3a_adapters_expand_long_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
-    CUtensorMap tm_b, tm_base, tm_out;
+    CUtensorMap tm_b, tm_base, tm_out, tm_base32, tm_out32;
     constexpr int box = long_stage<O>::box;
-    if (!encode(&tm_b, 3, a.b, 2, a.rank, a.out_width, a.adapters, a.rank, 32, kLongCols) || !encode(&tm_base, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, kLongRows) ||
-        !encode(&tm_out, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, kLongRows)) {
+    if (!encode(&tm_b, 3, a.b, 2, a.rank, a.out_width, a.adapters, a.rank, 32, kLongCols) || !encode(&tm_base, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, 1) ||
+        !encode(&tm_out, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, 1) || !encode(&tm_base32, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, kLongRows) ||
+        !encode(&tm_out32, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, kLongRows)) {
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    const int tiles = (a.rows + kLongRows - 1) / kLongRows;
-    {   hy3a_launch l(dim3((a.rows + 15) / 16, a.cuts * ((rank_blocks + 1) / 2)), dim3(32 * kReduceWarps), 0, stream);
+    const int tiles = most_tiles(a, kLongRows), rank_blocks = (a.rank + 31) / 32, pitch = rank_blocks * 32 + 8;
+    {   hy3a_launch l(dim3(2 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
         if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
     hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, a);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, tm_base32, tm_out32, a);
 }
 
 int check_sizes(const char *who, int rows, int width, int rank) {
@@ -529,6 +558,17 @@ int check_sizes(const char *who, int rows, int width, int rank) {
     return 0;
 }
 int cuts_of(int width) { return (width + kCut - 1) / kCut; }
+/* workspace: offsets of its parts, in bytes (a tile has a row at least) */
+struct workspace { size_t list, tiles, u, total; };
+workspace layout(int rows, int width, int rank) {
+    auto up256 = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    workspace w;
+    w.list = 256;                             /* the number of tiles lies before it */
+    w.tiles = w.list + up256((size_t)rows * sizeof(int));
+    w.u = w.tiles + up256((size_t)(rows + 1) * sizeof(adapter_tile));
+    w.total = w.u + up256((size_t)cuts_of(width) * rows * rank * sizeof(float));
+    return w;
+}
 
 } /* namespace */
 
@@ -543,7 +583,7 @@ extern "C" {
 
 size_t hy3a_adapters_workspace(int rows, int width, int rank) {
     if (check_sizes("adapters_workspace", rows, width, rank)) return 0;
-    return (size_t)cuts_of(width) * rows * rank * sizeof(float);
+    return layout(rows, width, rank).total;
 }
 
 int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, int adapters, int rank, const void *x, size_t x_stride, int base_dtype,
@@ -564,9 +604,11 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
     if (out_stride < (size_t)out_width && rows > 1) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: out rows of %d overlap at a stride of %zu", out_width, out_stride);
     int dev, sms;
     if ((rc = hy3a_layer_device("adapters", &dev, &sms))) return rc;
-    const size_t need = hy3a_adapters_workspace(rows, width, rank);
-    if (work_bytes < need) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: the workspace has %zu bytes, %zu are needed (hy3a_adapters_workspace)", work_bytes, need);
-    const adapter_args a = {x, base, a_, b_, x_stride, base_stride, out_stride, ids, scales, out, (float *)work, rows, width, out_width, adapters, rank, cuts_of(width), 0};
+    const workspace w = layout(rows, width, rank);
+    if (work_bytes < w.total) return hy3a_fail(NULL, HY3A_EINVAL, "adapters: the workspace has %zu bytes, %zu are needed (hy3a_adapters_workspace)", work_bytes, w.total);
+    char *m = (char *)work;
+    const adapter_args a = {x, base, a_, b_, x_stride, base_stride, out_stride, ids, scales, out, (float *)(m + w.u), (int *)(m + w.list), (adapter_tile *)(m + w.tiles), (int *)m,
+                            rows, width, out_width, adapters, rank, cuts_of(width), 0};
     cudaError_t e;
     const char *what = NULL;
     if (dtype == HY3A_F16) e = base_dtype == HY3A_F32 ? launch<__half, float>(a, dev, stream, &what) : launch<__half, __half>(a, dev, stream, &what);

@@ -17,11 +17,13 @@
 #include <algorithm>
 
 #include "experts.h"
+#include "grouping.cuh"
 
 namespace {
 
 using namespace hy3a_layer;
 
+constexpr int kMaxHeld = kGroupThreads;
 constexpr int kFewMost = 32;           /* slots of a call below which its products run here */
 
 /* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
@@ -46,94 +48,15 @@ __device__ __forceinline__ int local_expert(const expert_args &a, int id) {
     return id >= 0 && e >= 0 && e < a.held ? e : -1;
 }
 
-/* ---- 1. plan: one block, or a cluster of 8 that share the slots ---------------------------------------------------------
- * Each block counts its part of the slots, all read all counts, and each lists its part.  65 536 slots: 37 us with one block, TWO with 8. */
-constexpr int kPlanThreads = 1024, kMaxHeld = 1024, kPlanCluster = 8, kPlanShared = 4096;      /* slots from which blocks share them */
-__device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ int peer_value(const int *p, unsigned rank) {
-    unsigned a = (unsigned)__cvta_generic_to_shared(p);
-    int v;
-    asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(a) : "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
+/* ---- 1. plan ------------------------------------------------------------------------------------------------------------ */
 template <int BLOCKS>
-__global__ void __launch_bounds__(kPlanThreads) hy3a_experts_plan_kernel(const expert_args a) {
-    __shared__ int s_count[kMaxHeld], s_next[kMaxHeld], s_warp[2][32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned me = BLOCKS > 1 ? cluster_rank() : 0;
-    const int per = (a.slots + BLOCKS - 1) / BLOCKS, begin = min(a.slots, (int)me * per), end = min(a.slots, begin + per);
+__global__ void __launch_bounds__(kGroupThreads) hy3a_experts_plan_kernel(const expert_args a) {
     pdl_release();
-    for (int e = tid; e < a.held; e += kPlanThreads) s_count[e] = 0;
-    __syncthreads();
-    pdl_wait();
-#pragma unroll 4
-    for (int i = begin + tid; i < end; i += kPlanThreads) {
-        const int e = local_expert(a, a.ids[i]);
-        if (e >= 0) atomicAdd(&s_count[e], 1);
-    }
-    if (BLOCKS > 1) cluster_sync(); else __syncthreads();
-    /* a thread per expert: its slots, those of the blocks before this one, its tiles; exclusive sums over the experts */
-    int n = 0, earlier = 0;
-    if (tid < a.held) {
-        if (BLOCKS == 1) n = s_count[tid];
-        else {
-#pragma unroll
-            for (int r = 0; r < BLOCKS; r++) {
-                const int c = peer_value(&s_count[tid], r);
-                n += c;
-                if (r < (int)me) earlier += c;
-            }
-        }
-    }
-    const int tiles = (n + kTileSlots - 1) / kTileSlots;
-    int sum[2] = {n, tiles};
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int u = __shfl_up_sync(0xffffffffu, sum[i], o);
-            if (lane >= o) sum[i] += u;
-        }
-#pragma unroll
-    for (int i = 0; i < 2; i++) if (lane == 31) s_warp[i][warp] = sum[i];
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        int w = s_warp[i][lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += u;
-        }
-        if (i == 1) total = __shfl_sync(0xffffffffu, w, 31);
-        const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-        sum[i] += warp ? before : 0;
-    }
-    const int p0 = sum[0] - n, first = sum[1] - tiles;
-    if (tid < a.held) {
-        s_next[tid] = p0 + earlier;           /* where the block's next slot of the expert goes */
-        if (me == 0) {
-            for (int j = 0; j < tiles; j++) a.tiles[first + j] = {tid, first, tiles, p0, n};
-        }
-    }
-    if (tid == 0 && me == 0) *a.n_tiles = total;
-    __syncthreads();
-#pragma unroll 4
-    for (int i = begin + tid; i < end; i += kPlanThreads) {
-        const int e = local_expert(a, a.ids[i]);
-        if (e >= 0) {
-            const int p = atomicAdd(&s_next[e], 1);
-            a.row[p] = i / a.top_k;
-            a.place[i] = p;
-        }
-    }
-    if (BLOCKS > 1) cluster_sync();           /* nobody leaves while its counts are read */
+    const int tiles = group_items<BLOCKS, 1, false>(
+        a.slots, a.held, kTileSlots, [&](int i) { return local_expert(a, a.ids[i]); },
+        [&](int e, int p0, int n, int first, int count) { for (int j = 0; j < count; j++) a.tiles[first + j] = {e, first, count, p0, n}; },
+        [&](int i, int p) { a.row[p] = i / a.top_k; a.place[i] = p; });
+    if (threadIdx.x == 0 && (BLOCKS == 1 || cluster_rank() == 0)) *a.n_tiles = tiles;
 }
 
 /* ---- calls with few slots (at most 31; the others: experts_umma.cu) -----------------------------------------------------
@@ -313,10 +236,10 @@ cudaError_t launch(const expert_args &a, int device, int sms, void *stream, cons
      * 1032 x 200 for 1, 10 rows 7 / 17, 9.4 / 17.8 */
     if (a.slots < kFewMost) return launch_few<T>(a, stream);
     cudaError_t e;
-    const bool shared = a.slots >= kPlanShared;
-    {   hy3a_launch l(dim3(shared ? kPlanCluster : 1), dim3(kPlanThreads), 0, stream);
-        if (shared) l.cluster(kPlanCluster);
-        if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<kPlanCluster>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<1>, a)) != cudaSuccess) return e; }
+    const bool shared = a.slots >= kGroupShared;
+    {   hy3a_launch l(dim3(shared ? kGroupCluster : 1), dim3(kGroupThreads), 0, stream);
+        if (shared) l.cluster(kGroupCluster);
+        if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<kGroupCluster>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_plan_kernel<1>, a)) != cudaSuccess) return e; }
     if ((e = hy3a_experts_launch_umma(a, type<T>::code, device, sms, stream, what)) != cudaSuccess) return e;
     hy3a_launch l(dim3(a.rows, (a.hidden / 8 + 255) / 256), dim3(256), 0, stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_experts_combine_kernel<T>, a);

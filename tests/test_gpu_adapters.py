@@ -183,3 +183,30 @@ def test_refusals(cuda):
             hy3_b200.adapters(*bad)
     with pytest.raises(AssertionError):
         hy3_b200.adapters(x, base, a, b, ids, s, out=torch.empty((4, 72), dtype=x.dtype, device=cuda))
+
+
+@pytest.mark.parametrize("rows,n,out", [(9, 1, 264), (40, 2047, 72), (40, 2048, 72), (600, 3000, 136), (513, 500, 1032), (5000, 3, 136)])
+def test_many_adapters_and_rows_in_any_order(cuda, rows, n, out):
+    """Adapters beyond those whose rows can be listed, rows of one adapter that lie apart, and rows shared by several blocks of the plan."""
+    import torch
+    import hy3_b200
+    args = list(make(rows, n, 8, 64, out))
+    check(hy3_b200.adapters(*args), args)
+    turn = torch.randperm(rows, device=cuda)
+    want = hy3_b200.adapters(*args)
+    got = hy3_b200.adapters(args[0][turn].contiguous(), args[1][turn].contiguous(), args[2], args[3], args[4][turn].contiguous(), args[5])
+    assert torch.equal(got, want[turn])
+
+
+@pytest.mark.parametrize("rows", [300, 1100])
+def test_long_rows_in_place_in_any_order(cuda, rows):
+    """Rows that are fetched and stored by their numbers, some of them twice, where the output lies over base."""
+    import torch
+    import hy3_b200
+    for base in ("float32", "bfloat16"):
+        args = make(rows, 7, 40, 128, 1096, base=base)
+        want = hy3_b200.adapters(*args)
+        check(want, args)
+        got = args[1].clone()
+        hy3_b200.adapters(args[0], got, *args[2:], out=got)
+        assert torch.equal(got, want)
