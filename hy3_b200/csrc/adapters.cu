@@ -3,8 +3,10 @@
  *
  *      out[t] = base[t] + scales[a] * B_a (A_a x[t]),   a = ids[t]
  *
- * u = A_a x enters the second product as two numbers of the rows' type, a rounded value and the rest, so that an fp32 result keeps about 17 (bf16)
- * or 22 (fp16) bits of it; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.
+ * u = A_a x enters the second product as two numbers of the rows' type, a rounded value and the rest, which leave 2^-17 (bf16) or 2^-22 (fp16) of a row's
+ * largest; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.  bf16 rows on an fp32 base take a
+ * third number in short inputs (2^-25).  In long ones the products bound the expansion, and a third would take half as much again;
+ * two leave an error of 6e-7 of the result where the adapter adds a third of it.
  *
  * Rows are worked on in tiles of one adapter, so that its weights are read once for all of a tile, whatever the order of the rows:
  *   up to 8 rows        one launch: a cluster of blocks for each adapter that occurs (short kernel);
@@ -138,8 +140,8 @@ __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_ker
 
 /* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers;
  * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros). */
-template <class T, int TOK, int THREADS, int NQ, class U>
-__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_hi, T *s_lo, float *s_back) {
+template <class T, int TOK, int THREADS, int TERMS, int NQ, class U>
+__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_u /* [TERMS][TOK][pitch] */, float *s_back) {
     constexpr int PT = THREADS / TOK;
     const int i = threadIdx.x / PT, sub = threadIdx.x % PT;
     const bool on = (any >> i) & 1;
@@ -174,21 +176,26 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
     for (int q = 0; q < NQ; q++) {
         const int r = 4 * (sub + PT * q);
         if (r < pitch - 8) {
-            const float f[4] = {v[q].x * to, v[q].y * to, v[q].z * to, v[q].w * to};
-            T hi[4], lo[4];
+            float f[4] = {v[q].x * to, v[q].y * to, v[q].z * to, v[q].w * to};
 #pragma unroll
-            for (int z = 0; z < 4; z++) { hi[z] = type<T>::down(f[z]); lo[z] = type<T>::down(isinf(type<T>::up(hi[z])) ? 0.f : f[z] - type<T>::up(hi[z])); }
-            *reinterpret_cast<uint2 *>(s_hi + i * pitch + r) = *reinterpret_cast<const uint2 *>(hi);
-            *reinterpret_cast<uint2 *>(s_lo + i * pitch + r) = *reinterpret_cast<const uint2 *>(lo);
+            for (int k = 0; k < TERMS; k++) {
+                T part[4];
+#pragma unroll
+                for (int z = 0; z < 4; z++) {
+                    part[z] = type<T>::down(f[z]);
+                    f[z] = isinf(type<T>::up(part[z])) ? 0.f : f[z] - type<T>::up(part[z]);
+                }
+                *reinterpret_cast<uint2 *>(s_u + (k * TOK + i) * pitch + r) = *reinterpret_cast<const uint2 *>(part);
+            }
         }
     }
 }
-template <class T, int TOK, int THREADS, class U>
-__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_hi, T *s_lo, float *s_back) {
+template <class T, int TOK, int THREADS, int TERMS, class U>
+__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_u /* [TERMS][TOK][pitch] */, float *s_back) {
     constexpr int MOST = kMaxRank * TOK / 4 / THREADS;             /* four ranks at a time of a thread, at the largest rank */
-    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, (MOST + 7) / 8>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
-    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, (MOST + 1) / 2>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
-    else put_u_of<T, TOK, THREADS, MOST>(a, u, parts, scale, any, pitch, s_hi, s_lo, s_back);
+    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, TERMS, (MOST + 7) / 8>(a, u, parts, scale, any, pitch, s_u, s_back);
+    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, TERMS, (MOST + 1) / 2>(a, u, parts, scale, any, pitch, s_u, s_back);
+    else put_u_of<T, TOK, THREADS, TERMS, MOST>(a, u, parts, scale, any, pitch, s_u, s_back);
 }
 
 /* The columns of the output are the M side of the second product; which of a warp's 64 is which row of it is free, and chosen so that a
@@ -204,12 +211,13 @@ constexpr int kShortBlocks = 8, kShortWarps = 8;
 template <class T, class O, bool WIDE, bool LISTED>
 __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kernel(const adapter_args a) {
     constexpr int PER = 16 / sizeof(O), NB = 8 / PER, RB = 4;            /* blocks of 16 ranks at a time */
+    constexpr int TERMS = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
     __shared__ float s_sum[kShortWarps][RB][4][32];
     __shared__ alignas(16) float s_part[8 * kMaxRank];                   /* [row][rank] of the block's share of the width */
-    __shared__ alignas(16) uint8_t s_u[2 * 8 * (kMaxRank + 8) * sizeof(T)];
+    __shared__ alignas(16) uint8_t s_u_raw[TERMS * 8 * (kMaxRank + 8) * sizeof(T)];
     __shared__ float s_back[8];
     const int pitch = (a.rank + 31) / 32 * 32 + 8;                       /* elements of a row of u: 16 bytes more than a multiple of 64 */
-    T *s_hi = reinterpret_cast<T *>(s_u), *s_lo = s_hi + 8 * pitch;
+    T *s_u = reinterpret_cast<T *>(s_u_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int share = blockIdx.y % kShortBlocks, c_begin = blockIdx.y * a.span, n_end = min(a.out_width, c_begin + a.span);
     pdl_release();
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     cluster_arrive();
     cluster_wait();
     const unsigned part = (unsigned)__cvta_generic_to_shared(s_part);
-    put_u<T, 8, 32 * kShortWarps>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, ad < 0 ? 0.f : a.scales[ad], any, pitch, s_hi, s_lo, s_back);
+    put_u<T, 8, 32 * kShortWarps, TERMS>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, ad < 0 ? 0.f : a.scales[ad], any, pitch, s_u, s_back);
     __syncwarp();
     cluster_arrive();                        /* the others' shares have been read */
     __syncthreads();
@@ -301,9 +309,12 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
                 uint4 f[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] = r < a.rank && n0 + column<O>(g, j) < n_end ? load_row(w + (size_t)column<O>(g, j) * a.rank + r) : zero16();
-                const uint4 hi = *reinterpret_cast<const uint4 *>(s_hi + g * pitch + r), lo = *reinterpret_cast<const uint4 *>(s_lo + g * pitch + r);
 #pragma unroll
-                for (int j = 0; j < 4; j++) { mma32<T>(acc[j], f[2 * j], f[2 * j + 1], lo); mma32<T>(acc[j], f[2 * j], f[2 * j + 1], hi); }
+                for (int k = TERMS - 1; k >= 0; k--) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(s_u + (k * 8 + g) * pitch + r);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma32<T>(acc[j], f[2 * j], f[2 * j + 1], v);
+                }
             }
         }
 #pragma unroll
@@ -443,7 +454,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
             }
         }
     } else {
-        if (ad >= 0) put_u<T, kLongRows, 128>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_hi, s_lo, s_back);
+        if (ad >= 0) put_u<T, kLongRows, 128, 2>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_hi, s_back);
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const T *u_hi = s_hi + g * pitch + t * 8, *u_lo = s_lo + g * pitch + t * 8;
         const int col = warp * 32, groups = (d.count + 7) >> 3;
