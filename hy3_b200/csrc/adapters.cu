@@ -138,6 +138,9 @@ __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_ker
     }
 }
 
+/* numbers of the rows' type that stand for one of u */
+template <class T, class O> constexpr int kTermsOf = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
+
 /* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers;
  * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros). */
 template <class T, int TOK, int THREADS, int TERMS, int NQ, class U>
@@ -211,7 +214,7 @@ constexpr int kShortBlocks = 8, kShortWarps = 8;
 template <class T, class O, bool WIDE, bool LISTED>
 __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kernel(const adapter_args a) {
     constexpr int PER = 16 / sizeof(O), NB = 8 / PER, RB = 4;            /* blocks of 16 ranks at a time */
-    constexpr int TERMS = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
+    constexpr int TERMS = kTermsOf<T, O>;
     __shared__ float s_sum[kShortWarps][RB][4][32];
     __shared__ alignas(16) float s_part[8 * kMaxRank];                   /* [row][rank] of the block's share of the width */
     __shared__ alignas(16) uint8_t s_u_raw[TERMS * 8 * (kMaxRank + 8) * sizeof(T)];
@@ -376,9 +379,10 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
                                                                                 const adapter_args a) {
     extern __shared__ uint8_t s_bytes[];
     using stage = long_stage<O>;
+    constexpr int TERMS = kTermsOf<T, O>;
     uint8_t *ring = s_bytes + ((1024u - (smem_u32(s_bytes) & 1023u)) & 1023u);
     const int chunks = (a.rank + 31) >> 5, pitch = chunks * 32 + 8;      /* elements of a row of u: 16 bytes more than a multiple of 64 */
-    T *s_hi = reinterpret_cast<T *>(ring + kLongStages * stage::bytes), *s_lo = s_hi + kLongRows * pitch;
+    T *s_u = reinterpret_cast<T *>(ring + kLongStages * stage::bytes);
     __shared__ float s_back[kLongRows];
     __shared__ alignas(16) int s_rows[kLongRows];
     __shared__ alignas(8) unsigned long long s_bar[3 * kLongStages];
@@ -454,9 +458,9 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
             }
         }
     } else {
-        if (ad >= 0) put_u<T, kLongRows, 128, 2>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_hi, s_back);
+        if (ad >= 0) put_u<T, kLongRows, 128, TERMS>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_u, s_back);
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        const T *u_hi = s_hi + g * pitch + t * 8, *u_lo = s_lo + g * pitch + t * 8;
+        const T *u_at = s_u + g * pitch + t * 8;
         const int col = warp * 32, groups = (d.count + 7) >> 3;
         bool ok = true;
         for (int tile = 0; tile < columns && ok; tile++) {
@@ -475,9 +479,12 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (i >= groups) continue;
-                        const uint4 hi = *reinterpret_cast<const uint4 *>(u_hi + 8 * i * pitch + in * 32), lo = *reinterpret_cast<const uint4 *>(u_lo + 8 * i * pitch + in * 32);
 #pragma unroll
-                        for (int m = 0; m < 2; m++) { mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], lo); mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], hi); }
+                        for (int k = TERMS - 1; k >= 0; k--) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(u_at + (k * kLongRows + 8 * i) * pitch + in * 32);
+#pragma unroll
+                            for (int m = 0; m < 2; m++) mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], v);
+                        }
                     }
                 }
                 if (in == per - 1) {
@@ -539,7 +546,7 @@ cudaError_t launch(const adapter_args &a, int device, void *stream, const char *
         if (shared) l.cluster(kGroupCluster);
         if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<kGroupCluster>, a, tile_rows) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<1>, a, tile_rows)) != cudaSuccess) return e; }
     if (shorts) return launch_short<T, O, true>(a, wide, stream);
-    constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kMostSmem = kRing + 2 * kLongRows * (kMaxRank + 8) * sizeof(T);
+    constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kTerms = kTermsOf<T, O>, kMostSmem = kRing + kTerms * kLongRows * (kMaxRank + 8) * sizeof(T);
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
         if ((e = cudaFuncSetAttribute(hy3a_adapters_expand_long_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
@@ -557,7 +564,7 @@ cudaError_t launch(const adapter_args &a, int device, void *stream, const char *
     {   hy3a_launch l(dim3(2 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
         if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
-    hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)2 * kLongRows * pitch * sizeof(T), stream);
+    hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)kTerms * kLongRows * pitch * sizeof(T), stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, tm_base32, tm_out32, a);
 }
 
