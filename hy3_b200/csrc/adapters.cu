@@ -5,13 +5,12 @@
  *
  * u = A_a x enters the second product as two numbers of the rows' type, a rounded value and the rest, which leave 2^-17 (bf16) or 2^-22 (fp16) of a row's
  * largest; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.  bf16 rows on an fp32 base take a
- * third number in short inputs (2^-25).  In long ones the products bound the expansion, and a third would take half as much again;
- * two leave an error of 6e-7 of the result where the adapter adds a third of it.
+ * third number (2^-25): two left an error of 1e-6 of the result.
  *
  * Rows are worked on in tiles of one adapter, so that its weights are read once for all of a tile, whatever the order of the rows:
- *   up to 8 rows        one launch: a cluster of blocks for each adapter that occurs (short kernel);
- *   up to kShort rows   the rows are listed by adapter (grouping.cuh) in tiles of 8, and each tile is a cluster's;
- *   more                listed in tiles of 32; 1. reduce: u[s][t] = A_a x[t] over the s-th 1024 of the width, fp32; 2. expand.
+ *   up to 8 rows        one launch: clusters of blocks for each adapter that occurs (short kernel);
+ *   up to kShort rows   one launch: the rows are listed by adapter within it, in tiles of 8, and each tile is a cluster's or a few clusters';
+ *   more                listed by a launch of their own (grouping.cuh) in tiles of 32; 1. reduce: u[s][t] = A_a x[t] over the s-th 1024 of the width, fp32; 2. expand.
  * Parts of u are added in their order wherever they meet.
  */
 #include <math.h>
@@ -76,11 +75,11 @@ __device__ __forceinline__ unsigned rows_of(int id, int ad) { return __ballot_sy
 constexpr int kPlanShared = 512;                          /* rows from which the blocks of a cluster share them: their warps take turns (2048 rows 11.5 us with one block) */
 constexpr int kMaxListed = 2 * kGroupThreads - 1;       /* adapters whose rows can be listed */
 template <int BLOCKS>
-__global__ void __launch_bounds__(kGroupThreads) hy3a_adapters_plan_kernel(const adapter_args a, int tile_rows) {
+__global__ void __launch_bounds__(kGroupThreads) hy3a_adapters_plan_kernel(const adapter_args a) {
     pdl_release();
     const int tiles = group_items<BLOCKS, 2, true>(
-        a.rows, a.adapters + 1, tile_rows, [&](int i) { const int id = a.ids[i]; return id >= 0 && id < a.adapters ? id : a.adapters; },
-        [&](int ad, int p0, int n, int first, int count) { for (int j = 0; j < count; j++) a.tiles[first + j] = {ad < a.adapters ? ad : -1, p0 + j * tile_rows, min(tile_rows, n - j * tile_rows), 0}; },
+        a.rows, a.adapters + 1, kLongRows, [&](int i) { const int id = a.ids[i]; return id >= 0 && id < a.adapters ? id : a.adapters; },
+        [&](int ad, int p0, int n, int first, int count) { for (int j = 0; j < count; j++) a.tiles[first + j] = {ad < a.adapters ? ad : -1, p0 + j * kLongRows, min(kLongRows, n - j * kLongRows), 0}; },
         [&](int i, int p) { a.list[p] = i; });
     if (threadIdx.x == 0 && (BLOCKS == 1 || cluster_rank() == 0)) *a.n_tiles = tiles;
 }
@@ -206,11 +205,16 @@ __device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int par
  * instruction of the warp then moves 128 contiguous bytes of each of four rows: fp32 two runs of 4 columns a lane, 16-bit types one of 8. */
 template <class O> __device__ __forceinline__ int column(int g, int col) { return sizeof(O) == 4 ? (col & 4) * 8 + g * 4 + (col & 3) : g * 8 + col; }
 
-/* ---- short inputs: cluster of 8 blocks = (a tile of 8 rows, 8 x `span` columns) --------------------------------------------------
- * LISTED: the tile is one of the table's, whose rows are listed; otherwise 8 rows in their order, and one of the adapters among them (blockIdx.z).
+/* ---- short inputs: cluster of 8 blocks = (a tile of 8 rows of one adapter, 8 x `span` columns) ----------------------------------
+ * LISTED: each block lists the rows by adapter itself, 256 at a time (blockIdx.x), and takes the tile of its number (a launch that lists them took
+ * 5 us: 64 rows of a few prompts on 4096 -> 10240 11.9 with it, 10.4 without; 16 rows of as many requests on 8192 -> 4096 12.3, 10.3); otherwise (up to 8 rows) a
+ * warp finds the adapter of its number among them.
  * Each block multiplies the rows by an eighth of A's width, the blocks meet in shared memory, and each adds its columns: one launch, u never
  * leaves the chip, and A is read once for 8 x span columns.  B is asked of L2 and base of memory before the first product begins. */
-constexpr int kShortBlocks = 8, kShortWarps = 8;
+constexpr int kShortBlocks = 8, kShortWarps = 8, kShortListed = 32 * kShortWarps;
+/* clusters for which a listed input's columns are divided: about as many as fit at once (two blocks an SM).  us a pass with 32 / 64 / 96: 64 rows of a few
+ * prompts on 4096 -> 10240 10.4 / 14.2 / 14.1, of as many requests 12.3 / 15.1 / 20.2, on 8192 -> 4096 17.7 / 22.5 / 25.1. */
+constexpr int kShortClusters = 32;
 template <class T, class O, bool WIDE, bool LISTED>
 __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kernel(const adapter_args a) {
     constexpr int PER = 16 / sizeof(O), NB = 8 / PER, RB = 4;            /* blocks of 16 ranks at a time */
@@ -222,28 +226,58 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     const int pitch = (a.rank + 31) / 32 * 32 + 8;                       /* elements of a row of u: 16 bytes more than a multiple of 64 */
     T *s_u = reinterpret_cast<T *>(s_u_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int share = blockIdx.y % kShortBlocks, c_begin = blockIdx.y * a.span, n_end = min(a.out_width, c_begin + a.span);
+    const int share = blockIdx.y % kShortBlocks;
     pdl_release();
     pdl_wait();
     /* lane i (and i + 8, ...) keeps row i of the tile */
-    int row, ad;
+    int row, ad, group = blockIdx.y / kShortBlocks, span = a.span;
     unsigned rows, any;                                                  /* the block's rows, and those with an adapter */
     if (LISTED) {
-        const adapter_tile d = a.tiles[blockIdx.x];                      /* (the table has a line for each block that is launched; asked for together) */
-        if ((int)blockIdx.x >= *a.n_tiles) return;                       /* (so do the cluster's others) */
-        row = a.list[d.first + min(lane & 7, d.count - 1)];
-        ad = d.adapter;
-        rows = (1u << d.count) - 1u;
+        __shared__ alignas(16) int s_id[kShortListed];
+        __shared__ int s_heads[kShortWarps], s_row[8], s_tile[2] /* adapter, place of its first row among the adapter's */, s_rows;
+        const int first = blockIdx.x * kShortListed, my = id_of(a, first + tid), listed = min(kShortListed, a.rows - first);
+        s_id[tid] = my;
+        if (tid == 0) s_rows = 0;
+        __syncthreads();
+        /* the row's place among its adapter's; every eighth of them begins a tile, and the block takes the one of its number */
+        int place = 0;
+#pragma unroll 8
+        for (int i = 0, n = tid < listed ? tid : 0; i < n; i += 4) {
+            const int4 id = *reinterpret_cast<const int4 *>(s_id + i);
+            place += (id.x == my) + (i + 1 < tid && id.y == my) + (i + 2 < tid && id.z == my) + (i + 3 < tid && id.w == my);
+        }
+        const bool head = tid < listed && (place & 7) == 0;
+        const unsigned heads = __ballot_sync(0xffffffffu, head);
+        if (lane == 0) s_heads[warp] = __popc(heads);
+        __syncthreads();
+        int before = 0, tiles = 0;
+        for (int w = 0; w < kShortWarps; w++) { tiles += s_heads[w]; if (w < warp) before += s_heads[w]; }
+        const int groups = max(1, min(kShortClusters / tiles, (a.out_width + kShortBlocks * span - 1) / (kShortBlocks * span))), tile = blockIdx.z % tiles;
+        group = blockIdx.z / tiles;
+        if (group >= groups) return;                                     /* (so do the cluster's others) */
+        const int each = (a.out_width + kShortBlocks * groups - 1) / (kShortBlocks * groups), pass = each <= kShortWarps * kExpandCols ? kExpandCols : kShortWarps * kExpandCols;
+        span = (each + pass - 1) / pass * pass;
+        if (head && before + __popc(heads & ((1u << lane) - 1u)) == tile) { s_tile[0] = my; s_tile[1] = place; }
+        __syncthreads();
+        ad = s_tile[0];
+        const int at = place - s_tile[1];
+        const bool mine = tid < listed && my == ad && at >= 0 && at < 8;
+        if (mine) { s_row[at] = first + tid; atomicAdd(&s_rows, 1); }
+        __syncthreads();
+        const int count = s_rows;
+        row = s_row[min(lane & 7, count - 1)];
+        rows = (1u << count) - 1u;
         any = ad < 0 ? 0u : rows;
     } else {
-        row = min((int)blockIdx.x * 8 + (lane & 7), a.rows - 1);
-        const int my = lane < 8 ? id_of(a, blockIdx.x * 8 + lane) : -1;
-        const unsigned with = __ballot_sync(0xffffffffu, my >= 0), none = __ballot_sync(0xffffffffu, lane < 8 && (int)blockIdx.x * 8 + lane < a.rows && my < 0);
+        row = min(lane & 7, a.rows - 1);
+        const int my = lane < 8 ? id_of(a, lane) : -1;
+        const unsigned with = __ballot_sync(0xffffffffu, my >= 0), none = __ballot_sync(0xffffffffu, lane < 8 && lane < a.rows && my < 0);
         ad = nth_adapter(my, with, blockIdx.z);
         if (ad < 0 && blockIdx.z > 0) return;
         any = rows_of(my, ad);
         rows = any | (blockIdx.z == 0 ? none : 0u);                      /* rows without an adapter go with the first */
     }
+    const int c_begin = (group * kShortBlocks + share) * span, n_end = min(a.out_width, c_begin + span);
     const int row_g = __shfl_sync(0xffffffffu, row, g), row_t[2] = {__shfl_sync(0xffffffffu, row, 2 * t), __shfl_sync(0xffffffffu, row, 2 * t + 1)};
     const T *const b = reinterpret_cast<const T *>(a.b) + (size_t)(ad < 0 ? 0 : ad) * a.out_width * a.rank;
     if (any && c_begin < n_end)
@@ -525,13 +559,13 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
 /* Rows up to which tiles of 8 are taken (us a pass, tiles of 8 / of 32): 64, 128 and 256 rows of as many requests on 8192 -> 4096 20.1 / 21.5, 28.6 / 30.0,
  * 30.4 / 32.0; of a few prompts on 4096 -> 10240 11.9 / 18.5, 17.2 / 19.9, 26.7 / 23.8. */
 constexpr int kShort = 128;
-int most_tiles(const adapter_args &a, int tile_rows) { return a.rows / tile_rows + std::min(a.rows, a.adapters + 1); }
 
 template <class T, class O, bool LISTED>
 cudaError_t launch_short(adapter_args a, bool wide, void *stream) {
-    a.span = a.rows <= 8 ? 256 : 512;
-    const int groups = (a.out_width + kShortBlocks * a.span - 1) / (kShortBlocks * a.span);
-    hy3a_launch l(LISTED ? dim3(most_tiles(a, 8), kShortBlocks * groups) : dim3((a.rows + 7) / 8, kShortBlocks * groups, std::min({8, a.rows, a.adapters})), dim3(32 * kShortWarps), 0, stream);
+    a.span = LISTED ? 512 : 256;           /* at least, where the kernel chooses */
+    const int groups = (a.out_width + kShortBlocks * a.span - 1) / (kShortBlocks * a.span), chunk = std::min(a.rows, kShortListed);
+    hy3a_launch l(LISTED ? dim3((a.rows + kShortListed - 1) / kShortListed, kShortBlocks, std::max(kShortClusters, chunk / 8 + std::min(chunk, a.adapters + 1)))
+                         : dim3(1, kShortBlocks * groups, std::min(a.rows, a.adapters)), dim3(32 * kShortWarps), 0, stream);
     l.cluster(1, kShortBlocks);
     return wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, true, LISTED>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, false, LISTED>, a);
 }
@@ -539,13 +573,12 @@ template <class T, class O>
 cudaError_t launch(const adapter_args &a, int device, void *stream, const char **what) {
     cudaError_t e;
     const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
-    if (a.rows <= 8 || a.adapters > kMaxListed) return launch_short<T, O, false>(a, wide, stream);
-    const bool shared = a.rows >= kPlanShared, shorts = a.rows <= kShort || a.base_stride < (size_t)a.out_width;      /* (rows of base that overlap have no tensor map) */
-    const int tile_rows = shorts ? 8 : kLongRows;
+    if (a.rows <= 8) return launch_short<T, O, false>(a, wide, stream);
+    if (a.rows <= kShort || a.adapters > kMaxListed || a.base_stride < (size_t)a.out_width /* rows that overlap have no tensor map */) return launch_short<T, O, true>(a, wide, stream);
+    const bool shared = a.rows >= kPlanShared;
     {   hy3a_launch l(dim3(shared ? kGroupCluster : 1), dim3(kGroupThreads), 0, stream);
         if (shared) l.cluster(kGroupCluster);
-        if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<kGroupCluster>, a, tile_rows) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<1>, a, tile_rows)) != cudaSuccess) return e; }
-    if (shorts) return launch_short<T, O, true>(a, wide, stream);
+        if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<kGroupCluster>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<1>, a)) != cudaSuccess) return e; }
     constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kTerms = kTermsOf<T, O>, kMostSmem = kRing + kTerms * kLongRows * (kMaxRank + 8) * sizeof(T);
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
@@ -560,7 +593,7 @@ cudaError_t launch(const adapter_args &a, int device, void *stream, const char *
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    const int tiles = most_tiles(a, kLongRows), rank_blocks = (a.rank + 31) / 32, pitch = rank_blocks * 32 + 8;
+    const int tiles = a.rows / kLongRows + std::min(a.rows, a.adapters + 1), rank_blocks = (a.rank + 31) / 32, pitch = rank_blocks * 32 + 8;
     {   hy3a_launch l(dim3(2 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
         if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
     const int across = (a.out_width + kLongCols - 1) / kLongCols;
