@@ -10,7 +10,7 @@
  * Rows are worked on in tiles of one adapter, so that its weights are read once for all of a tile, whatever the order of the rows:
  *   up to 8 rows        one launch: clusters of blocks for each adapter that occurs (short kernel);
  *   up to kShort rows   one launch: the rows are listed by adapter within it, in tiles of 8, and each tile is a cluster's or a few clusters';
- *   more                listed by a launch of their own (grouping.cuh) in tiles of 32; 1. reduce: u[s][t] = A_a x[t] over the s-th 1024 of the width, fp32; 2. expand.
+ *   more                listed by a launch of their own (grouping.cuh) in tiles of 64; 1. reduce: u[s][t] = A_a x[t] over the s-th 2048 of the width, fp32; 2. expand.
  * Parts of u are added in their order wherever they meet.
  */
 #include <math.h>
@@ -27,9 +27,9 @@ using namespace hy3a_layer;
 using namespace hy3a_ring;
 
 constexpr int kMaxRank = 256, kMaxWidth = 1 << 20;
-constexpr int kCut = 1024;           /* k's of a reduce block: 128 of each of its 8 warps */
+constexpr int kCut = 2048;           /* k's of a reduce block: 256 of each of its 8 warps (1024: 2048 rows on 8192 -> 4096 48.4 -> 55.7 us a pass, 512 of width 4096 25.0 -> 23.5) */
 constexpr int kReduceWarps = 8, kExpandCols = 64 /* columns of a warp at a time */;
-constexpr int kLongRows = 32, kLongCols = 128, kLongStages = 4, kLongThreads = 192, kLongTiles = 5;
+constexpr int kLongRows = 64, kLongCols = 128, kLongStages = 4;
 
 /* `count` listed rows from `first` on, all of one adapter (-1: none) */
 struct adapter_tile { int adapter, first, count, unused; };
@@ -141,9 +141,10 @@ __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_ker
 template <class T, class O> constexpr int kTermsOf = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
 
 /* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers;
- * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros). */
-template <class T, int TOK, int THREADS, int TERMS, int NQ, class U>
-__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_u /* [TERMS][TOK][pitch] */, float *s_back) {
+ * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros); `ranks`: how many are
+ * written, those past the last as zeros; place(term, row, rank): where four go. */
+template <class T, int TOK, int THREADS, int TERMS, int NQ, class U, class P>
+__device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int parts, float scale, unsigned long long any, int ranks, const P &place, float *s_back) {
     constexpr int PT = THREADS / TOK;
     const int i = threadIdx.x / PT, sub = threadIdx.x % PT;
     const bool on = (any >> i) & 1;
@@ -177,7 +178,7 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
         const int r = 4 * (sub + PT * q);
-        if (r < pitch - 8) {
+        if (r < ranks) {
             float f[4] = {v[q].x * to, v[q].y * to, v[q].z * to, v[q].w * to};
 #pragma unroll
             for (int k = 0; k < TERMS; k++) {
@@ -187,17 +188,17 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
                     part[z] = type<T>::down(f[z]);
                     f[z] = isinf(type<T>::up(part[z])) ? 0.f : f[z] - type<T>::up(part[z]);
                 }
-                *reinterpret_cast<uint2 *>(s_u + (k * TOK + i) * pitch + r) = *reinterpret_cast<const uint2 *>(part);
+                *reinterpret_cast<uint2 *>(place(k, i, r)) = *reinterpret_cast<const uint2 *>(part);
             }
         }
     }
 }
-template <class T, int TOK, int THREADS, int TERMS, class U>
-__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, float scale, unsigned any, int pitch, T *s_u /* [TERMS][TOK][pitch] */, float *s_back) {
+template <class T, int TOK, int THREADS, int TERMS, class U, class P>
+__device__ __forceinline__ void put_u(const adapter_args &a, const U &u, int parts, float scale, unsigned long long any, int ranks, const P &place, float *s_back) {
     constexpr int MOST = kMaxRank * TOK / 4 / THREADS;             /* four ranks at a time of a thread, at the largest rank */
-    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, TERMS, (MOST + 7) / 8>(a, u, parts, scale, any, pitch, s_u, s_back);
-    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, TERMS, (MOST + 1) / 2>(a, u, parts, scale, any, pitch, s_u, s_back);
-    else put_u_of<T, TOK, THREADS, TERMS, MOST>(a, u, parts, scale, any, pitch, s_u, s_back);
+    if (a.rank <= kMaxRank / 8) put_u_of<T, TOK, THREADS, TERMS, (MOST + 7) / 8>(a, u, parts, scale, any, ranks, place, s_back);
+    else if (a.rank <= kMaxRank / 2) put_u_of<T, TOK, THREADS, TERMS, (MOST + 1) / 2>(a, u, parts, scale, any, ranks, place, s_back);
+    else put_u_of<T, TOK, THREADS, TERMS, MOST>(a, u, parts, scale, any, ranks, place, s_back);
 }
 
 /* The columns of the output are the M side of the second product; which of a warp's 64 is which row of it is free, and chosen so that a
@@ -334,7 +335,8 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     cluster_arrive();
     cluster_wait();
     const unsigned part = (unsigned)__cvta_generic_to_shared(s_part);
-    put_u<T, 8, 32 * kShortWarps, TERMS>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, ad < 0 ? 0.f : a.scales[ad], any, pitch, s_u, s_back);
+    put_u<T, 8, 32 * kShortWarps, TERMS>(a, [&](int c, int i, int r) { return peer_value(part + (unsigned)(i * a.rank + r) * 4u, (unsigned)c); }, kShortBlocks, ad < 0 ? 0.f : a.scales[ad], any, pitch - 8,
+                                               [&](int k, int i, int r) { return s_u + (k * 8 + i) * pitch + r; }, s_back);
     __syncwarp();
     cluster_arrive();                        /* the others' shares have been read */
     __syncthreads();
@@ -377,183 +379,184 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
     cluster_wait();
 }
 
-/* ---- 2. expand, long inputs: block = (a tile of 32 rows, 4 column tiles of 128) -------------------------------------------
- * Units (column tile, 32 ranks) go through a ring of 4 stages that TMA fills: 128 rows of B of 32 ranks, and with the last unit of a column tile the
- * tile of base, as one box where the rows are neighbours (a prompt's), four rows at a time by their numbers otherwise (tile::gather4, tile::scatter4:
- * 54 us of 2048 rows on 4096 -> 10240 become 76); it becomes the tile of the output where it lies and leaves the same way.  Bounds are the tensor maps'.  Warps 0-3 multiply (32 rows x 32 columns each), warp 4 fetches, warp 5 stores.  Base and output are
- * what this kernel has to move (168 MB for 2048 rows of 10240 in fp32); written with loads and stores of the multiplying warps, their addresses took
- * more issue slots than the products. */
-template <class O> struct long_stage {
-    static constexpr int box = 128 / sizeof(O) /* columns of a box: 128 bytes */, base_bytes = kLongRows * kLongCols * sizeof(O), b_bytes = kLongCols * 64, bytes = b_bytes + base_bytes;
-};
-enum { A_FULL = 0, A_DONE = kLongStages, A_EMPTY = 2 * kLongStages };
+/* ---- 2. expand, long inputs: block = (a tile of up to 64 rows, some tiles of 128 columns, 256 in 16-bit types), two an SM -------------------
+ * Base and output are what this kernel has to move (168 MB for 2048 rows of 10240 in fp32, of 50 us a pass in all; a copy of as many bytes by rows of 128
+ * in this form runs at 5.6 TB/s).  Columns are the M side of tcgen05.mma, rows the N side: an accumulator's lane is a column of the output, so that a
+ * warp adds base and stores straight from tensor memory, 128 bytes of a row at a time, whatever rows the list names.  In 16-bit types a lane has
+ * two neighbouring columns, one in each of two accumulators: B's columns come in by their parity.  Warps 0-7 prepare u and then move the quarter w % 4 of
+ * the columns of rows 32 (w / 4) ..; warp 8 fetches B (128 columns x 64 ranks a stage, 128-byte swizzle), warp 9 multiplies, into two sets of accumulators in turn.
+ * Measured beside it, 2048 rows on 4096 -> 10240 with 32 / 128 ranks: warp-level products over a ring of tensor copies 63 / 159, this 50 / 73; base and
+ * output through shared memory by a bulk copy of each row, one block an SM, 67 / 92. */
+constexpr int kLongWarps = 8, kLongThreads = 32 * (kLongWarps + 2), kStageBytes = kLongCols * 128;
+enum { A_FULL = 0, A_EMPTY = kLongStages, A_TFULL = 2 * kLongStages, A_TEMPTY = A_TFULL + 2, A_COUNT = A_TEMPTY + 2 };
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
-__device__ __forceinline__ void tma_gather4(unsigned dst, const CUtensorMap *map, unsigned bar, int x, const int4 &row) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w) : "memory");
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+/* K-major operand, 128-byte swizzle: 8-row groups 1024 B apart, descriptor version 1, layout 2 */
+__device__ __forceinline__ unsigned long long make_desc(unsigned saddr) {
+    return (unsigned long long)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void umma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tma_store(const CUtensorMap *map, unsigned src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void umma_commit(unsigned bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tmem_ld8(unsigned taddr, unsigned (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tma_scatter4(const CUtensorMap *map, unsigned src, int x, const int4 &row) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile::scatter4.bulk_group [%0, {%2, %3, %4, %5, %6}], [%1];"
-                 ::"l"(map), "r"(src), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w) : "memory");
-}
-
 template <class T, class O>
-__global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_base,
-                                                                                const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_base32, const __grid_constant__ CUtensorMap tm_out32,
-                                                                                const adapter_args a) {
+__global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_kernel(const __grid_constant__ CUtensorMap tm_b, const adapter_args a, int stages, int blocks) {
     extern __shared__ uint8_t s_bytes[];
-    using stage = long_stage<O>;
-    constexpr int TERMS = kTermsOf<T, O>;
-    uint8_t *ring = s_bytes + ((1024u - (smem_u32(s_bytes) & 1023u)) & 1023u);
-    const int chunks = (a.rank + 31) >> 5, pitch = chunks * 32 + 8;      /* elements of a row of u: 16 bytes more than a multiple of 64 */
-    T *s_u = reinterpret_cast<T *>(ring + kLongStages * stage::bytes);
+    constexpr int TERMS = kTermsOf<T, O>, PER = 4 / sizeof(O) /* columns of a lane */, COLS = kLongCols * PER, ACC = kLongRows * PER /* columns of tensor memory of a unit */;
+    uint8_t *ring = s_bytes + ((1024u - (smem_u32(s_bytes) & 1023u)) & 1023u), *s_u = ring + stages * kStageBytes;      /* u: [term][64 ranks][row] */
     __shared__ float s_back[kLongRows];
-    __shared__ alignas(16) int s_rows[kLongRows];
-    __shared__ alignas(8) unsigned long long s_bar[3 * kLongStages];
+    __shared__ size_t s_base[kLongRows], s_out[kLongRows];               /* where the rows begin, in words of 4 bytes */
+    __shared__ alignas(8) unsigned long long s_bar[A_COUNT];
+    __shared__ unsigned s_tmem;
     __shared__ int s_abort_flag;
     volatile int *s_abort = &s_abort_flag;
     const unsigned bar0 = smem_u32(s_bar);
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int across = (a.out_width + kLongCols - 1) / kLongCols;
-    const int c_first = blockIdx.y * kLongTiles, columns = min(kLongTiles, across - c_first);      /* column tiles */
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, panels = (a.rank + 63) >> 6, across = (a.out_width + COLS - 1) / COLS;
     if (tid == 0) {
         s_abort_flag = 0;
-        for (int i = 0; i < kLongStages; i++) { mbar_init(bar0 + 8 * (A_FULL + i), 1); mbar_init(bar0 + 8 * (A_DONE + i), 4); mbar_init(bar0 + 8 * (A_EMPTY + i), 1); }
+        for (int i = 0; i < stages; i++) { mbar_init(bar0 + 8 * (A_FULL + i), 1); mbar_init(bar0 + 8 * (A_EMPTY + i), 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(bar0 + 8 * (A_TFULL + i), 1); mbar_init(bar0 + 8 * (A_TEMPTY + i), kLongWarps); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_release();
-    pdl_wait();
-    const adapter_tile d = a.tiles[blockIdx.x];
-    if ((int)blockIdx.x >= *a.n_tiles) return;
-    const int ad = d.adapter, last_row = d.count - 1;
-    if (warp == 0) s_rows[lane] = a.list[d.first + min(lane, last_row)];     /* places past the last row stand for it: what is stored there twice is the same */
+    if (warp == kLongWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(2u * ACC) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    const int per = ad < 0 ? 1 : chunks;                                 /* units of a column tile */
-    const bool run = last_row == kLongRows - 1 && s_rows[last_row] - s_rows[0] == last_row;      /* the listed rows ascend: 32 neighbours are one box */
-    unsigned st = 0, ph = 0;
-    if (warp == 5) {
-        /* gives the stages back, those with output when it has been read */
-        if (lane == 0) {
-            int pending = -1;
-            bool ok = true;
-            for (int tile = 0; tile < columns && ok; tile++) {
-                const int c0 = (c_first + tile) * kLongCols;
-                for (int in = 0; in < per; in++) {
-                    if (!(ok = mbar_wait(bar0 + 8 * (A_DONE + st), ph, s_abort, g_err, 32u))) break;
-                    const bool last = in == per - 1;
-                    if (last) {
-                        const unsigned src = smem_u32(ring) + st * stage::bytes + stage::b_bytes;
-                        for (int i = 0; i < kLongCols / stage::box; i++)
-                            if (c0 + i * stage::box >= a.out_width) break;
-                            else if (run) tma_store(&tm_out32, src + i * kLongRows * 128, c0 + i * stage::box, s_rows[0]);
-                            else
-                                for (int q = 0; q <= last_row >> 2; q++) tma_scatter4(&tm_out, src + i * kLongRows * 128 + q * 512, c0 + i * stage::box, *reinterpret_cast<const int4 *>(s_rows + 4 * q));
-                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = s_tmem;
+    pdl_release();                           /* not before the tensor memory is there: the next kernel could take it and wait for this one */
+    pdl_wait();
+    /* the column tiles of a row tile are divided among as many blocks as fit at once */
+    const int tiles = *a.n_tiles, groups = max(1, min(blocks / tiles, across)), span = (across + groups - 1) / groups, c_first = ((int)blockIdx.x / tiles) * span;
+    const int columns = (int)blockIdx.x / tiles < groups ? min(span, across - c_first) : 0;
+    const adapter_tile d = a.tiles[(int)blockIdx.x % tiles];
+    const int ad = d.adapter;
+    if (tid < kLongRows) {
+        const int row = a.list[d.first + min(tid, d.count - 1)];
+        s_base[tid] = (size_t)row * (a.base_stride / PER);
+        s_out[tid] = (size_t)row * (a.out_stride / PER);
+    }
+    __syncthreads();
+    if (columns > 0 && (ad >= 0 || warp < kLongWarps)) {
+        if (warp == kLongWarps) {
+            if (lane == 0) {
+                int st = 0;
+                unsigned ph = 0;
+                bool ok = true;
+                for (int c = 0; c < columns && ok; c++)
+                    for (int p = 0; p < panels * PER; p++) {
+                        if (!(ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 30u))) break;
+                        mbar_expect_tx(bar0 + 8 * (A_FULL + st), kStageBytes);
+                        tma_load(smem_u32(ring) + st * kStageBytes, &tm_b, bar0 + 8 * (A_FULL + st), p / PER * 64, p % PER, (c_first + c) * kLongCols, ad);
+                        if (++st == stages) { st = 0; ph ^= 1u; }
                     }
-                    if (pending >= 0) {                 /* the output before this unit's */
-                        if (last) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        mbar_arrive(bar0 + 8 * (A_EMPTY + pending));
-                    }
-                    pending = last ? (int)st : -1;
-                    if (!last) mbar_arrive(bar0 + 8 * (A_EMPTY + st));
-                    if (++st == kLongStages) { st = 0; ph ^= 1u; }
+                for (int i = 0; i < stages && ok; i++) {                 /* the last commits have reached their barriers before the block ends */
+                    ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 34u);
+                    if (++st == stages) { st = 0; ph ^= 1u; }
                 }
             }
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        }
-    } else if (warp == 4) {
-        if (lane == 0) {
-            bool ok = true;
-            for (int tile = 0; tile < columns && ok; tile++) {
-                const int c0 = (c_first + tile) * kLongCols, boxes = min(kLongCols / stage::box, (a.out_width - c0 + stage::box - 1) / stage::box), fours = (last_row >> 2) + 1;
-                for (int in = 0; in < per; in++) {
-                    if (!(ok = mbar_wait(bar0 + 8 * (A_EMPTY + st), ph ^ 1u, s_abort, g_err, 30u))) break;
-                    const unsigned full = bar0 + 8 * (A_FULL + st), dst = smem_u32(ring) + st * stage::bytes;
-                    const bool last = in == per - 1;
-                    mbar_expect_tx(full, (ad < 0 ? 0 : stage::b_bytes) + (last ? boxes * fours * 512 : 0));
-                    if (ad >= 0) tma_load(dst, &tm_b, full, in * 32, c0, ad);
-                    if (last)
-                        for (int i = 0; i < boxes; i++)
-                            if (run) tma_load(dst + stage::b_bytes + i * kLongRows * 128, &tm_base32, full, c0 + i * stage::box, s_rows[0]);
-                            else for (int q = 0; q < fours; q++) tma_gather4(dst + stage::b_bytes + i * kLongRows * 128 + q * 512, &tm_base, full, c0 + i * stage::box, *reinterpret_cast<const int4 *>(s_rows + 4 * q));
-                    if (++st == kLongStages) { st = 0; ph ^= 1u; }
-                }
-            }
-        }
-    } else {
-        if (ad >= 0) put_u<T, kLongRows, 128, TERMS>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + min(i, last_row)) * a.rank + r); }, a.cuts, a.scales[ad], ~0u, pitch, s_u, s_back);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const T *u_at = s_u + g * pitch + t * 8;
-        const int col = warp * 32, groups = (d.count + 7) >> 3;
-        bool ok = true;
-        for (int tile = 0; tile < columns && ok; tile++) {
-            float acc[2][4][4] = {};
-            for (int in = 0; in < per; in++) {
-                if (!(ok = mbar_wait(bar0 + 8 * (A_FULL + st), ph, s_abort, g_err, 31u))) break;
-                uint8_t *const at = ring + st * stage::bytes;
-                if (ad >= 0) {
-                    /* product m of the warp's two: its row g is column 4g + 2m, row g + 8 the one behind it */
-                    uint4 f[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int n = col + 4 * g + j;
-                        f[j] = *reinterpret_cast<const uint4 *>(at + n * 64 + ((t ^ ((n >> 1) & 3)) << 4));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (i >= groups) continue;
-#pragma unroll
+        } else if (warp == kLongWarps + 1) {
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * (kLongWarps + 1)) : "memory");
+            if (lane == 0) {
+                constexpr unsigned kType = type<T>::code == HY3A_BF16 ? (1u << 7) | (1u << 10) : 0u;
+                const unsigned idesc = (1u << 4) | kType | (((unsigned)(d.count + 15) >> 4) << 18) | ((kLongCols >> 4) << 24);
+                int st = 0;
+                unsigned ph = 0;
+                bool ok = true;
+                for (int c = 0; c < columns && ok; c++) {
+                    const int buf = c & 1;
+                    if (!(ok = mbar_wait(bar0 + 8 * (A_TEMPTY + buf), ((c >> 1) & 1) ^ 1, s_abort, g_err, 32u))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    for (int p = 0; p < panels * PER; p++) {
+                        if (!(ok = mbar_wait(bar0 + 8 * (A_FULL + st), ph, s_abort, g_err, 31u))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const int panel = p / PER, steps = min(4, (a.rank - panel * 64 + 15) >> 4);
+                        const unsigned long long da = make_desc(smem_u32(ring) + st * kStageBytes);
                         for (int k = TERMS - 1; k >= 0; k--) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(u_at + (k * kLongRows + 8 * i) * pitch + in * 32);
-#pragma unroll
-                            for (int m = 0; m < 2; m++) mma32<T>(acc[m][i], f[2 * m], f[2 * m + 1], v);
+                            const unsigned long long db = make_desc(smem_u32(s_u) + (k * panels + panel) * kLongRows * 128);
+                            for (int i = 0; i < steps; i++) umma(tmem + buf * ACC + p % PER * kLongRows, da + 2 * i, db + 2 * i, idesc, panel > 0 || k < TERMS - 1 || i > 0);
                         }
+                        umma_commit(bar0 + 8 * (A_EMPTY + st));
+                        if (++st == stages) { st = 0; ph ^= 1u; }
+                    }
+                    if (ok) umma_commit(bar0 + 8 * (A_TFULL + buf));
+                }
+            }
+        } else {
+            const int r0 = (warp >> 2) * 32, count = d.count - r0;
+            if (ad >= 0) {
+                put_u<T, kLongRows, 32 * kLongWarps, TERMS>(a, [&](int c, int i, int r) { return *reinterpret_cast<const float4 *>(a.u + ((size_t)c * a.rows + d.first + i) * a.rank + r); },
+                                                            a.cuts, a.scales[ad], ~0ull >> (kLongRows - d.count), (a.rank + 15) & ~15,
+                                                            [&](int k, int i, int r) { return s_u + (k * panels + (r >> 6)) * kLongRows * 128 + i * 128 + ((((r >> 3) & 7) ^ (i & 7)) << 4) + (r & 7) * 2; }, s_back);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * (kLongWarps + 1)) : "memory");
+            }
+            for (int c = 0; c < columns; c++) {
+                const int n = (c_first + c) * COLS + (warp & 3) * 32 * PER + lane * PER, buf = c & 1;
+                const bool in = n < a.out_width, whole = count >= 32 && n + (32 - lane) * PER <= a.out_width;
+                const unsigned *const base = reinterpret_cast<const unsigned *>(reinterpret_cast<const O *>(a.base) + n);
+                unsigned *const out = reinterpret_cast<unsigned *>(reinterpret_cast<O *>(a.out) + n);
+                unsigned held[32];
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) held[j] = base[s_base[r0 + j]];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) if (in && j < count) held[j] = base[s_base[r0 + j]];
+                }
+                if (ad < 0) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) if (in && j < count) out[s_out[r0 + j]] = held[j];
+                    continue;
+                }
+                if (!mbar_wait(bar0 + 8 * (A_TFULL + buf), (c >> 1) & 1, s_abort, g_err, 33u)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                constexpr int STEP = 16 / PER;
+#pragma unroll
+                for (int h = 0; h < 32; h += STEP) {
+                    if (h >= count) continue;
+                    unsigned v[2][8];                /* rows and the 8 behind them, or a row's two columns */
+                    const unsigned at = tmem + ((unsigned)((warp & 3) * 32) << 16) + buf * ACC + r0 + h;
+                    tmem_ld8(at, v[0]);
+                    tmem_ld8(at + (PER == 2 ? kLongRows : 8), v[1]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    auto sum = [&](int j) {
+                        const float by = s_back[r0 + h + j];
+                        unsigned o = held[h + j];
+                        O *const e = reinterpret_cast<O *>(&o);
+#pragma unroll
+                        for (int z = 0; z < PER; z++) e[z] = type<O>::down(type<O>::up(e[z]) + by * __uint_as_float(PER == 2 ? v[z][j & 7] : v[j >> 3][j & 7]));
+                        out[s_out[r0 + h + j]] = o;
+                    };
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < STEP; j++) sum(j);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < STEP; j++) if (in && h + j < count) sum(j);
                     }
                 }
-                if (in == per - 1) {
-                    if (ad >= 0) {
-                        struct alignas(4 * sizeof(O)) four { O v[4]; };
-                        four o[4][2];
-                        /* columns 4g .. 4g + 3 of row 8i + 2t + c */
-                        auto place = [&](int i, int c) {
-                            const int row = 8 * i + 2 * t + c, b = (col + 4 * g) * (int)sizeof(O);           /* byte of the tile's row */
-                            return reinterpret_cast<four *>(at + stage::b_bytes + (b >> 7) * kLongRows * 128 + row * 128 + ((((b >> 4) & 7) ^ (row & 7)) << 4) + (b & 15));
-                        };
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int c = 0; c < 2; c++) if (i < groups) o[i][c] = *place(i, c);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int c = 0; c < 2; c++) {
-                                if (i >= groups) continue;
-                                const float back = s_back[8 * i + 2 * t + c];
-#pragma unroll
-                                for (int z = 0; z < 4; z++) o[i][c].v[z] = type<O>::down(type<O>::up(o[i][c].v[z]) + back * acc[z >> 1][i][(z & 1) * 2 + c]);
-                                *place(i, c) = o[i][c];
-                            }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar0 + 8 * (A_DONE + st));
-                if (++st == kLongStages) { st = 0; ph ^= 1u; }
+                if (lane == 0) mbar_arrive(bar0 + 8 * (A_TEMPTY + buf));
             }
         }
     }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the unit that was given up are still on their way */
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == kLongWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * ACC) : "memory");
 }
 
 /* Rows up to which tiles of 8 are taken (us a pass, tiles of 8 / of 32): 64, 128 and 256 rows of as many requests on 8192 -> 4096 20.1 / 21.5, 28.6 / 30.0,
@@ -569,36 +572,42 @@ cudaError_t launch_short(adapter_args a, bool wide, void *stream) {
     l.cluster(1, kShortBlocks);
     return wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, true, LISTED>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_short_kernel<T, O, false, LISTED>, a);
 }
+/* B as [adapter][column / per][column % per][rank]; boxes of 128 columns that are `per` apart, of 64 ranks */
+bool encode_columns(CUtensorMap *m, const adapter_args &a, int per) {
+    const encode_tiled_fn enc = encoder();
+    const cuuint64_t line = (cuuint64_t)a.rank * 2, dims[4] = {(cuuint64_t)a.rank, (cuuint64_t)per, (cuuint64_t)(a.out_width / per), (cuuint64_t)a.adapters}, strides[3] = {line, line * per, line * a.out_width};
+    const cuuint32_t box[4] = {64, 1, kLongCols, 1}, one[4] = {1, 1, 1, 1};
+    return enc && enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(a.b), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 template <class T, class O>
-cudaError_t launch(const adapter_args &a, int device, void *stream, const char **what) {
+cudaError_t launch(const adapter_args &a, int device, int sms, void *stream, const char **what) {
     cudaError_t e;
     const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
     if (a.rows <= 8) return launch_short<T, O, false>(a, wide, stream);
-    if (a.rows <= kShort || a.adapters > kMaxListed || a.base_stride < (size_t)a.out_width /* rows that overlap have no tensor map */) return launch_short<T, O, true>(a, wide, stream);
+    if (a.rows <= kShort || a.adapters > kMaxListed) return launch_short<T, O, true>(a, wide, stream);
     const bool shared = a.rows >= kPlanShared;
     {   hy3a_launch l(dim3(shared ? kGroupCluster : 1), dim3(kGroupThreads), 0, stream);
         if (shared) l.cluster(kGroupCluster);
         if ((e = shared ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<kGroupCluster>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_plan_kernel<1>, a)) != cudaSuccess) return e; }
-    constexpr int kRing = kLongStages * long_stage<O>::bytes + 1024, kTerms = kTermsOf<T, O>, kMostSmem = kRing + kTerms * kLongRows * (kMaxRank + 8) * sizeof(T);
+    constexpr int kTerms = kTermsOf<T, O>, kMostSmem = 1024 + kLongStages * kStageBytes + kTerms * (kMaxRank / 64) * kLongRows * 128, kHalf = 113000 /* of an SM, static shared memory left out */;
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
         if ((e = cudaFuncSetAttribute(hy3a_adapters_expand_long_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
-    CUtensorMap tm_b, tm_base, tm_out, tm_base32, tm_out32;
-    constexpr int box = long_stage<O>::box;
-    if (!encode(&tm_b, 3, a.b, 2, a.rank, a.out_width, a.adapters, a.rank, 32, kLongCols) || !encode(&tm_base, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, 1) ||
-        !encode(&tm_out, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, 1) || !encode(&tm_base32, 2, a.base, sizeof(O), a.out_width, a.rows, 1, a.base_stride, box, kLongRows) ||
-        !encode(&tm_out32, 2, a.out, sizeof(O), a.out_width, a.rows, 1, a.out_stride, box, kLongRows)) {
+    CUtensorMap tm_b;
+    if (!encode_columns(&tm_b, a, 4 / sizeof(O))) {
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    const int tiles = a.rows / kLongRows + std::min(a.rows, a.adapters + 1), rank_blocks = (a.rank + 31) / 32, pitch = rank_blocks * 32 + 8;
-    {   hy3a_launch l(dim3(2 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
+    const int tiles = a.rows / kLongRows + std::min(a.rows, a.adapters + 1), rank_blocks = (a.rank + 31) / 32;
+    {   hy3a_launch l(dim3(kLongRows / 16 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
         if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
-    const int across = (a.out_width + kLongCols - 1) / kLongCols;
-    hy3a_launch l(dim3(tiles, (across + kLongTiles - 1) / kLongTiles), dim3(kLongThreads), kRing + (size_t)kTerms * kLongRows * pitch * sizeof(T), stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, tm_base, tm_out, tm_base32, tm_out32, a);
+    /* two blocks an SM while u leaves room for two stages at least */
+    const int u_bytes = kTerms * ((a.rank + 63) / 64) * kLongRows * 128, room = (kHalf - 1024 - u_bytes) / kStageBytes, stages = room < 2 ? kLongStages : std::min(kLongStages, room), blocks = (room < 2 ? 1 : 2) * sms;
+    hy3a_launch l(dim3(std::max(blocks, tiles)), dim3(kLongThreads), 1024 + stages * kStageBytes + u_bytes, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_adapters_expand_long_kernel<T, O>, tm_b, a, stages, blocks);
 }
 
 int check_sizes(const char *who, int rows, int width, int rank) {
@@ -662,8 +671,8 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
                             rows, width, out_width, adapters, rank, cuts_of(width), 0};
     cudaError_t e;
     const char *what = NULL;
-    if (dtype == HY3A_F16) e = base_dtype == HY3A_F32 ? launch<__half, float>(a, dev, stream, &what) : launch<__half, __half>(a, dev, stream, &what);
-    else e = base_dtype == HY3A_F32 ? launch<__nv_bfloat16, float>(a, dev, stream, &what) : launch<__nv_bfloat16, __nv_bfloat16>(a, dev, stream, &what);
+    if (dtype == HY3A_F16) e = base_dtype == HY3A_F32 ? launch<__half, float>(a, dev, sms, stream, &what) : launch<__half, __half>(a, dev, sms, stream, &what);
+    else e = base_dtype == HY3A_F32 ? launch<__nv_bfloat16, float>(a, dev, sms, stream, &what) : launch<__nv_bfloat16, __nv_bfloat16>(a, dev, sms, stream, &what);
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "adapters: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;
 }

@@ -359,9 +359,9 @@ cudaError_t launch(const expert_args &a, const maps &m, int device, int sms, voi
 cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device, int sms, void *stream, const char **what) {
     *what = nullptr;
     maps m;
-    const bool ok = encode(&m.gate, 3, a.gate, 2, a.hidden, a.inter, a.held, a.hidden, 64, 16) && encode(&m.up, 3, a.up, 2, a.hidden, a.inter, a.held, a.hidden, 64, 16) &&
-                    encode(&m.down, 3, a.down, 2, a.inter, a.hidden, a.held, a.inter, 64, 128) && encode(&m.x, 2, a.x, 2, a.hidden, a.rows, 1, a.x_stride, 64, 1) &&
-                    encode(&m.h, 3, a.h, 2, a.inter, a.slots, 1, a.inter, 64, 8);
+    const bool ok = encode(&m.gate, 3, a.gate, a.hidden, a.inter, a.held, a.hidden, 64, 16) && encode(&m.up, 3, a.up, a.hidden, a.inter, a.held, a.hidden, 64, 16) &&
+                    encode(&m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 64, 128) && encode(&m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 64, 1) &&
+                    encode(&m.h, 3, a.h, a.inter, a.slots, 1, a.inter, 64, 8);
     if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
     return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
 }

@@ -56,14 +56,15 @@ static inline encode_tiled_fn encoder() {
     }();
     return fn;
 }
-/* [depth][rows][inner] with dense depths (rank 3), or [rows][inner] (rank 2), rows `stride` elements apart; boxes of box_rows x box_inner */
-static inline bool encode(CUtensorMap *m, int rank, const void *base, int element, size_t inner, size_t rows, size_t depth, size_t stride, int box_inner, int box_rows) {
+/* 16-bit elements, [depth][rows][inner] with dense depths (rank 3), or [rows][inner] (rank 2), rows `stride` elements apart; boxes of box_rows x
+ * box_inner (128 bytes) */
+static inline bool encode(CUtensorMap *m, int rank, const void *base, size_t inner, size_t rows, size_t depth, size_t stride, int box_inner, int box_rows) {
     const encode_tiled_fn enc = encoder();
-    const cuuint64_t dims[3] = {inner, rows, depth}, strides[2] = {stride * element, stride * rows * element};
+    const cuuint64_t dims[3] = {inner, rows, depth}, strides[2] = {2 * stride, 2 * stride * rows};
     const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
     /* (16-bit types are moved alike) */
-    return enc && enc(m, element == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      box_inner * element == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return enc && enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 } /* namespace hy3a_ring */
