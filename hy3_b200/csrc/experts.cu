@@ -53,7 +53,7 @@ template <int BLOCKS>
 __global__ void __launch_bounds__(kGroupThreads) hy3a_experts_plan_kernel(const expert_args a) {
     pdl_release();
     const int tiles = group_items<BLOCKS, 1, false>(
-        a.slots, a.held, kTileSlots, [&](int i) { return local_expert(a, a.ids[i]); },
+        a.slots, a.held, kTileSlots, [&](int i) { const int e = local_expert(a, a.ids[i]); if (e < 0) a.place[i] = -1; return e; },
         [&](int e, int p0, int n, int first, int count) { for (int j = 0; j < count; j++) a.tiles[first + j] = {e, first, count, p0, n}; },
         [&](int i, int p) { a.row[p] = i / a.top_k; a.place[i] = p; });
     if (threadIdx.x == 0 && (BLOCKS == 1 || cluster_rank() == 0)) *a.n_tiles = tiles;
@@ -181,17 +181,17 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
 }
 
 /* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------
- * (The ids, weights and places come from launches that are complete before `down` lets this one begin.)  A warp for a whole row, 32 columns a
- * lane in flight, takes 45 us instead of 41 for 8192 rows of 4096. */
+ * (The weights and places come from launches that are complete before `down` lets this one begin.)  Bound by the chain of its loads: 34 us by itself for
+ * 8192 rows of 4096 with a slot each, whose bytes take 20; 38 with the ids looked at instead of places of -1, more with a warp for a whole row, or the
+ * loads of four slots together (57). */
 template <class T>
 __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
     pdl_release();
     const int row = blockIdx.x, d = (blockIdx.y * 256 + threadIdx.x) * 8, lane = threadIdx.x & 31;
     const size_t s0 = (size_t)row * a.top_k;
-    const bool mine = lane < a.top_k && local_expert(a, a.ids[s0 + lane]) >= 0;
-    const float w_lane = mine ? a.weights[s0 + lane] : 0.f;
-    const int place = mine ? a.place[s0 + lane] : 0;
-    unsigned todo = __ballot_sync(0xffffffffu, mine);
+    const int place = lane < a.top_k ? a.place[s0 + lane] : -1;
+    const float w_lane = lane < a.top_k ? a.weights[s0 + lane] : 0.f;
+    unsigned todo = __ballot_sync(0xffffffffu, place >= 0);
     const bool in = d < a.hidden;
     pdl_wait();
     float sum[8] = {};
@@ -232,8 +232,8 @@ cudaError_t launch_few(const expert_args &a, void *stream) {
 }
 template <class T>
 cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
-    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 57.7 / 70.5, 107 / 113, 155 / 154; fp16, 3 of 10 of
-     * 1032 x 200 for 1, 10 rows 7 / 17, 9.4 / 17.8 */
+    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 55.2 / 67.9, 95 / 110, 138 / 149; fp16, 3 of 10 of
+     * 1032 x 200 for 1, 10 rows 7.5 / 18.4, 9.9 / 16.9 */
     if (a.slots < kFewMost) return launch_few<T>(a, stream);
     cudaError_t e;
     const bool shared = a.slots >= kGroupShared;

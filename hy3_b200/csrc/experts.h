@@ -19,7 +19,7 @@ struct expert_args {
     void *out;
     size_t out_stride;
     int rows, top_k, hidden, inter, held, first, slots;
-    int *row, *place;   /* [slots] rows of the listed slots, expert by expert; where each slot is in that list */
+    int *row, *place;   /* [slots] rows of the listed slots, expert by expert; where each slot is in that list (-1: not) */
     expert_tile *tiles; /* [*n_tiles] */
     int *n_tiles;
     void *h;            /* [slots][inter], in the order of the list (few slots: of the slots) */
