@@ -559,9 +559,10 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
     if (warp == kLongWarps + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * ACC) : "memory");
 }
 
-/* Rows up to which tiles of 8 are taken (us a pass, tiles of 8 / of 32): 64, 128 and 256 rows of as many requests on 8192 -> 4096 20.1 / 21.5, 28.6 / 30.0,
- * 30.4 / 32.0; of a few prompts on 4096 -> 10240 11.9 / 18.5, 17.2 / 19.9, 26.7 / 23.8. */
-constexpr int kShort = 128;
+/* Rows up to which the short kernel is taken (us a pass, short / long): 128, 160, 200 and 256 rows of as many requests on 8192 -> 4096 27.5 / 28.4, 28.9 / 29.1,
+ * 30.5 / 29.7, 32.3 / 30.5; of 7 prompts on 4096 -> 10240 14.5 / 16.0, 15.1 / 16.2, 15.6 / 16.4, 22.6 / 17.9; of 40 adapters on 600 -> 5000 11.5 / 15.4, 14.2 / 16.7,
+ * 18.4 / 17.6, 22.0 / 18.5. */
+constexpr int kShort = 192;
 
 template <class T, class O, bool LISTED>
 cudaError_t launch_short(adapter_args a, bool wide, void *stream) {
