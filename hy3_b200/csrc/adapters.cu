@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_ker
 /* numbers of the rows' type that stand for one of u */
 template <class T, class O> constexpr int kTermsOf = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
 
-/* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into two numbers;
+/* Puts a tile's u into shared memory: the sum of its parts (u(part, row, rank): four ranks), in their order, the scale, the split into TERMS numbers;
  * neighbouring threads share a row, four ranks each at a time.  `any`: the rows that have an adapter (the others get zeros); `ranks`: how many are
  * written, those past the last as zeros; place(term, row, rank): where four go. */
 template <class T, int TOK, int THREADS, int TERMS, int NQ, class U, class P>

@@ -37,7 +37,7 @@ workspace layout(long long slots, int hidden, int inter, int held) {
     w.place = w.row + up256((size_t)slots * 4);
     w.tiles = w.place + up256((size_t)slots * 4);
     w.h = w.tiles + 256 + up256(((size_t)slots / kTileSlots + (slots < held ? slots : held)) * sizeof(expert_tile));     /* their number, then the table */
-    w.q = w.h + up256((size_t)slots * inter * 2);
+    w.q = w.h + up256((size_t)slots * inter * (slots < kFewMost ? 4 : 2));
     w.scale = w.q + up256((size_t)slots * hidden * 2);
     w.total = w.scale + up256((size_t)slots * ((hidden + 31) / 32) * 4);
     return w;
@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(kGroupThreads) hy3a_experts_plan_kernel(const 
 
 /* ---- calls with few slots (at most 31; the others: experts_umma.cu) -----------------------------------------------------
  * Two launches, without a plan: every warp sees all slots.  The first slot of an expert leads, and takes the expert's other slots along, 8 at a
- * time (more than 8 read the weights again, from L2).  Fragments come straight from global memory (layer.h), 8 loads of 32 bytes in
+ * time (more than 8 read the weights again, from L2).  h is kept as two numbers of the rows' type, the rounded value and the rest: with so few
+ * values the error that one leaves is now and then more than half as large again as that of the result's own rounding (1 row of 192 experts 55.2 us a pass with one, 54.8 with two).  Fragments come straight from global memory (layer.h), 8 loads of 32 bytes in
  * flight a lane. */
 constexpr int kFewWarps = 8, kFewLoads = 4 /* k blocks of 64 in flight */;
 /* lane s: expert of slot s (-1: none), the slots of the same expert */
@@ -122,7 +123,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(
             float lo = 0.f, hi = 0.f;
 #pragma unroll
             for (int w = 0; w < kFewWarps; w++) { lo += s_sum[w][c][from]; hi += s_sum[w][2 + c][from]; }
-            if (to >= 0 && m0 + m < M) reinterpret_cast<T *>(a.h)[(size_t)to * M + m0 + m] = type<T>::down(__fdividef(lo, 1.f + __expf(-lo)) * hi);
+            if (to >= 0 && m0 + m < M) {
+                const float v = __fdividef(lo, 1.f + __expf(-lo)) * hi;
+                const T h = type<T>::down(v);
+                T *at = reinterpret_cast<T *>(a.h) + (size_t)to * M + m0 + m;
+                *at = h;
+                at[(size_t)a.slots * M] = type<T>::down(isinf(type<T>::up(h)) ? 0.f : v - type<T>::up(h));
+            }
         }
     }
 }
@@ -138,6 +145,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
     const unsigned any = __ballot_sync(0xffffffffu, mine >= 0), leaders = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(same) - 1);
     const int n = __popc(leaders), shares = n ? max(1, kFewWarps / n) : 1;
     const int K = a.inter, M = a.hidden, m0 = blockIdx.x * 16, step = shares * 64;
+    const size_t rest = (size_t)a.slots * K;
     bool waited = false;
     for (int unit = warp; unit < n * shares; unit += kFewWarps) {
         const int which = unit / shares, share = unit - which * shares, lead = nth_bit(leaders, which);
@@ -148,17 +156,24 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
         for (int base = 0; base < __popc(slots); base += 8) {
             const int s = nth_bit(slots, base + g);
             const T *h = s >= 0 ? reinterpret_cast<const T *>(a.h) + (size_t)s * K : nullptr;
-            float acc[4] = {};
+            float acc[4] = {}, acc_rest[4] = {};
             for (int kb = share * 64; kb < K; kb += step * kFewLoads) {
                 k16 lo[kFewLoads], hi[kFewLoads];
                 few_load<T, WIDE>(lo, hi, w_lo, w_hi, has_lo, has_hi, kb + t * 16, step, K);
                 if (!waited) { pdl_wait(); waited = true; }
-                few_multiply<T, WIDE>(acc, lo, hi, h, kb + t * 16, step, K);
+                const int k = kb + t * 16;
+#pragma unroll
+                for (int u = 0; u < kFewLoads; u++) {
+                    const int left = h ? K - k - u * step : 0;
+                    const k16 v = load16<WIDE, false>(h + k + u * step, left), r = load16<WIDE, false>(h + rest + k + u * step, left);
+                    mma64<T>(acc, lo[u], hi[u], v);
+                    mma64<T>(acc_rest, lo[u], hi[u], r);
+                }
             }
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int to = nth_bit(slots, base + 2 * t + (c & 1));
-                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = acc[c];
+                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = acc[c] + acc_rest[c];
             }
         }
     }
@@ -232,8 +247,8 @@ cudaError_t launch_few(const expert_args &a, void *stream) {
 }
 template <class T>
 cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
-    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 55.2 / 67.9, 95 / 110, 138 / 149; fp16, 3 of 10 of
-     * 1032 x 200 for 1, 10 rows 7.5 / 18.4, 9.9 / 16.9 */
+    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 54.8 / 67.9, 95 / 110, 137 / 149; fp16, 3 of 10 of
+     * 1032 x 200 for 1, 10 rows 8.0 / 18.4, 10.4 / 16.9 */
     if (a.slots < kFewMost) return launch_few<T>(a, stream);
     cudaError_t e;
     const bool shared = a.slots >= kGroupShared;

@@ -22,7 +22,7 @@ struct expert_args {
     int *row, *place;   /* [slots] rows of the listed slots, expert by expert; where each slot is in that list (-1: not) */
     expert_tile *tiles; /* [*n_tiles] */
     int *n_tiles;
-    void *h;            /* [slots][inter], in the order of the list (few slots: of the slots) */
+    void *h;            /* [slots][inter], in the order of the list (few slots: of the slots, and as much again, the rest) */
     short *q;           /* [slots][hidden], in the order of the list: y in 16 bits; with 2^e the power of two below the largest magnitude of 32 neighbours, multiples of 2^(e - 14) */
     float *q_scale;     /* [slots][hidden / 32, rounded up] that scale */
 };
