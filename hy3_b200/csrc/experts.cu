@@ -6,7 +6,7 @@
  * A slot is a (row, choice) pair, t * top_k + j.  Four launches, all on the stream, nothing read back:
  *   1. plan      counts the slots of each held expert, lists them expert by expert, and cuts the lists into tiles;
  *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand);
- *   3. down      y of every listed slot, in fixed point (experts.h);
+ *   3. down      y of every listed slot, fp32;
  *   4. combine   sums a row's slots in the order of j, fp32, and rounds once.
  * Fewer than 32 slots take two, gate / up and down with the sum.
  * Slots whose id is outside [first_expert, first_expert + held) are left out everywhere.  The place of a slot within its expert's list
@@ -28,7 +28,7 @@ constexpr int kFewMost = 32;           /* slots of a call below which its produc
 
 /* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
 struct workspace {
-    size_t row, place, tiles, h, q, scale, total;
+    size_t row, place, tiles, h, y, total;
 };
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 workspace layout(long long slots, int hidden, int inter, int held) {
@@ -37,9 +37,8 @@ workspace layout(long long slots, int hidden, int inter, int held) {
     w.place = w.row + up256((size_t)slots * 4);
     w.tiles = w.place + up256((size_t)slots * 4);
     w.h = w.tiles + 256 + up256(((size_t)slots / kTileSlots + (slots < held ? slots : held)) * sizeof(expert_tile));     /* their number, then the table */
-    w.q = w.h + up256((size_t)slots * inter * (slots < kFewMost ? 4 : 2));
-    w.scale = w.q + up256((size_t)slots * hidden * 2);
-    w.total = w.scale + up256((size_t)slots * ((hidden + 31) / 32) * 4);
+    w.y = w.h + up256((size_t)slots * inter * (slots < kFewMost ? 4 : 2));
+    w.total = w.y + up256((size_t)slots * hidden * 4);
     return w;
 }
 
@@ -196,9 +195,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
 }
 
 /* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------
- * (The weights and places come from launches that are complete before `down` lets this one begin.)  Bound by the chain of its loads: 34 us by itself for
- * 8192 rows of 4096 with a slot each, whose bytes take 20; 38 with the ids looked at instead of places of -1, more with a warp for a whole row, or the
- * loads of four slots together (57). */
+ * (The weights and places come from launches that are complete before `down` lets this one begin.)  Bound by the chain of its loads and by memory: 8192 rows
+ * of 4096 with a slot each are 201 MB. */
 template <class T>
 __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
     pdl_release();
@@ -217,17 +215,9 @@ __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_
         const float w = __shfl_sync(0xffffffffu, w_lane, j);
         const size_t p = (size_t)__shfl_sync(0xffffffffu, place, j);
         if (!in) continue;
-        const uint4 v = *reinterpret_cast<const uint4 *>(a.q + p * a.hidden + d);
-        const float scale = a.q_scale[p * ((a.hidden + 31) >> 5) + (d >> 5)];
-        const unsigned u[4] = {v.x, v.y, v.z, v.w};
-        if (scale >= 0.f) {
-            const float ws = w * scale;
-#pragma unroll
-            for (int i = 0; i < 4; i++) { sum[2 * i] += ws * (float)(short)(u[i] & 0xffff); sum[2 * i + 1] += ws * (float)(short)(u[i] >> 16); }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) { sum[2 * i] += w * __uint_as_float(u[i] << 16); sum[2 * i + 1] += w * __uint_as_float(u[i] & 0xffff0000u); }
-        }
+        const float4 *const y = reinterpret_cast<const float4 *>(a.y + p * a.hidden + d), lo = y[0], hi = y[1];
+        sum[0] += w * lo.x; sum[1] += w * lo.y; sum[2] += w * lo.z; sum[3] += w * lo.w;
+        sum[4] += w * hi.x; sum[5] += w * hi.y; sum[6] += w * hi.z; sum[7] += w * hi.w;
     }
     if (!in) return;
     T o[8];
@@ -302,7 +292,7 @@ int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int i
     if ((rc = hy3a_layer_device("experts", &dev, &sms))) return rc;
     char *b = (char *)work;
     expert_args a = {x, x_stride, ids, weights, gate, up, down, out, out_stride, rows, top_k, hidden, inter, held, first_expert, rows * top_k,
-                     (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles), b + w.h, (short *)(b + w.q), (float *)(b + w.scale)};
+                     (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles), b + w.h, (float *)(b + w.y)};
     const char *what = NULL;
     const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, dev, sms, stream, &what) : launch<__nv_bfloat16>(a, dev, sms, stream, &what);
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", what ? what : cudaGetErrorString(e));

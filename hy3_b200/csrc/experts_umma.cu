@@ -82,12 +82,10 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 /* 32 bytes */
-__device__ __forceinline__ void store32(void *p, const unsigned (&v)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+__device__ __forceinline__ void store32(void *p, const float4 &a, const float4 &b) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(a.x), "f"(a.y), "f"(a.z), "f"(a.w), "f"(b.x), "f"(b.y), "f"(b.z), "f"(b.w) : "memory");
 }
-__device__ __forceinline__ short to_short(float v) { short r; asm("cvt.rni.sat.s16.f32 %0, %1;" : "=h"(r) : "f"(v)); return r; }
 
 /* what a tile is: its expert, weight rows from m0 (gate / up: pairs) and n of the listed slots from p0 */
 struct where { int e, m0, p0, n; };
@@ -260,13 +258,11 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         }
     } else {
         /* ===================== epilogue: warp w has weight rows 32 (w % 4) .. + 31 of the CTA, and every other 16 slots =====================
-         * A lane has a weight row, and what is stored is a slot's row: 16 slots at a time turn in a patch of shared memory, and leave as 16 or
-         * 32 bytes a lane (a store for each slot, of 32 neighbouring values, takes the warp 90 clocks beside the copies and products). */
+         * A lane has a weight row, and what is stored is a slot's row: 16 slots at a time turn in a patch of shared memory, and leave as 32 bytes of y or 16 of
+         * h a lane (a store for each slot, of 32 neighbouring values, takes the warp 90 clocks beside the copies and products). */
         unsigned buf = 0, tph = 0;
         const int quarter = warp & 3, sl = lane & 15, half = lane >> 4;
         uint8_t *patch = sm + kOffPatch + warp * kPatch;
-        const int scales = (a.hidden + 31) >> 5;
-        const bool whole = !(a.hidden & 15);
         tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
         for (where w; walk.take(w);) {
             if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, g_err, 23u)) break;
@@ -275,41 +271,17 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             for (int c0 = (warp >> 2) * 16; c0 < w.n; c0 += 32) {
                 unsigned v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * 256u + c0, v);
-                const int p = w.p0 + c0 + sl;
                 if (DOWN) {
-                    const bool has = m0 + lane < a.hidden;
 #pragma unroll
-                    for (int j = 0; j < 16; j++) *reinterpret_cast<float *>(patch + j * kPitch + lane * 4) = has ? __uint_as_float(v[j]) : 0.f;
+                    for (int j = 0; j < 16; j++) *reinterpret_cast<unsigned *>(patch + j * kPitch + lane * 4) = v[j];
                     __syncwarp();
-                    /* half a slot's 32 values */
-                    float f[16], top = 0.f;
+                    /* four lanes a line of 128 bytes */
+                    const int d = m0 + (lane & 3) * 8;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float4 x = *reinterpret_cast<const float4 *>(patch + sl * kPitch + half * 64 + j * 16);
-                        f[4 * j] = x.x; f[4 * j + 1] = x.y; f[4 * j + 2] = x.z; f[4 * j + 3] = x.w;
-                        top = max_nan(max_nan(top, max_nan(fabsf(x.x), fabsf(x.y))), max_nan(fabsf(x.z), fabsf(x.w)));
-                    }
-                    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const unsigned ex = __float_as_uint(top) >> 23;                  /* 2^(ex - 127) <= it */
-                    const bool nil = ex < 27, odd = ex >= 255;
-                    const float times = __uint_as_float((nil || odd ? 0u : 268u - ex) << 23);
-                    unsigned o[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = (unsigned)(unsigned short)to_short(f[2 * j] * times) | ((unsigned)(unsigned short)to_short(f[2 * j + 1] * times) << 16);
-                    if (__any_sync(0xffffffffu, odd)) {
-                        if (odd) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) o[j] = (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * j])) | ((unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * j + 1])) << 16);
-                        }
-                    }
-                    if (c0 + sl < w.n && m0 < a.hidden) {
-                        short *q = a.q + (size_t)p * a.hidden + m0 + half * 16;
-                        if (whole && m0 + half * 16 + 16 <= a.hidden) store32(q, o);
-                        else {                                                      /* rows of 16 bytes only, or the last of them */
-                            if (m0 + half * 16 + 8 <= a.hidden) *reinterpret_cast<uint4 *>(q) = make_uint4(o[0], o[1], o[2], o[3]);
-                            if (m0 + half * 16 + 16 <= a.hidden) *reinterpret_cast<uint4 *>(q + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-                        }
-                        if (half == 0) a.q_scale[(size_t)p * scales + (m0 >> 5)] = odd ? -1.f : __uint_as_float((nil ? 0u : ex - 14u) << 23);
+                    for (int i = 0; i < 2; i++) {
+                        const int j = i * 8 + (lane >> 2);
+                        const float4 *const from = reinterpret_cast<const float4 *>(patch + j * kPitch + (lane & 3) * 32);
+                        if (c0 + j < w.n && d < a.hidden) store32(a.y + (size_t)(w.p0 + c0 + j) * a.hidden + d, from[0], from[1]);
                     }
                 } else {
                     /* lanes below 16 have the gate, the others the up of one pair; of two slots each half finishes one */
@@ -321,7 +293,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
                     }
                     __syncwarp();
                     const uint4 o = *reinterpret_cast<const uint4 *>(patch + sl * 48 + half * 16);
-                    if (c0 + sl < w.n && m0 + half * 8 < a.inter) *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.h) + (size_t)p * a.inter + m0 + half * 8) = o;
+                    if (c0 + sl < w.n && m0 + half * 8 < a.inter) *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.h) + (size_t)(w.p0 + c0 + sl) * a.inter + m0 + half * 8) = o;
                 }
                 __syncwarp();
             }
