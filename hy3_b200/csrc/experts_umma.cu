@@ -116,18 +116,20 @@ struct tile_walk {
 };
 
 /* The steps of one tile for one producer warp: its weight box, and MINE of the tile's slot rows (gathers of 4, or boxes of 8), whose number is a
- * constant here so that the row numbers stay where the copy instruction reads them from: looked up in every step, a gather cost 52 clocks. */
+ * constant here so that the row numbers stay where the copy instruction reads them from: looked up in every step, a gather cost 52 clocks.
+ * Each warp has a weight box in every step, so that no stage is filled, and none given back, before each has seen the stage's last phase end: one that
+ * only waits may fall a ring behind, and a wait that has missed a phase ends with the next but one, or never. */
 struct ring_state { unsigned st, ph; };
 template <bool DOWN, int MINE>
 __device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, const CUtensorMap *tm_rows, unsigned sbase, unsigned bar0, volatile int *s_abort, int steps, int ahead /* steps whose weights are under way */, unsigned bytes /* 0: not the one that counts */,
                                         int part, int m, int e, const int4 (&row)[4], unsigned lead) {
     unsigned st = q.st, ph = q.ph;
     for (int s = 0; s < steps; s++) {
-        if (!mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
+        /* (a stage whose weights are under way has not been used before) */
+        if (s >= ahead && !mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
         const unsigned full = cluster_addr(bar0 + 8u * (B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
         if (bytes && lead && s >= ahead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
-        if (!DOWN) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
-        else if (part == 0 && s >= ahead) tma_box(sa, tm_w, full, s * 64, m, e, lead);
+        if (s >= ahead) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
             if (DOWN) tma_box(sb + (part + kProducers * i) * 1024, tm_rows, full, s * 64, row[i].x, 0, lead);
@@ -200,15 +202,14 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             }
             const unsigned bytes = part == 0 && rank == 0 ? 2 * kABytes + N * 128 : 0;
             const CUtensorMap *tm = !DOWN && (part & 1) ? &tm_w1 : &tm_w0;
-            const int m = DOWN ? w.m0 + (int)rank * 128 : w.m0 + (int)rank * 64 + (part >> 1) * 16;
+            const int m = w.m0 + (DOWN ? (int)rank * 128 + part * 16 : (int)rank * 64 + (part >> 1) * 16);
             if (DOWN && walk.t == pair) {
                 ahead = min(steps, kStages);
-                if (part == 0)
-                    for (int s = 0; s < ahead; s++) {
-                        const unsigned full = cluster_addr(BAR(B_FULL + s), 0);
-                        if (bytes && lead) mbar_expect_tx(BAR(B_FULL + s), bytes);
-                        tma_box(sbase + s * (kABytes + kBBytes), tm, full, s * 64, m, w.e, lead);
-                    }
+                for (int s = 0; s < ahead; s++) {
+                    const unsigned full = cluster_addr(BAR(B_FULL + s), 0);
+                    if (bytes && lead) mbar_expect_tx(BAR(B_FULL + s), bytes);
+                    tma_box(sbase + s * (kABytes + kBBytes) + part * 2048, tm, full, s * 64, m, w.e, lead);
+                }
                 pdl_wait();
             }
             bool ok;
@@ -336,7 +337,7 @@ cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device
     *what = nullptr;
     maps m;
     const bool ok = encode(&m.gate, 3, a.gate, a.hidden, a.inter, a.held, a.hidden, 64, 16) && encode(&m.up, 3, a.up, a.hidden, a.inter, a.held, a.hidden, 64, 16) &&
-                    encode(&m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 64, 128) && encode(&m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 64, 1) &&
+                    encode(&m.down, 3, a.down, a.inter, a.hidden, a.held, a.inter, 64, 16) && encode(&m.x, 2, a.x, a.hidden, a.rows, 1, a.x_stride, 64, 1) &&
                     encode(&m.h, 3, a.h, a.inter, a.slots, 1, a.inter, 64, 8);
     if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
     return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
