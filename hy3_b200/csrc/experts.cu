@@ -5,10 +5,11 @@
  *
  * A slot is a (row, choice) pair, t * top_k + j.  Four launches, all on the stream, nothing read back:
  *   1. plan      counts the slots of each held expert, lists them expert by expert, and cuts the lists into tiles;
- *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand);
+ *   2. gate/up   h = silu(gate x) * (up x) of every listed slot, rounded once to the rows' type (it is the next product's operand; fp16 rows take a launch
+ *                for that, which brings each slot's h near the top of the type's range first: products of two sums may be beyond it, and below);
  *   3. down      y of every listed slot, fp32;
  *   4. combine   sums a row's slots in the order of j, fp32, and rounds once.
- * Fewer than 32 slots take two, gate / up and down with the sum.
+ * Fewer than 32 slots take no plan: gate / up (and the range), and down with the sum.
  * Slots whose id is outside [first_expert, first_expert + held) are left out everywhere.  The place of a slot within its expert's list
  * comes from an atomic and may differ from run to run; no sum depends on it, so results do not.
  */
@@ -28,7 +29,7 @@ constexpr int kFewMost = 32;           /* slots of a call below which its produc
 
 /* ---- workspace: offsets of its parts, in bytes ------------------------------------------------------------------------ */
 struct workspace {
-    size_t row, place, tiles, h, y, total;
+    size_t row, place, tiles, h, back, y, total;
 };
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 workspace layout(long long slots, int hidden, int inter, int held) {
@@ -37,8 +38,9 @@ workspace layout(long long slots, int hidden, int inter, int held) {
     w.place = w.row + up256((size_t)slots * 4);
     w.tiles = w.place + up256((size_t)slots * 4);
     w.h = w.tiles + 256 + up256(((size_t)slots / kTileSlots + (slots < held ? slots : held)) * sizeof(expert_tile));     /* their number, then the table */
-    w.y = w.h + up256((size_t)slots * inter * (slots < kFewMost ? 4 : 2));
-    w.total = w.y + up256((size_t)slots * hidden * 4);
+    w.back = w.h + up256((size_t)slots * inter * (slots < kFewMost ? 4 : 2));
+    w.y = w.back + up256((size_t)slots * 4);
+    w.total = w.y + up256((size_t)slots * std::max(hidden, inter) * 4);        /* y, and before it h in fp32 */
     return w;
 }
 
@@ -58,11 +60,63 @@ __global__ void __launch_bounds__(kGroupThreads) hy3a_experts_plan_kernel(const 
     if (threadIdx.x == 0 && (BLOCKS == 1 || cluster_rank() == 0)) *a.n_tiles = tiles;
 }
 
+/* ---- fp16 rows, between gate / up and down: h as fp16 holds it ------------------------------------------------------------
+ * The products of two sums may be beyond the type's range, or so small that it keeps few of their bits, where the result is neither.  A warp takes a slot (a
+ * block, up to two slots an SM), and brings its largest value into [2^14, 2^15) on the way to fp16: 2^-38 of it is kept.  us a pass, without / with it: 1 row
+ * of 192 experts 54.1 / 57.0, 8 rows 313 / 318, 2048 rows 1277 / 1344, 8192 rows on 24 held experts 377 / 413, 333 rows of 10 small ones 22.6 / 27.0.  Two blocks an SM find room beside gate / up, and
+ * are there when it ends. */
+/* the larger of m and |v|, if that is finite */
+__device__ __forceinline__ float most_finite(float m, float v) { return fabsf(v) <= 3.402823466e38f ? fmaxf(m, fabsf(v)) : m; }
+constexpr int kRangeThreads = 256, kRangeBlocks = 2 /* an SM */;
+/* EACH: threads of a slot, 32 or, if there are no more slots than blocks, all of a block */
+template <bool FEW, int EACH>
+__global__ void __launch_bounds__(kRangeThreads) hy3a_experts_range_kernel(const expert_args a) {
+    pdl_release();                          /* (gate / up let this launch begin behind its own wait: the plan is complete, here and for `down`) */
+    const int sub = threadIdx.x % EACH, quads = a.inter >> 2, tiles = FEW ? 0 : *a.n_tiles;
+    const int listed = FEW ? a.slots : (tiles ? a.tiles[tiles - 1].p0 + a.tiles[tiles - 1].count : 0);      /* (few: those without an expert too, nobody reads theirs) */
+    pdl_wait();
+    for (int p = (blockIdx.x * kRangeThreads + threadIdx.x) / EACH; p < listed; p += gridDim.x * kRangeThreads / EACH) {
+        const float4 *const from = reinterpret_cast<const float4 *>(a.wide + (size_t)p * a.inter);
+        float most = 0.f;
+#pragma unroll 4
+        for (int i = sub; i < quads; i += EACH) {
+            const float4 v = from[i];
+            most = most_finite(most_finite(most_finite(most_finite(most, v.x), v.y), v.z), v.w);
+        }
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+        if (EACH > 32) {
+            __shared__ float s_most[kRangeThreads / 32];
+            if ((sub & 31) == 0) s_most[sub >> 5] = most;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kRangeThreads / 32; w++) most = fmaxf(most, s_most[w]);
+        }
+        /* 2^n that does it, at most 2^100; and its inverse */
+        const int n = most > 0.f ? min(141 - (int)(__float_as_uint(most) >> 23), 100) : 0;
+        const float by = __uint_as_float((unsigned)(127 + n) << 23);
+        if (sub == 0) a.back[p] = __uint_as_float((unsigned)(127 - n) << 23);
+        __half *const h = reinterpret_cast<__half *>(a.h) + (size_t)p * a.inter;
+#pragma unroll 4
+        for (int i = sub; i < quads; i += EACH) {
+            const float4 v = from[i];
+            const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+            __half one[4], rest[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                one[z] = __float2half_rn(f[z]);
+                rest[z] = __float2half_rn(isinf(f[z]) ? 0.f : f[z] - __half2float(one[z]));
+            }
+            *reinterpret_cast<uint2 *>(h + 4 * i) = *reinterpret_cast<const uint2 *>(one);
+            if (FEW) *reinterpret_cast<uint2 *>(h + (size_t)a.slots * a.inter + 4 * i) = *reinterpret_cast<const uint2 *>(rest);
+        }
+    }
+}
+
 /* ---- calls with few slots (at most 31; the others: experts_umma.cu) -----------------------------------------------------
- * Two launches, without a plan: every warp sees all slots.  The first slot of an expert leads, and takes the expert's other slots along, 8 at a
- * time (more than 8 read the weights again, from L2).  h is kept as two numbers of the rows' type, the rounded value and the rest: with so few
- * values the error that one leaves is now and then more than half as large again as that of the result's own rounding (1 row of 192 experts 55.2 us a pass with one, 54.8 with two).  Fragments come straight from global memory (layer.h), 8 loads of 32 bytes in
- * flight a lane. */
+ * Two launches (fp16 rows three), without a plan: every warp sees all slots.  The first slot of an expert leads, and takes the expert's other slots along, 8 at a
+ * time (more than 8 read the weights again, from L2).  h enters the second product as two numbers of the rows' type, the rounded value and the
+ * rest: with so few values the error that one number leaves is now and then more than half as large again as that of the result's own rounding.
+ * Fragments come straight from global memory (layer.h), 8 loads of 32 bytes in flight a lane. */
 constexpr int kFewWarps = 8, kFewLoads = 4 /* k blocks of 64 in flight */;
 /* lane s: expert of slot s (-1: none), the slots of the same expert */
 __device__ __forceinline__ int few_slots(const expert_args &a, unsigned &same) {
@@ -124,10 +178,13 @@ __global__ void __launch_bounds__(32 * kFewWarps, 3) hy3a_experts_few_up_kernel(
             for (int w = 0; w < kFewWarps; w++) { lo += s_sum[w][c][from]; hi += s_sum[w][2 + c][from]; }
             if (to >= 0 && m0 + m < M) {
                 const float v = __fdividef(lo, 1.f + __expf(-lo)) * hi;
-                const T h = type<T>::down(v);
-                T *at = reinterpret_cast<T *>(a.h) + (size_t)to * M + m0 + m;
-                *at = h;
-                at[(size_t)a.slots * M] = type<T>::down(isinf(type<T>::up(h)) ? 0.f : v - type<T>::up(h));
+                const size_t at = (size_t)to * M + m0 + m;
+                if (type<T>::code == HY3A_F16) a.wide[at] = v;
+                else {
+                    const T h = type<T>::down(v);
+                    reinterpret_cast<T *>(a.h)[at] = h;
+                    reinterpret_cast<T *>(a.h)[at + (size_t)a.slots * M] = type<T>::down(isinf(type<T>::up(h)) ? 0.f : v - type<T>::up(h));
+                }
             }
         }
     }
@@ -172,7 +229,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int to = nth_bit(slots, base + 2 * t + (c & 1));
-                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = acc[c] + acc_rest[c];
+                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = (type<T>::code == HY3A_F16 ? a.back[to] : 1.f) * (acc[c] + acc_rest[c]);
             }
         }
     }
@@ -232,6 +289,11 @@ cudaError_t launch_few(const expert_args &a, void *stream) {
     const bool wide_up = wide_rows({a.x, a.gate, a.up}, {a.x_stride, (size_t)a.hidden}), wide_down = wide_rows({a.down}, {(size_t)a.inter});
     const cudaError_t e = wide_up ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_few_up_kernel<T, false>, a);
     if (e != cudaSuccess) return e;
+    if (type<T>::code == HY3A_F16) {
+        hy3a_launch r(dim3(a.slots), dim3(kRangeThreads), 0, stream);
+        const cudaError_t e = cudaLaunchKernelEx(&r.cfg, hy3a_experts_range_kernel<true, kRangeThreads>, a);
+        if (e != cudaSuccess) return e;
+    }
     hy3a_launch d(dim3((a.hidden + 15) / 16), dim3(32 * kFewWarps), 0, stream);
     return wide_down ? cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T, true>, a) : cudaLaunchKernelEx(&d.cfg, hy3a_experts_few_down_kernel<T, false>, a);
 }
@@ -264,6 +326,12 @@ int check_sizes(const char *who, int rows, int top_k, int hidden, int inter, int
 
 } /* namespace */
 
+cudaError_t hy3a_experts_launch_range(const expert_args &a, int sms, void *stream) {
+    const int most = kRangeBlocks * sms, each = kRangeThreads / 32;
+    hy3a_launch l(dim3(a.slots <= most ? a.slots : std::min((a.slots + each - 1) / each, most)), dim3(kRangeThreads), 0, stream);
+    return a.slots <= most ? cudaLaunchKernelEx(&l.cfg, hy3a_experts_range_kernel<false, kRangeThreads>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_experts_range_kernel<false, 32>, a);
+}
+
 extern "C" {
 
 size_t hy3a_experts_workspace(int rows, int top_k, int hidden, int inter, int held) {
@@ -292,7 +360,7 @@ int hy3a_experts(void *stream, int dtype, int rows, int top_k, int hidden, int i
     if ((rc = hy3a_layer_device("experts", &dev, &sms))) return rc;
     char *b = (char *)work;
     expert_args a = {x, x_stride, ids, weights, gate, up, down, out, out_stride, rows, top_k, hidden, inter, held, first_expert, rows * top_k,
-                     (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles), b + w.h, (float *)(b + w.y)};
+                     (int *)(b + w.row), (int *)(b + w.place), (expert_tile *)(b + w.tiles + 256), (int *)(b + w.tiles), b + w.h, (float *)(b + w.y), (float *)(b + w.back), (float *)(b + w.y)};
     const char *what = NULL;
     const cudaError_t e = dtype == HY3A_F16 ? launch<__half>(a, dev, sms, stream, &what) : launch<__nv_bfloat16>(a, dev, sms, stream, &what);
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "experts: %s", what ? what : cudaGetErrorString(e));

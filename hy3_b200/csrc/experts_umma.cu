@@ -9,7 +9,7 @@
  *             (tile::gather4), rows of h, which lie in the order of the list, as boxes of 8, all with 128-byte swizzle; the byte counts of
  *             both CTAs go to the leader's barriers;
  *   warp 16   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step; commits reach both CTAs;
- *   warps 0-7 epilogue: tcgen05.ld, then h or y.
+ *   warps 0-7 epilogue: tcgen05.ld, then h (of fp16 rows in fp32, for the launch that brings it into range) or y.
  * Gate / up: 16 gate rows and the 16 up rows of the same index alternate in the tile, so that a pair's halves lie 16 lanes apart in one
  * warp and meet in a shuffle.
  *
@@ -24,6 +24,7 @@
  * through, and TMEM is always released.
  */
 #include <atomic>
+#include <type_traits>
 
 #include "experts.h"
 #include "ring.cuh"
@@ -174,8 +175,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *s_tmem;
-    /* Gate / up lets the next launch begin behind its own wait: that one finds the plan complete, and fetches its first weights before it waits
-     * for h. */
+    /* Gate / up lets the next launch begin behind its own wait (and so does the one between the two): `down` finds the plan complete, and fetches its first
+     * weights before it waits for h. */
     if (!DOWN) pdl_wait();
     pdl_release();
     const int total = *a.n_tiles * m_tiles;
@@ -259,8 +260,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         }
     } else {
         /* ===================== epilogue: warp w has weight rows 32 (w % 4) .. + 31 of the CTA, and every other 16 slots =====================
-         * A lane has a weight row, and what is stored is a slot's row: 16 slots at a time turn in a patch of shared memory, and leave as 32 bytes of y or 16 of
-         * h a lane (a store for each slot, of 32 neighbouring values, takes the warp 90 clocks beside the copies and products). */
+         * A lane has a weight row, and what is stored is a slot's row: 16 slots at a time turn in a patch of shared memory, and leave as 32 bytes of y (or of h in fp32) or
+         * 16 of h a lane (a store for each slot, of 32 neighbouring values, takes the warp 90 clocks beside the copies and products). */
         unsigned buf = 0, tph = 0;
         const int quarter = warp & 3, sl = lane & 15, half = lane >> 4;
         uint8_t *patch = sm + kOffPatch + warp * kPatch;
@@ -282,19 +283,31 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
                     for (int i = 0; i < 2; i++) {
                         const int j = i * 8 + (lane >> 2);
                         const float4 *const from = reinterpret_cast<const float4 *>(patch + j * kPitch + (lane & 3) * 32);
-                        if (c0 + j < w.n && d < a.hidden) store32(a.y + (size_t)(w.p0 + c0 + j) * a.hidden + d, from[0], from[1]);
+                        if (c0 + j >= w.n || d >= a.hidden) continue;
+                        float4 lo = from[0], hi = from[1];
+                        if (type<T>::code == HY3A_F16) {
+                            const float by = a.back[w.p0 + c0 + j];
+                            lo.x *= by; lo.y *= by; lo.z *= by; lo.w *= by; hi.x *= by; hi.y *= by; hi.z *= by; hi.w *= by;
+                        }
+                        store32(a.y + (size_t)(w.p0 + c0 + j) * a.hidden + d, lo, hi);
                     }
                 } else {
                     /* lanes below 16 have the gate, the others the up of one pair; of two slots each half finishes one */
+                    using H = typename std::conditional<type<T>::code == HY3A_F16, float, T>::type;       /* what is stored */
+                    constexpr int kPitchH = 16 * sizeof(H) + 16;
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
                         const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(half ? v[j] : v[j + 1]), 16);
                         const float g = half ? other : __uint_as_float(v[j]), u = half ? __uint_as_float(v[j + 1]) : other;
-                        *reinterpret_cast<T *>(patch + (j + half) * 48 + sl * 2) = type<T>::down(__fdividef(g, 1.f + __expf(-g)) * u);
+                        *reinterpret_cast<H *>(patch + (j + half) * kPitchH + sl * sizeof(H)) = type<H>::down(__fdividef(g, 1.f + __expf(-g)) * u);
                     }
                     __syncwarp();
-                    const uint4 o = *reinterpret_cast<const uint4 *>(patch + sl * 48 + half * 16);
-                    if (c0 + sl < w.n && m0 + half * 8 < a.inter) *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.h) + (size_t)(w.p0 + c0 + sl) * a.inter + m0 + half * 8) = o;
+                    if (c0 + sl < w.n && m0 + half * 8 < a.inter) {
+                        const uint8_t *const from = patch + sl * kPitchH + half * 8 * sizeof(H);
+                        const size_t at = (size_t)(w.p0 + c0 + sl) * a.inter + m0 + half * 8;
+                        if (type<T>::code == HY3A_F16) store32(a.wide + at, *reinterpret_cast<const float4 *>(from), *reinterpret_cast<const float4 *>(from + 16));
+                        else *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.h) + at) = *reinterpret_cast<const uint4 *>(from);
+                    }
                 }
                 __syncwarp();
             }
@@ -327,6 +340,7 @@ cudaError_t launch(const expert_args &a, const maps &m, int device, int sms, voi
     const dim3 grid(sms & ~1);
     {   hy3a_launch l(grid, dim3(kThreads), kSmem, stream);
         if ((e = cudaLaunchKernelEx(&l.cfg, hy3a_experts_umma_kernel<T, false>, m.gate, m.up, m.x, a)) != cudaSuccess) return e; }
+    if (type<T>::code == HY3A_F16 && (e = hy3a_experts_launch_range(a, sms, stream)) != cudaSuccess) return e;
     hy3a_launch l(grid, dim3(kThreads), kSmem, stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_experts_umma_kernel<T, true>, m.down, m.down, m.h, a);
 }

@@ -269,7 +269,8 @@ int hy3a_route(void *stream, int dtype, int rows, int experts, const void *logit
  * e = ids[t][j], sums in fp32.  The experts [first_expert, first_expert + held) are held here; slots with another id (-1 among them) are
  * left out, and a row without any is 0: ranks that split the experts add their outputs up.  dtype HY3A_F16 or HY3A_BF16 is that of x
  * [rows][hidden], out and the weights gate, up [held][inter][hidden] and down [held][hidden][inter] (dense); the gated products are
- * rounded to it once between the two (calls of fewer than 32 slots keep twice its bits).  hidden and inter are multiples of 8 up to 65536,
+ * rounded to it once between the two, fp16 on a power-of-two scale of each slot, so that they may lie beyond the type's range (calls of fewer than 32 slots
+ * keep twice its bits: a row's result may differ in its last bits between a call of 31 slots and one of 32).  hidden and inter are multiples of 8 up to 65536,
  * row strides multiples of 8, held and top_k at most 1024 and 32; pointers 16-byte aligned, the workspace (hy3a_experts_workspace bytes, 0 on bad sizes) 256.  out must not overlap x.
  * The result depends on the inputs alone, not on how slots are ordered within an expert.                                     */
 size_t hy3a_experts_workspace(int rows, int top_k, int hidden, int inter, int held);
