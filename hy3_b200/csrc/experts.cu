@@ -229,7 +229,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int to = nth_bit(slots, base + 2 * t + (c & 1));
-                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = (type<T>::code == HY3A_F16 ? a.back[to] : 1.f) * (acc[c] + acc_rest[c]);
+                /* (an infinite weight meets both numbers of h, whose signs may differ: then the first has it) */
+                const float y = fabsf(acc[c]) <= 3.402823466e38f ? acc[c] + acc_rest[c] : acc[c];
+                if (to >= 0) s_y[share][to][g + (c >> 1) * 8] = type<T>::code == HY3A_F16 ? a.back[to] * y : y;
             }
         }
     }
