@@ -3,9 +3,10 @@
  *
  *      out[t] = base[t] + scales[a] * B_a (A_a x[t]),   a = ids[t]
  *
- * u = A_a x enters the second product as two numbers of the rows' type, a rounded value and the rest, which leave 2^-17 (bf16) or 2^-22 (fp16) of a row's
- * largest; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.  bf16 rows on an fp32 base take a
- * third number (2^-25): two left an error of 1e-6 of the result.
+ * u = A_a x enters the second product as two numbers of the rows' type, the next smaller value and the rest, which leave 2^-16 (bf16) or 2^-22 (fp16) of a
+ * row's largest; each row of u is brought to a largest value in [1, 2) first and back afterwards, which keeps fp16 in range.  bf16 rows on an fp32 base take a
+ * third number (2^-24): two left an error of 1e-6 of the result.  The numbers have the sign of u, and none is 0 unless u is: an infinite weight meets each of
+ * them, and gives the infinity that it gives with u (rounded to nearest they leave half as much, and NaN there).
  *
  * Rows are worked on in tiles of one adapter, so that its weights are read once for all of a tile, whatever the order of the rows:
  *   up to 8 rows        one launch: clusters of blocks for each adapter that occurs (short kernel);
@@ -137,6 +138,19 @@ __global__ void __launch_bounds__(32 * kReduceWarps, 2) hy3a_adapters_reduce_ker
     }
 }
 
+/* the value of the rows' type next below |f| with f's sign, but not 0, and what it leaves of f (0, infinities and NaN: themselves; an infinity leaves 1) */
+template <class T> __device__ __forceinline__ T below(float &f) {
+    T t = type<T>::cut(f);
+    if (type<T>::up(t) == f && f != 0.f && !isinf(f)) t = type<T>::step_down(t);
+    if (type<T>::up(t) == 0.f && f != 0.f) { t = type<T>::least(f); f = 2.f * type<T>::up(t); }
+    f = isinf(f) ? copysignf(1.f, f) : f - type<T>::up(t);
+    return t;
+}
+/* the nearest one, but 0 of 0 alone */
+template <class T> __device__ __forceinline__ T nearest(float f) {
+    const T t = type<T>::down(f);
+    return type<T>::up(t) == 0.f && f != 0.f ? type<T>::least(f) : t;
+}
 /* numbers of the rows' type that stand for one of u */
 template <class T, class O> constexpr int kTermsOf = sizeof(O) == 4 && type<T>::code == HY3A_BF16 ? 3 : 2;
 
@@ -170,11 +184,10 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
     }
 #pragma unroll
     for (int o = 1; o < PT; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    /* 2^-floor(log2 m) of the largest finite value; subnormal or no values stay as they are */
-    const int ex = (int)(__float_as_uint(m) >> 23);
-    const bool usual = ex > 0 && ex < 254;
-    const float to = usual ? __uint_as_float((unsigned)(254 - ex) << 23) : 1.f;
-    if (sub == 0) s_back[i] = usual ? __uint_as_float((unsigned)ex << 23) : 1.f;
+    /* 2^-floor(log2 m) of the largest finite value, as far as fp32 has that and its inverse (no value: 1) */
+    const unsigned ex = m > 0.f ? (unsigned)min(max((int)(254u - (__float_as_uint(m) >> 23)), 1), 253) : 127u;
+    const float to = __uint_as_float(ex << 23);
+    if (sub == 0) s_back[i] = __uint_as_float((254u - ex) << 23);
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
         const int r = 4 * (sub + PT * q);
@@ -184,10 +197,7 @@ __device__ __forceinline__ void put_u_of(const adapter_args &a, const U &u, int 
             for (int k = 0; k < TERMS; k++) {
                 T part[4];
 #pragma unroll
-                for (int z = 0; z < 4; z++) {
-                    part[z] = type<T>::down(f[z]);
-                    f[z] = isinf(type<T>::up(part[z])) ? 0.f : f[z] - type<T>::up(part[z]);
-                }
+                for (int z = 0; z < 4; z++) part[z] = k < TERMS - 1 ? below<T>(f[z]) : nearest<T>(f[z]);
                 *reinterpret_cast<uint2 *>(place(k, i, r)) = *reinterpret_cast<const uint2 *>(part);
             }
         }

@@ -52,6 +52,9 @@ template <> struct type<__nv_bfloat16> {
     static constexpr int code = HY3A_BF16;
     static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ __nv_bfloat16 cut(float v) { return __float2bfloat16_rz(v); }
+    static __device__ __forceinline__ __nv_bfloat16 step_down(__nv_bfloat16 v) { return __ushort_as_bfloat16(__bfloat16_as_ushort(v) - 1); }      /* next towards 0, of what is not 0 */
+    static __device__ __forceinline__ __nv_bfloat16 least(float v) { return __ushort_as_bfloat16(v < 0.f ? 0x8080 : 0x0080); }                      /* smallest normal number of v's sign */
     static __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -61,6 +64,9 @@ template <> struct type<__half> {
     static constexpr int code = HY3A_F16;
     static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ __half cut(float v) { return __float2half_rz(v); }
+    static __device__ __forceinline__ __half step_down(__half v) { return __ushort_as_half(__half_as_ushort(v) - 1); }
+    static __device__ __forceinline__ __half least(float v) { return __ushort_as_half(v < 0.f ? 0x8001 : 0x0001); }      /* (subnormal: the normal ones begin at 2^-14) */
     static __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
