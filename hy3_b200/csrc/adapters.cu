@@ -612,7 +612,8 @@ cudaError_t launch(const adapter_args &a, int device, int sms, void *stream, con
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    const int tiles = a.rows / kLongRows + std::min(a.rows, a.adapters + 1), rank_blocks = (a.rank + 31) / 32;
+    /* most tiles that there can be: every adapter's last one, and a tile has a row at least (the table has a line more than rows) */
+    const int tiles = std::min(a.rows, a.rows / kLongRows + std::min(a.rows, a.adapters + 1)), rank_blocks = (a.rank + 31) / 32;
     {   hy3a_launch l(dim3(kLongRows / 16 * tiles, a.cuts * rank_blocks), dim3(32 * kReduceWarps), 0, stream);
         if ((e = wide ? cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_adapters_reduce_kernel<T, 2, 2, false>, a)) != cudaSuccess) return e; }
     /* two blocks an SM while u leaves room for two stages at least */
