@@ -9,6 +9,7 @@
  */
 #include <Python.h>
 
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -182,6 +183,15 @@ bool fits(std::initializer_list<int64_t> v) { for (int64_t n : v) if (n < 0 || n
 at::Tensor workspace(size_t bytes, const at::Tensor &x) { return at::empty({(int64_t)(bytes ? bytes : 1)}, x.options().dtype(at::kByte)); }
 void *as_stream(PyObject *o) { return PyLong_AsVoidPtr(o); }
 
+/* Whether autograd would look for a gradient here: there is none, and an output without one would end it unseen. */
+bool wants_grad(std::initializer_list<const at::Tensor *> v) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor *t : v) if (t && t->requires_grad()) return true;
+    return false;
+}
+/* what was written into has changed, for those that keep it for a backward pass */
+void changed(const at::Tensor *t) { if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version(); }
+
 /* route(stream, logits, bias, top_k, score, groups, top_groups, renormalize, scale) -> (ids, weights) */
 PyObject *route(PyObject *const *a, Py_ssize_t na) {
     if (na != 9) return refuse("route: 9 arguments");
@@ -196,6 +206,7 @@ PyObject *route(PyObject *const *a, Py_ssize_t na) {
     if (!l || !l->is_cuda() || !matrix(l) || dtype_code(l) < 0) return refuse("route: logits are a CUDA matrix of fp32, fp16 or bf16 with dense rows");
     const int64_t rows = l->size(0), n = l->size(1);
     if (bias && (!dense(bias, at::kFloat, *l) || bias->numel() != n)) return refuse("route: bias is fp32 [experts] on the logits' device");
+    if (wants_grad({l, bias})) return refuse("route: computes no gradients: call it under torch.no_grad()");
     if (!fits({rows, n})) return refuse("route: sizes do not fit an int");
     const int64_t k = v[0] < 0 ? 0 : v[0];
     c10::DeviceGuard guard(l->device());
@@ -235,6 +246,7 @@ PyObject *experts(PyObject *const *a, Py_ssize_t na) {
         return refuse("experts: gate and up [held, inter, hidden] and down [held, hidden, inter] are contiguous, of x's type and on its device");
     const int64_t held = gate->size(0), inter = gate->size(1), k = ids->size(1);
     if (given && (!on_gpu_with(given, *x) || given->scalar_type() != type || !matrix(given) || given->sizes() != x->sizes())) return refuse("experts: out is like x");
+    if (wants_grad({x, w, gate, up, down, given})) return refuse("experts: computes no gradients: call it under torch.no_grad()");
     if (!fits({rows, hidden, held, inter, k})) return refuse("experts: sizes do not fit an int");
     c10::DeviceGuard guard(x->device());
     at::Tensor out = given ? *given : at::empty({rows, hidden}, x->options());
@@ -250,7 +262,9 @@ PyObject *experts(PyObject *const *a, Py_ssize_t na) {
     Py_BEGIN_ALLOW_THREADS
     rc = f_experts(stream, dt, (int)rows, (int)k, (int)hidden, (int)inter, (int)held, first, xp, sx, ip, wp, gp, up_, dp, op, so, kp, bytes);
     Py_END_ALLOW_THREADS
-    return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    if (rc) return PyLong_FromLong(rc);
+    changed(given);
+    return THPVariable_Wrap(out);
 }
 /* adapters(stream, x, base, a, b, ids, scales, out) -> out */
 PyObject *adapters(PyObject *const *a, Py_ssize_t na) {
@@ -271,6 +285,7 @@ PyObject *adapters(PyObject *const *a, Py_ssize_t na) {
     if (!dense(ids, at::kInt, *x) || ids->dim() != 1 || ids->size(0) != rows || !dense(sc, at::kFloat, *x) || sc->numel() != n)
         return refuse("adapters: ids are int32 [rows], scales fp32 [adapters], on x's device");
     if (given && (!on_gpu_with(given, *x) || given->scalar_type() != base->scalar_type() || !matrix(given) || given->sizes() != base->sizes())) return refuse("adapters: out is like base");
+    if (wants_grad({x, base, la, lb, sc, given})) return refuse("adapters: computes no gradients: call it under torch.no_grad()");
     if (!fits({rows, width, wide, n, rank})) return refuse("adapters: sizes do not fit an int");
     c10::DeviceGuard guard(x->device());
     at::Tensor out = given ? *given : at::empty({rows, wide}, base->options());
@@ -286,7 +301,9 @@ PyObject *adapters(PyObject *const *a, Py_ssize_t na) {
     Py_BEGIN_ALLOW_THREADS
     rc = f_adapters(stream, dt, (int)rows, (int)width, (int)wide, (int)n, (int)rank, xp, sx, bt, bp, sb, ap, b2, ip, sp, op, so, kp, bytes);
     Py_END_ALLOW_THREADS
-    return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+    if (rc) return PyLong_FromLong(rc);
+    changed(given);
+    return THPVariable_Wrap(out);
 }
 /* bind(addresses of hy3a_batch_set, _append, _decode_step, _prefill, _route, _experts_workspace, _experts, _adapters_workspace, _adapters) */
 PyObject *bind(PyObject *const *a, Py_ssize_t na) {

@@ -2,8 +2,8 @@
 
 They are functions, without a context: work is enqueued on torch's current stream of the tensors' device, outputs and workspaces come
 from torch's allocator, nothing is copied to the host or kept between calls, and calls can be captured in a graph.  Sizes and pointers
-that the library refuses raise `Hy3AttnError`, tensors of another kind than stated `AssertionError`.  include/hy3_attn.h has the
-semantics in full.
+that the library refuses raise `Hy3AttnError`, tensors of another kind than stated `AssertionError`, and so do tensors that require gradients,
+outside of torch.no_grad(): there is no backward pass.  include/hy3_attn.h has the semantics in full.
 """
 from ._lib import Hy3AttnError, load_library, load_native
 
