@@ -61,6 +61,7 @@ PROTOTYPES = {
     "hy3a_adapters_workspace": (_sz, [_i, _i, _i]),
     "hy3a_adapters": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz]),
     "hy3a_layer_sync": (_i, [_vp]),
+    "hy3a_layer_wait_out": (_i, [_vp, _i]),
     "hy3a_launch_count": (_u64, [_vp]),
     "hy3a_decode_schedule_kv": (_i, [_i, _i, _ip, _i, _i, _i, _llp, _llp, _llp]),
     "hy3a_decode_schedule": (_i, [_i, _ip, _i, _i, _i, _llp, _llp, _llp]),

@@ -357,6 +357,11 @@ cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device
     return dtype == HY3A_BF16 ? launch<__nv_bfloat16>(a, m, device, sms, stream) : launch<__half>(a, m, device, sms, stream);
 }
 
+static __global__ void hy3a_experts_wait_out_kernel() { wait_out(g_err, 29u); }
+cudaError_t hy3a_experts_wait_out(void *stream) {
+    hy3a_experts_wait_out_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
+    return cudaGetLastError();
+}
 cudaError_t hy3a_experts_error(unsigned *err) {
     const unsigned none[2] = {0, 0};
     cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));

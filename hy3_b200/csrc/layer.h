@@ -24,6 +24,9 @@ int hy3a_layer_device(const char *who, int *device, int *sms);
 /* The files' error words {code, where} of the first wait that ran out on the current device; read and cleared. */
 cudaError_t hy3a_experts_error(unsigned *err);
 cudaError_t hy3a_adapters_error(unsigned *err);
+/* a launch of the file's with one wait that runs out */
+cudaError_t hy3a_experts_wait_out(void *stream);
+cudaError_t hy3a_adapters_wait_out(void *stream);
 
 /* launch configuration with programmatic stream serialisation: the kernels wait (pdl_wait) before they touch memory */
 struct hy3a_launch {

@@ -37,6 +37,14 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatil
     if (atomicCAS(err, 0u, 2u) == 0u) err[1] = where;
     return false;
 }
+/* one wait that nothing ends (hy3a_layer_wait_out) */
+__device__ __forceinline__ void wait_out(unsigned *err, unsigned where) {
+    __shared__ alignas(8) unsigned long long s_bar;
+    __shared__ int s_abort;
+    s_abort = 0;
+    mbar_init(smem_u32(&s_bar), 1);
+    mbar_wait(smem_u32(&s_bar), 0u, &s_abort, err, where);
+}
 __device__ __forceinline__ unsigned elect_one() {
     unsigned p;
     asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(p));

@@ -301,3 +301,12 @@ extern "C" int hy3a_layer_sync(void *stream) {
         if (err[i][0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "%s: a device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", i ? "adapters" : "experts", err[i][0], err[i][1]);
     return HY3A_OK;
 }
+
+extern "C" int hy3a_layer_wait_out(void *stream, int which) {
+    if (which != 0 && which != 1) return hy3a_fail(NULL, HY3A_EINVAL, "layer_wait_out: which %d not in {0,1}", which);
+    int dev, sms, rc = hy3a_layer_device("layer_wait_out", &dev, &sms);
+    if (rc) return rc;
+    const cudaError_t e = which ? hy3a_adapters_wait_out(stream) : hy3a_experts_wait_out(stream);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_wait_out: %s", cudaGetErrorString(e));
+    return HY3A_OK;
+}

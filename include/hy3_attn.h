@@ -292,6 +292,8 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
  * hy3a_experts or hy3a_adapters ran out on the current device since the last call (it then returned early, and outputs since are
  * not valid).  */
 int hy3a_layer_sync(void *stream);
+/* For checks of that report: a launch with one bounded wait of hy3a_experts (which 0) or hy3a_adapters (1) that nothing ends; it returns after half a second. */
+int hy3a_layer_wait_out(void *stream, int which);
 
 /* ---- introspection ------------------------------------------------------------------*/
 /* Number of kernels this library has launched on ctx since creation. */
