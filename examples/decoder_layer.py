@@ -67,8 +67,8 @@ class DecoderLayer:
         shared = torch.mm(torch.nn.functional.silu(torch.mm(h, self.shared_gate.T)) * torch.mm(h, self.shared_up.T), self.shared_down.T)
         return x + routed.float() + shared.float(), ids, weights
 
-    def prompt(self, seq, x, adapter):
-        """Rows x of a fresh request `seq`, with its adapter (-1: none), in chunks."""
+    def prompt(self, seq, x, adapter, routed=None):
+        """Rows x of a fresh request `seq`, with its adapter (-1: none), in chunks; each chunk's experts and weights are appended to `routed`."""
         out = []
         for t in range(0, x.shape[0], self.chunk):
             part = x[t:t + self.chunk]
@@ -77,7 +77,10 @@ class DecoderLayer:
             self.ctx.batch_set([seq] * n, list(range(t, t + n)))
             q, k, v = self.project(part, which)
             self.ctx.append(0, q, k, v, q_out=False, q_out16=self.q16[:n])
-            out.append(self.finish(part, self.ctx.prefill(0, seq, t, self.q16[:n]), which)[0])
+            rows, *experts = self.finish(part, self.ctx.prefill(0, seq, t, self.q16[:n]), which)
+            out.append(rows)
+            if routed is not None:
+                routed.append(experts)
         return torch.cat(out)
 
     def step(self, seqs, slots, x, adapter):
