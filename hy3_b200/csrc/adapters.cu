@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(32 * kShortWarps, 2) hy3a_adapters_short_kerne
  * warp adds base and stores straight from tensor memory, 128 bytes of a row at a time, whatever rows the list names.  In 16-bit types a lane has
  * two neighbouring columns, one in each of two accumulators: B's columns come in by their parity.  Warps 0-7 prepare u and then move the quarter w % 4 of
  * the columns of rows 32 (w / 4) ..; warp 8 fetches B (128 columns x 64 ranks a stage, 128-byte swizzle), warp 9 multiplies, into two sets of accumulators in turn.
- * Measured beside it, 2048 rows on 4096 -> 10240 with 32 / 128 ranks: warp-level products over a ring of tensor copies 63 / 159, this 50 / 73; base and
+ * Measured beside it, 2048 rows on 4096 -> 10240 with 32 / 128 ranks: warp-level products over a ring of tensor copies 63 / 159, this 50 / 78; base and
  * output through shared memory by a bulk copy of each row, one block an SM, 67 / 92. */
 constexpr int kLongWarps = 8, kLongThreads = 32 * (kLongWarps + 2), kStageBytes = kLongCols * 128;
 enum { A_FULL = 0, A_EMPTY = kLongStages, A_TFULL = 2 * kLongStages, A_TEMPTY = A_TFULL + 2, A_COUNT = A_TEMPTY + 2 };
@@ -596,6 +596,8 @@ cudaError_t launch(const adapter_args &a, int device, int sms, void *stream, con
     cudaError_t e;
     const bool wide = wide_rows({a.x, a.a}, {a.x_stride, (size_t)a.width});
     if (a.rows <= 8) return launch_short<T, O, false>(a, wide, stream);
+    /* (the plan's array holds no more adapters: beyond, tiles of 8 rows read A and B for each.  us a pass with 2047 / 2048 adapters of rank 64 on 8192 -> 4096: 2048 rows
+     * of 7 prompts 121 / 326, of as many requests 416 / 784, 300 rows of as many requests 93 / 121) */
     if (a.rows <= kShort || a.adapters > kMaxListed) return launch_short<T, O, true>(a, wide, stream);
     const bool shared = a.rows >= kPlanShared;
     {   hy3a_launch l(dim3(shared ? kGroupCluster : 1), dim3(kGroupThreads), 0, stream);

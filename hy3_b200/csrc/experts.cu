@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) hy3a_experts_few_down_kerne
 }
 
 /* ---- 4. combine: a thread per 8 columns of a row ------------------------------------------------------------------------
- * (The weights and places come from launches that are complete before `down` lets this one begin.)  Bound by the chain of its loads and by memory: 8192 rows
- * of 4096 with a slot each are 201 MB. */
+ * (The weights and places come from launches that are complete before `down` lets this one begin.)  Bound by the chain of its loads and by memory: 39 us by
+ * itself for 8192 rows of 4096 with a slot each, whose 201 MB take 31. */
 template <class T>
 __global__ void __launch_bounds__(256) hy3a_experts_combine_kernel(const expert_args a) {
     pdl_release();
@@ -301,8 +301,8 @@ cudaError_t launch_few(const expert_args &a, void *stream) {
 }
 template <class T>
 cudaError_t launch(const expert_args &a, int device, int sms, void *stream, const char **what) {
-    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 54.8 / 67.9, 95 / 110, 137 / 149; fp16, 3 of 10 of
-     * 1032 x 200 for 1, 10 rows 8.0 / 18.4, 10.4 / 16.9 */
+    /* us a pass, few / umma: bf16, 8 of 192 experts of 4096 x 1536 for 1, 2, 3 rows 54.4 / 67.5, 94.5 / 110, 137 / 149; fp16, the same for 1, 3 rows 57.3 / 70.5,
+     * 141 / 153, 3 of 10 of 1032 x 200 for 1, 10 rows 11.3 / 17.2, 12.4 / 18.1 */
     if (a.slots < kFewMost) return launch_few<T>(a, stream);
     cudaError_t e;
     const bool shared = a.slots >= kGroupShared;

@@ -16,8 +16,9 @@
  * Pairs take tiles in turn: (slots' tile, 256 weight rows), the tiles of an expert's slots innermost, so that pairs that work on the same weights
  * at the same time find them in L2.
  *
- * With few slots an expert the kernels read weights (64 rows on 192 experts of 4096 x 1536: 6.8 GB in 943 us, 7.2 TB/s); with many, gate / up by itself
- * keeps the tensor pipe busy 77 % of the time (8192 slots on 24 experts: 1.07 PFLOP/s, power-limited).  CTAs by themselves (cta_group::1, 128 weight rows) instead of pairs are 1 %
+ * With few slots an expert the kernels read weights (64 rows ask for 162 of 192 experts of 4096 x 1536: 6.1 GB in 928 us, 6.6 TB/s); with many, gate / up by itself
+ * keeps the tensor pipe busy 78 % of the time, down 59 % (8192 slots on 24 experts; 1.07 PFLOP/s in gate / up from a cold start; passes for seconds run at
+ * 1241 MHz, the median under the power limit, of 1965).  CTAs by themselves (cta_group::1, 128 weight rows) instead of pairs are 1 %
  * faster where weights are read and 30 % slower where products are computed: an SM's share of weights is the same.
  *
  * Every wait is bounded; one that runs out raises the CTA's abort flag and a code in the error word (hy3a_layer_sync), lets all warps fall

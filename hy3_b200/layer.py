@@ -34,7 +34,7 @@ def route(logits, bias=None, top_k=8, score="sigmoid", groups=1, top_groups=1, r
     [rows, top_k], weights fp32 [rows, top_k]).
 
     Scores s = sigmoid or softmax of the logits; s + bias picks, s weighs.  A logit of -inf closes its expert for the row; with groups > 1
-    only the experts of the best `top_groups` groups of neighbours stay open (a group stands with the sum of its two best).  The `top_k`
+    only the experts of the best `top_groups` groups of neighbours stay open (a group stands with the sum of its two best, whatever the score).  The `top_k`
     best in descending order, ties to the lowest index; -1 with weight 0 where none is left.  Weights are divided by their sum if
     `renormalize`, times `scale`."""
     return _out(load_native().route(_stream(logits), logits, bias, top_k, SCORES[score], groups, top_groups, renormalize, scale))
@@ -45,7 +45,8 @@ def experts(x, ids, weights, gate, up, down, first_expert=0, out=None):
     e = ids[t, j] - first_expert.
 
     x [rows, hidden] fp16 or bf16 (row stride free), ids int32 and weights fp32 [rows, top_k] (as `route` gives them), gate and up
-    [held, inter, hidden], down [held, hidden, inter] of x's type, dense.  Slots of experts that are not held here are left out: ranks that
+    [held, inter, hidden], down [held, hidden, inter] of x's type, dense.  Sums are fp32; between the two products the gated ones are rounded to
+    x's type (fp16: on a scale of each slot; fewer than 32 slots in all keep twice the bits).  Slots of experts that are not held here are left out: ranks that
     split the experts add their outputs up.  Returns out [rows, hidden] of x's type."""
     return _out(load_native().experts(_stream(x), x, ids, weights, gate, up, down, first_expert, out))
 
