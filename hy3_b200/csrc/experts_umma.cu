@@ -176,8 +176,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *s_tmem;
-    /* Gate / up lets the next launch begin behind its own wait (and so does the one between the two): `down` finds the plan complete, and fetches its first
-     * weights before it waits for h. */
+    /* Gate / up lets the next launch begin behind its own wait, and the one that fp16 rows have between the two lets `down` begin at once: `down` finds the plan
+     * complete, and fetches its first weights before it waits for h. */
     if (!DOWN) pdl_wait();
     pdl_release();
     const int total = *a.n_tiles * m_tiles;

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(32 * kWarps) hy3a_route_kernel(const route_arg
             b1 = b1 == -INFINITY ? b1 : (row_nan ? kLowest : __fdiv_rn(b1, d));
             b2 = b2 == -INFINITY ? b2 : (row_nan ? kLowest : __fdiv_rn(b2, d));
         }
-        const float stands = b2 == -INFINITY ? b1 : fmaxf(__fadd_rn(b1, b2), kLowest);      /* (two NaN stand before nothing, too) */
+        const float stands = b2 == -INFINITY ? b1 : fmaxf(__fadd_rn(b1, b2), kLowest);      /* (two NaN: still before a group without open experts) */
         /* groups that come before this one: better, or as good with a lower index (o > mine, or o >= mine: a key is at least 1) */
         const unsigned mine = ordered(stands);
         int before = 0;
