@@ -60,6 +60,9 @@ PROTOTYPES = {
     "hy3a_experts": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz]),
     "hy3a_adapters_workspace": (_sz, [_i, _i, _i]),
     "hy3a_adapters": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz]),
+    "hy3a_quantize4": (_i, [_vp, _i, _i, _i, _i, _vp, _sz, _i, _vp, _vp]),
+    "hy3a_linear4": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _sz, _vp, _vp, _i, _vp, _sz]),
+    "hy3a_logprobs": (_i, [_vp, _i, _i, _i, _vp, _sz, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "hy3a_layer_sync": (_i, [_vp]),
     "hy3a_layer_wait_out": (_i, [_vp, _i]),
     "hy3a_launch_count": (_u64, [_vp]),
@@ -92,7 +95,8 @@ def load_library():
 
 
 _bound = None
-BOUND = ("batch_set", "append", "decode_step", "prefill", "route", "experts_workspace", "experts", "adapters_workspace", "adapters")
+BOUND = ("batch_set", "append", "decode_step", "prefill", "route", "experts_workspace", "experts", "adapters_workspace", "adapters",
+         "quantize4", "linear4", "logprobs")
 
 
 def load_native():

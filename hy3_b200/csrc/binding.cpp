@@ -1,6 +1,6 @@
 /*
  * binding.cpp -- the per-step calls of Hy3Attn (attn.py) as native functions: batch_set, append, decode_step, prefill; and the operators
- * beside the attention (layer.py): route, experts, adapters.
+ * beside the attention (layer.py): route, experts, adapters, quantize4, linear4, logprobs.
  *
  * A decode step of a short context takes 6 to 9 us on the GPU; the same call through ctypes cost the host 6.6 us (four to seven
  * tensors asked for their strides, types and addresses one attribute at a time, 11 to 15 arguments converted one by one).  Here the
@@ -12,6 +12,7 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/hy3_attn.h"
@@ -27,6 +28,9 @@ decltype(&hy3a_experts_workspace) f_experts_workspace;
 decltype(&hy3a_experts) f_experts;
 decltype(&hy3a_adapters_workspace) f_adapters_workspace;
 decltype(&hy3a_adapters) f_adapters;
+decltype(&hy3a_quantize4) f_quantize4;
+decltype(&hy3a_linear4) f_linear4;
+decltype(&hy3a_logprobs) f_logprobs;
 
 constexpr int64_t kH = HY3A_N_HEAD, kD = HY3A_HEAD_DIM;
 
@@ -305,23 +309,137 @@ PyObject *adapters(PyObject *const *a, Py_ssize_t na) {
     changed(given);
     return THPVariable_Wrap(out);
 }
-/* bind(addresses of hy3a_batch_set, _append, _decode_step, _prefill, _route, _experts_workspace, _experts, _adapters_workspace, _adapters) */
+/* a torch.dtype, `fallback` for None */
+bool scalar_type(PyObject *o, at::ScalarType fallback, at::ScalarType &t) {
+    t = fallback;
+    if (o == Py_None) return true;
+    if (!THPDtype_Check(o)) { PyErr_SetString(PyExc_TypeError, "expected a torch.dtype or None"); return false; }
+    t = reinterpret_cast<THPDtype *>(o)->scalar_type;
+    return true;
+}
+int code_of(at::ScalarType t) { return t == at::kFloat ? HY3A_F32 : (t == at::kHalf ? HY3A_F16 : (t == at::kBFloat16 ? HY3A_BF16 : -1)); }
+
+/* quantize4(stream, w, group, dtype) -> (codes, scales) */
+PyObject *quantize4(PyObject *const *a, Py_ssize_t na) {
+    if (na != 4) return refuse("quantize4: 4 arguments");
+    void *stream = as_stream(a[0]);
+    const at::Tensor *w;
+    if (PyErr_Occurred() || !tensor(a[1], w)) return nullptr;
+    const int group = as_int(a[2]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!w || !w->is_cuda() || !matrix(w) || dtype_code(w) < 0) return refuse("quantize4: w is a CUDA matrix of fp32, fp16 or bf16 with dense rows");
+    at::ScalarType type;
+    if (!scalar_type(a[3], w->scalar_type() == at::kHalf ? at::kHalf : at::kBFloat16, type)) return nullptr;
+    if (type != at::kHalf && type != at::kBFloat16) return refuse("quantize4: dtype is fp16 or bf16");
+    if (wants_grad({w})) return refuse("quantize4: computes no gradients: call it under torch.no_grad()");
+    const int64_t out = w->size(0), width = w->size(1);
+    if (!fits({out, width})) return refuse("quantize4: sizes do not fit an int");
+    const int64_t groups = group > 0 ? (width + group - 1) / group : 0;
+    c10::DeviceGuard guard(w->device());
+    at::Tensor codes = at::empty({out, width / 2}, w->options().dtype(at::kByte)), scales = at::empty({out, groups}, w->options().dtype(type));
+    const void *wp = w->data_ptr();
+    void *cp = codes.data_ptr(), *sp = scales.data_ptr();
+    const size_t stride = row_stride(w);
+    const int wt = dtype_code(w), st = code_of(type);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_quantize4(stream, wt, (int)out, (int)width, group, wp, stride, st, cp, sp);
+    Py_END_ALLOW_THREADS
+    if (rc) return PyLong_FromLong(rc);
+    PyObject *pc = THPVariable_Wrap(codes), *ps = THPVariable_Wrap(scales), *r = pc && ps ? PyTuple_Pack(2, pc, ps) : nullptr;
+    Py_XDECREF(pc);
+    Py_XDECREF(ps);
+    return r;
+}
+/* linear4(stream, x, codes, scales, out_dtype, out) -> out */
+PyObject *linear4(PyObject *const *a, Py_ssize_t na) {
+    if (na != 6) return refuse("linear4: 6 arguments");
+    void *stream = as_stream(a[0]);
+    const at::Tensor *x, *codes, *scales, *given;
+    if (PyErr_Occurred() || !tensor(a[1], x) || !tensor(a[2], codes) || !tensor(a[3], scales) || !tensor(a[5], given)) return nullptr;
+    if (!x || !codes || !scales) return refuse("linear4: tensors, and out or None");
+    const at::ScalarType type = x->scalar_type();
+    if (!x->is_cuda() || !matrix(x) || (type != at::kHalf && type != at::kBFloat16)) return refuse("linear4: x is a CUDA matrix of fp16 or bf16 with dense rows");
+    const int64_t rows = x->size(0), width = x->size(1);
+    if (codes->dim() != 2 || codes->size(1) * 2 != width || !dense(codes, at::kByte, *x) || scales->dim() != 2 || scales->size(0) != codes->size(0) || !dense(scales, type, *x))
+        return refuse("linear4: codes are contiguous uint8 [out_width, width / 2], scales [out_width, groups] of x's type, on its device");
+    const int64_t wide = codes->size(0), groups = scales->size(1);
+    /* (two sizes that make as many groups make one of them: it does not matter which is meant) */
+    int group = 0;
+    for (int g = 32; g <= 128 && !group; g *= 2) if ((width + g - 1) / g == groups) group = g;
+    if (!group) return refuse("linear4: scales are one for each 32, 64 or 128 neighbours in a row");
+    at::ScalarType result;
+    if (!scalar_type(a[4], given ? given->scalar_type() : type, result)) return nullptr;
+    if (result != type && result != at::kFloat) return refuse("linear4: the result is of x's type or fp32");
+    if (given && (!on_gpu_with(given, *x) || given->scalar_type() != result || !matrix(given) || given->size(0) != rows || given->size(1) != wide)) return refuse("linear4: out is a matrix [rows, out_width] of the result's type on x's device");
+    if (wants_grad({x, scales, given})) return refuse("linear4: computes no gradients: call it under torch.no_grad()");
+    if (!fits({rows, width, wide})) return refuse("linear4: sizes do not fit an int");
+    c10::DeviceGuard guard(x->device());
+    at::Tensor out = given ? *given : at::empty({rows, wide}, x->options().dtype(result));
+    const int dt = dtype_code(x), ot = code_of(result);
+    const void *xp = x->data_ptr(), *cp = codes->data_ptr(), *sp = scales->data_ptr();
+    void *op = out.data_ptr();
+    const size_t sx = row_stride(x), so = row_stride(&out);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_linear4(stream, dt, (int)rows, (int)width, (int)wide, group, xp, sx, cp, sp, ot, op, so);
+    Py_END_ALLOW_THREADS
+    if (rc) return PyLong_FromLong(rc);
+    changed(given);
+    return THPVariable_Wrap(out);
+}
+/* logprobs(stream, logits, tokens, top_k) -> (log probabilities or None, entropy, ids, their log probabilities) */
+PyObject *logprobs(PyObject *const *a, Py_ssize_t na) {
+    if (na != 4) return refuse("logprobs: 4 arguments");
+    void *stream = as_stream(a[0]);
+    const at::Tensor *l, *tokens;
+    if (PyErr_Occurred() || !tensor(a[1], l) || !tensor(a[2], tokens)) return nullptr;
+    const int top_k = as_int(a[3]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!l || !l->is_cuda() || !matrix(l) || dtype_code(l) < 0) return refuse("logprobs: logits are a CUDA matrix of fp32, fp16 or bf16 with dense rows");
+    const int64_t rows = l->size(0), vocab = l->size(1);
+    if (tokens && (tokens->dim() < 1 || tokens->dim() > 2 || tokens->size(0) != rows || !dense(tokens, at::kInt, *l))) return refuse("logprobs: tokens are contiguous int32 [rows] or [rows, asked] on the logits' device");
+    const int64_t asked = !tokens ? 0 : (tokens->dim() == 1 ? 1 : tokens->size(1));
+    if (wants_grad({l})) return refuse("logprobs: computes no gradients: call it under torch.no_grad()");
+    if (!fits({rows, vocab, asked})) return refuse("logprobs: sizes do not fit an int");
+    const int64_t k = top_k < 0 ? 0 : top_k;
+    c10::DeviceGuard guard(l->device());
+    const at::TensorOptions f32 = l->options().dtype(at::kFloat);
+    at::Tensor logp = tokens ? at::empty(tokens->sizes(), f32) : at::Tensor(), entropy = at::empty({rows}, f32), ids = at::empty({rows, k}, l->options().dtype(at::kInt)), top = at::empty({rows, k}, f32);
+    const void *lp = l->data_ptr();
+    const int *tp = ptr<const int>(tokens);
+    float *ap = tokens ? (float *)logp.data_ptr() : nullptr, *ep = (float *)entropy.data_ptr(), *pp = (float *)top.data_ptr();
+    int *ip = (int *)ids.data_ptr();
+    const size_t stride = row_stride(l);
+    const int dt = dtype_code(l);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f_logprobs(stream, dt, (int)rows, (int)vocab, lp, stride, tp, (int)asked, top_k, ap, ep, ip, pp);
+    Py_END_ALLOW_THREADS
+    if (rc) return PyLong_FromLong(rc);
+    PyObject *v[4] = {tokens ? THPVariable_Wrap(logp) : Py_NewRef(Py_None), THPVariable_Wrap(entropy), THPVariable_Wrap(ids), THPVariable_Wrap(top)};
+    PyObject *r = v[0] && v[1] && v[2] && v[3] ? PyTuple_Pack(4, v[0], v[1], v[2], v[3]) : nullptr;
+    for (PyObject *o : v) Py_XDECREF(o);
+    return r;
+}
+/* bind(addresses of hy3a_batch_set, _append, _decode_step, _prefill, _route, _experts_workspace, _experts, _adapters_workspace, _adapters, _quantize4, _linear4, _logprobs) */
 PyObject *bind(PyObject *const *a, Py_ssize_t na) {
-    if (na != 9) return refuse("bind: 9 addresses");
-    void *f[9];
-    for (int i = 0; i < 9; i++) {
+    if (na != 12) return refuse("bind: 12 addresses");
+    void *f[12];
+    for (int i = 0; i < 12; i++) {
         f[i] = PyLong_AsVoidPtr(a[i]);
         if (PyErr_Occurred()) return nullptr;
     }
     f_batch_set = (decltype(f_batch_set))f[0]; f_append = (decltype(f_append))f[1]; f_decode_step = (decltype(f_decode_step))f[2]; f_prefill = (decltype(f_prefill))f[3];
     f_route = (decltype(f_route))f[4]; f_experts_workspace = (decltype(f_experts_workspace))f[5]; f_experts = (decltype(f_experts))f[6];
     f_adapters_workspace = (decltype(f_adapters_workspace))f[7]; f_adapters = (decltype(f_adapters))f[8];
+    f_quantize4 = (decltype(f_quantize4))f[9]; f_linear4 = (decltype(f_linear4))f[10]; f_logprobs = (decltype(f_logprobs))f[11];
     Py_RETURN_NONE;
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(batch_set), METHOD(append), METHOD(decode_step), METHOD(prefill),
-                         METHOD(route), METHOD(experts), METHOD(adapters), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(route), METHOD(experts), METHOD(adapters), METHOD(quantize4), METHOD(linear4), METHOD(logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 
 } /* namespace */

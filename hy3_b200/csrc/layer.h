@@ -1,6 +1,6 @@
 /*
- * layer.h -- what the operators beside the attention share (route.cu, experts.cu, adapters.cu): the device check and launch attributes on
- * the host; 16-byte loads, conversions and the warp-level matrix product on the device.
+ * layer.h -- what the operators beside the attention share (route.cu, experts.cu, adapters.cu, quantize4.cu, linear4.cu, logprobs.cu): the device check and
+ * launch attributes on the host; 16-byte loads, conversions and the warp-level matrix product on the device.
  *
  * The warp-level product takes its fragments straight from global memory.  mma.m16n8k16 wants of lane (g = lane / 4, t = lane % 4) the
  * k's {2t, 2t+1, 2t+8, 2t+9} of rows g and g + 8 of A and of column g of B.  A sum does not mind the order of its terms, so k is
@@ -21,12 +21,17 @@
 /* The current device's number and SM count; refuses devices that sm_100a code cannot run on. */
 int hy3a_layer_device(const char *who, int *device, int *sms);
 
+/* Whether sizes of a matrix in 4 bits are in their limits: 0 or HY3A_EINVAL. */
+int hy3a_quant4_sizes(const char *who, int out_width, int width, int group);
+
 /* The files' error words {code, where} of the first wait that ran out on the current device; read and cleared. */
 cudaError_t hy3a_experts_error(unsigned *err);
 cudaError_t hy3a_adapters_error(unsigned *err);
+cudaError_t hy3a_linear4_error(unsigned *err);
 /* a launch of the file's with one wait that runs out */
 cudaError_t hy3a_experts_wait_out(void *stream);
 cudaError_t hy3a_adapters_wait_out(void *stream);
+cudaError_t hy3a_linear4_wait_out(void *stream);
 
 /* launch configuration with programmatic stream serialisation: the kernels wait (pdl_wait) before they touch memory */
 struct hy3a_launch {

@@ -1,0 +1,50 @@
+/* linear4.h -- what the kernels of hy3a_linear4 share (linear4.cu: few rows; linear4_umma.cu: many). */
+#ifndef HY3A_LINEAR4_H
+#define HY3A_LINEAR4_H
+
+#include "layer.h"
+
+struct linear4_args {
+    const void *x;            /* [rows][width], 16-bit type T */
+    size_t x_stride;
+    const uint8_t *codes;     /* [out_width][width / 2] */
+    const void *scales;       /* [out_width][groups], T */
+    void *out;                /* [rows][out_width], T or fp32 */
+    size_t out_stride;
+    int rows, width, out_width, group, groups;
+    int wide;                 /* out is fp32 */
+};
+
+namespace hy3a_layer {
+
+/* Codes become numbers of the rows' type by their bits: with a code c in the lowest bits of the mantissa, 0x4300 | c is 128 + c in bf16 and 0x6400 | c is 1024 + c in
+ * fp16 (with c four bits higher 1024 + 16 c), and the subtraction of 128 + 8, or 1024 + 8, is exact.  A word's codes k = 0 .. 7 come as the pairs (0, 4), (1, 5),
+ * (2, 6), (3, 7). */
+__device__ __forceinline__ unsigned and_or(unsigned a, unsigned mask, unsigned bits) {
+    unsigned r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+    return r;
+}
+template <class T> struct steps;
+template <> struct steps<__nv_bfloat16> {
+    static __device__ __forceinline__ void of(unsigned w, unsigned (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned c = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+            asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(c), "r"(0x43084308u));
+        }
+    }
+};
+template <> struct steps<__half> {
+    static __device__ __forceinline__ void of(unsigned w, unsigned (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const unsigned u = i ? w >> 8 : w, lo = and_or(u, 0x000f000fu, 0x64006400u), hi = and_or(u, 0x00f000f0u, 0x64006400u);
+            asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(lo), "r"(0x64086408u));
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[i + 1]) : "r"(hi), "r"(0x2c002c00u) /* 1 / 16 */, "r"(0xd480d480u) /* -72 */);
+        }
+    }
+};
+
+} /* namespace hy3a_layer */
+#endif

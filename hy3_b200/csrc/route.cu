@@ -292,21 +292,23 @@ extern "C" int hy3a_route(void *stream, int dtype, int rows, int experts, const 
 }
 
 extern "C" int hy3a_layer_sync(void *stream) {
-    unsigned err[2][2] = {{0, 0}, {0, 0}};
+    static const char *const names[3] = {"experts", "adapters", "linear4"};
+    unsigned err[3][2] = {{0, 0}, {0, 0}, {0, 0}};
     cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
     if (e == cudaSuccess) e = hy3a_experts_error(err[0]);
     if (e == cudaSuccess) e = hy3a_adapters_error(err[1]);
+    if (e == cudaSuccess) e = hy3a_linear4_error(err[2]);
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_sync: %s", cudaGetErrorString(e));
-    for (int i = 0; i < 2; i++)
-        if (err[i][0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "%s: a device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", i ? "adapters" : "experts", err[i][0], err[i][1]);
+    for (int i = 0; i < 3; i++)
+        if (err[i][0]) return hy3a_fail(NULL, HY3A_ETIMEOUT, "%s: a device-side bounded wait ran out (code %u, where %u): outputs since the last check are not valid", names[i], err[i][0], err[i][1]);
     return HY3A_OK;
 }
 
 extern "C" int hy3a_layer_wait_out(void *stream, int which) {
-    if (which != 0 && which != 1) return hy3a_fail(NULL, HY3A_EINVAL, "layer_wait_out: which %d not in {0,1}", which);
+    if (which != 0 && which != 1 && which != 4) return hy3a_fail(NULL, HY3A_EINVAL, "layer_wait_out: which %d not in {0,1,4}", which);
     int dev, sms, rc = hy3a_layer_device("layer_wait_out", &dev, &sms);
     if (rc) return rc;
-    const cudaError_t e = which ? hy3a_adapters_wait_out(stream) : hy3a_experts_wait_out(stream);
+    const cudaError_t e = which == 4 ? hy3a_linear4_wait_out(stream) : (which ? hy3a_adapters_wait_out(stream) : hy3a_experts_wait_out(stream));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "layer_wait_out: %s", cudaGetErrorString(e));
     return HY3A_OK;
 }

@@ -1,4 +1,5 @@
-"""The operators beside the attention in a layer, on torch CUDA tensors: routing to experts, the experts' products, and low-rank adapters.
+"""The operators beside the attention, on torch CUDA tensors: routing to experts, the experts' products, and low-rank adapters; weights in 4 bits and
+rows' products with them; log probabilities of logits.
 
 They are functions, without a context: work is enqueued on torch's current stream of the tensors' device, outputs and workspaces come
 from torch's allocator, nothing is copied to the host or kept between calls, and calls can be captured in a graph.  Sizes and pointers
@@ -59,9 +60,36 @@ def adapters(x, base, a, b, ids, scales, out=None):
     return _out(load_native().adapters(_stream(x), x, base, a, b, ids, scales, out))
 
 
+def quantize4(w, group=64, dtype=None):
+    """Weights in 4 bits: w [out_width, width] fp32 / fp16 / bf16 (row stride free) -> (codes uint8 [out_width, width / 2], scales [out_width, groups]).
+
+    Each `group` (32, 64 or 128) neighbours of a row share a scale s of type `dtype` (fp16 or bf16; default: w's, bf16 for fp32), a weight is (q - 8) * s, and a
+    byte has the codes q of two neighbours, the first in its low half.  The value of the largest magnitude gets q = 0, 8 steps from 0: s is minus an eighth of it.
+    width is a multiple of 32 (the last group may be short).  A group with a NaN or an infinity has a scale that is not finite."""
+    return _out(load_native().quantize4(_stream(w), w, group, dtype))
+
+
+def linear4(x, codes, scales, out_dtype=None, out=None):
+    """Rows times a matrix in 4 bits: out[t, o] = sum_k (q[o, k] - 8) * s[o, k / group] * x[t, k], codes and scales as `quantize4` gives them.
+
+    x [rows, width] fp16 or bf16 (row stride free), scales of x's type; the group's size follows from their number.  The result [rows, out_width] is of x's type,
+    or fp32 (`out_dtype`, or out's).  Sums are fp32.  Returns out."""
+    return _out(load_native().linear4(_stream(x), x, codes, scales, out_dtype, out))
+
+
+def logprobs(logits, tokens=None, top_k=0):
+    """Log probabilities under softmax: logits [rows, vocab] fp32 / fp16 / bf16 (row stride free), tokens int32 [rows] or [rows, asked] or None -> (log
+    probabilities of the tokens, of their shape (None without), entropy [rows], ids int32 [rows, top_k], their log probabilities [rows, top_k]), fp32.
+
+    The top_k (at most 32) most likely tokens in descending order, ties to the lowest index.  A logit of -inf closes its token: -inf if it is asked for, and
+    where no open one is left the ids are -1, with -inf.  A row without open tokens has the entropy 0.  The token -1 asks for none and gets 0, others outside
+    the vocabulary get NaN.  Rows with a NaN or +inf get NaN; their ids are in range, NaN below every number."""
+    return _out(load_native().logprobs(_stream(logits), logits, tokens, top_k))
+
+
 def layer_sync(device=None):
     """Waits for torch's current stream on `device` (default: the current one), and raises `Hy3AttnError` if a bounded device-side wait of
-    `experts` or `adapters` ran out there since the last call."""
+    `experts`, `adapters` or `linear4` ran out there since the last call."""
     import torch
     with torch.cuda.device(device):
         rc = load_library().hy3a_layer_sync(torch.cuda.current_stream().cuda_stream)

@@ -244,7 +244,7 @@ int hy3a_fill_random(hy3a_ctx *ctx, int layer, int seq, int t0, int n, uint64_t 
 
 /* ---- operators beside the attention -------------------------------------------------------
  * What else a layer does with rows that are chosen one by one: the experts that a row is routed to, and the low-rank adapter
- * of its request.  (The reference routes and multiplies on the CPU or with a warp per weight row, hy3.c:1266-1303, hy3_gpu.cu:75-130; it
+ * of its request; shared projections and the output head on weights in 4 bits, and what is asked of the logits.  (The reference routes and multiplies on the CPU or with a warp per weight row, hy3.c:1266-1303, hy3_gpu.cu:75-130; it
  * has no adapters.)  They need no context: the stream (a cudaStream_t) and the workspace are arguments, work is enqueued on the
  * current device, which has to be the stream's, nothing is allocated, copied to the host or kept between calls, and all of
  * them can be captured in a graph.  Messages: hy3a_last_error(NULL) of the calling thread.  A workspace may be used again by the
@@ -288,11 +288,36 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
                   const void *base, size_t base_stride, const void *a, const void *b, const int *ids, const float *scales, void *out,
                   size_t out_stride, void *work, size_t work_bytes);
 
+/* Weights in 4 bits: each `group` (32, 64 or 128) neighbours of a row of w [out_width][width] (w_dtype HY3A_F32 / F16 / BF16, rows w_stride elements
+ * apart) share a scale s of type `dtype` (HY3A_F16 or HY3A_BF16), and a weight is (q - 8) * s with 0 <= q < 16:
+ *   e = the group's largest value if that is larger than minus its smallest, else its smallest;  s = -e / 8, rounded to nearest;
+ *   q = min(max(rint(w / s), -8), 7) + 8, w / s in fp32; 8 where s is 0 or not finite (a NaN or an infinity in the group, or |e| too large for the type).
+ * codes [out_width][width / 2] bytes, the even element in the low half; scales [out_width][ceil(width / group)], both dense.  width: a multiple of 32 up to
+ * 65536; the last group may be short.  w and codes are 16-byte aligned, rows of w start on 16-byte boundaries.
+ * (The reference's 4-bit weights have scales in two levels and minima, hy3_gpu.cu:75-130; it quantises none.)                 */
+int hy3a_quantize4(void *stream, int w_dtype, int out_width, int width, int group, const void *w, size_t w_stride, int dtype, void *codes, void *scales);
+
+/* Rows times a matrix in 4 bits, in hy3a_quantize4's format: out[t][o] = sum over k of (q[o][k] - 8) * s[o][k / group] * x[t][k].  x [rows][width] and
+ * the scales are of dtype HY3A_F16 or HY3A_BF16, out [rows][out_width] of out_dtype: that, or HY3A_F32.  Sums are fp32.  x and codes are 16-byte aligned, and rows of x start on
+ * 16-byte boundaries; scales and out are aligned to their types.  out must not overlap x.                                     */
+int hy3a_linear4(void *stream, int dtype, int rows, int width, int out_width, int group, const void *x, size_t x_stride, const void *codes, const void *scales,
+                 int out_dtype, void *out, size_t out_stride);
+
+/* Log probabilities of given tokens, entropy and the best alternatives of rows of logits (dtype HY3A_F32 / F16 / BF16, [rows][vocab], `stride` elements from
+ * row to row), p = softmax of a row, in fp32:
+ *   - asked_logp [rows][asked]: log p of tokens [rows][asked]; 0 for the token -1 (padding), NaN for others outside [0, vocab).  asked may be 0 (both NULL);
+ *   - entropy [rows]: -sum p log p;
+ *   - top_ids, top_logp [rows][top_k]: the top_k (at most 32; 0: both NULL) most likely tokens in descending order, ties to the lowest index, and their log p.
+ * A logit of -inf closes its token: its log p is -inf, it is no alternative, and -1 with -inf stands where none is left.  A row of closed tokens has the entropy
+ * 0.  A row with a NaN or +inf has NaN for its values (0 for the token -1 all the same); its ids are in range, NaN counts below every number.  vocab: at most 2^24, asked: at most 1024. */
+int hy3a_logprobs(void *stream, int dtype, int rows, int vocab, const void *logits, size_t stride, const int *tokens, int asked, int top_k,
+                  float *asked_logp, float *entropy, int *top_ids, float *top_logp);
+
 /* cudaStreamSynchronize on the stream + read of the operators' device error words: HY3A_ETIMEOUT if a bounded device-side wait of
- * hy3a_experts or hy3a_adapters ran out on the current device since the last call (it then returned early, and outputs since are
+ * hy3a_experts, hy3a_adapters or hy3a_linear4 ran out on the current device since the last call (it then returned early, and outputs since are
  * not valid).  */
 int hy3a_layer_sync(void *stream);
-/* For checks of that report: a launch with one bounded wait of hy3a_experts (which 0) or hy3a_adapters (1) that nothing ends; it returns after half a second. */
+/* For checks of that report: a launch with one bounded wait of hy3a_experts (which 0), hy3a_adapters (1) or hy3a_linear4 (4) that nothing ends; it returns after half a second. */
 int hy3a_layer_wait_out(void *stream, int which);
 
 /* ---- introspection ------------------------------------------------------------------*/
