@@ -6,9 +6,10 @@
  * The inner sums are warp-level products (mma.m16n8k16, fp32 sums) of 16 outputs with 8 rows: the differences are exact in the rows' type and so are the
  * products; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
  *
- * A block takes a contiguous part of the outputs (all parts alike to one output), in tiles of 16, and streams their codes through a ring of shared memory: a
- * stage is a tile's codes for 4096 k's (or all, where there are fewer), each output's by a bulk copy of its own, so that all blocks have 100 KB and more under way, and its scales in words
- * (cp.async: their rows start anywhere).  The 16 warps share the k's; each keeps its part of x in registers for the whole launch.  Their sums meet in shared memory.
+ * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
+ * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, so that all blocks have 170 KB under way.  (A bulk copy for
+ * each output keeps the issuing lane busy for longer than its bytes take.)  The 16 warps share the k's; each keeps its part of x in registers for the whole launch, and reads its scales two
+ * stages ahead.  Their sums meet in shared memory, where a warp of their own adds them up.
  *
  * mma wants of lane (g = lane / 4, t = lane % 4) four k's of outputs g and g + 8, and of row g; k's are renamed so that lane t has neighbouring ones, those of a word
  * (32 k's of 4 lanes) the least: a block of 32, 64 or 128 k's, one group's, is 1, 2 or 4 words a lane.
@@ -23,26 +24,30 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kWarps = 16, kThreads = 32 * (kWarps + 1), kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16;
-constexpr int kRingBytes = 200 * 1024, kOffBar = 0, kOffPart = 512, kPartPitch = kTile * kRows, kOffRing = kOffPart + 2 * kWarps * kPartPitch * 4;
+constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2), kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16;
+constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
+constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
+constexpr int kRingBytes = 180 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
+enum { B_FULL = 0, B_EMPTY = kMaxStages, B_READY = 2 * kMaxStages, B_TAKEN = 2 * kMaxStages + kParts, B_COUNT = 2 * kMaxStages + 2 * kParts };
+static_assert(8 * B_COUNT <= 512, "barriers");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
 struct few_args {
     linear4_args a;
-    int pitch /* bytes of an output's codes in a stage */, scale_pitch /* words of its scales */, stage_bytes, stages, passes /* stages of a tile */;
+    int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stages, passes /* stages of a tile */, per /* groups of a warp in a stage */;
+    int whole;                /* rows of codes are whole lines */
 };
 
-__device__ __forceinline__ void bulk_copy(unsigned dst, const void *src, unsigned bytes, unsigned bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(0x12F0000000000000ull) /* evict first */ : "memory");
+/* Copies are issued in uniform control flow by one elected lane (lead): a lane's own operands cost each 50 clocks and more. */
+__device__ __forceinline__ void copy_lines(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, int z, unsigned long long policy, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %7, 0;\n"
+                 " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void copy_word(unsigned dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void arrive_behind_copies(unsigned bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
-template <class T> __device__ __forceinline__ float scale_at(unsigned addr) {
-    unsigned short v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
-    return type<T>::up(*reinterpret_cast<const T *>(&v));
+template <class T> __device__ __forceinline__ float unpack(unsigned v, bool hi) {
+    const unsigned short u = (unsigned short)(hi ? v >> 16 : v);
+    return type<T>::up(*reinterpret_cast<const T *>(&u));
 }
 
 /* x of a lane for a block of 32 W k's from k0 on, in the pairs' order; zeros past the width, and where the row is none */
@@ -58,6 +63,13 @@ template <class T, int W> __device__ __forceinline__ void load_x(const T *row, b
         x[4 * w + 3] = __byte_perm(v.y, v.w, 0x7632);
     }
 }
+/* type<T>::mma with sums from 0 */
+template <class T> __device__ __forceinline__ void mma_first(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    if (type<T>::code == HY3A_BF16) asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                                        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+             : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 /* W words at an address of shared memory */
 template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsigned (&v)[W]) {
     if (W == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[W > 2 ? 2 : 0]), "=r"(v[W > 3 ? 3 : 0]) : "r"(addr));
@@ -67,155 +79,227 @@ template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsig
 
 /* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each */
 template <class T, int W, int P>
-__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const few_args f) {
-    extern __shared__ __align__(128) uint8_t s_raw[];
-    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1;
+__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm, const few_args f) {
+    extern __shared__ uint8_t s_raw[];
+    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kAhead = P == 1 ? 2 : (P ? 1 : 0) /* tiles */;
     const linear4_args &a = f.a;
-    __shared__ int s_abort_flag;
-    volatile int *s_abort = &s_abort_flag;
-    const unsigned sbase = smem_u32(s_raw), bar0 = sbase + kOffBar, ring = sbase + kOffRing;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int first = (int)((long long)a.out_width * blockIdx.x / gridDim.x), last = (int)((long long)a.out_width * (blockIdx.x + 1) / gridDim.x);
+    uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT);
+    const unsigned ring = smem_u32(sm), bar0 = ring + kOffBar, stage_bytes = (kTile / kBox) * f.box_bytes;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int boxes = (a.out_width + kBox - 1) / kBox, first = kBox * (int)((long long)boxes * blockIdx.x / gridDim.x), last = min(a.out_width, kBox * (int)((long long)boxes * (blockIdx.x + 1) / gridDim.x));
     const int t0 = blockIdx.y * kRows, rows = min(kRows, a.rows - t0);
-#define FULL(i) (bar0 + 8u * (unsigned)(i))
-#define EMPTY(i) (bar0 + 8u * (unsigned)(kMaxStages + (i)))
+    /* outputs g and g + 8 of the products are outputs mine and mine + 8 of the tile: such that lanes that read together find their words in different banks */
+    const int mine_of = W == 4 ? (g & 1) * 4 + (g >> 1) : ((g >> 1) & 1) * 4 + (g & 1) * 2 + (g >> 2);
+#define BAR(i) (bar0 + 8u * (unsigned)(i))
     if (tid == 0) {
-        s_abort_flag = 0;
-        for (int i = 0; i < f.stages; i++) { mbar_init(FULL(i), 33); mbar_init(EMPTY(i), kWarps); }
+        *s_abort = 0;
+        for (int i = 0; i < f.stages; i++) { mbar_init(BAR(B_FULL + i), 1); mbar_init(BAR(B_EMPTY + i), kWarps); }
+        for (int i = 0; i < kParts; i++) { mbar_init(BAR(B_READY + i), kWarps); mbar_init(BAR(B_TAKEN + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == kProducer && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&tm) : "memory");
     __syncthreads();
     pdl_release();
     pdl_wait();
     int st = 0;
     unsigned ph = 0;
-    if (warp == kWarps) {
+    if (warp == kProducer) {
         /* ===================== producer ===================== */
+        const unsigned lead = elect_one();
+        unsigned long long policy;
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         bool ok = true;
-        const T *scales = reinterpret_cast<const T *>(a.scales);
         for (int o0 = first; o0 < last && ok; o0 += kTile) {
-            const int n = min(kTile, last - o0);
+            const int n = (min(kTile, last - o0) + kBox - 1) / kBox;
             for (int p = 0; p < f.passes; p++) {
-                if (!(ok = mbar_wait(EMPTY(st), ph ^ 1u, s_abort, g_err, 40u))) break;
-                const unsigned to = ring + st * f.stage_bytes;
-                const unsigned bytes = (unsigned)min(kStageK, a.width - p * kStageK) / 2;
-                if (lane == 0) mbar_expect_tx(FULL(st), n * bytes);
-                __syncwarp();
-                if (lane < n) bulk_copy(to + lane * f.pitch, a.codes + (size_t)(o0 + lane) * (a.width / 2) + p * (kStageK / 2), bytes, FULL(st));
-                const int j0 = p * (kStageK / kGroup), count = min(kStageK / kGroup, a.groups - j0);
-                for (int r = 0; r < n; r++) {
-                    const uintptr_t at = (uintptr_t)(scales + (size_t)(o0 + r) * a.groups + j0);
-                    const int words = (int)(((at & 3) + 2 * count + 3) >> 2);
-                    for (int i = lane; i < words; i += 32) copy_word(to + kTile * f.pitch + (r * f.scale_pitch + i) * 4, reinterpret_cast<const void *>((at & ~(uintptr_t)3) + 4 * i));
+                if (!(ok = mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, g_err, 40u))) break;
+                const unsigned to = ring + st * stage_bytes, full = BAR(B_FULL + st);
+                /* (what lies past the matrix comes as zeros, and counts) */
+                if (lead) mbar_expect_tx(full, n * f.lines * kBox * kLine);
+                for (int q = 0; q < n; q++) {
+                    if (f.whole) copy_lines(to + q * f.box_bytes, &tm, full, 0, o0 + q * kBox, p * (kStageK / 2 / kLine), policy, lead);
+                    else for (int c = 0; c < f.lines; c++) copy_lines(to + q * f.box_bytes + c * kBox * kLine, &tm, full, p * (kStageK / 2) + c * kLine, o0 + q * kBox, 0, policy, lead);
                 }
-                arrive_behind_copies(FULL(st));
                 if (++st == f.stages) { st = 0; ph ^= 1u; }
             }
         }
+    } else if (warp == kFinisher) {
+        /* ===================== the warps' parts, added up in the warps' order; a lane has an output and four rows ===================== */
+        const int o = lane >> 1, r0 = (lane & 1) * 4;
+        int turn = 0;
+        for (int o0 = first; o0 < last; o0 += kTile, turn++) {
+            const int buf = turn % kParts;
+            if (!mbar_wait(BAR(B_READY + buf), (turn / kParts) & 1, s_abort, g_err, 42u)) break;
+            const float *part = reinterpret_cast<const float *>(sm + kOffPart) + buf * kWarps * kPart + lane * 4;
+            float4 sum = *reinterpret_cast<const float4 *>(part);
+#pragma unroll
+            for (int w = 1; w < kWarps; w++) {
+                const float4 v = *reinterpret_cast<const float4 *>(part + w * kPart);
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf));
+            if (o0 + o < last) {
+                const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (r0 + r >= rows) break;
+                    const size_t to = (size_t)(t0 + r0 + r) * a.out_stride + o0 + o;
+                    if (a.wide) reinterpret_cast<float *>(a.out)[to] = v[r];
+                    else reinterpret_cast<T *>(a.out)[to] = type<T>::down(v[r]);
+                }
+            }
+        }
     } else {
-        /* ===================== products ===================== */
+        /* ===================== products: a warp has `mine` groups of a stage, one behind the other ===================== */
         unsigned x[kSets][kMine][4 * W];
         const T *row = reinterpret_cast<const T *>(a.x) + (size_t)(t0 + min(g, rows - 1)) * a.x_stride;
+        const int g0 = warp * f.per;
         if (P) {
 #pragma unroll
             for (int p = 0; p < kSets; p++)
 #pragma unroll
-                for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows, p * kStageK + (warp + kWarps * i) * kGroup, a.width, x[p][i]);
+                for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, x[p][i]);
         }
-        bool ok = true;
-        int turn = 0;
-        for (int o0 = first; o0 < last; o0 += kTile, turn++) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            const auto stage = [&](int p, unsigned (&xs)[kMine][4 * W]) {
-                ok = ok && mbar_wait(FULL(st), ph, s_abort, g_err, 41u);
-                if (ok) {
-                    const unsigned at = ring + st * f.stage_bytes, lo = at + g * f.pitch + t * 4 * W;
-                    const uintptr_t s_lo = (uintptr_t)(reinterpret_cast<const T *>(a.scales) + (size_t)(o0 + g) * a.groups + p * (kStageK / kGroup)), s_hi = s_lo + (size_t)8 * a.groups * 2;
-                    const unsigned sc = at + kTile * f.pitch, sc_lo = sc + g * f.scale_pitch * 4 + (unsigned)(s_lo & 2), sc_hi = sc + (g + 8) * f.scale_pitch * 4 + (unsigned)(s_hi & 2);
+        /* where the lane's words are in a stage: line c of four outputs lies behind line c - 1, its 16-byte parts in an order that goes by their address (128-byte swizzle) */
+        unsigned at[kMine];
 #pragma unroll
-                    for (int i = 0; i < kMine; i++) {
-                        const int j = warp + kWarps * i;
-                        if (p * kStageK + j * kGroup < a.width) {
-                            unsigned wl[W], wh[W];
-                            load_words<W>(lo + j * 16 * W, wl);
-                            load_words<W>(lo + 8 * f.pitch + j * 16 * W, wh);
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < kMine; i++) {
+            const unsigned in_row = (unsigned)((g0 + i) * 16 * W + t * 4 * W), line = (unsigned)(mine_of >> 2) * f.box_bytes + (in_row >> 7) * (kBox * kLine) + (unsigned)(mine_of & 3) * kLine;
+            at[i] = ring + line + ((in_row & 127u) ^ ((line >> 3) & 0x70u));
+        }
+        const unsigned eight = 2 * f.box_bytes;
+        /* Scales of the lane's two outputs, group 4 i + t of the warp's for i = 0 ..: those of a tile are asked for kAhead tiles before, into registers that nothing
+         * touches until then. */
+        unsigned short sc[kAhead + 1][kSets][kPacks][2];
+        const auto fetch = [&](int o0, int p, unsigned short (&to)[kPacks][2]) {
 #pragma unroll
-                            for (int w = 0; w < W; w++) {
-                                unsigned vl[4], vh[4];
-                                steps<T>::of(wl[w], vl);
-                                steps<T>::of(wh[w], vh);
-                                type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], xs[i][4 * w], xs[i][4 * w + 1]);
-                                type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], xs[i][4 * w + 2], xs[i][4 * w + 3]);
-                            }
-                            const float s0 = scale_at<T>(sc_lo + 2 * j), s1 = scale_at<T>(sc_hi + 2 * j);
-                            acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
-                            acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
+            for (int i = 0; i < kPacks; i++) {
+                const int j = p * (kStageK / kGroup) + g0 + 4 * i + t, o = o0 + mine_of;
+                const unsigned short *const s = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)o * a.groups + j;
+                const bool there = 4 * i + t < f.per && j < a.groups;
+                to[i][0] = to[i][1] = 0;
+                if (there && o < last) to[i][0] = s[0];
+                if (there && o + 8 < last) to[i][1] = s[(size_t)8 * a.groups];
+            }
+        };
+        const auto stage = [&](int p, unsigned (&xs)[kMine][4 * W], const unsigned short (&scales)[kPacks][2], float (&acc)[4]) {
+            const int mine = min(f.per, a.groups - p * (kStageK / kGroup) - g0);
+            if (mbar_wait(BAR(B_FULL + st), ph, s_abort, g_err, 41u)) {
+                const unsigned by = st * stage_bytes;
+                unsigned both[kPacks];
+#pragma unroll
+                for (int i = 0; i < kPacks; i++) both[i] = (unsigned)scales[i][0] | (unsigned)scales[i][1] << 16;
+#pragma unroll
+                for (int i = 0; i < kMine; i++) {
+                    if (i < mine) {
+                        unsigned wl[W], wh[W];
+                        load_words<W>(at[i] + by, wl);
+                        load_words<W>(at[i] + by + eight, wh);
+                        float d[4];
+#pragma unroll
+                        for (int w = 0; w < W; w++) {
+                            unsigned vl[4], vh[4];
+                            steps<T>::of(wl[w], vl);
+                            steps<T>::of(wh[w], vh);
+                            if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], xs[i][0], xs[i][1]);
+                            else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], xs[i][4 * w], xs[i][4 * w + 1]);
+                            type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], xs[i][4 * w + 2], xs[i][4 * w + 3]);
                         }
+                        const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
+                        const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
+                        acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
+                        acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(EMPTY(st));
-                if (++st == f.stages) { st = 0; ph ^= 1u; }
-            };
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_EMPTY + st));
+            if (++st == f.stages) { st = 0; ph ^= 1u; }
+        };
+        int turn = 0;
+        /* a tile with its scales in set `now`, those of the tile kAhead further on to set `ahead`; false: given up */
+        const auto tile = [&](int o0, unsigned short (&now)[kSets][kPacks][2], unsigned short (&ahead)[kSets][kPacks][2]) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
             if (P) {
 #pragma unroll
-                for (int p = 0; p < kSets; p++) stage(p, x[p]);
+                for (int p = 0; p < kSets; p++) fetch(o0 + kAhead * kTile, p, ahead[p]);
+#pragma unroll
+                for (int p = 0; p < kSets; p++) stage(p, x[p], now[p], acc);
             } else {
                 for (int p = 0; p < f.passes; p++) {
+                    fetch(o0, p, now[0]);
 #pragma unroll
-                    for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows, p * kStageK + (warp + kWarps * i) * kGroup, a.width, x[0][i]);
-                    stage(p, x[0]);
+                    for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, x[0][i]);
+                    stage(p, x[0], now[0], acc);
                 }
             }
-            /* the warps' sums, [output][row], added up in the warps' order by four warps of them, others for each tile */
-            float *const part = reinterpret_cast<float *>(s_raw + kOffPart) + (turn & 1) * kWarps * kPartPitch;
-            *reinterpret_cast<float2 *>(part + warp * kPartPitch + g * kRows + 2 * t) = make_float2(acc[0], acc[1]);
-            *reinterpret_cast<float2 *>(part + warp * kPartPitch + (g + 8) * kRows + 2 * t) = make_float2(acc[2], acc[3]);
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory");
-            if ((warp >> 2) == (turn & 3)) {
-                const int q = (warp & 3) * 32 + lane, o = q & 15, r = q >> 4;
-                float sum = 0.f;
+            const int buf = turn % kParts;
+            if (turn >= kParts && !mbar_wait(BAR(B_TAKEN + buf), (turn / kParts - 1) & 1, s_abort, g_err, 43u)) return false;
+            float *const part = reinterpret_cast<float *>(sm + kOffPart) + (buf * kWarps + warp) * kPart;       /* [output][row] */
+            *reinterpret_cast<float2 *>(part + mine_of * kRows + 2 * t) = make_float2(acc[0], acc[1]);
+            *reinterpret_cast<float2 *>(part + (mine_of + 8) * kRows + 2 * t) = make_float2(acc[2], acc[3]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_READY + buf));
+            turn++;
+            return true;
+        };
+        if (P) {
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) sum += part[w * kPartPitch + o * kRows + r];
-                if (r < rows && o0 + o < last) {
-                    const size_t to = (size_t)(t0 + r) * a.out_stride + o0 + o;
-                    if (a.wide) reinterpret_cast<float *>(a.out)[to] = sum;
-                    else reinterpret_cast<T *>(a.out)[to] = type<T>::down(sum);
-                }
-            }
+            for (int i = 0; i < kAhead; i++)
+#pragma unroll
+                for (int p = 0; p < kSets; p++) fetch(first + i * kTile, p, sc[i][p]);
+        }
+        for (int o0 = first; o0 < last; o0 += (kAhead + 1) * kTile) {
+            bool more = true;
+#pragma unroll
+            for (int i = 0; i <= kAhead; i++) more = more && o0 + i * kTile < last && tile(o0 + i * kTile, sc[i], sc[(i + kAhead) % (kAhead + 1)]);
+            if (!more) break;
         }
     }
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of a stage that was given up are still on their way */
-#undef FULL
-#undef EMPTY
+#undef BAR
 }
 
 template <class T, int W, int P>
-cudaError_t launch(const few_args &f, int device, int sms, void *stream) {
+cudaError_t launch(const CUtensorMap &tm, const few_args &f, int device, int sms, void *stream) {
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
-    const int smem = kOffRing + kRingBytes;
     cudaError_t e;
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
-        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
-    hy3a_launch l(dim3(f.a.out_width < sms ? f.a.out_width : sms, (f.a.rows + kRows - 1) / kRows), dim3(kThreads), smem, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P>, f);
+    const int boxes = (f.a.out_width + kBox - 1) / kBox;
+    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(kThreads), kSmem, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P>, tm, f);
 }
 template <class T, int W>
-cudaError_t launch_passes(const few_args &f, int device, int sms, void *stream) {
-    return f.passes == 1 ? launch<T, W, 1>(f, device, sms, stream) : (f.passes == 2 ? launch<T, W, 2>(f, device, sms, stream) : launch<T, W, 0>(f, device, sms, stream));
+cudaError_t launch_group(const CUtensorMap &tm, const few_args &f, int device, int sms, void *stream) {
+    if (f.passes == 1) return launch<T, W, 1>(tm, f, device, sms, stream);
+    constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers) */
+    return f.passes == 2 ? launch<T, W, kTwo>(tm, f, device, sms, stream) : launch<T, W, 0>(tm, f, device, sms, stream);
 }
 template <class T>
-cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream) {
-    const int words = a.group / 32, k = a.width < kStageK ? a.width : kStageK;
-    few_args f = {a, ((k / 2 + 127) & ~127) + 16 * words, ((k + a.group - 1) / a.group / 2 + 1) | 1, 0, 0, (a.width + kStageK - 1) / kStageK};
-    f.stage_bytes = kTile * (f.pitch + 4 * f.scale_pitch);
-    f.stages = kRingBytes / f.stage_bytes < kMaxStages ? kRingBytes / f.stage_bytes : kMaxStages;
-    if (words == 1) return launch_passes<T, 1>(f, device, sms, stream);
-    if (words == 2) return launch_passes<T, 2>(f, device, sms, stream);
-    return launch_passes<T, 4>(f, device, sms, stream);
+cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream, const char **what) {
+    const int k = a.width < kStageK ? a.width : kStageK, bytes = a.width / 2;
+    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, ((k + a.group - 1) / a.group + kWarps - 1) / kWarps, bytes % kLine == 0};
+    f.box_bytes = (f.lines | 1) * kBox * kLine;
+    f.stages = kRingBytes / (kTile / kBox * f.box_bytes);
+    if (f.stages > kMaxStages) f.stages = kMaxStages;
+    /* rows of whole lines: [lines][outputs][128 bytes], all lines of a stage in a copy; else [outputs][bytes], a line in a copy */
+    CUtensorMap tm;
+    const encode_tiled_fn enc = encoder();
+    const cuuint64_t dims[3] = {(cuuint64_t)(f.whole ? kLine : bytes), (cuuint64_t)a.out_width, (cuuint64_t)(f.whole ? bytes / kLine : 1)}, strides[2] = {(cuuint64_t)bytes, (cuuint64_t)(f.whole ? kLine : 16)};
+    const cuuint32_t box[3] = {kLine, kBox, (cuuint32_t)(f.whole ? f.lines : 1)}, one[3] = {1, 1, 1};
+    if (!enc || enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        *what = "no tensor map (cuTensorMapEncodeTiled)";
+        return cudaErrorInvalidValue;
+    }
+    if (a.group == 32) return launch_group<T, 1>(tm, f, device, sms, stream);
+    if (a.group == 64) return launch_group<T, 2>(tm, f, device, sms, stream);
+    return launch_group<T, 4>(tm, f, device, sms, stream);
 }
 
 } /* namespace */
@@ -243,8 +327,9 @@ extern "C" int hy3a_linear4(void *stream, int dtype, int rows, int width, int ou
     int dev, sms;
     if ((rc = hy3a_layer_device("linear4", &dev, &sms))) return rc;
     const linear4_args a = {x, x_stride, (const uint8_t *)codes, scales, out, out_stride, rows, width, out_width, group, (width + group - 1) / group, out_dtype == HY3A_F32};
-    const cudaError_t e = dtype == HY3A_BF16 ? launch_few<__nv_bfloat16>(a, dev, sms, stream) : launch_few<__half>(a, dev, sms, stream);
-    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "linear4: %s", cudaGetErrorString(e));
+    const char *what = NULL;
+    const cudaError_t e = dtype == HY3A_BF16 ? launch_few<__nv_bfloat16>(a, dev, sms, stream, &what) : launch_few<__half>(a, dev, sms, stream, &what);
+    if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "linear4: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;
 }
 
