@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhy3attn.so")
 DROPIN_LIB = os.path.join(HERE, "libhy3_gpu.so")
 NATIVE = os.path.join(HERE, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
-SOURCES = ["append.cu", "decode.cu", "decode_umma.cu", "prefill.cu", "route.cu", "experts.cu", "experts_umma.cu", "adapters.cu", "quantize4.cu", "linear4.cu", "logprobs.cu", "capi.cu", "selftest.cu"]
+SOURCES = ["append.cu", "decode.cu", "decode_umma.cu", "prefill.cu", "route.cu", "experts.cu", "experts_umma.cu", "adapters.cu", "quantize4.cu", "linear4.cu", "linear4_umma.cu", "logprobs.cu", "capi.cu", "selftest.cu"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC,-fvisibility=default", "-I", os.path.join(ROOT, "include")]
 

@@ -24,10 +24,10 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2), kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16;
+constexpr int kMostWarps = 16, kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16;
 constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
 constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
-constexpr int kRingBytes = 180 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
+constexpr int kRingBytes = 180 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kMostWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
 enum { B_FULL = 0, B_EMPTY = kMaxStages, B_READY = 2 * kMaxStages, B_TAKEN = 2 * kMaxStages + kParts, B_COUNT = 2 * kMaxStages + 2 * kParts };
 static_assert(8 * B_COUNT <= 512, "barriers");
 
@@ -35,7 +35,7 @@ __device__ unsigned g_err[2];         /* {code, where} of the first wait that ra
 
 struct few_args {
     linear4_args a;
-    int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stages, passes /* stages of a tile */, per /* groups of a warp in a stage */;
+    int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stages, passes /* stages of a tile */, in_stage /* groups of a stage */, per /* of a warp */;
     int whole;                /* rows of codes are whole lines */
 };
 
@@ -78,10 +78,10 @@ template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsig
 }
 
 /* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each */
-template <class T, int W, int P>
-__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm, const few_args f) {
+template <class T, int W, int P, int kWarps>
+__global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm, const few_args f) {
     extern __shared__ uint8_t s_raw[];
-    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kAhead = P == 1 ? 2 : (P ? 1 : 0) /* tiles */;
+    constexpr int kProducer = kWarps, kFinisher = kWarps + 1, kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kAhead = P == 1 ? 2 : (P ? 1 : 0) /* tiles */;
     const linear4_args &a = f.a;
     uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT);
@@ -191,27 +191,32 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                 unsigned both[kPacks];
 #pragma unroll
                 for (int i = 0; i < kPacks; i++) both[i] = (unsigned)scales[i][0] | (unsigned)scales[i][1] << 16;
+                const auto group = [&](int i) {
+                    unsigned wl[W], wh[W];
+                    load_words<W>(at[i] + by, wl);
+                    load_words<W>(at[i] + by + eight, wh);
+                    float d[4];
 #pragma unroll
-                for (int i = 0; i < kMine; i++) {
-                    if (i < mine) {
-                        unsigned wl[W], wh[W];
-                        load_words<W>(at[i] + by, wl);
-                        load_words<W>(at[i] + by + eight, wh);
-                        float d[4];
-#pragma unroll
-                        for (int w = 0; w < W; w++) {
-                            unsigned vl[4], vh[4];
-                            steps<T>::of(wl[w], vl);
-                            steps<T>::of(wh[w], vh);
-                            if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], xs[i][0], xs[i][1]);
-                            else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], xs[i][4 * w], xs[i][4 * w + 1]);
-                            type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], xs[i][4 * w + 2], xs[i][4 * w + 3]);
-                        }
-                        const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
-                        const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
-                        acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
-                        acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
+                    for (int w = 0; w < W; w++) {
+                        unsigned vl[4], vh[4];
+                        steps<T>::of(wl[w], vl);
+                        steps<T>::of(wh[w], vh);
+                        if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], xs[i][0], xs[i][1]);
+                        else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], xs[i][4 * w], xs[i][4 * w + 1]);
+                        type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], xs[i][4 * w + 2], xs[i][4 * w + 3]);
                     }
+                    const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
+                    const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
+                    acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
+                    acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
+                };
+                /* (without branches between them the groups' chains overlap) */
+                if (mine == kMine) {
+#pragma unroll
+                    for (int i = 0; i < kMine; i++) group(i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kMine; i++) if (i < mine) group(i);
                 }
             }
             __syncwarp();
@@ -263,16 +268,18 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
 }
 
 template <class T, int W, int P>
-cudaError_t launch(const CUtensorMap &tm, const few_args &f, int device, int sms, void *stream) {
+cudaError_t launch(const CUtensorMap &tm, few_args f, int device, int sms, void *stream) {
+    constexpr int kWarps = 16;
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     cudaError_t e;
+    f.per = (f.in_stage + kWarps - 1) / kWarps;
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
-        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P, kWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
     const int boxes = (f.a.out_width + kBox - 1) / kBox;
-    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(kThreads), kSmem, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P>, tm, f);
+    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(32 * (kWarps + 2)), kSmem, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, kWarps>, tm, f);
 }
 template <class T, int W>
 cudaError_t launch_group(const CUtensorMap &tm, const few_args &f, int device, int sms, void *stream) {
@@ -283,7 +290,7 @@ cudaError_t launch_group(const CUtensorMap &tm, const few_args &f, int device, i
 template <class T>
 cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream, const char **what) {
     const int k = a.width < kStageK ? a.width : kStageK, bytes = a.width / 2;
-    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, ((k + a.group - 1) / a.group + kWarps - 1) / kWarps, bytes % kLine == 0};
+    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0};
     f.box_bytes = (f.lines | 1) * kBox * kLine;
     f.stages = kRingBytes / (kTile / kBox * f.box_bytes);
     if (f.stages > kMaxStages) f.stages = kMaxStages;
@@ -328,7 +335,8 @@ extern "C" int hy3a_linear4(void *stream, int dtype, int rows, int width, int ou
     if ((rc = hy3a_layer_device("linear4", &dev, &sms))) return rc;
     const linear4_args a = {x, x_stride, (const uint8_t *)codes, scales, out, out_stride, rows, width, out_width, group, (width + group - 1) / group, out_dtype == HY3A_F32};
     const char *what = NULL;
-    const cudaError_t e = dtype == HY3A_BF16 ? launch_few<__nv_bfloat16>(a, dev, sms, stream, &what) : launch_few<__half>(a, dev, sms, stream, &what);
+    const cudaError_t e = rows > kRows ? hy3a_linear4_launch_many(a, dtype, dev, sms, stream, &what)
+                        : (dtype == HY3A_BF16 ? launch_few<__nv_bfloat16>(a, dev, sms, stream, &what) : launch_few<__half>(a, dev, sms, stream, &what));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "linear4: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;
 }
@@ -341,6 +349,6 @@ cudaError_t hy3a_linear4_wait_out(void *stream) {
 cudaError_t hy3a_linear4_error(unsigned *err) {
     const unsigned none[2] = {0, 0};
     cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
-    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
-    return e;
+    if (e == cudaSuccess && err[0]) return cudaMemcpyToSymbol(g_err, none, sizeof(none));
+    return e == cudaSuccess ? hy3a_linear4_many_error(err) : e;
 }

@@ -15,6 +15,10 @@ struct linear4_args {
     int wide;                 /* out is fp32 */
 };
 
+/* linear4_umma.cu: any number of rows; *what: why, where it is not CUDA's error */
+cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, int sms, void *stream, const char **what);
+cudaError_t hy3a_linear4_many_error(unsigned *err);
+
 namespace hy3a_layer {
 
 /* Codes become numbers of the rows' type by their bits: with a code c in the lowest bits of the mantissa, 0x4300 | c is 128 + c in bf16 and 0x6400 | c is 1024 + c in

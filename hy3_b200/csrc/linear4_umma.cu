@@ -1,0 +1,389 @@
+/*
+ * linear4_umma.cu -- rows through a matrix in 4 bits, many rows: on 5th-generation tensor cores (tcgen05 + TMEM + TMA).
+ *
+ * The weights are the M side of the product and the rows its N side (up to 256).  A pair of CTAs (cta_group::2) works on 256 outputs: each has 128 of them, and half of the
+ * rows of x in shared memory.  Codes become weights on their way: a thread has an output, reads its codes of 64 k's from shared memory, and stores (code - 8) * scale
+ * as the A operand into tensor memory, from where the product takes it; shared memory sees 4 bits a weight, and the tensor cores read only x from there.  Per CTA:
+ *   warps 0-7 weights: each four of them (a lane quarter each) every other step of 64 k's; afterwards the results;
+ *   warp 8    TMA producer: codes, 128 k's at a time, and x, 64 k's at a time;
+ *   warp 9    MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
+ *
+ * Rounding: a weight has up to 15 bits (fp16) or 11 (bf16).  Where the result is of the rows' type the weight is rounded to it once; where the result is fp32 it enters as
+ * two numbers, the rounded one and the rest, which is exact.  Results that are not finite (a rounded weight over the type's largest, an infinite x that meets the rest)
+ * are computed again from the definition, by the warp that finds them.
+ *
+ * Where tiles are few, the CTAs of a cluster share the k's of a tile; their sums meet in shared memory, and are added in the order of the k's.
+ *
+ * Every wait is bounded; one that runs out raises the CTA's abort flag and a code in the error word (hy3a_layer_sync), lets all warps fall through, and TMEM is always
+ * released.
+ */
+#include <atomic>
+
+#include "linear4.h"
+#include "ring.cuh"
+
+namespace {
+
+using namespace hy3a_layer;
+using namespace hy3a_ring;
+
+constexpr int kWorkers = 8, kProducer = kWorkers, kIssuer = kWorkers + 1, kThreads = 32 * (kWorkers + 2);
+constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
+constexpr int kMostSteps = 8, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kMostSteps * kStepBytes, kSmem = kOffBar + 512 + 1024;
+constexpr int kAColumn = 256;          /* tensor memory: the sums, then the stages of A */
+enum { B_CODES = 0, B_CODES_FREE = kUnits, B_X = 2 * kUnits, B_A = 2 * kUnits + kMostSteps, B_FREE = 2 * kUnits + 2 * kMostSteps, B_SUMS = 2 * kUnits + 3 * kMostSteps, B_COUNT };
+static_assert(8 * B_COUNT + 16 <= 512, "barriers");
+static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
+
+__device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
+
+struct many_args {
+    linear4_args a;
+    int columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits;
+};
+
+__device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ unsigned cluster_addr(unsigned addr, unsigned rank) {
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void tma_codes(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, unsigned long long policy, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %6, 0;\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "l"(policy), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void tma_rows(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %5, 0;\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(lead) : "memory");
+}
+/* K-major operand, 128-byte swizzle: 8-row groups 1024 B apart, descriptor version 1, layout 2 */
+__device__ __forceinline__ unsigned long long make_desc(unsigned saddr) {
+    return (unsigned long long)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+/* A in tensor memory */
+__device__ __forceinline__ void umma_lead(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate, unsigned lead) {
+    asm volatile("{\n .reg .pred p, e;\n setp.ne.b32 e, %5, 0;\n setp.ne.b32 p, %4, 0;\n @e tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void umma_commit_lead(unsigned bar, unsigned short ctas, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}"
+                 ::"r"(bar), "r"(lead), "h"(ctas) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+template <class T> struct pair_of;
+template <> struct pair_of<__nv_bfloat16> {
+    static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
+};
+template <> struct pair_of<__half> {
+    static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
+};
+
+/* out[t][o] from the definition, by a warp */
+template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {
+    const int lane = threadIdx.x & 31;
+    const T *const x = reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride, *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
+    const uint8_t *const codes = a.codes + (size_t)o * (a.width / 2);
+    float sum = 0.f;
+    for (int k = 2 * lane; k < a.width; k += 64) {
+        const int both = codes[k >> 1];
+        const float s = type<T>::up(scales[k / a.group]);
+        sum = fmaf((float)((both & 15) - 8) * s, type<T>::up(x[k]), sum);
+        sum = fmaf((float)((both >> 4) - 8) * s, type<T>::up(x[k + 1]), sum);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    return sum;
+}
+/* v of the lanes that are `mine`, of output o and row t: what is not finite is computed again */
+template <class T> __device__ __forceinline__ float settled(const linear4_args &a, float v, bool mine, int t, int o) {
+    unsigned todo = __ballot_sync(0xffffffffu, mine && !(fabsf(v) < INFINITY));
+    while (todo) {
+        const int l = __ffs(todo) - 1;
+        const float again = plain<T>(a, __shfl_sync(0xffffffffu, t, l), __shfl_sync(0xffffffffu, o, l));
+        if ((int)(threadIdx.x & 31) == l) v = again;
+        todo &= todo - 1;
+    }
+    return v;
+}
+
+/* WIDE: the result is fp32, weights are two numbers.  PER: scales of 64 k's (groups of 32: two) */
+template <class T, bool WIDE, int PER>
+__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
+    extern __shared__ uint8_t s_raw[];
+    constexpr int kSteps = WIDE ? 4 : 8 /* stages of x and A */, kAWide = WIDE ? 64 : 32 /* columns of a stage of A */;
+    const linear4_args &a = f.a;
+    uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
+    const unsigned sbase = smem_u32(sm), bar0 = sbase + kOffBar;
+    volatile unsigned *s_tmem = reinterpret_cast<volatile unsigned *>(sm + kOffBar + 8 * B_COUNT);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT + 4);
+#define BAR(i) (bar0 + 8u * (unsigned)(i))
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31;
+    const unsigned me = cluster_rank(), leader = me & ~1u, rank = me & 1u;
+    const int split = me >> 1, tile = blockIdx.x / (2 * f.splits), m_tile = tile % f.m_tiles, row0 = tile / f.m_tiles * f.columns;
+    const int u0 = (int)((long long)f.units * split / f.splits), u1 = (int)((long long)f.units * (split + 1) / f.splits), steps = 2 * (u1 - u0);
+    const int m0 = m_tile * 256 + (int)rank * 128, N = f.columns, rows = min(N, a.rows - row0);
+
+    if (tid == 0) {
+        *s_abort = 0;
+        for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), kWorkers); }
+        for (int i = 0; i < kSteps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), kWorkers /* four of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
+        mbar_init(BAR(B_SUMS), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kProducer && lane < 2) {
+        const CUtensorMap *m = lane == 0 ? &tm_codes : &tm_x;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar0 + 8u * B_COUNT), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = *s_tmem;
+    pdl_release();
+    pdl_wait();
+
+    if (warp == kProducer) {
+        /* ===================== producer ===================== */
+        const unsigned lead = elect_one();
+        unsigned long long policy;
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        int unit = 0, st = 0;
+        unsigned uph = 0, ph = 0;
+        bool ok = true;
+        /* (codes run ahead of x: as far as their ring goes) */
+        int asked = u0;
+        for (int s = 0; s < steps && ok; s++) {
+            while (asked < u1 && asked - u0 - (s >> 1) < kUnits) {
+                if (!(ok = mbar_wait(BAR(B_CODES_FREE + unit), uph ^ 1u, s_abort, g_err, 50u))) break;
+                if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
+                tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), asked * (kUnit / 2), m0, policy, lead);
+                asked++;
+                if (++unit == kUnits) { unit = 0; uph ^= 1u; }
+            }
+            if (!ok || !(ok = mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
+            if (lead && rank == 0) mbar_expect_tx(BAR(B_X + st), N * 128);
+            tma_rows(sbase + kOffX + st * kStepBytes, &tm_x, cluster_addr(BAR(B_X + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
+            if (++st == kSteps) { st = 0; ph ^= 1u; }
+        }
+        /* the last commits reach the barriers of both CTAs before either leaves */
+        for (int i = 0; i < kSteps && !*s_abort; i++) {
+            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 52u)) break;
+            if (++st == kSteps) { st = 0; ph ^= 1u; }
+        }
+    } else if (warp == kIssuer) {
+        if (rank == 0) {
+            /* ===================== MMA issuer: uniform control flow, one elected lane issues ===================== */
+            const unsigned lead = elect_one();
+            constexpr unsigned kType = type<T>::code == HY3A_BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const unsigned idesc = (1u << 4) | kType | (((unsigned)N >> 3) << 17) | ((256u >> 4) << 24);
+            const unsigned short both = (unsigned short)(3u << leader);
+            int st = 0;
+            unsigned ph = 0;
+            bool ok = true;
+            for (int s = 0; s < steps; s++) {
+                if (!(ok = mbar_wait(BAR(B_X + st), ph, s_abort, g_err, 53u) && mbar_wait(BAR(B_A + st), ph, s_abort, g_err, 54u))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned long long db = make_desc(sbase + kOffX + st * kStepBytes);
+                const unsigned da = tmem + kAColumn + st * kAWide;
+#pragma unroll
+                for (int k = 0; k < 4; k++) umma_lead(tmem, da + 8 * k, db + 2 * k, idesc, s + k > 0, lead);
+                if (WIDE) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) umma_lead(tmem, da + 32 + 8 * k, db + 2 * k, idesc, 1, lead);
+                }
+                umma_commit_lead(BAR(B_FREE + st), both, lead);
+                if (++st == kSteps) { st = 0; ph ^= 1u; }
+            }
+            if (ok) umma_commit_lead(BAR(B_SUMS), both, lead);
+        }
+    } else {
+        /* ===================== weights: a thread has an output; each four warps every other step ===================== */
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, o = m0 + r;
+        const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
+        const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
+        const unsigned to_a = tmem + kAColumn + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
+        unsigned short sc[3][PER];
+        const auto fetch = [&](int s, unsigned short (&to)[PER]) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int j = (u0 * kUnit + s * 64 + 32 * i) >> shift;
+                to[i] = 0;
+                if (s < steps && j < a.groups) to[i] = scales[j];
+            }
+        };
+        int st = half, unit = 0;
+        unsigned ph = 0, uph = 0;
+        const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
+            fetch(s + 4, ahead);
+            if (!mbar_wait(BAR(B_CODES + unit), uph, s_abort, g_err, 55u)) return false;
+            uint4 c[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const unsigned at = from + unit * kUnitBytes + (((unsigned)(half * 2 + i) ^ turn) << 4);
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[i].x), "=r"(c[i].y), "=r"(c[i].z), "=r"(c[i].w) : "r"(at));
+            }
+            const unsigned w[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
+            unsigned hi[32], lo[WIDE ? 32 : 1];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const unsigned s2 = __byte_perm(now[i * PER / 8], 0, 0x1010);
+                unsigned v[4];
+                hy3a_layer::steps<T>::of(w[i], v);
+                const unsigned n[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    hi[4 * i + j] = pair_of<T>::mul(n[j], s2);
+                    if (WIDE) lo[WIDE ? 4 * i + j : 0] = pair_of<T>::rest(n[j], s2, hi[4 * i + j]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(B_CODES_FREE + unit));
+            if (++unit == kUnits) { unit = 0; uph ^= 1u; }
+            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            tmem_st32(to_a + st * kAWide, hi);
+            if constexpr (WIDE) tmem_st32(to_a + st * kAWide + 32, lo);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_A + st), leader));
+            st += 2;
+            if (st >= kSteps) { st -= kSteps; ph ^= 1u; }
+            return true;
+        };
+        fetch(half, sc[0]);
+        fetch(half + 2, sc[1]);
+        bool ok = true;
+        for (int s = half; s < steps && ok; s += 6) {
+            ok = step(s, sc[0], sc[2]);
+            if (ok && s + 2 < steps) ok = step(s + 2, sc[1], sc[0]);
+            if (ok && s + 4 < steps) ok = step(s + 4, sc[2], sc[1]);
+        }
+        /* ===================== results: a lane has an output, the warp every other 16 rows ===================== */
+        if (ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 57u)) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int c0 = half * 16; c0 < rows; c0 += 32) {
+                unsigned v[16];
+                tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    if (c0 + j >= rows) break;
+                    if (f.splits > 1) { *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = __uint_as_float(v[j]); continue; }
+                    const bool mine = o < a.out_width;
+                    const float y = settled<T>(a, __uint_as_float(v[j]), mine, row0 + c0 + j, o);
+                    if (!mine) continue;
+                    const size_t to = (size_t)(row0 + c0 + j) * a.out_stride + o;
+                    if (WIDE) reinterpret_cast<float *>(a.out)[to] = y;
+                    else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the step that was given up are still on their way */
+    cluster_sync();
+    if (f.splits > 1) {
+        /* each CTA adds up the rows of its share, in the order of the k's */
+        if (warp < kWorkers && !*s_abort) {
+            const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
+            for (int c = first + (tid >> 7); c < last; c += 2) {
+                float y = 0.f;
+                for (int i = 0; i < f.splits; i++) {
+                    float v;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(sbase + (c * 128 + r) * 4, 2 * i + rank)) : "memory");
+                    y += v;
+                }
+                const bool mine = o < a.out_width;
+                y = settled<T>(a, y, mine, row0 + c, o);
+                if (!mine) continue;
+                const size_t to = (size_t)(row0 + c) * a.out_stride + o;
+                if (WIDE) reinterpret_cast<float *>(a.out)[to] = y;
+                else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == kIssuer) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+#undef BAR
+}
+
+template <class T, bool WIDE, int PER>
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
+    static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
+    cudaError_t e;
+    if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
+        if ((e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if (device < 64) ready[device].store(true, std::memory_order_release);
+    }
+    hy3a_launch l(dim3((unsigned)tiles * 2 * f.splits), dim3(kThreads), kSmem, stream);
+    l.cluster(2 * f.splits);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_umma_kernel<T, WIDE, PER>, codes, x, f);
+}
+template <class T>
+cudaError_t launch_type(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
+    if (f.a.group == 32) return f.a.wide ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 2>(codes, x, f, tiles, device, stream);
+    return f.a.wide ? launch<T, true, 1>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
+}
+
+} /* namespace */
+
+cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, int sms, void *stream, const char **what) {
+    many_args f = {a, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1};
+    const int pairs = sms / 2;
+    /* Row tiles: as few as there have to be, or more where their tiles then take less time: rounds of all pairs times a tile's rows. */
+    int row_tiles = (a.rows + 255) / 256;
+    long long least = -1;
+    for (int n = row_tiles; n <= row_tiles + 4; n++) {
+        const int columns = ((a.rows + n - 1) / n + 15) & ~15, need = (a.rows + columns - 1) / columns;
+        const long long rounds = ((long long)need * f.m_tiles + pairs - 1) / pairs, cost = rounds * (columns + 32);
+        if (least < 0 || cost < least) { least = cost; row_tiles = need; f.columns = columns; }
+    }
+    const long long tiles = (long long)row_tiles * f.m_tiles;
+    while (f.splits < 4 && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
+    *what = NULL;
+    CUtensorMap codes, x;
+    const encode_tiled_fn enc = encoder();
+    const cuuint64_t dims[2] = {(cuuint64_t)(a.width / 2), (cuuint64_t)a.out_width}, strides[1] = {(cuuint64_t)(a.width / 2)};
+    const cuuint32_t box[2] = {kUnit / 2, 128}, one[2] = {1, 1};
+    const bool ok = enc && enc(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS &&
+                    encode(&x, 2, a.x, a.width, a.rows, 1, a.x_stride, 64, f.columns / 2);
+    if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
+    if (tiles * 2 * f.splits > 0x7fffffffll) { *what = "too many tiles"; return cudaErrorInvalidValue; }
+    return dtype == HY3A_BF16 ? launch_type<__nv_bfloat16>(codes, x, f, (int)tiles, device, stream) : launch_type<__half>(codes, x, f, (int)tiles, device, stream);
+}
+
+cudaError_t hy3a_linear4_many_error(unsigned *err) {
+    const unsigned none[2] = {0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
+    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
+    return e;
+}
