@@ -37,6 +37,7 @@ struct few_args {
     linear4_args a;
     int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stages, passes /* stages of a tile */, in_stage /* groups of a stage */, per /* of a warp */;
     int whole;                /* rows of codes are whole lines */
+    unsigned zero;            /* 0, which the compiler does not know */
 };
 
 /* Copies are issued in uniform control flow by one elected lane (lead): a lane's own operands cost each 50 clocks and more. */
@@ -220,7 +221,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(cons
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(B_EMPTY + st));
+            /* (an arrival does not wait for loads that are under way, so it takes something of the sums that they went into) */
+            if (lane == 0) mbar_arrive(BAR(B_EMPTY + st) + ((__float_as_uint(acc[0]) | __float_as_uint(acc[2])) & f.zero));
             if (++st == f.stages) { st = 0; ph ^= 1u; }
         };
         int turn = 0;
@@ -290,7 +292,7 @@ cudaError_t launch_group(const CUtensorMap &tm, const few_args &f, int device, i
 template <class T>
 cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream, const char **what) {
     const int k = a.width < kStageK ? a.width : kStageK, bytes = a.width / 2;
-    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0};
+    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0, 0u};
     f.box_bytes = (f.lines | 1) * kBox * kLine;
     f.stages = kRingBytes / (kTile / kBox * f.box_bytes);
     if (f.stages > kMaxStages) f.stages = kMaxStages;

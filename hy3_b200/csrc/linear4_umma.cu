@@ -4,9 +4,9 @@
  * The weights are the M side of the product and the rows its N side (up to 256).  A pair of CTAs (cta_group::2) works on 256 outputs: each has 128 of them, and half of the
  * rows of x in shared memory.  Codes become weights on their way: a thread has an output, reads its codes of 64 k's from shared memory, and stores (code - 8) * scale
  * as the A operand into tensor memory, from where the product takes it; shared memory sees 4 bits a weight, and the tensor cores read only x from there.  Per CTA:
- *   warps 0-7 weights: each four of them (a lane quarter each) every other step of 64 k's; afterwards the results;
- *   warp 8    TMA producer: codes, 128 k's at a time, and x, 64 k's at a time;
- *   warp 9    MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
+ *   warps 0-15 weights: each four of them (a lane quarter each) every fourth step of 64 k's; afterwards the results;
+ *   warp 16   TMA producer: codes, 128 k's at a time, and x, 64 k's at a time;
+ *   warp 17   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
  *
  * Rounding: a weight has up to 15 bits (fp16) or 11 (bf16).  Where the result is of the rows' type the weight is rounded to it once; where the result is fp32 it enters as
  * two numbers, the rounded one and the rest, which is exact.  Results that are not finite (a rounded weight over the type's largest, an infinite x that meets the rest)
@@ -27,12 +27,13 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kWorkers = 8, kProducer = kWorkers, kIssuer = kWorkers + 1, kThreads = 32 * (kWorkers + 2);
+constexpr int kTeams = 4 /* of four warps: a warp for each 32 outputs */, kWorkers = 4 * kTeams, kProducer = kWorkers, kIssuer = kWorkers + 1, kThreads = 32 * (kWorkers + 2);
 constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
 constexpr int kMostSteps = 8, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kMostSteps * kStepBytes, kSmem = kOffBar + 512 + 1024;
 constexpr int kAColumn = 256;          /* tensor memory: the sums, then the stages of A */
 enum { B_CODES = 0, B_CODES_FREE = kUnits, B_X = 2 * kUnits, B_A = 2 * kUnits + kMostSteps, B_FREE = 2 * kUnits + 2 * kMostSteps, B_SUMS = 2 * kUnits + 3 * kMostSteps, B_COUNT };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
+static_assert(kMostSteps % kTeams == 0 && kUnits % (kTeams / 2) == 0, "teams' turns");
 static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
@@ -52,7 +53,9 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+/* Relaxed: what it tells of lies in tensor memory, is waited for (tcgen05.wait::st) and ordered by tcgen05.fence::before_thread_sync.  A release in the cluster's scope would
+ * wait for all else that the warp has under way, the scales asked for ahead among it (64 rows on 10240 x 4096: 49 us). */
+__device__ __forceinline__ void mbar_arrive_cluster(unsigned bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void tma_codes(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, unsigned long long policy, unsigned lead) {
     asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %6, 0;\n"
                  " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;\n}"
@@ -144,8 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
 
     if (tid == 0) {
         *s_abort = 0;
-        for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), kWorkers); }
-        for (int i = 0; i < kSteps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), kWorkers /* four of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
+        for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), 8 /* two teams */); }
+        for (int i = 0; i < kSteps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), 8 /* a team of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
         mbar_init(BAR(B_SUMS), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -220,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             if (ok) umma_commit_lead(BAR(B_SUMS), both, lead);
         }
     } else {
-        /* ===================== weights: a thread has an output; each four warps every other step ===================== */
-        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane, o = m0 + r;
+        /* ===================== weights: a thread has an output; each team takes every fourth step ===================== */
+        const int quarter = warp & 3, team = warp >> 2, half = team & 1 /* of a unit */, r = quarter * 32 + lane, o = m0 + r;
         const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
         const unsigned to_a = tmem + kAColumn + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
@@ -234,10 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
                 if (s < steps && j < a.groups) to[i] = scales[j];
             }
         };
-        int st = half, unit = 0;
+        int st = team, unit = team >> 1;
         unsigned ph = 0, uph = 0;
         const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
-            fetch(s + 4, ahead);
+            fetch(s + 2 * kTeams, ahead);
             if (!mbar_wait(BAR(B_CODES + unit), uph, s_abort, g_err, 55u)) return false;
             uint4 c[2];
 #pragma unroll
@@ -259,33 +262,35 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
                     if (WIDE) lo[WIDE ? 4 * i + j : 0] = pair_of<T>::rest(n[j], s2, hi[4 * i + j]);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(B_CODES_FREE + unit));
-            if (++unit == kUnits) { unit = 0; uph ^= 1u; }
             if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
+            __syncwarp();              /* (lanes may leave the wait one by one; what follows is the whole warp's) */
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             tmem_st32(to_a + st * kAWide, hi);
             if constexpr (WIDE) tmem_st32(to_a + st * kAWide + 32, lo);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_A + st), leader));
-            st += 2;
+            /* (the codes are given back behind a store that needed them: an arrival does not wait for loads that are under way) */
+            if (lane == 0) { mbar_arrive_cluster(cluster_addr(BAR(B_A + st), leader)); mbar_arrive(BAR(B_CODES_FREE + unit)); }
+            unit += kTeams / 2;
+            if (unit >= kUnits) { unit -= kUnits; uph ^= 1u; }
+            st += kTeams;
             if (st >= kSteps) { st -= kSteps; ph ^= 1u; }
             return true;
         };
-        fetch(half, sc[0]);
-        fetch(half + 2, sc[1]);
+        fetch(team, sc[0]);
+        fetch(team + kTeams, sc[1]);
         bool ok = true;
-        for (int s = half; s < steps && ok; s += 6) {
+        for (int s = team; s < steps && ok; s += 3 * kTeams) {
             ok = step(s, sc[0], sc[2]);
-            if (ok && s + 2 < steps) ok = step(s + 2, sc[1], sc[0]);
-            if (ok && s + 4 < steps) ok = step(s + 4, sc[2], sc[1]);
+            if (ok && s + kTeams < steps) ok = step(s + kTeams, sc[1], sc[0]);
+            if (ok && s + 2 * kTeams < steps) ok = step(s + 2 * kTeams, sc[2], sc[1]);
         }
-        /* ===================== results: a lane has an output, the warp every other 16 rows ===================== */
+        /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
         if (ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 57u)) {
+            __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int c0 = half * 16; c0 < rows; c0 += 32) {
+            for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
                 unsigned v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
 #pragma unroll
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
         /* each CTA adds up the rows of its share, in the order of the k's */
         if (warp < kWorkers && !*s_abort) {
             const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
-            for (int c = first + (tid >> 7); c < last; c += 2) {
+            for (int c = first + (tid >> 7); c < last; c += kTeams) {
                 float y = 0.f;
                 for (int i = 0; i < f.splits; i++) {
                     float v;
