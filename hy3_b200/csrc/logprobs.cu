@@ -7,11 +7,12 @@
  * alone: a token that is nearly certain keeps the digits of its log probability.  The terms of H are all positive.
  *
  * A row is a block's, or the blocks' of a cluster where rows are few.  A warp shares m, so that it seldom rises: past the first vectors nearly all take the
- * branch without it.
+ * branch without it, and of those that raise it only the vectors that have the new m are looked at logit by logit.
  *
- * The top k are found without a second pass over the row: a thread keeps its largest logit and the vector of 16 bytes that had it; the k-th largest of 128
- * such keys, of four threads each, is no larger than the k-th largest logit; the few threads whose own key reaches it look through their vectors again, and the few logits
- * that reach it are ranked by (value, lowest index).  Rows with a NaN or an infinity, and rows where too many reach it, are searched k times instead.
+ * The top k are found without a second pass over the row: a thread keeps its largest logit and the vector of 16 bytes that had it; the k-th largest of 32
+ * such keys, of the threads of a lane each, is no larger than the k-th largest logit; the few threads whose own key reaches it look through their vectors again (the last
+ * ones are still in registers), and the few logits that reach it are ranked by (value, lowest index).  Rows with a NaN or an infinity, and rows where too many reach
+ * it, are searched k times instead.
  */
 #include <math.h>
 
@@ -21,8 +22,10 @@ namespace {
 
 using namespace hy3a_layer;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
-constexpr int kKeys = 128;                    /* groups of threads among whose largest logits the threshold is looked for */
+/* Threads of a block: four blocks an SM where a row is a block's, so that one's end runs beside the others' loads; two where it is a cluster's, so that a row of 131072 logits is
+ * one round of loads. */
+constexpr int kAlone = 256, kShared = 512, kMaxCluster = 8;
+constexpr int kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
 constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
 
 struct logprobs_args {
@@ -46,9 +49,8 @@ __device__ __forceinline__ unsigned peer(const void *p, unsigned rank) {
     asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(a) : "r"(rank));
     return a;
 }
-__device__ __forceinline__ float peer_float(const float *p, unsigned rank) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer(p, rank)) : "memory"); return v; }
 __device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }      /* (not of NaN) */
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -57,7 +59,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 /* What is kept of some logits: their maximum m, how many equal it, the sum of e^(l - m) of the others, and of e^(l - m) (m - l). */
-struct part { float m, n, s, t; };
+struct __align__(16) part { float m, n, s, t; };
 /* p seen from a maximum that is no smaller: n and s of the logits below it go to s */
 __device__ __forceinline__ void raise(part &p, float m) {
     if (p.m == m) return;             /* (also: no logits on either side) */
@@ -119,138 +121,151 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long key) {
     const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(key >> 32) == hi ? (unsigned)key : 0u);
     return (unsigned long long)hi << 32 | lo;
 }
-__device__ __forceinline__ void order(unsigned long long &a, unsigned long long &b) { if (a < b) { const unsigned long long c = a; a = b; b = c; } }
-/* the k-th largest of kKeys keys, 0 if fewer are open; one warp */
-__device__ __forceinline__ unsigned long long kth_largest(const unsigned long long *keys, int k) {
-    static_assert(kKeys == 128, "four keys a lane");
-    const int lane = threadIdx.x & 31;
-    unsigned long long q[4], most = 0;
+/* the k-th largest of the lanes' keys, 0 if fewer are open */
+__device__ __forceinline__ unsigned long long kth_largest(unsigned long long key, int k) {
+    int before = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) q[j] = keys[lane + 32 * j];
-    order(q[0], q[1]); order(q[2], q[3]); order(q[0], q[2]); order(q[1], q[3]); order(q[1], q[2]);
-    for (int i = 0; i < k; i++) {
-        most = warp_max(q[0]);
-        if (closed(most)) return 0;
-        if (q[0] == most) { q[0] = q[1]; q[1] = q[2]; q[2] = q[3]; q[3] = 0; }
-    }
-    return most;
+    for (int i = 1; i < 32; i++) before += __shfl_xor_sync(0xffffffffu, key, i) > key;
+    const unsigned at = __ballot_sync(0xffffffffu, before == k - 1 && !closed(key));        /* (open keys differ) */
+    return at ? __shfl_sync(0xffffffffu, key, __ffs(at) - 1) : 0;
 }
+/* two numbers at a time */
+struct f2 { float x, y; };
+__device__ __forceinline__ unsigned long long bits(f2 v) { unsigned long long r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y)); return r; }
+__device__ __forceinline__ f2 pair(unsigned long long v) { f2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { unsigned long long r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c))); return pair(r); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { unsigned long long r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return pair(r); }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { unsigned long long r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return pair(r); }
 
-template <class T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) hy3a_logprobs_kernel(const logprobs_args a) {
-    constexpr int kOf = row_of<T>::kOf, kAtOnce = 32 / kOf;        /* vectors of a thread that are on their way together */
-    __shared__ part s_part[kWarps], s_all;
+/* What a thread has of its logits so far; the sums in two halves. */
+struct running {
+    float m, n;
+    f2 s, t;
+    __device__ __forceinline__ part all() const { return {m, n, s.x + s.y, t.x + t.y}; }
+    /* logits below m */
+    template <int N> __device__ __forceinline__ void add_below(const float (&v)[N]) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            f2 d = fma2({v[j], v[j + 1]}, {-1.f, -1.f}, {m, m});
+            d = {min_nan(d.x, 200.f), min_nan(d.y, 200.f)};         /* (e^-200 is 0, and so is 0 times it) */
+            const f2 a = mul2(d, {-kLog2e, -kLog2e}), e = {ex2(a.x), ex2(a.y)};
+            s = add2(s, e);
+            t = fma2(e, d, t);
+        }
+    }
+    /* logits up to m, -inf among them also where m is that */
+    template <int N> __device__ __forceinline__ void add(const float (&v)[N]) {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const float d = v[j] == -INFINITY ? 200.f : min_nan(m - v[j], 200.f), e = d == 0.f ? 0.f : ex2(d * -kLog2e);
+            n += d == 0.f ? 1.f : 0.f;
+            s.x += e;
+            t.x = fmaf(e, d, t.x);
+        }
+    }
+};
+
+template <class T, bool TOP, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kernel(const logprobs_args a) {
+    constexpr int kWarps = kThreads / 32, kOf = row_of<T>::kOf, kAtOnce = 32 / kOf;        /* vectors of a thread that are on their way together */
+    constexpr bool kCluster = kThreads == kShared;
+    __shared__ part s_part[kWarps], s_all[kMaxCluster];
     __shared__ float s_max, s_log;
-    __shared__ unsigned long long s_key[TOP ? kKeys : 1], s_threshold, s_list[TOP ? kList : 1];
+    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_threshold[kMaxCluster], s_list[TOP ? kList : 1];
     __shared__ unsigned s_listed;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cluster = a.cluster, me = cluster > 1 ? (int)cluster_rank() : 0, row = blockIdx.x / cluster;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cluster = kCluster ? a.cluster : 1, me = kCluster ? (int)cluster_rank() : 0, row = kCluster ? blockIdx.x / cluster : blockIdx.x;
     pdl_release();
     pdl_wait();
     const row_of<T> r(a, row);
     const int per = (r.vectors + cluster - 1) / cluster, first = me * per, last = min(r.vectors, first + per);       /* the block's vectors */
     if (tid == 0) s_listed = 0;
+    if (kCluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-    part p = {-INFINITY, 0.f, 0.f, 0.f};
+    running p = {-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}};
     float best = -INFINITY;                /* the thread's largest logit, */
     int best_at = 0;                       /* and the first vector that has it */
-    for (int i0 = first + warp * 32; i0 < last; i0 += kThreads * kAtOnce) {
-        float v[kAtOnce][kOf];
+    float v[kAtOnce][kOf];                 /* (the last ones stay) */
+    int i0 = first + warp * 32;
+    for (;; i0 += kThreads * kAtOnce) {
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
             const int i = i0 + u * kThreads + lane;
             r.load(i < last ? i : -1, v[u]);
         }
-        float most = -INFINITY;
+        float vm[kAtOnce], most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
-            float vm = v[u][0];
+            vm[u] = v[u][0];
 #pragma unroll
-            for (int j = 1; j < kOf; j++) vm = fmaxf(vm, v[u][j]);
-            if (TOP && vm > best) { best = vm; best_at = i0 + u * kThreads + lane; }
-            most = fmaxf(most, vm);
+            for (int j = 1; j < kOf; j++) vm[u] = fmaxf(vm[u], v[u][j]);
+            if (TOP && vm[u] > best) { best = vm[u]; best_at = i0 + u * kThreads + lane; }
+            most = fmaxf(most, vm[u]);
         }
         if (__any_sync(0xffffffffu, most >= p.m)) {
-            const float m = warp_max(fmaxf(most, p.m));
-            raise(p, m);
+            part q = p.all();
+            raise(q, warp_max(fmaxf(most, p.m)));
+            p = {q.m, q.n, {q.s, 0.f}, {q.t, 0.f}};
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++)
-#pragma unroll
-                for (int j = 0; j < kOf; j++) {
-                    const float d = v[u][j] == -INFINITY ? -200.f : max_nan(v[u][j] - m, -200.f);
-                    const float e = d == 0.f ? 0.f : ex2(d * kLog2e);
-                    p.n += d == 0.f ? 1.f : 0.f;
-                    p.s += e;
-                    p.t = fmaf(e, -d, p.t);
-                }
+            for (int u = 0; u < kAtOnce; u++) {
+                if (p.m == -INFINITY || __any_sync(0xffffffffu, vm[u] >= p.m)) p.add(v[u]);
+                else p.add_below(v[u]);
+            }
         } else {
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++)
-#pragma unroll
-                for (int j = 0; j < kOf; j++) {
-                    const float d = max_nan(v[u][j] - p.m, -200.f);
-                    const float e = ex2(d * kLog2e);
-                    p.s += e;
-                    p.t = fmaf(e, -d, p.t);
-                }
+            for (int u = 0; u < kAtOnce; u++) p.add_below(v[u]);
         }
+        if (i0 + kThreads * kAtOnce >= last) break;
     }
-    p.n = warp_sum(p.n); p.s = warp_sum(p.s); p.t = warp_sum(p.t);
-    if (lane == 0) s_part[warp] = p;
+    part q = p.all();
+    q.n = warp_sum(q.n); q.s = warp_sum(q.s); q.t = warp_sum(q.t);
+    if (lane == 0) s_part[warp] = q;
     const unsigned long long mine = TOP ? key_of(best, best_at) : 0;        /* (here a key has the vector's number for the logit's) */
-    if (TOP) {
-        unsigned long long key = mine;
-#pragma unroll
-        for (int o = 1; o < kThreads / kKeys; o <<= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-            key = other > key ? other : key;
-        }
-        if (tid % (kThreads / kKeys) == 0) s_key[tid / (kThreads / kKeys)] = key;
-    }
+    if (TOP) s_key[tid] = mine;
     __syncthreads();
+    if (kCluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");              /* all blocks are there: they write to each other now */
     if (warp == 0) {
-        part q = lane < kWarps ? s_part[lane] : part{-INFINITY, 0.f, 0.f, 0.f};
+        q = lane < kWarps ? s_part[lane] : part{-INFINITY, 0.f, 0.f, 0.f};
         raise(q, warp_max(q.m));
         q.n = warp_sum(q.n); q.s = warp_sum(q.s); q.t = warp_sum(q.t);
-        if (lane == 0) s_all = q;
+        if (lane == 0) {
+            if (kCluster) asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(peer(&s_all[me], 0)), "f"(q.m), "f"(q.n), "f"(q.s), "f"(q.t) : "memory");
+            else s_all[0] = q;
+        }
     } else if (TOP && warp == 1) {
-        const unsigned long long key = kth_largest(s_key, a.top_k);
-        if (lane == 0) s_threshold = key;
+        unsigned long long key = s_key[lane];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) { const unsigned long long other = s_key[32 * w + lane]; key = other > key ? other : key; }
+        key = kth_largest(key, a.top_k);
+        /* what each block is sure of, all may rely on */
+        if (!kCluster) { if (lane == 0) s_threshold[0] = key; }
+        else if (lane < cluster) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer(&s_threshold[me], lane)), "l"(key) : "memory");
     }
     meet(cluster);
     if (TOP) {
-        /* what each block is sure of, all may rely on */
-        unsigned long long threshold = s_threshold;
-        for (int c = 0; c < cluster; c++) {
-            if (cluster == 1) break;
-            unsigned long long other;
-            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(other) : "r"(peer(&s_threshold, c)) : "memory");
-            threshold = other > threshold ? other : threshold;
-        }
+        unsigned long long threshold = s_threshold[0];
+        if (kCluster) for (int c = 1; c < cluster; c++) threshold = s_threshold[c] > threshold ? s_threshold[c] : threshold;
         if (!closed(mine) && mine >= threshold) {
             const unsigned count = peer(&s_listed, 0), list = peer(s_list, 0);
-            for (int i0 = first + tid; i0 < last; i0 += kThreads * kAtOnce) {
-                float v[kAtOnce][kOf];
+            const auto look = [&](const float (&x)[kOf], int i) {
 #pragma unroll
-                for (int u = 0; u < kAtOnce; u++) r.load(i0 + u * kThreads < last ? i0 + u * kThreads : -1, v[u]);
+                for (int j = 0; j < kOf; j++) {
+                    if (x[j] == -INFINITY || key_of(x[j], i) < threshold) continue;
+                    unsigned at;
+                    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
+                    if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(x[j], i * kOf + j - r.skip)) : "memory");
+                }
+            };
 #pragma unroll
-                for (int u = 0; u < kAtOnce; u++)
-#pragma unroll
-                    for (int j = 0; j < kOf; j++) {
-                        const int i = i0 + u * kThreads;
-                        if (v[u][j] == -INFINITY || key_of(v[u][j], i) < threshold) continue;
-                        unsigned at;
-                        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
-                        if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(v[u][j], i * kOf + j - r.skip)) : "memory");
-                    }
+            for (int u = 0; u < kAtOnce; u++) look(v[u], i0 + u * kThreads + lane);
+            for (int i = first + tid; i < i0; i += kThreads) {
+                r.load(i, v[0]);
+                look(v[0], i);
             }
         }
     }
     if (me == 0 && tid == 0) {
-        part q = s_all;
-        for (int c = 1; c < cluster; c++) {
-            const part o = {peer_float(&s_all.m, c), peer_float(&s_all.n, c), peer_float(&s_all.s, c), peer_float(&s_all.t, c)};
-            join(q, o);
-        }
+        q = s_all[0];
+        for (int c = 1; c < cluster; c++) join(q, s_all[c]);
         const bool none = q.m == -INFINITY && !isnan(q.s);             /* nothing is open */
         s_max = q.m;
         s_log = none ? 0.f : (q.n == 1.f ? log1pf(q.s) : logf(q.n + q.s));
@@ -271,10 +286,10 @@ __global__ void __launch_bounds__(kThreads, 2) hy3a_logprobs_kernel(const logpro
     if (!TOP) return;
     int *const ids = a.top_ids + (size_t)row * a.top_k;
     float *const top = a.top_logp + (size_t)row * a.top_k;
-    const auto put = [&](int rank, unsigned long long key) {
+    const auto put = [&](int at, unsigned long long key) {
         const unsigned u = (unsigned)(key >> 32);
-        ids[rank] = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
-        top[rank] = closed(key) ? -INFINITY : logp(__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u));
+        ids[at] = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
+        top[at] = closed(key) ? -INFINITY : logp(__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u));
     };
     const unsigned n = s_listed;
     if (n <= kList && !isnan(log_all)) {
@@ -309,12 +324,14 @@ __global__ void __launch_bounds__(kThreads, 2) hy3a_logprobs_kernel(const logpro
     }
 }
 
-template <class T>
+template <class T, int kThreads>
 cudaError_t launch(const logprobs_args &a, void *stream) {
     hy3a_launch l(dim3((unsigned)a.rows * a.cluster), dim3(kThreads), 0, stream);
-    if (a.cluster > 1) l.cluster(a.cluster);
-    return a.top_k ? cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, true>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, false>, a);
+    if (kThreads == kShared) l.cluster(a.cluster);
+    return a.top_k ? cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, true, kThreads>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, false, kThreads>, a);
 }
+template <class T>
+cudaError_t launch_type(const logprobs_args &a, void *stream) { return a.cluster > 1 ? launch<T, kShared>(a, stream) : launch<T, kAlone>(a, stream); }
 
 } /* namespace */
 
@@ -332,11 +349,11 @@ extern "C" int hy3a_logprobs(void *stream, int dtype, int rows, int vocab, const
         return hy3a_fail(NULL, HY3A_EINVAL, "logprobs: a pointer is not aligned to its type");
     int dev, sms, rc = hy3a_layer_device("logprobs", &dev, &sms);
     if (rc) return rc;
-    /* Blocks of a row: as many as fit on the device at once for all rows (two an SM), up to a portable cluster, and with a step of the loop for each at least. */
-    int cluster = 8;
-    while (cluster > 1 && ((long long)rows * cluster > 2 * sms || (size_t)vocab * el < (size_t)cluster * kThreads * 128)) cluster >>= 1;
+    /* Blocks of a row: as many as fit on the device at once for all rows (two an SM), up to a portable cluster, and with half a round of loads for each at least. */
+    int cluster = kMaxCluster;
+    while (cluster > 1 && ((long long)rows * cluster > 2 * sms || vocab < cluster * kShared * 16)) cluster >>= 1;
     const logprobs_args a = {logits, stride, tokens, asked_logp, entropy, top_logp, top_ids, rows, vocab, asked, top_k, cluster};
-    const cudaError_t e = dtype == HY3A_F32 ? launch<float>(a, stream) : (dtype == HY3A_F16 ? launch<__half>(a, stream) : launch<__nv_bfloat16>(a, stream));
+    const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "logprobs: %s", cudaGetErrorString(e));
     return HY3A_OK;
 }
