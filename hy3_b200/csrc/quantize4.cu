@@ -6,7 +6,7 @@
  *
  * so that the value of the largest magnitude is 8 steps from 0, on the side that has 8.  Codes are counted in steps of the rounded scale, with IEEE division.
  *
- * A lane takes 16 neighbours, two to eight lanes meet for a group.  Memory bounds it if the instructions stay below that: a division and two conversions for each value keep
+ * A lane takes 32 neighbours, one to four lanes meet for a group.  Memory bounds it if the instructions stay below that: a division and two conversions for each value keep
  * the unit of special functions busy for three times as long (120832 x 4096 bf16: 572 us).
  */
 #include "layer.h"
@@ -23,7 +23,7 @@ struct quantize_args {
     uint8_t *codes;
     void *scales;
     int out;
-    int units;           /* of 16 values in a row, */
+    int units;           /* of 32 values in a row, */
     int padded;          /* and in a row of full groups */
     int groups;
     int shift;           /* 2^shift threads take a row */
@@ -32,26 +32,26 @@ struct quantize_args {
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-/* 16 values and the bounds of theirs (and 0, which changes neither bound that counts); those of 16 bits are compared two at a time */
+/* 32 values and the bounds of theirs (and 0, which changes neither bound that counts); those of 16 bits are compared two at a time */
 template <class W> struct values;
 template <> struct values<float> {
-    uint4 raw[4];
+    uint4 raw[8];
     __device__ __forceinline__ void load(const void *p) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < 8; i++) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
     }
     __device__ __forceinline__ float at(int j) const { const uint4 &r = raw[j / 4]; return __uint_as_float(j % 4 == 0 ? r.x : (j % 4 == 1 ? r.y : (j % 4 == 2 ? r.z : r.w))); }
     __device__ __forceinline__ void bounds(float &hi, float &lo) const {
         hi = lo = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; j++) { hi = max_nan(hi, at(j)); lo = min_nan(lo, at(j)); }
+        for (int j = 0; j < 32; j++) { hi = max_nan(hi, at(j)); lo = min_nan(lo, at(j)); }
     }
 };
 template <class W> struct values16 {
-    uint4 raw[2];
+    uint4 raw[4];
     __device__ __forceinline__ void load(const void *p) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+        for (int i = 0; i < 4; i++) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
     }
     __device__ __forceinline__ unsigned word(int i) const { const uint4 &r = raw[i / 4]; return i % 4 == 0 ? r.x : (i % 4 == 1 ? r.y : (i % 4 == 2 ? r.z : r.w)); }
     __device__ __forceinline__ float at(int j) const {
@@ -61,7 +61,7 @@ template <class W> struct values16 {
     template <class Max, class Min> __device__ __forceinline__ void bounds_by(float &hi, float &lo, const Max &most, const Min &least) const {
         unsigned h = 0u, l = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; i++) { h = most(h, word(i)); l = least(l, word(i)); }
+        for (int i = 0; i < 16; i++) { h = most(h, word(i)); l = least(l, word(i)); }
         const unsigned short a[4] = {(unsigned short)h, (unsigned short)(h >> 16), (unsigned short)l, (unsigned short)(l >> 16)};
         hi = max_nan(type<W>::up(*reinterpret_cast<const W *>(&a[0])), type<W>::up(*reinterpret_cast<const W *>(&a[1])));
         lo = min_nan(type<W>::up(*reinterpret_cast<const W *>(&a[2])), type<W>::up(*reinterpret_cast<const W *>(&a[3])));
@@ -86,7 +86,7 @@ __device__ __noinline__ unsigned code_of(float v, float s) {
     return (unsigned)((int)fminf(fmaxf(rintf(__fdiv_rn(v, s)), -8.f), 7.f) + 8);
 }
 
-/* r = 3 2^22 + 8 + rint(w / s) by a product with 1 / s: the code in its last bits; off: how far w / s is from what it was rounded to.  Two at a time. */
+/* r = 3 2^22 + 8 + rint(w / s): the code in its last bits; off: how far w / s is from what it was rounded to.  Two at a time. */
 constexpr float kMagic = 12582920.f;
 struct f2 { float x, y; };
 __device__ __forceinline__ unsigned long long bits(f2 v) { unsigned long long r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y)); return r; }
@@ -101,14 +101,14 @@ __device__ __forceinline__ void rounded(f2 w, float inverse, f2 &r, f2 &off) {
 /* GROUP: values of a group.  A row is taken by 2^shift threads of a block. */
 template <class W, class S, int GROUP>
 __global__ void __launch_bounds__(kThreads) hy3a_quantize4_kernel(const quantize_args a) {
-    constexpr int kLanes = GROUP / 16;
+    constexpr int kLanes = GROUP / 32;
     const int first = threadIdx.x & ((1 << a.shift) - 1), step = gridDim.x << (8 - a.shift);       /* (in a row; rows) */
     int row = (blockIdx.x << (8 - a.shift)) + (threadIdx.x >> a.shift), unit = first;
     pdl_release();
     pdl_wait();
     /* the next values are on their way while these are worked on */
     values<W> next;
-    const auto load = [&]() { if (row < a.out && unit < a.units) next.load(reinterpret_cast<const W *>(a.w) + (size_t)row * a.stride + (size_t)unit * 16); };
+    const auto load = [&]() { if (row < a.out && unit < a.units) next.load(reinterpret_cast<const W *>(a.w) + (size_t)row * a.stride + (size_t)unit * 32); };
     load();
     /* (lanes meet by groups, and the threads of a row go as far as its groups: those of a warp have the same number of turns) */
     while (__any_sync(0xffffffffu, row < a.out)) {
@@ -129,37 +129,41 @@ __global__ void __launch_bounds__(kThreads) hy3a_quantize4_kernel(const quantize
             const float far = hi > -lo ? hi : lo;
             const S s = type<S>::down(__fadd_rn(far * -0.125f, 0.f));       /* (no -0) */
             const float step_size = type<S>::up(s), inverse = __fdividef(1.f, step_size);
-            /* A product with 1 / s is off by 2^-19 at most and a quotient by 2^-21, so they are rounded alike but within 2^-18 of the middle between two codes; steps are
-             * more than 8 and a little where the scale is subnormal, and 1 / s is no use where it is 0 or not finite. */
+            /* A product with 1 / s is off by 2^-19 at most.  Quotients of numbers of 16 bits are in the middle between two codes, or 2^-13 and more beside it, so that
+             * products are as good once they are rounded to multiples of 2^-16.  Of fp32 values, whose quotients are off by 2^-21 and may be any, those within 2^-18 of the middle are divided.
+             * Steps are more than 8 and a little where the scale is subnormal, and 1 / s is no use where it is 0 or not finite. */
             const bool regular = fabsf(fmaf(far, inverse, 8.f)) < 0.4f;
             constexpr float kNear = 0.5f - 0x1p-18f;
-            float off = 0.f;
-            unsigned word[2];
+            unsigned word[4];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                word[h] = 0u - (0x4B400000u + 0xB4000000u + 0x40000000u);       /* the bits of 3 2^22, eight times, four further each time */
+            for (int h = 0; h < 4; h++) {
+                /* codes k and k + 4 of a word as the 16-bit halves of one number, 8 + 8 at most */
+                float off = 0.f;
+                word[h] = 0u;
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
+                for (int k = 0; k < 4; k++) {
                     f2 r, e;
-                    rounded({v.at(8 * h + j), v.at(8 * h + j + 1)}, inverse, r, e);
-                    off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
-                    word[h] += __float_as_uint(fminf(r.x, kMagic + 7.f)) << (4 * j);
-                    word[h] += __float_as_uint(fminf(r.y, kMagic + 7.f)) << (4 * j + 4);
+                    if (sizeof(W) == 2) r = add2(fma2({v.at(8 * h + k), v.at(8 * h + k + 4)}, {inverse, inverse}, {192.f, 192.f}), {kMagic - 192.f, kMagic - 192.f});      /* (192 + t: steps of 2^-16) */
+                    else {
+                        rounded({v.at(8 * h + k), v.at(8 * h + k + 4)}, inverse, r, e);
+                        off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
+                    }
+                    unsigned c = __byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x5410);
+                    asm("min.u16x2 %0, %0, %1;" : "+r"(c) : "r"(0x000f000fu));
+                    word[h] += c << (4 * k);
                 }
-            }
-            if (!regular || !(off < kNear)) {
+                if (!regular || !(off < kNear)) {
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const f2 w = {v.at(8 * h + j), v.at(8 * h + j + 1)};
+                    for (int k = 0; k < 4; k++) {
+                        const f2 w = {v.at(8 * h + k), v.at(8 * h + k + 4)};
                         f2 r, e;
                         rounded(w, inverse, r, e);
-                        if (!regular || !(fabsf(e.x) < kNear)) word[h] = (word[h] & ~(15u << (4 * j))) | code_of(w.x, step_size) << (4 * j);
-                        if (!regular || !(fabsf(e.y) < kNear)) word[h] = (word[h] & ~(15u << (4 * j + 4))) | code_of(w.y, step_size) << (4 * j + 4);
+                        if (!regular || !(fabsf(e.x) < kNear)) word[h] = (word[h] & ~(15u << (4 * k))) | code_of(w.x, step_size) << (4 * k);
+                        if (!regular || !(fabsf(e.y) < kNear)) word[h] = (word[h] & ~(15u << (4 * k + 16))) | code_of(w.y, step_size) << (4 * k + 16);
                     }
+                }
             }
-            *reinterpret_cast<uint2 *>(a.codes + ((size_t)row_now * a.units + unit_now) * 8) = make_uint2(word[0], word[1]);
+            *reinterpret_cast<uint4 *>(a.codes + ((size_t)row_now * a.units + unit_now) * 16) = make_uint4(word[0], word[1], word[2], word[3]);
             if (unit_now % kLanes == 0) reinterpret_cast<S *>(a.scales)[(size_t)row_now * a.groups + unit_now / kLanes] = s;
         }
     }
@@ -194,7 +198,7 @@ extern "C" int hy3a_quantize4(void *stream, int w_dtype, int out_width, int widt
     int dev, sms;
     if ((rc = hy3a_layer_device("quantize4", &dev, &sms))) return rc;
     const int groups = (width + group - 1) / group;
-    quantize_args a = {w, w_stride, (uint8_t *)codes, scales, out_width, width / 16, groups * (group / 16), groups, 3};
+    quantize_args a = {w, w_stride, (uint8_t *)codes, scales, out_width, width / 32, groups * (group / 32), groups, 2};
     while (a.shift < 8 && (1 << a.shift) < a.padded) a.shift++;
     const cudaError_t e = w_dtype == HY3A_F32 ? launch_type<float>(a, dtype, group, sms, stream)
                         : (w_dtype == HY3A_F16 ? launch_type<__half>(a, dtype, group, sms, stream) : launch_type<__nv_bfloat16>(a, dtype, group, sms, stream));
