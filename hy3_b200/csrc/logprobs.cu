@@ -22,8 +22,8 @@ namespace {
 
 using namespace hy3a_layer;
 
-/* Threads of a block: four blocks an SM where a row is a block's, so that one's end runs beside the others' loads; two where it is a cluster's, so that a row of 131072 logits is
- * one round of loads. */
+/* Threads of a block: four blocks an SM where there are more rows than SMs, so that one's end runs beside the others' loads; else one, and the blocks of a cluster for a row where rows
+ * are fewer still: 131072 fp32 logits are one round of loads for 8 of them. */
 constexpr int kAlone = 256, kShared = 512, kMaxCluster = 8;
 constexpr int kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
 constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
@@ -34,7 +34,7 @@ struct logprobs_args {
     const int *tokens;
     float *asked_logp, *entropy, *top_logp;
     int *top_ids;
-    int rows, vocab, asked, top_k, cluster;
+    int rows, vocab, asked, top_k, cluster /* blocks of a row; 0: one by itself */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -84,22 +84,53 @@ template <class T> struct row_of {
         vectors = (end + kOf - 1) / kOf;
     }
     /* vector i, -inf in place of what is not the row's */
-    __device__ __forceinline__ void load(int i, float (&v)[kOf]) const {
-        if (i >= vectors || i < 0) {
-#pragma unroll
-            for (int j = 0; j < kOf; j++) v[j] = -INFINITY;
-        } else if ((i == 0 && skip) || (i + 1) * kOf > end) {
-#pragma unroll
-            for (int j = 0; j < kOf; j++) v[j] = i * kOf + j >= skip && i * kOf + j < end ? type<T>::up(base[i * kOf + j]) : -INFINITY;
-        } else {
-            uint4 raw;
-            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w) : "l"(base + (size_t)i * kOf));
-            const T *const r = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-            for (int j = 0; j < kOf; j++) v[j] = type<T>::up(r[j]);
+    __device__ __forceinline__ uint4 load(int i) const {
+        constexpr unsigned kClosed = sizeof(T) == 4 ? 0xff800000u : (type<T>::code == HY3A_BF16 ? 0xff80ff80u : 0xfc00fc00u);
+        uint4 raw = make_uint4(kClosed, kClosed, kClosed, kClosed);
+        const int at = i * kOf;
+        if (i >= 0 && at >= skip && at + kOf <= end)
+            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w) : "l"(base + at));
+        else if (i >= 0 && at < end) {
+            /* an edge, shifted in from above (rare: in few instructions) */
+#pragma unroll 1
+            for (int j = 0; j < kOf; j++) {
+                unsigned v = kClosed;
+                if (at + j >= skip && at + j < end) v = bits_of(base + at + j);
+                const auto next = [](unsigned lo, unsigned hi) { return sizeof(T) == 4 ? hi : __funnelshift_r(lo, hi, 16); };
+                raw = make_uint4(next(raw.x, raw.y), next(raw.y, raw.z), next(raw.z, raw.w), next(raw.w, v));
+            }
         }
+        return raw;
     }
+    static __device__ __forceinline__ unsigned bits_of(const T *p) { return sizeof(T) == 4 ? *reinterpret_cast<const unsigned *>(p) : *reinterpret_cast<const unsigned short *>(p); }
 };
+/* the u-th of several vectors */
+template <int N> __device__ __forceinline__ uint4 pick(const uint4 (&raw)[N], int u) {
+    uint4 r = raw[0];
+#pragma unroll
+    for (int k = 1; k < N; k++) if (u == k) r = raw[k];
+    return r;
+}
+/* a vector's logits, and the largest of them that is a number */
+template <class T> __device__ __forceinline__ void logits_of(const uint4 &r, float (&v)[4]) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w); }
+__device__ __forceinline__ float largest(const uint4 &r, float) { return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))); }
+template <class T> __device__ __forceinline__ void logits_of16(const uint4 &r, float (&v)[8]) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned short u[2] = {(unsigned short)w[i], (unsigned short)(w[i] >> 16)};
+        v[2 * i] = type<T>::up(*reinterpret_cast<const T *>(&u[0]));
+        v[2 * i + 1] = type<T>::up(*reinterpret_cast<const T *>(&u[1]));
+    }
+}
+template <class T> __device__ __forceinline__ void logits_of(const uint4 &r, float (&v)[8]) { logits_of16<T>(r, v); }
+__device__ __forceinline__ unsigned largest2(unsigned a, unsigned b, __nv_bfloat16) { unsigned r; asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ unsigned largest2(unsigned a, unsigned b, __half) { unsigned r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+template <class T> __device__ __forceinline__ float largest(const uint4 &r, T t) {
+    const unsigned m = largest2(largest2(r.x, r.y, t), largest2(r.z, r.w, t), t);
+    const unsigned short u[2] = {(unsigned short)m, (unsigned short)(m >> 16)};
+    return fmaxf(type<T>::up(*reinterpret_cast<const T *>(&u[0])), type<T>::up(*reinterpret_cast<const T *>(&u[1])));
+}
 
 /* order of floats as unsigned numbers, NaN below all but what is closed (0) */
 __device__ __forceinline__ unsigned ordered(float v) {
@@ -107,6 +138,7 @@ __device__ __forceinline__ unsigned ordered(float v) {
     return v == -INFINITY ? 0u : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ unsigned long long key_of(float v, int i) { return (unsigned long long)ordered(v) << 32 | (0xffffffffu - (unsigned)i); }
+__device__ __forceinline__ float value_of(unsigned long long key) { const unsigned u = (unsigned)(key >> 32); return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 __device__ __forceinline__ bool closed(unsigned long long key) { return (key >> 32) == 0; }
 
 /* parts of two sets of logits as one's */
@@ -137,6 +169,10 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { unsigned long long r; asm
 __device__ __forceinline__ f2 add2(f2 a, f2 b) { unsigned long long r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return pair(r); }
 __device__ __forceinline__ f2 mul2(f2 a, f2 b) { unsigned long long r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return pair(r); }
 
+/* a load that stays where it stands */
+__device__ __forceinline__ float load_now(const float *p) { float v; asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p)); return v; }
+template <class T> __device__ __forceinline__ T load_now(const T *p) { unsigned short v; asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p)); return *reinterpret_cast<T *>(&v); }
+
 /* What a thread has of its logits so far; the sums in two halves. */
 struct running {
     float m, n;
@@ -166,12 +202,12 @@ struct running {
 };
 
 template <class T, bool TOP, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kernel(const logprobs_args a) {
-    constexpr int kWarps = kThreads / 32, kOf = row_of<T>::kOf, kAtOnce = 32 / kOf;        /* vectors of a thread that are on their way together */
+__global__ void __launch_bounds__(kThreads, kThreads == kAlone ? 4 : 1) hy3a_logprobs_kernel(const logprobs_args a) {
+    constexpr int kWarps = kThreads / 32, kOf = row_of<T>::kOf, kAtOnce = 8;        /* vectors of a thread that are on their way together */
     constexpr bool kCluster = kThreads == kShared;
     __shared__ part s_part[kWarps], s_all[kMaxCluster];
     __shared__ float s_max, s_log;
-    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_threshold[kMaxCluster], s_list[TOP ? kList : 1];
+    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_lanes[TOP ? kMaxCluster : 1][32], s_list[TOP ? kList : 1];
     __shared__ unsigned s_listed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cluster = kCluster ? a.cluster : 1, me = kCluster ? (int)cluster_rank() : 0, row = kCluster ? blockIdx.x / cluster : blockIdx.x;
     pdl_release();
@@ -181,46 +217,56 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kerne
     if (tid == 0) s_listed = 0;
     if (kCluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
+    int token = -1;           /* (loaded here, its logit behind the loop, both used at the end) */
+    if (me == 0 && tid < a.asked) asm volatile("ld.global.s32 %0, [%1];" : "=r"(token) : "l"(a.tokens + (size_t)row * a.asked + tid));
     running p = {-INFINITY, 0.f, {0.f, 0.f}, {0.f, 0.f}};
     float best = -INFINITY;                /* the thread's largest logit, */
     int best_at = 0;                       /* and the first vector that has it */
-    float v[kAtOnce][kOf];                 /* (the last ones stay) */
+    uint4 raw[kAtOnce];                    /* (the last ones stay) */
     int i0 = first + warp * 32;
     for (;; i0 += kThreads * kAtOnce) {
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
             const int i = i0 + u * kThreads + lane;
-            r.load(i < last ? i : -1, v[u]);
+            raw[u] = r.load(i < last ? i : -1);
         }
-        float vm[kAtOnce], most = -INFINITY;
+        float most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
-            vm[u] = v[u][0];
-#pragma unroll
-            for (int j = 1; j < kOf; j++) vm[u] = fmaxf(vm[u], v[u][j]);
-            if (TOP && vm[u] > best) { best = vm[u]; best_at = i0 + u * kThreads + lane; }
-            most = fmaxf(most, vm[u]);
+            const float vm = largest(raw[u], T());
+            if (TOP && vm > best) { best = vm; best_at = i0 + u * kThreads + lane; }
+            most = fmaxf(most, vm);
         }
+        /* where m rises, the vectors that have it (or all, as long as nothing is open) are looked at logit by logit, one piece of code for all: code that is run once is fetched once */
+        unsigned with_m = 0u;
         if (__any_sync(0xffffffffu, most >= p.m)) {
             part q = p.all();
             raise(q, warp_max(fmaxf(most, p.m)));
             p = {q.m, q.n, {q.s, 0.f}, {q.t, 0.f}};
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) {
-                if (p.m == -INFINITY || __any_sync(0xffffffffu, vm[u] >= p.m)) p.add(v[u]);
-                else p.add_below(v[u]);
+            for (int u = 0; u < kAtOnce; u++) with_m |= __any_sync(0xffffffffu, largest(raw[u], T()) >= p.m || p.m == -INFINITY) ? 1u << u : 0u;
+            for (unsigned todo = with_m; todo; todo &= todo - 1) {
+                float v[kOf];
+                logits_of<T>(pick(raw, __ffs(todo) - 1), v);
+                p.add(v);
             }
-        } else {
+        }
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) p.add_below(v[u]);
+        for (int u = 0; u < kAtOnce; u++) {
+            if ((with_m >> u) & 1) continue;
+            float v[kOf];
+            logits_of<T>(raw[u], v);
+            p.add_below(v);
         }
         if (i0 + kThreads * kAtOnce >= last) break;
     }
+    const T *const logits = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.stride;
+    T token_logit = type<T>::down(0.f);
+    if (me == 0 && token >= 0 && token < a.vocab) token_logit = load_now(logits + token);
     part q = p.all();
     q.n = warp_sum(q.n); q.s = warp_sum(q.s); q.t = warp_sum(q.t);
     if (lane == 0) s_part[warp] = q;
-    const unsigned long long mine = TOP ? key_of(best, best_at) : 0;        /* (here a key has the vector's number for the logit's) */
-    if (TOP) s_key[tid] = mine;
+    if (TOP) s_key[tid] = key_of(best, best_at);        /* (here a key has the vector's number for the logit's) */
     __syncthreads();
     if (kCluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");              /* all blocks are there: they write to each other now */
     if (warp == 0) {
@@ -235,31 +281,41 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kerne
         unsigned long long key = s_key[lane];
 #pragma unroll
         for (int w = 1; w < kWarps; w++) { const unsigned long long other = s_key[32 * w + lane]; key = other > key ? other : key; }
-        key = kth_largest(key, a.top_k);
-        /* what each block is sure of, all may rely on */
-        if (!kCluster) { if (lane == 0) s_threshold[0] = key; }
-        else if (lane < cluster) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer(&s_threshold[me], lane)), "l"(key) : "memory");
+        if (!kCluster) s_lanes[0][lane] = key;
+        else for (int c = 0; c < cluster; c++) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer(&s_lanes[me][lane], c)), "l"(key) : "memory");
     }
     meet(cluster);
     if (TOP) {
-        unsigned long long threshold = s_threshold[0];
-        if (kCluster) for (int c = 1; c < cluster; c++) threshold = s_threshold[c] > threshold ? s_threshold[c] : threshold;
-        if (!closed(mine) && mine >= threshold) {
+        /* the largest of each lane's threads, in all blocks; every warp finds the k-th of them (0: fewer are open) */
+        unsigned long long key = s_lanes[0][lane];
+        if (kCluster) for (int c = 1; c < cluster; c++) key = s_lanes[c][lane] > key ? s_lanes[c][lane] : key;
+        key = kth_largest(key, a.top_k);
+        const float least = closed(key) ? -INFINITY : value_of(key);
+        const int least_at = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
+        const auto reaches = [&](float l, int i) { return l > least || (l == least && i <= least_at); };
+        if (reaches(best, best_at)) {
             const unsigned count = peer(&s_listed, 0), list = peer(s_list, 0);
-            const auto look = [&](const float (&x)[kOf], int i) {
+            /* the last round's vectors, then those of the rounds before */
+            for (int i = i0 + lane;;) {
+                unsigned todo = 0u;
 #pragma unroll
-                for (int j = 0; j < kOf; j++) {
-                    if (x[j] == -INFINITY || key_of(x[j], i) < threshold) continue;
-                    unsigned at;
-                    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
-                    if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(x[j], i * kOf + j - r.skip)) : "memory");
+                for (int u = 0; u < kAtOnce; u++) todo |= reaches(largest(raw[u], T()), i + u * kThreads) ? 1u << u : 0u;
+                for (; todo; todo &= todo - 1) {
+                    const int u = __ffs(todo) - 1, vector = i + u * kThreads;
+                    float v[kOf];
+                    logits_of<T>(pick(raw, u), v);
+#pragma unroll
+                    for (int j = 0; j < kOf; j++) {
+                        if (!reaches(v[j], vector)) continue;
+                        unsigned at;
+                        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
+                        if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(v[j], vector * kOf + j - r.skip)) : "memory");
+                    }
                 }
-            };
+                i -= kThreads * kAtOnce;
+                if (i < first) break;
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) look(v[u], i0 + u * kThreads + lane);
-            for (int i = first + tid; i < i0; i += kThreads) {
-                r.load(i, v[0]);
-                look(v[0], i);
+                for (int u = 0; u < kAtOnce; u++) raw[u] = r.load(i + u * kThreads);
             }
         }
     }
@@ -278,18 +334,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kerne
     /* (a closed logit has -inf, also where nothing is open, and NaN where the sum is one) */
     const auto logp = [&](float l) { return l == -INFINITY && !isnan(log_all) ? -INFINITY : (l - m) - log_all; };
     for (int j = tid; j < a.asked; j += kThreads) {
-        const int token = a.tokens[(size_t)row * a.asked + j];
-        float v = token == -1 ? 0.f : NAN;
-        if (token >= 0 && token < a.vocab) v = logp(type<T>::up(reinterpret_cast<const T *>(a.logits)[(size_t)row * a.stride + token]));
-        a.asked_logp[(size_t)row * a.asked + j] = v;
+        if (j != tid) {
+            token = a.tokens[(size_t)row * a.asked + j];
+            if (token >= 0 && token < a.vocab) token_logit = logits[token];
+        }
+        a.asked_logp[(size_t)row * a.asked + j] = token >= 0 && token < a.vocab ? logp(type<T>::up(token_logit)) : (token == -1 ? 0.f : NAN);
     }
     if (!TOP) return;
     int *const ids = a.top_ids + (size_t)row * a.top_k;
     float *const top = a.top_logp + (size_t)row * a.top_k;
     const auto put = [&](int at, unsigned long long key) {
-        const unsigned u = (unsigned)(key >> 32);
         ids[at] = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
-        top[at] = closed(key) ? -INFINITY : logp(__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u));
+        top[at] = closed(key) ? -INFINITY : logp(value_of(key));
     };
     const unsigned n = s_listed;
     if (n <= kList && !isnan(log_all)) {
@@ -307,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kerne
         unsigned long long most = 0;
         for (int i = tid; i < r.vectors; i += kThreads) {
             float v[kOf];
-            r.load(i, v);
+            logits_of<T>(r.load(i), v);
 #pragma unroll
             for (int j = 0; j < kOf; j++) {
                 const unsigned long long key = key_of(v[j], i * kOf + j - r.skip);
@@ -326,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) hy3a_logprobs_kerne
 
 template <class T, int kThreads>
 cudaError_t launch(const logprobs_args &a, void *stream) {
-    hy3a_launch l(dim3((unsigned)a.rows * a.cluster), dim3(kThreads), 0, stream);
+    hy3a_launch l(dim3((unsigned)a.rows * (kThreads == kShared ? a.cluster : 1)), dim3(kThreads), 0, stream);
     if (kThreads == kShared) l.cluster(a.cluster);
     return a.top_k ? cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, true, kThreads>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, false, kThreads>, a);
 }
 template <class T>
-cudaError_t launch_type(const logprobs_args &a, void *stream) { return a.cluster > 1 ? launch<T, kShared>(a, stream) : launch<T, kAlone>(a, stream); }
+cudaError_t launch_type(const logprobs_args &a, void *stream) { return a.cluster ? launch<T, kShared>(a, stream) : launch<T, kAlone>(a, stream); }
 
 } /* namespace */
 
@@ -349,9 +405,10 @@ extern "C" int hy3a_logprobs(void *stream, int dtype, int rows, int vocab, const
         return hy3a_fail(NULL, HY3A_EINVAL, "logprobs: a pointer is not aligned to its type");
     int dev, sms, rc = hy3a_layer_device("logprobs", &dev, &sms);
     if (rc) return rc;
-    /* Blocks of a row: as many as fit on the device at once for all rows (two an SM), up to a portable cluster, and with half a round of loads for each at least. */
-    int cluster = kMaxCluster;
-    while (cluster > 1 && ((long long)rows * cluster > 2 * sms || vocab < cluster * kShared * 16)) cluster >>= 1;
+    /* Blocks of a row: none but one where there are more rows than SMs; else as many as fit on the device at once for all rows, up to a portable cluster, and with half a round of
+     * loads for each at least. */
+    int cluster = rows > sms ? 0 : kMaxCluster;
+    while (cluster > 1 && (rows * cluster > sms || vocab < cluster * kShared * 16)) cluster >>= 1;
     const logprobs_args a = {logits, stride, tokens, asked_logp, entropy, top_logp, top_ids, rows, vocab, asked, top_k, cluster};
     const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "logprobs: %s", cudaGetErrorString(e));
