@@ -1,20 +1,24 @@
 /*
- * linear4.cu -- rows through a matrix of 4-bit codes with a scale for each group of neighbours in a row (hy3a_linear4), few rows:
+ * linear4.cu -- rows through a matrix of 4-bit codes with a scale for each group of neighbours in a row (hy3a_linear4), up to 8 rows:
  *
  *      y[t][o] = sum over groups j of scales[o][j] * sum over k of group j of (code[o][k] - 8) x[t][k]
  *
- * The inner sums are warp-level products (mma.m16n8k16, fp32 sums) of 16 outputs with 8 rows: the differences are exact in the rows' type and so are the
- * products; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
+ * The inner sums are warp-level products of 16 outputs with 8 columns; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
+ *   2 to 8 rows  the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products;
+ *   one row      the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
+ *                below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 11, and
+ *                -8 sum d comes in as the sum's first value.  (120832 x 4096: 63 us with the row as a column.)
  *
  * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
- * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, so that all blocks have 170 KB under way.  (A bulk copy for
- * each output keeps the issuing lane busy for longer than its bytes take.)  The 16 warps share the k's; each keeps its part of x in registers for the whole launch, and reads its scales two
- * stages ahead.  Their sums meet in shared memory, where a warp of their own adds them up.
+ * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way.  (A bulk copy
+ * for each output keeps the issuing lane busy for longer than its bytes take.)  The 16 warps share the k's; each keeps its part of x in registers for the whole launch.  Their
+ * sums meet in shared memory, where a warp of their own adds them up.  Short launches wait for instructions as much as for codes: loops that are run a few times are not unrolled.
  *
- * mma wants of lane (g = lane / 4, t = lane % 4) four k's of outputs g and g + 8, and of row g; k's are renamed so that lane t has neighbouring ones, those of a word
+ * mma wants of lane (g = lane / 4, t = lane % 4) four k's of outputs g and g + 8, and of column g; k's are renamed so that lane t has neighbouring ones, those of a word
  * (32 k's of 4 lanes) the least: a block of 32, 64 or 128 k's, one group's, is 1, 2 or 4 words a lane.
  */
 #include <atomic>
+#include <type_traits>
 
 #include "linear4.h"
 #include "ring.cuh"
@@ -24,19 +28,23 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kMostWarps = 16, kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16;
+constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2);
+constexpr int kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24;
 constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
 constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
-constexpr int kRingBytes = 180 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kMostWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
+constexpr int kRingBytes = 184 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
 enum { B_FULL = 0, B_EMPTY = kMaxStages, B_READY = 2 * kMaxStages, B_TAKEN = 2 * kMaxStages + kParts, B_COUNT = 2 * kMaxStages + 2 * kParts };
-static_assert(8 * B_COUNT <= 512, "barriers");
+static_assert(8 * B_COUNT + 8 <= 512, "barriers");
+static_assert(kStageK / 8 * 8 * 8 <= kParts * kWarps * kPart * 4, "the digits of a stage's k's lie where the parts do later");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
 struct few_args {
     linear4_args a;
-    int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stages, passes /* stages of a tile */, in_stage /* groups of a stage */, per /* of a warp */;
+    int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stage_bytes, stages, passes /* stages of a tile */;
+    int in_stage /* groups of a stage */, per /* of a warp */;
     int whole;                /* rows of codes are whole lines */
+    int scale_pitch;          /* bytes of an output's scales in a stage; 0: rows of scales do not start on 16-byte boundaries, and are read where they lie */
     unsigned zero;            /* 0, which the compiler does not know */
 };
 
@@ -46,12 +54,29 @@ __device__ __forceinline__ void copy_lines(unsigned dst, const CUtensorMap *map,
                  " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;\n}"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy), "r"(lead) : "memory");
 }
+__device__ __forceinline__ void copy_scales(unsigned dst, const CUtensorMap *map, unsigned bar, int x, int y, unsigned lead) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %5, 0;\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void meet_workers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
 template <class T> __device__ __forceinline__ float unpack(unsigned v, bool hi) {
     const unsigned short u = (unsigned short)(hi ? v >> 16 : v);
     return type<T>::up(*reinterpret_cast<const T *>(&u));
 }
+__device__ __forceinline__ unsigned scale_at(unsigned addr) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+    return v;
+}
+/* W words at an address of shared memory */
+template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsigned (&v)[W]) {
+    if (W == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[W > 2 ? 2 : 0]), "=r"(v[W > 3 ? 3 : 0]) : "r"(addr));
+    else if (W == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[W > 1 ? 1 : 0]) : "r"(addr));
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(addr));
+}
 
-/* x of a lane for a block of 32 W k's from k0 on, in the pairs' order; zeros past the width, and where the row is none */
+/* ---- rows as columns: x of a lane for a group from k0 on, in the pairs' order; zeros past the width, and where the row is none ---- */
 template <class T, int W> __device__ __forceinline__ void load_x(const T *row, bool there, int k0, int width, unsigned (&x)[4 * W]) {
     const int k = k0 + (threadIdx.x & 3) * 8 * W;
 #pragma unroll
@@ -71,35 +96,106 @@ template <class T> __device__ __forceinline__ void mma_first(float (&d)[4], unsi
     else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
              : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-/* W words at an address of shared memory */
-template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsigned (&v)[W]) {
-    if (W == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[W > 2 ? 2 : 0]), "=r"(v[W > 3 ? 3 : 0]) : "r"(addr));
-    else if (W == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[W > 1 ? 1 : 0]) : "r"(addr));
-    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(addr));
+template <class T, int W> struct row_columns {
+    unsigned x[4 * W];
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4], float &by) const {
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            unsigned vl[4], vh[4];
+            steps<T>::of(wl[w], vl);
+            steps<T>::of(wh[w], vh);
+            if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], x[0], x[1]);
+            else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], x[4 * w], x[4 * w + 1]);
+            type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], x[4 * w + 2], x[4 * w + 3]);
+        }
+        by = 1.f;
+    }
+};
+
+/* ---- digits as columns ---- */
+constexpr int kFirstSum = 0x4B400000;        /* 3 2^22 as a float: what is added to it as an integer, up to 2^22, is added to the float */
+template <int W> struct digit_columns {
+    unsigned x[2 * W];                /* the column's digits of even and odd k's of each word */
+    int first[2];                     /* kFirstSum - 8 sum of digits, of columns 2 t and 2 t + 1 */
+    float unit;                       /* 2^(E - 7) */
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4], float &by) const {
+        int n[4] = {first[0], first[1], first[0], first[1]};
+#pragma unroll
+        for (int w = 0; w < W; w++)
+            asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                : "+r"(n[0]), "+r"(n[1]), "+r"(n[2]), "+r"(n[3])
+                : "r"(wl[w] & 0x0f0f0f0fu), "r"(wh[w] & 0x0f0f0f0fu), "r"((wl[w] >> 4) & 0x0f0f0f0fu), "r"((wh[w] >> 4) & 0x0f0f0f0fu), "r"(x[2 * w]), "r"(x[2 * w + 1]));
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] = __int_as_float(n[i]) - __int_as_float(kFirstSum);
+        by = unit;
+    }
+};
+__device__ __forceinline__ unsigned shift_left(unsigned v, int by) { unsigned r; asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }        /* (0 by 32 and more, and by less than 0) */
+__device__ __forceinline__ unsigned shift_right(unsigned v, int by) { unsigned r; asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }
+
+/* The digits of 8 k's from k on, a thread's share of a stage's: word `word` of the stage.  Row c = group * W + word of its lane holds the digits of four lanes, 8 bytes for
+ * each column and lane, column j in place j ^ (c & 7): banks.  Sets bit 0 of *odd where x is NaN, bit 1 where it is infinite. */
+template <class T, int W> __device__ __forceinline__ void store_digits(const T *row, int k, int width, int word, uint8_t *digits, float *units, int *odd) {
+    uint4 raw = zero16();
+    if (k < width) raw = load_row(row + k);
+    const unsigned pairs[4] = {raw.x, raw.y, raw.z, raw.w};
+    unsigned m[8], sign = 0;          /* |x| = m 2^(ex - 137), m < 2^11 */
+    int ex[8], most = 1;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const unsigned u = __float_as_uint(unpack<T>(pairs[i / 2], i & 1)), e = (u >> 23) & 255u;
+        m[i] = ((u >> 13) & 0x3ffu) | (e ? 0x400u : 0u);
+        ex[i] = max((int)e, 1);
+        most = max(most, ex[i]);
+        sign |= (u >> 31) << i;
+        if (e == 255u) atomicOr(odd, u & 0x7fffffu ? 1 : 2);
+    }
+#pragma unroll
+    for (int o = 1; o < 4 * W; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int c = word / (4 * W) * W + word % W, t = word / W & 3;
+    if (word % (4 * W) == 0) units[word / (4 * W)] = most > 6 ? __int_as_float((most - 6) << 23) : __int_as_float(1 << (16 + most));
+#pragma unroll 1
+    for (int j = 0; j < 8; j++) {
+        unsigned b[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int by = 7 * j - 4 + ex[i] - most;
+            const unsigned d = (shift_left(m[i], by) | shift_right(m[i], -by)) & 127u, s = 0u - ((sign >> i) & 1u);
+            b[i & 1] |= (((d ^ s) - s) & 255u) << (8 * (i >> 1));
+        }
+        *reinterpret_cast<uint2 *>(digits + c * 256 + ((j ^ (c & 7)) * 4 + t) * 8) = make_uint2(b[0], b[1]);
+    }
 }
 
-/* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each */
-template <class T, int W, int P, int kWarps>
-__global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm, const few_args f) {
+/* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each; ONE: one row */
+template <class T, int W, int P, bool ONE>
+__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_scales, const few_args f) {
     extern __shared__ uint8_t s_raw[];
-    constexpr int kProducer = kWarps, kFinisher = kWarps + 1, kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kAhead = P == 1 ? 2 : (P ? 1 : 0) /* tiles */;
+    using columns = typename std::conditional<ONE, digit_columns<W>, row_columns<T, W>>::type;
+    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4;
+    __shared__ float s_units[ONE ? kStageK / kGroup : 1];
     const linear4_args &a = f.a;
     uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     volatile int *s_abort = reinterpret_cast<volatile int *>(sm + kOffBar + 8 * B_COUNT);
-    const unsigned ring = smem_u32(sm), bar0 = ring + kOffBar, stage_bytes = (kTile / kBox) * f.box_bytes;
+    int *s_odd = reinterpret_cast<int *>(sm + kOffBar + 8 * B_COUNT + 4);
+    const unsigned ring = smem_u32(sm), bar0 = ring + kOffBar;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int boxes = (a.out_width + kBox - 1) / kBox, first = kBox * (int)((long long)boxes * blockIdx.x / gridDim.x), last = min(a.out_width, kBox * (int)((long long)boxes * (blockIdx.x + 1) / gridDim.x));
-    const int t0 = blockIdx.y * kRows, rows = min(kRows, a.rows - t0);
+    const int rows = ONE ? 1 : a.rows;
     /* outputs g and g + 8 of the products are outputs mine and mine + 8 of the tile: such that lanes that read together find their words in different banks */
     const int mine_of = W == 4 ? (g & 1) * 4 + (g >> 1) : ((g >> 1) & 1) * 4 + (g & 1) * 2 + (g >> 2);
 #define BAR(i) (bar0 + 8u * (unsigned)(i))
     if (tid == 0) {
         *s_abort = 0;
+        *s_odd = 0;
         for (int i = 0; i < f.stages; i++) { mbar_init(BAR(B_FULL + i), 1); mbar_init(BAR(B_EMPTY + i), kWarps); }
         for (int i = 0; i < kParts; i++) { mbar_init(BAR(B_READY + i), kWarps); mbar_init(BAR(B_TAKEN + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kProducer && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&tm) : "memory");
+    if (warp == kProducer && lane < 2) {
+        const CUtensorMap *m = lane == 0 ? &tm_codes : &tm_scales;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
     __syncthreads();
     pdl_release();
     pdl_wait();
@@ -115,20 +211,23 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(cons
             const int n = (min(kTile, last - o0) + kBox - 1) / kBox;
             for (int p = 0; p < f.passes; p++) {
                 if (!(ok = mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, g_err, 40u))) break;
-                const unsigned to = ring + st * stage_bytes, full = BAR(B_FULL + st);
+                const unsigned to = ring + st * f.stage_bytes, full = BAR(B_FULL + st);
                 /* (what lies past the matrix comes as zeros, and counts) */
-                if (lead) mbar_expect_tx(full, n * f.lines * kBox * kLine);
+                if (lead) mbar_expect_tx(full, n * f.lines * kBox * kLine + kTile * f.scale_pitch);
+#pragma unroll 1
                 for (int q = 0; q < n; q++) {
-                    if (f.whole) copy_lines(to + q * f.box_bytes, &tm, full, 0, o0 + q * kBox, p * (kStageK / 2 / kLine), policy, lead);
-                    else for (int c = 0; c < f.lines; c++) copy_lines(to + q * f.box_bytes + c * kBox * kLine, &tm, full, p * (kStageK / 2) + c * kLine, o0 + q * kBox, 0, policy, lead);
+                    if (f.whole) copy_lines(to + q * f.box_bytes, &tm_codes, full, 0, o0 + q * kBox, p * (kStageK / 2 / kLine), policy, lead);
+                    else for (int c = 0; c < f.lines; c++) copy_lines(to + q * f.box_bytes + c * kBox * kLine, &tm_codes, full, p * (kStageK / 2) + c * kLine, o0 + q * kBox, 0, policy, lead);
                 }
+                if (f.scale_pitch) copy_scales(to + (kTile / kBox) * f.box_bytes, &tm_scales, full, p * (kStageK / kGroup), o0, lead);
                 if (++st == f.stages) { st = 0; ph ^= 1u; }
             }
         }
     } else if (warp == kFinisher) {
-        /* ===================== the warps' parts, added up in the warps' order; a lane has an output and four rows ===================== */
+        /* ===================== the warps' parts, added up in the warps' order; a lane has an output and four columns ===================== */
         const int o = lane >> 1, r0 = (lane & 1) * 4;
         int turn = 0;
+#pragma unroll 1
         for (int o0 = first; o0 < last; o0 += kTile, turn++) {
             const int buf = turn % kParts;
             if (!mbar_wait(BAR(B_READY + buf), (turn / kParts) & 1, s_abort, g_err, 42u)) break;
@@ -140,28 +239,71 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(cons
                 sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf));
-            if (o0 + o < last) {
-                const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    if (r0 + r >= rows) break;
-                    const size_t to = (size_t)(t0 + r0 + r) * a.out_stride + o0 + o;
-                    if (a.wide) reinterpret_cast<float *>(a.out)[to] = v[r];
-                    else reinterpret_cast<T *>(a.out)[to] = type<T>::down(v[r]);
+            /* (an arrival does not wait for loads that are under way, so it takes something of the sums that they went into) */
+            if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf) + (__float_as_uint(sum.x) & f.zero));
+            float v[4] = {sum.x, sum.y, sum.z, sum.w};
+            const auto put = [&](int r, float y) {
+                const size_t to = (size_t)r * a.out_stride + o0 + o;
+                if (a.wide) reinterpret_cast<float *>(a.out)[to] = y;
+                else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
+            };
+            if (ONE) {
+                /* digits: column c counts 2^-7c; an x that is not finite has none */
+                float y = (v[0] + v[1] * 0x1p-7f + (v[2] * 0x1p-14f + v[3] * 0x1p-21f)) * (r0 ? 0x1p-28f : 1.f);
+                y += __shfl_xor_sync(0xffffffffu, y, 1);
+                const int odd = *reinterpret_cast<volatile int *>(s_odd);
+                if (odd & 1) y = NAN;
+                else if (odd) {
+#pragma unroll 1
+                    for (int i = 0; i < kTile && o0 + i < last; i++) {
+                        const float again = plain<T>(a, 0, o0 + i);
+                        if (o == i) y = again;
+                    }
                 }
+                if (r0 == 0 && o0 + o < last) put(0, y);
+            } else if (o0 + o < last) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) if (r0 + r < rows) put(r0 + r, v[r]);
             }
         }
     } else {
-        /* ===================== products: a warp has `mine` groups of a stage, one behind the other ===================== */
-        unsigned x[kSets][kMine][4 * W];
-        const T *row = reinterpret_cast<const T *>(a.x) + (size_t)(t0 + min(g, rows - 1)) * a.x_stride;
+        /* ===================== products: a warp has `per` groups of a stage, one behind the other ===================== */
+        columns x[kSets][kMine];
+        const T *row = reinterpret_cast<const T *>(a.x) + (ONE ? 0 : (size_t)min(g, rows - 1) * a.x_stride);
         const int g0 = warp * f.per;
+        const auto load_columns = [&](columns (&to)[kMine], int p) {
+            if constexpr (ONE) {
+                uint8_t *const digits = sm + kOffPart;
+                meet_workers();
+                store_digits<T, W>(row, p * kStageK + tid * 8, a.width, tid, digits, s_units, s_odd);
+                meet_workers();
+#pragma unroll
+                for (int i = 0; i < kMine; i++) {
+                    const bool there = i < f.per && g0 + i < kStageK / kGroup;
+                    int sum = 0;
+#pragma unroll
+                    for (int w = 0; w < W; w++) {
+                        const int c = (g0 + i) * W + w;
+                        const uint2 d = there ? *reinterpret_cast<const uint2 *>(digits + c * 256 + ((g ^ (c & 7)) * 4 + t) * 8) : make_uint2(0, 0);
+                        to[i].x[2 * w] = d.x;
+                        to[i].x[2 * w + 1] = d.y;
+                        sum = __dp4a((int)d.x, 0x01010101, __dp4a((int)d.y, 0x01010101, sum));
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                    for (int k = 0; k < 2; k++) to[i].first[k] = kFirstSum - 8 * __shfl_sync(0xffffffffu, sum, (2 * t + k) * 4);
+                    to[i].unit = there ? s_units[g0 + i] : 0.f;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, to[i].x);
+            }
+        };
         if (P) {
 #pragma unroll
-            for (int p = 0; p < kSets; p++)
-#pragma unroll
-                for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, x[p][i]);
+            for (int p = 0; p < kSets; p++) load_columns(x[p], p);
+            if (ONE) meet_workers();          /* (where the digits lay, parts come) */
         }
         /* where the lane's words are in a stage: line c of four outputs lies behind line c - 1, its 16-byte parts in an order that goes by their address (128-byte swizzle) */
         unsigned at[kMine];
@@ -170,145 +312,128 @@ __global__ void __launch_bounds__(32 * (kWarps + 2), 1) hy3a_linear4_kernel(cons
             const unsigned in_row = (unsigned)((g0 + i) * 16 * W + t * 4 * W), line = (unsigned)(mine_of >> 2) * f.box_bytes + (in_row >> 7) * (kBox * kLine) + (unsigned)(mine_of & 3) * kLine;
             at[i] = ring + line + ((in_row & 127u) ^ ((line >> 3) & 0x70u));
         }
-        const unsigned eight = 2 * f.box_bytes;
-        /* Scales of the lane's two outputs, group 4 i + t of the warp's for i = 0 ..: those of a tile are asked for kAhead tiles before, into registers that nothing
-         * touches until then. */
-        unsigned short sc[kAhead + 1][kSets][kPacks][2];
-        const auto fetch = [&](int o0, int p, unsigned short (&to)[kPacks][2]) {
-#pragma unroll
-            for (int i = 0; i < kPacks; i++) {
-                const int j = p * (kStageK / kGroup) + g0 + 4 * i + t, o = o0 + mine_of;
-                const unsigned short *const s = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)o * a.groups + j;
-                const bool there = 4 * i + t < f.per && j < a.groups;
-                to[i][0] = to[i][1] = 0;
-                if (there && o < last) to[i][0] = s[0];
-                if (there && o + 8 < last) to[i][1] = s[(size_t)8 * a.groups];
-            }
-        };
-        const auto stage = [&](int p, unsigned (&xs)[kMine][4 * W], const unsigned short (&scales)[kPacks][2], float (&acc)[4]) {
+        const unsigned eight = 2 * f.box_bytes, scales_at = ring + (kTile / kBox) * f.box_bytes + mine_of * f.scale_pitch + (g0 + t) * 2;
+        int turn = 0;
+        const auto stage = [&](int o0, int p, const columns (&xs)[kMine], float (&acc)[4]) {
             const int mine = min(f.per, a.groups - p * (kStageK / kGroup) - g0);
+            /* scales of the lane's two outputs, group 4 i + t of the warp's for i = 0 .. */
+            unsigned both[kPacks];
+            if (!f.scale_pitch) {
+#pragma unroll
+                for (int i = 0; i < kPacks; i++) {
+                    const unsigned short *const s = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)(o0 + mine_of) * a.groups + p * (kStageK / kGroup) + g0 + 4 * i + t;
+                    both[i] = 0u;
+                    if (4 * i + t < mine && o0 + mine_of < last) both[i] = s[0];
+                    if (4 * i + t < mine && o0 + mine_of + 8 < last) both[i] |= (unsigned)s[(size_t)8 * a.groups] << 16;
+                }
+            }
             if (mbar_wait(BAR(B_FULL + st), ph, s_abort, g_err, 41u)) {
-                const unsigned by = st * stage_bytes;
-                unsigned both[kPacks];
+                const unsigned by = st * f.stage_bytes;
+                if (f.scale_pitch) {
 #pragma unroll
-                for (int i = 0; i < kPacks; i++) both[i] = (unsigned)scales[i][0] | (unsigned)scales[i][1] << 16;
-                const auto group = [&](int i) {
-                    unsigned wl[W], wh[W];
-                    load_words<W>(at[i] + by, wl);
-                    load_words<W>(at[i] + by + eight, wh);
-                    float d[4];
+                    for (int i = 0; i < kPacks; i++) both[i] = 4 * i + t < mine ? scale_at(scales_at + by + 8 * i) | scale_at(scales_at + by + 8 * i + 8 * f.scale_pitch) << 16 : 0u;
+                }
+                /* Groups that are not there have x and scales of 0, and codes of any value.  (Without branches between them the groups' chains overlap.) */
+                constexpr int kHalf = kMine > 1 ? kMine / 2 : 1;
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        unsigned vl[4], vh[4];
-                        steps<T>::of(wl[w], vl);
-                        steps<T>::of(wh[w], vh);
-                        if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], xs[i][0], xs[i][1]);
-                        else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], xs[i][4 * w], xs[i][4 * w + 1]);
-                        type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], xs[i][4 * w + 2], xs[i][4 * w + 3]);
+                for (int h = 0; h < kMine; h += kHalf) {
+                    if (h >= mine) break;
+#pragma unroll
+                    for (int i = h; i < h + kHalf; i++) {
+                        unsigned wl[W], wh[W];
+                        load_words<W>(at[i] + by, wl);
+                        load_words<W>(at[i] + by + eight, wh);
+                        float d[4], unit;
+                        xs[i].sums(wl, wh, d, unit);
+                        const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
+                        float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
+                        if (ONE) { s0 *= unit; s1 *= unit; }
+                        acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
+                        acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
                     }
-                    const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
-                    const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
-                    acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
-                    acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
-                };
-                /* (without branches between them the groups' chains overlap) */
-                if (mine == kMine) {
-#pragma unroll
-                    for (int i = 0; i < kMine; i++) group(i);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kMine; i++) if (i < mine) group(i);
                 }
             }
             __syncwarp();
-            /* (an arrival does not wait for loads that are under way, so it takes something of the sums that they went into) */
             if (lane == 0) mbar_arrive(BAR(B_EMPTY + st) + ((__float_as_uint(acc[0]) | __float_as_uint(acc[2])) & f.zero));
             if (++st == f.stages) { st = 0; ph ^= 1u; }
         };
-        int turn = 0;
-        /* a tile with its scales in set `now`, those of the tile kAhead further on to set `ahead`; false: given up */
-        const auto tile = [&](int o0, unsigned short (&now)[kSets][kPacks][2], unsigned short (&ahead)[kSets][kPacks][2]) {
+#pragma unroll 1
+        for (int o0 = first; o0 < last; o0 += kTile, turn++) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             if (P) {
 #pragma unroll
-                for (int p = 0; p < kSets; p++) fetch(o0 + kAhead * kTile, p, ahead[p]);
-#pragma unroll
-                for (int p = 0; p < kSets; p++) stage(p, x[p], now[p], acc);
+                for (int p = 0; p < kSets; p++) stage(o0, p, x[p], acc);
             } else {
+#pragma unroll 1
                 for (int p = 0; p < f.passes; p++) {
-                    fetch(o0, p, now[0]);
-#pragma unroll
-                    for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, x[0][i]);
-                    stage(p, x[0], now[0], acc);
+                    load_columns(x[0], p);
+                    stage(o0, p, x[0], acc);
                 }
             }
             const int buf = turn % kParts;
-            if (turn >= kParts && !mbar_wait(BAR(B_TAKEN + buf), (turn / kParts - 1) & 1, s_abort, g_err, 43u)) return false;
-            float *const part = reinterpret_cast<float *>(sm + kOffPart) + (buf * kWarps + warp) * kPart;       /* [output][row] */
+            if (turn >= kParts && !mbar_wait(BAR(B_TAKEN + buf), (turn / kParts - 1) & 1, s_abort, g_err, 43u)) break;
+            float *const part = reinterpret_cast<float *>(sm + kOffPart) + (buf * kWarps + warp) * kPart;       /* [output][column] */
             *reinterpret_cast<float2 *>(part + mine_of * kRows + 2 * t) = make_float2(acc[0], acc[1]);
             *reinterpret_cast<float2 *>(part + (mine_of + 8) * kRows + 2 * t) = make_float2(acc[2], acc[3]);
             __syncwarp();
             if (lane == 0) mbar_arrive(BAR(B_READY + buf));
-            turn++;
-            return true;
-        };
-        if (P) {
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-#pragma unroll
-                for (int p = 0; p < kSets; p++) fetch(first + i * kTile, p, sc[i][p]);
-        }
-        for (int o0 = first; o0 < last; o0 += (kAhead + 1) * kTile) {
-            bool more = true;
-#pragma unroll
-            for (int i = 0; i <= kAhead; i++) more = more && o0 + i * kTile < last && tile(o0 + i * kTile, sc[i], sc[(i + kAhead) % (kAhead + 1)]);
-            if (!more) break;
         }
     }
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of a stage that was given up are still on their way */
 #undef BAR
 }
 
-template <class T, int W, int P>
-cudaError_t launch(const CUtensorMap &tm, few_args f, int device, int sms, void *stream) {
-    constexpr int kWarps = 16;
+template <class T, int W, int P, bool ONE>
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     cudaError_t e;
-    f.per = (f.in_stage + kWarps - 1) / kWarps;
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
-        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P, kWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
     const int boxes = (f.a.out_width + kBox - 1) / kBox;
-    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(32 * (kWarps + 2)), kSmem, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, kWarps>, tm, f);
+    hy3a_launch l(dim3(boxes < sms ? boxes : sms), dim3(kThreads), kSmem, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE>, codes, scales, f);
 }
 template <class T, int W>
-cudaError_t launch_group(const CUtensorMap &tm, const few_args &f, int device, int sms, void *stream) {
-    if (f.passes == 1) return launch<T, W, 1>(tm, f, device, sms, stream);
-    constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers) */
-    return f.passes == 2 ? launch<T, W, kTwo>(tm, f, device, sms, stream) : launch<T, W, 0>(tm, f, device, sms, stream);
+cudaError_t launch_group(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
+    constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers for two stages' x) */
+    if (f.passes == 1) return f.a.rows == 1 ? launch<T, W, 1, true>(codes, scales, f, device, sms, stream) : launch<T, W, 1, false>(codes, scales, f, device, sms, stream);
+    if (f.passes == 2 && kTwo) return f.a.rows == 1 ? launch<T, W, kTwo, kTwo != 0>(codes, scales, f, device, sms, stream) : launch<T, W, kTwo, false>(codes, scales, f, device, sms, stream);
+    return launch<T, W, 0, false>(codes, scales, f, device, sms, stream);
 }
 template <class T>
 cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream, const char **what) {
     const int k = a.width < kStageK ? a.width : kStageK, bytes = a.width / 2;
-    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0, 0u};
+    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0, 0, 0u};
+    f.per = (f.in_stage + kWarps - 1) / kWarps;
     f.box_bytes = (f.lines | 1) * kBox * kLine;
-    f.stages = kRingBytes / (kTile / kBox * f.box_bytes);
+    const bool boxed = a.groups % 8 == 0 && (uintptr_t)a.scales % 16 == 0;
+    if (boxed) f.scale_pitch = 2 * (a.groups < kStageK / a.group ? a.groups : kStageK / a.group);
+    f.stage_bytes = (kTile / kBox * f.box_bytes + kTile * f.scale_pitch + 1023) & ~1023;
+    f.stages = kRingBytes / f.stage_bytes;
     if (f.stages > kMaxStages) f.stages = kMaxStages;
     /* rows of whole lines: [lines][outputs][128 bytes], all lines of a stage in a copy; else [outputs][bytes], a line in a copy */
-    CUtensorMap tm;
+    CUtensorMap codes, scales = {};
     const encode_tiled_fn enc = encoder();
+    const cuuint32_t one[3] = {1, 1, 1};
     const cuuint64_t dims[3] = {(cuuint64_t)(f.whole ? kLine : bytes), (cuuint64_t)a.out_width, (cuuint64_t)(f.whole ? bytes / kLine : 1)}, strides[2] = {(cuuint64_t)bytes, (cuuint64_t)(f.whole ? kLine : 16)};
-    const cuuint32_t box[3] = {kLine, kBox, (cuuint32_t)(f.whole ? f.lines : 1)}, one[3] = {1, 1, 1};
-    if (!enc || enc(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    const cuuint32_t box[3] = {kLine, kBox, (cuuint32_t)(f.whole ? f.lines : 1)};
+    bool ok = enc && enc(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    if (boxed && ok) {
+        const cuuint64_t sdims[2] = {(cuuint64_t)a.groups, (cuuint64_t)a.out_width}, sstrides[1] = {2ull * a.groups};
+        const cuuint32_t sbox[2] = {(cuuint32_t)f.scale_pitch / 2, kTile};
+        ok = enc(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(a.scales), sdims, sstrides, sbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    if (!ok) {
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    if (a.group == 32) return launch_group<T, 1>(tm, f, device, sms, stream);
-    if (a.group == 64) return launch_group<T, 2>(tm, f, device, sms, stream);
-    return launch_group<T, 4>(tm, f, device, sms, stream);
+    if (a.group == 32) return launch_group<T, 1>(codes, scales, f, device, sms, stream);
+    if (a.group == 64) return launch_group<T, 2>(codes, scales, f, device, sms, stream);
+    return launch_group<T, 4>(codes, scales, f, device, sms, stream);
 }
 
 } /* namespace */
@@ -324,7 +449,7 @@ extern "C" int hy3a_linear4(void *stream, int dtype, int rows, int width, int ou
                             int out_dtype, void *out, size_t out_stride) {
     if (dtype != HY3A_F16 && dtype != HY3A_BF16) return hy3a_fail(NULL, HY3A_EINVAL, "linear4: dtype %d not in {1,2}", dtype);
     if (out_dtype != dtype && out_dtype != HY3A_F32) return hy3a_fail(NULL, HY3A_EINVAL, "linear4: out_dtype %d is neither the rows' nor fp32", out_dtype);
-    if (rows < 0) return hy3a_fail(NULL, HY3A_EINVAL, "linear4: rows %d < 0", rows);
+    if (rows < 0 || rows > kMaxRows) return hy3a_fail(NULL, HY3A_EINVAL, "linear4: rows %d not in [0,%d]", rows, kMaxRows);
     int rc = hy3a_quant4_sizes("linear4", out_width, width, group);
     if (rc) return rc;
     if (rows == 0 || out_width == 0) return HY3A_OK;

@@ -50,5 +50,21 @@ template <> struct steps<__half> {
     }
 };
 
+/* out[t][o] from the definition, by a warp */
+template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {
+    const int lane = threadIdx.x & 31;
+    const T *const x = reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride, *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
+    const uint8_t *const codes = a.codes + (size_t)o * (a.width / 2);
+    float sum = 0.f;
+    for (int k = 2 * lane; k < a.width; k += 64) {
+        const int both = codes[k >> 1];
+        const float s = type<T>::up(scales[k / a.group]);
+        sum = fmaf((float)((both & 15) - 8) * s, type<T>::up(x[k]), sum);
+        sum = fmaf((float)((both >> 4) - 8) * s, type<T>::up(x[k + 1]), sum);
+    }
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+    return sum;
+}
 } /* namespace hy3a_layer */
 #endif
