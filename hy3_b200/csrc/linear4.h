@@ -31,6 +31,15 @@ __device__ __forceinline__ unsigned and_or(unsigned a, unsigned mask, unsigned b
 }
 template <class T> struct steps;
 template <> struct steps<__nv_bfloat16> {
+    /* the same as the pairs (0, 1), (2, 3), (4, 5), (6, 7) */
+    static __device__ __forceinline__ void in_order(unsigned w, unsigned (&v)[4]) {
+        const unsigned odd = w >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned c = and_or(__byte_perm(w, odd, 0x4400 + 0x1111 * i), 0x000f000fu, 0x43004300u);
+            asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(c), "r"(0x43084308u));
+        }
+    }
     static __device__ __forceinline__ void of(unsigned w, unsigned (&v)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -40,6 +49,13 @@ template <> struct steps<__nv_bfloat16> {
     }
 };
 template <> struct steps<__half> {
+    static __device__ __forceinline__ void in_order(unsigned w, unsigned (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const unsigned c = and_or(__byte_perm(w, 0, 0x1111 * i), 0x00f0000fu, 0x64006400u);       /* 1024 + c, 1024 + 16 c */
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[i]) : "r"(c), "r"(0x2c003c00u) /* 1, 1 / 16 */, "r"(0xd480e408u) /* -1032, -72 */);
+        }
+    }
     static __device__ __forceinline__ void of(unsigned w, unsigned (&v)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {

@@ -5,8 +5,8 @@
  * rows of x in shared memory.  Codes become weights on their way: a thread has an output, reads its codes of 64 k's from shared memory, and stores (code - 8) * scale
  * as the A operand into tensor memory, from where the product takes it; shared memory sees 4 bits a weight, and the tensor cores read only x from there.  Per CTA:
  *   warps 0-15 weights: each four of them (a lane quarter each) every fourth step of 64 k's; afterwards the results;
- *   warp 16   TMA producer: codes, 128 k's at a time, and x, 64 k's at a time;
- *   warp 17   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
+ *   warps 16, 17 TMA producers: codes, 128 k's at a time, and x, 64 k's at a time;
+ *   warp 18   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
  *
  * Rounding: a weight has up to 15 bits (fp16) or 11 (bf16).  Where the result is of the rows' type the weight is rounded to it once; where the result is fp32 it enters as
  * two numbers, the rounded one and the rest, which is exact.  Results that are not finite (a rounded weight over the type's largest, an infinite x that meets the rest)
@@ -27,20 +27,20 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kTeams = 4 /* of four warps: a warp for each 32 outputs */, kWorkers = 4 * kTeams, kProducer = kWorkers, kIssuer = kWorkers + 1, kThreads = 32 * (kWorkers + 2);
+constexpr int kTeams = 4 /* of four warps: a warp for each 32 outputs */, kWorkers = 4 * kTeams, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
 constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
-constexpr int kMostSteps = 8, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kMostSteps * kStepBytes, kSmem = kOffBar + 512 + 1024;
-constexpr int kAColumn = 256;          /* tensor memory: the sums, then the stages of A */
+constexpr int kMostSplits = 4;
+constexpr int kMostSteps = 12 /* of x and A: as tensor memory has room for A beside the sums, and shared memory for x */, kXBytes = 8 * kStepBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
 enum { B_CODES = 0, B_CODES_FREE = kUnits, B_X = 2 * kUnits, B_A = 2 * kUnits + kMostSteps, B_FREE = 2 * kUnits + 2 * kMostSteps, B_SUMS = 2 * kUnits + 3 * kMostSteps, B_COUNT };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
-static_assert(kMostSteps % kTeams == 0 && kUnits % (kTeams / 2) == 0, "teams' turns");
+static_assert(kUnits % (kTeams / 2) == 0, "teams' turns");
 static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
 struct many_args {
     linear4_args a;
-    int columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits;
+    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -100,23 +100,54 @@ template <> struct pair_of<__half> {
     static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 
-/* v of the lanes that are `mine`, of output o and row t: what is not finite is computed again */
-template <class T> __device__ __forceinline__ float settled(const linear4_args &a, float v, bool mine, int t, int o) {
-    unsigned todo = __ballot_sync(0xffffffffu, mine && !(fabsf(v) < INFINITY));
-    while (todo) {
-        const int l = __ffs(todo) - 1;
-        const float again = plain<T>(a, __shfl_sync(0xffffffffu, t, l), __shfl_sync(0xffffffffu, o, l));
-        if ((int)(threadIdx.x & 31) == l) v = again;
-        todo &= todo - 1;
+/* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is computed again, by the whole warp (rare: one piece of code, not unrolled) */
+template <class T, int N> __device__ __forceinline__ void settle(const linear4_args &a, float (&y)[N], int n, int t, int o, bool mine) {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < N; j++) odd |= j < n && !(fabsf(y[j]) < INFINITY);
+    unsigned todo = __ballot_sync(0xffffffffu, odd && mine);
+#pragma unroll 1
+    for (; todo; todo &= todo - 1) {
+        const int l = __ffs(todo) - 1, its = __shfl_sync(0xffffffffu, o, l);
+#pragma unroll 1
+        for (int j = 0; j < n; j++) {
+            float was = y[0];
+#pragma unroll
+            for (int k = 1; k < N; k++) if (j == k) was = y[k];
+            if (fabsf(__shfl_sync(0xffffffffu, was, l)) < INFINITY) continue;
+            const float again = plain<T>(a, t + j, its);
+#pragma unroll
+            for (int k = 0; k < N; k++) if (j == k && (int)(threadIdx.x & 31) == l) y[k] = again;
+        }
     }
-    return v;
+}
+/* A lane's results of its output, row after row.  16-bit ones: neighbouring lanes exchange, so that one stores the even rows' two outputs and one the odd rows'. */
+template <class T, bool WIDE, int N> __device__ __forceinline__ void store(const linear4_args &a, const float (&y)[N], int n, int t, int o, int odd_stride) {
+    const bool mine = o < a.out_width;
+    if (WIDE) {
+#pragma unroll
+        for (int j = 0; j < N; j++) if (j < n && mine) reinterpret_cast<float *>(a.out)[(size_t)(t + j) * a.out_stride + o] = y[j];
+    } else if (odd_stride) {
+#pragma unroll
+        for (int j = 0; j < N; j++) if (j < n && mine) reinterpret_cast<T *>(a.out)[(size_t)(t + j) * a.out_stride + o] = type<T>::down(y[j]);
+    } else {
+        const int lane = threadIdx.x & 31, side = lane & 1;
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, side ? y[j] : y[j + 1], 1);
+            T two[2] = {type<T>::down(side ? other : y[j]), type<T>::down(side ? y[j + 1] : other)};
+            if (j + side < n && mine) *reinterpret_cast<unsigned *>(reinterpret_cast<T *>(a.out) + (size_t)(t + j + side) * a.out_stride + o - side) = *reinterpret_cast<const unsigned *>(two);
+        }
+    }
 }
 
 /* WIDE: the result is fp32, weights are two numbers.  PER: scales of 64 k's (groups of 32: two) */
 template <class T, bool WIDE, int PER>
 __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
     extern __shared__ uint8_t s_raw[];
-    constexpr int kSteps = WIDE ? 4 : 8 /* stages of x and A */, kAWide = WIDE ? 64 : 32 /* columns of a stage of A */;
+    constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */;
+    const int n_steps = f.steps;
+    const unsigned x_bytes_up = (f.columns * 64 + 1023) & ~1023u;          /* (half the rows of 64 k's, from 1024 to 1024) */
     const linear4_args &a = f.a;
     uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const unsigned sbase = smem_u32(sm), bar0 = sbase + kOffBar;
@@ -132,11 +163,11 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
     if (tid == 0) {
         *s_abort = 0;
         for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), 8 /* two teams */); }
-        for (int i = 0; i < kSteps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), 8 /* a team of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
+        for (int i = 0; i < n_steps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), 8 /* a team of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
         mbar_init(BAR(B_SUMS), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kProducer && lane < 2) {
+    if (warp == kCodes && lane < 2) {
         const CUtensorMap *m = lane == 0 ? &tm_codes : &tm_x;
         asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
@@ -152,33 +183,36 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
     pdl_release();
     pdl_wait();
 
-    if (warp == kProducer) {
-        /* ===================== producer ===================== */
+    if (warp == kCodes) {
+        /* ===================== producer of codes ===================== */
         const unsigned lead = elect_one();
         unsigned long long policy;
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-        int unit = 0, st = 0;
-        unsigned uph = 0, ph = 0;
-        bool ok = true;
-        /* (codes run ahead of x: as far as their ring goes) */
-        int asked = u0;
-        for (int s = 0; s < steps && ok; s++) {
-            while (asked < u1 && asked - u0 - (s >> 1) < kUnits) {
-                if (!(ok = mbar_wait(BAR(B_CODES_FREE + unit), uph ^ 1u, s_abort, g_err, 50u))) break;
-                if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
-                tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), asked * (kUnit / 2), m0, policy, lead);
-                asked++;
-                if (++unit == kUnits) { unit = 0; uph ^= 1u; }
-            }
-            if (!ok || !(ok = mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
+        int unit = 0;
+        unsigned ph = 0;
+#pragma unroll 1
+        for (int u = u0; u < u1; u++) {
+            if (!mbar_wait(BAR(B_CODES_FREE + unit), ph ^ 1u, s_abort, g_err, 50u)) break;
+            if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
+            tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), u * (kUnit / 2), m0, policy, lead);
+            if (++unit == kUnits) { unit = 0; ph ^= 1u; }
+        }
+    } else if (warp == kRowsOfX) {
+        /* ===================== producer of x ===================== */
+        const unsigned lead = elect_one();
+        int st = 0;
+        unsigned ph = 0;
+#pragma unroll 1
+        for (int s = 0; s < steps; s++) {
+            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u)) break;
             if (lead && rank == 0) mbar_expect_tx(BAR(B_X + st), N * 128);
-            tma_rows(sbase + kOffX + st * kStepBytes, &tm_x, cluster_addr(BAR(B_X + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
-            if (++st == kSteps) { st = 0; ph ^= 1u; }
+            tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_X + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
+            if (++st == n_steps) { st = 0; ph ^= 1u; }
         }
         /* the last commits reach the barriers of both CTAs before either leaves */
-        for (int i = 0; i < kSteps && !*s_abort; i++) {
+        for (int i = 0; i < n_steps && !*s_abort; i++) {
             if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 52u)) break;
-            if (++st == kSteps) { st = 0; ph ^= 1u; }
+            if (++st == n_steps) { st = 0; ph ^= 1u; }
         }
     } else if (warp == kIssuer) {
         if (rank == 0) {
@@ -193,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             for (int s = 0; s < steps; s++) {
                 if (!(ok = mbar_wait(BAR(B_X + st), ph, s_abort, g_err, 53u) && mbar_wait(BAR(B_A + st), ph, s_abort, g_err, 54u))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned long long db = make_desc(sbase + kOffX + st * kStepBytes);
-                const unsigned da = tmem + kAColumn + st * kAWide;
+                const unsigned long long db = make_desc(sbase + kOffX + st * x_bytes_up);
+                const unsigned da = tmem + f.a_column + st * kAWide;
 #pragma unroll
                 for (int k = 0; k < 4; k++) umma_lead(tmem, da + 8 * k, db + 2 * k, idesc, s + k > 0, lead);
                 if (WIDE) {
@@ -202,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
                     for (int k = 0; k < 4; k++) umma_lead(tmem, da + 32 + 8 * k, db + 2 * k, idesc, 1, lead);
                 }
                 umma_commit_lead(BAR(B_FREE + st), both, lead);
-                if (++st == kSteps) { st = 0; ph ^= 1u; }
+                if (++st == n_steps) { st = 0; ph ^= 1u; }
             }
             if (ok) umma_commit_lead(BAR(B_SUMS), both, lead);
         }
@@ -211,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
         const int quarter = warp & 3, team = warp >> 2, half = team & 1 /* of a unit */, r = quarter * 32 + lane, o = m0 + r;
         const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
-        const unsigned to_a = tmem + kAColumn + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
+        const unsigned to_a = tmem + f.a_column + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
         unsigned short sc[3][PER];
         const auto fetch = [&](int s, unsigned short (&to)[PER]) {
 #pragma unroll
@@ -237,9 +271,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const unsigned s2 = __byte_perm(now[i * PER / 8], 0, 0x1010);
-                unsigned v[4];
-                hy3a_layer::steps<T>::of(w[i], v);
-                const unsigned n[4] = {__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)};
+                unsigned n[4];
+                hy3a_layer::steps<T>::in_order(w[i], n);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     hi[4 * i + j] = pair_of<T>::mul(n[j], s2);
@@ -259,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             unit += kTeams / 2;
             if (unit >= kUnits) { unit -= kUnits; uph ^= 1u; }
             st += kTeams;
-            if (st >= kSteps) { st -= kSteps; ph ^= 1u; }
+            if (st >= n_steps) { st -= n_steps; ph ^= 1u; }
             return true;
         };
         fetch(team, sc[0]);
@@ -277,17 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
                 unsigned v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
+                const int n = min(16, rows - c0);
+                if (f.splits > 1) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    if (c0 + j >= rows) break;
-                    if (f.splits > 1) { *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = __uint_as_float(v[j]); continue; }
-                    const bool mine = o < a.out_width;
-                    const float y = settled<T>(a, __uint_as_float(v[j]), mine, row0 + c0 + j, o);
-                    if (!mine) continue;
-                    const size_t to = (size_t)(row0 + c0 + j) * a.out_stride + o;
-                    if (WIDE) reinterpret_cast<float *>(a.out)[to] = y;
-                    else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
+                    for (int j = 0; j < 16; j++) if (j < n) *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = __uint_as_float(v[j]);
+                    continue;
                 }
+                float y[16];
+#pragma unroll
+                for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
+                settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
+                store<T, WIDE>(a, y, n, row0 + c0, o, f.odd_out);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
@@ -301,19 +334,21 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
         /* each CTA adds up the rows of its share, in the order of the k's */
         if (warp < kWorkers && !*s_abort) {
             const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
-            for (int c = first + (tid >> 7); c < last; c += kTeams) {
-                float y = 0.f;
-                for (int i = 0; i < f.splits; i++) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(sbase + (c * 128 + r) * 4, 2 * i + rank)) : "memory");
-                    y += v;
-                }
-                const bool mine = o < a.out_width;
-                y = settled<T>(a, y, mine, row0 + c, o);
-                if (!mine) continue;
-                const size_t to = (size_t)(row0 + c) * a.out_stride + o;
-                if (WIDE) reinterpret_cast<float *>(a.out)[to] = y;
-                else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
+#pragma unroll 1
+            for (int c = first + 2 * (tid >> 7); c < last; c += 2 * kTeams) {
+                float part[kMostSplits][2], y[2] = {0.f, 0.f};
+                const int n = min(2, last - c);
+#pragma unroll
+                for (int i = 0; i < kMostSplits; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        part[i][j] = 0.f;
+                        if (i < f.splits && j < n) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[i][j]) : "r"(cluster_addr(sbase + ((c + j) * 128 + r) * 4, 2 * i + rank)) : "memory");
+                    }
+#pragma unroll
+                for (int i = 0; i < kMostSplits; i++) { y[0] += part[i][0]; y[1] += part[i][1]; }
+                settle<T>(a, y, n, row0 + c, o, o < a.out_width);
+                store<T, WIDE>(a, y, n, row0 + c, o, f.odd_out);
             }
         }
         __syncwarp();
@@ -345,7 +380,7 @@ cudaError_t launch_type(const CUtensorMap &codes, const CUtensorMap &x, const ma
 } /* namespace */
 
 cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, int sms, void *stream, const char **what) {
-    many_args f = {a, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1};
+    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0};
     const int pairs = sms / 2;
     /* Row tiles: as few as there have to be, or more where their tiles then take less time: rounds of all pairs times a tile's rows. */
     int row_tiles = (a.rows + 255) / 256;
@@ -356,7 +391,13 @@ cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int devic
         if (least < 0 || cost < least) { least = cost; row_tiles = need; f.columns = columns; }
     }
     const long long tiles = (long long)row_tiles * f.m_tiles;
-    while (f.splits < 4 && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
+    while (f.splits < kMostSplits && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
+    const int wide = a.wide ? 64 : 32;
+    f.steps = (512 - f.columns) / wide;
+    const int fit = kXBytes / ((f.columns * 64 + 1023) & ~1023);
+    if (f.steps > fit) f.steps = fit;
+    if (f.steps > kMostSteps) f.steps = kMostSteps;
+    f.a_column = 512 - f.steps * wide;
     *what = NULL;
     CUtensorMap codes, x;
     const encode_tiled_fn enc = encoder();
