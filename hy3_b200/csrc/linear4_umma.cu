@@ -6,11 +6,14 @@
  * as the A operand into tensor memory, from where the product takes it; shared memory sees 4 bits a weight, and the tensor cores read only x from there.  Per CTA:
  *   warps 0-15 weights: each four of them (a lane quarter each) every fourth step of 64 k's; afterwards the results;
  *   warps 16, 17 TMA producers: codes, 128 k's at a time, and x, 64 k's at a time;
- *   warp 18   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, 8 where the result is fp32.
+ *   warp 18   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step.
  *
- * Rounding: a weight has up to 15 bits (fp16) or 11 (bf16).  Where the result is of the rows' type the weight is rounded to it once; where the result is fp32 it enters as
- * two numbers, the rounded one and the rest, which is exact.  Results that are not finite (a rounded weight over the type's largest, an infinite x that meets the rest)
- * are computed again from the definition, by the warp that finds them.
+ * Results of the rows' type: a weight, of up to 15 bits (fp16) or 11 (bf16), is rounded to that type once, which leaves an error like the result's own rounding.  Results that are not finite (of weights
+ * rounded beyond the type's largest) are computed again from the definition, by the warp that finds them.
+ *
+ * Results in fp32: A is code - 8, which is exact, and a group's sum by itself; the tensor cores begin anew with each group, in one of four sums of up to 64 rows.  Warps 0-7 (every second step
+ * each four) make A, and warps 8-23 (every second group each eight) add scale * sum to results in registers, in fp32.  (Weights as two numbers, the rounded one and the rest, with one sum for all k's were twice the products, and
+ * the tensor cores' sums, which are cut off and not rounded, left an error of 5.6e-6 of the result over 4096 k's; 64 rows on 10240 x 4096 23.1 us.)
  *
  * Where tiles are few, the CTAs of a cluster share the k's of a tile; their sums meet in shared memory, and are added in the order of the k's.
  *
@@ -27,13 +30,11 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kTeams = 4 /* of four warps: a warp for each 32 outputs */, kWorkers = 4 * kTeams, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
 constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
 constexpr int kMostSplits = 4;
 constexpr int kMostSteps = 12 /* of x and A: as tensor memory has room for A beside the sums, and shared memory for x */, kXBytes = 8 * kStepBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
-enum { B_CODES = 0, B_CODES_FREE = kUnits, B_X = 2 * kUnits, B_A = 2 * kUnits + kMostSteps, B_FREE = 2 * kUnits + 2 * kMostSteps, B_SUMS = 2 * kUnits + 3 * kMostSteps, B_COUNT };
+enum { B_CODES = 0, B_CODES_FREE = kUnits, B_STEP = 2 * kUnits /* x and A of a step are there */, B_FREE = 2 * kUnits + kMostSteps, B_SUMS = 2 * kUnits + 2 * kMostSteps, B_GROUP, B_GROUP_FREE = B_GROUP + 4, B_COUNT = B_GROUP_FREE + 4 };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
-static_assert(kUnits % (kTeams / 2) == 0, "teams' turns");
 static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
@@ -90,14 +91,29 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, unsigned (&r)[16]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
+/* A wait's answer takes 100 clocks and more, also where nothing is waited for: the issuer looks at its barriers ahead of time, and waits only if that did not show them through.  What all_wait tells is the same
+ * for all lanes, and the compiler knows (where it does not, each product that the warp issues behind it costs 100 clocks). */
+__device__ __forceinline__ unsigned peek(unsigned bar, unsigned parity) {
+    unsigned ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __forceinline__ bool all_wait(unsigned seen, unsigned bar, unsigned parity, volatile int *abort_flag, unsigned where) {
+    return __all_sync(0xffffffffu, seen) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, g_err, where));
+}
+struct f2 { float x, y; };
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 c, a, b, c;\n mov.b64 {%0, %1}, c;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
 template <class T> struct pair_of;
 template <> struct pair_of<__nv_bfloat16> {
     static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 template <> struct pair_of<__half> {
     static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
-    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 
 /* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is computed again, by the whole warp (rare: one piece of code, not unrolled) */
@@ -141,11 +157,17 @@ template <class T, bool WIDE, int N> __device__ __forceinline__ void store(const
     }
 }
 
-/* WIDE: the result is fp32, weights are two numbers.  PER: scales of 64 k's (groups of 32: two) */
+/* The warps of a CTA: teams of four that make A (a warp for each 32 outputs), those that add up groups, two producers, the issuer. */
+template <bool WIDE> struct warps_of {
+    static constexpr int kTeams = WIDE ? 2 : 4, kAdders = WIDE ? 16 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
+};
+
+/* WIDE: the result is fp32, PER: products (of 16 k's) of a group; else PER: scales of 64 k's (groups of 32: two) */
 template <class T, bool WIDE, int PER>
-__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
+__global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
     extern __shared__ uint8_t s_raw[];
-    constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */;
+    using W = warps_of<WIDE>;
+    constexpr int kAWide = 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kBufs = 4, kGroupColumns = 64 /* WIDE: sums of a group */;
     const int n_steps = f.steps;
     const unsigned x_bytes_up = (f.columns * 64 + 1023) & ~1023u;          /* (half the rows of 64 k's, from 1024 to 1024) */
     const linear4_args &a = f.a;
@@ -163,8 +185,9 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
     if (tid == 0) {
         *s_abort = 0;
         for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), 8 /* two teams */); }
-        for (int i = 0; i < n_steps; i++) { mbar_init(BAR(B_X + i), 1); mbar_init(BAR(B_A + i), 8 /* a team of each CTA */); mbar_init(BAR(B_FREE + i), 1); }
+        for (int i = 0; i < n_steps; i++) { mbar_init(BAR(B_STEP + i), 9 /* a team of each CTA, and the bytes of x */); mbar_init(BAR(B_FREE + i), 1); }
         mbar_init(BAR(B_SUMS), 1);
+        for (int i = 0; i < kBufs; i++) { mbar_init(BAR(B_GROUP + i), 1); mbar_init(BAR(B_GROUP_FREE + i), 16 /* eight warps of each CTA */); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kCodes && lane < 2) {
@@ -205,8 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
 #pragma unroll 1
         for (int s = 0; s < steps; s++) {
             if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u)) break;
-            if (lead && rank == 0) mbar_expect_tx(BAR(B_X + st), N * 128);
-            tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_X + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
+            if (lead && rank == 0) mbar_expect_tx(BAR(B_STEP + st), N * 128);
+            tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
             if (++st == n_steps) { st = 0; ph ^= 1u; }
         }
         /* the last commits reach the barriers of both CTAs before either leaves */
@@ -221,35 +244,108 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             constexpr unsigned kType = type<T>::code == HY3A_BF16 ? (1u << 7) | (1u << 10) : 0u;
             const unsigned idesc = (1u << 4) | kType | (((unsigned)N >> 3) << 17) | ((256u >> 4) << 24);
             const unsigned short both = (unsigned short)(3u << leader);
-            int st = 0;
-            unsigned ph = 0;
+            int st = 0, buf = 0;
+            unsigned ph = 0, gph = 0, seen = 0, group_seen = WIDE ? peek(BAR(B_GROUP_FREE), 1u) : 0;
             bool ok = true;
             for (int s = 0; s < steps; s++) {
-                if (!(ok = mbar_wait(BAR(B_X + st), ph, s_abort, g_err, 53u) && mbar_wait(BAR(B_A + st), ph, s_abort, g_err, 54u))) break;
+                if (!(ok = all_wait(seen, BAR(B_STEP + st), ph, s_abort, 53u))) break;
+                const int next = st + 1 == n_steps ? 0 : st + 1;
+                const unsigned next_ph = next ? ph : ph ^ 1u;
+                seen = peek(BAR(B_STEP + next), next_ph);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned long long db = make_desc(sbase + kOffX + st * x_bytes_up);
                 const unsigned da = tmem + f.a_column + st * kAWide;
+                if (!WIDE) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) umma_lead(tmem, da + 8 * k, db + 2 * k, idesc, s + k > 0, lead);
-                if (WIDE) {
+                    for (int k = 0; k < 4; k++) umma_lead(tmem, da + 8 * k, db + 2 * k, idesc, s + k > 0, lead);
+                } else {
+                    constexpr int kRuns = PER == 2 ? 2 : 1, kInRun = 4 / kRuns;        /* products of a step that go to one sum */
+                    const bool begins = PER < 8 || s % 2 == 0, ends = PER < 8 || s % 2 == 1;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) umma_lead(tmem, da + 32 + 8 * k, db + 2 * k, idesc, 1, lead);
+                    for (int run = 0; run < kRuns; run++) {
+                        if (begins && !(ok = all_wait(group_seen, BAR(B_GROUP_FREE + buf), gph ^ 1u, s_abort, 59u))) break;
+                        const unsigned d = tmem + buf * kGroupColumns, group = BAR(B_GROUP + buf);
+                        if (ends) {
+                            if (++buf == kBufs) { buf = 0; gph ^= 1u; }
+                            group_seen = peek(BAR(B_GROUP_FREE + buf), gph ^ 1u);
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                        for (int k = run * kInRun; k < (run + 1) * kInRun; k++) umma_lead(d, da + 8 * k, db + 2 * k, idesc, !begins || k > run * kInRun, lead);
+                        if (ends) umma_commit_lead(group, both, lead);
+                    }
+                    if (!ok) break;
                 }
                 umma_commit_lead(BAR(B_FREE + st), both, lead);
-                if (++st == n_steps) { st = 0; ph ^= 1u; }
+                st = next;
+                ph = next_ph;
             }
             if (ok) umma_commit_lead(BAR(B_SUMS), both, lead);
         }
+    } else if (WIDE && warp >= 4 * kTeams) {
+        /* ===================== groups: eight warps take every other one; a lane has an output, the warp every other 16 rows ===================== */
+        const int quarter = warp & 3, half = (warp >> 2) & 1, set = (warp >> 3) - 1, r = quarter * 32 + lane, o = m0 + r;
+        const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
+        const int g0 = u0 * (kUnit / a.group), groups = (u1 - u0) * (kUnit / a.group);
+        f2 acc[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) acc[i][k] = {0.f, 0.f};
+        /* (scales are asked for three of the warp's groups before) */
+        unsigned short sc[3];
+        const auto fetch = [&](int j, unsigned short &to) { to = 0; if (j < groups && g0 + j < a.groups) to = scales[g0 + j]; };
+#pragma unroll
+        for (int q = 0; q < 3; q++) fetch(set + 2 * q, sc[q]);
+        bool ok = true;
+        int buf = set;
+        unsigned ph = 0;
+#pragma unroll 1
+        for (int j = set; j < groups && ok; j += 6) {
+#pragma unroll
+            for (int q = 0; q < 3; q++) {
+                if (!ok || j + 2 * q >= groups) break;
+                if (!(ok = mbar_wait(BAR(B_GROUP + buf), ph, s_abort, g_err, 60u))) break;
+                __syncwarp();
+                const unsigned group_free = cluster_addr(BAR(B_GROUP_FREE + buf), leader), from = tmem + ((unsigned)(quarter * 32) << 16) + buf * kGroupColumns;
+                buf ^= 2;
+                if (buf == set) ph ^= 1u;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float s = type<T>::up(*reinterpret_cast<const T *>(&sc[q]));
+                fetch(j + 2 * q + 6, sc[q]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int c0 = (2 * i + half) * 16;
+                    if (c0 >= N) break;
+                    unsigned v[16];
+                    tmem_ld16(from + c0, v);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) acc[i][k] = fma2({__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])}, {s, s}, acc[i][k]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(group_free);
+            }
+        }
+        /* (codes and x lie where the sums go: until the last product is through) */
+        if (ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 61u)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    if ((2 * i + half) * 16 + k < rows) *reinterpret_cast<float *>(sm + ((set * kGroupColumns + (2 * i + half) * 16 + k) * 128 + r) * 4) = k & 1 ? acc[i][k / 2].y : acc[i][k / 2].x;
+        }
     } else {
-        /* ===================== weights: a thread has an output; each team takes every fourth step ===================== */
+        /* ===================== weights: a thread has an output; each team takes every second or fourth step ===================== */
         const int quarter = warp & 3, team = warp >> 2, half = team & 1 /* of a unit */, r = quarter * 32 + lane, o = m0 + r;
         const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
         const unsigned to_a = tmem + f.a_column + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
-        unsigned short sc[3][PER];
-        const auto fetch = [&](int s, unsigned short (&to)[PER]) {
+        constexpr int kScales = WIDE ? 1 : PER;
+        unsigned short sc[3][kScales];
+        const auto fetch = [&](int s, unsigned short (&to)[kScales]) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
+            for (int i = 0; i < kScales; i++) {
                 const int j = (u0 * kUnit + s * 64 + 32 * i) >> shift;
                 to[i] = 0;
                 if (s < steps && j < a.groups) to[i] = scales[j];
@@ -257,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
         };
         int st = team, unit = team >> 1;
         unsigned ph = 0, uph = 0;
-        const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
-            fetch(s + 2 * kTeams, ahead);
+        const auto step = [&](int s, const unsigned short (&now)[kScales], unsigned short (&ahead)[kScales]) {
+            if (!WIDE) fetch(s + 2 * kTeams, ahead);
             if (!mbar_wait(BAR(B_CODES + unit), uph, s_abort, g_err, 55u)) return false;
             uint4 c[2];
 #pragma unroll
@@ -267,36 +363,34 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[i].x), "=r"(c[i].y), "=r"(c[i].z), "=r"(c[i].w) : "r"(at));
             }
             const unsigned w[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
-            unsigned hi[32], lo[WIDE ? 32 : 1];
+            unsigned weights[32];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const unsigned s2 = __byte_perm(now[i * PER / 8], 0, 0x1010);
                 unsigned n[4];
                 hy3a_layer::steps<T>::in_order(w[i], n);
+                const unsigned s2 = __byte_perm(now[i * kScales / 8], 0, 0x1010);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    hi[4 * i + j] = pair_of<T>::mul(n[j], s2);
-                    if (WIDE) lo[WIDE ? 4 * i + j : 0] = pair_of<T>::rest(n[j], s2, hi[4 * i + j]);
-                }
+                for (int j = 0; j < 4; j++) weights[4 * i + j] = WIDE ? n[j] : pair_of<T>::mul(n[j], s2);
             }
             if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
             __syncwarp();              /* (lanes may leave the wait one by one; what follows is the whole warp's) */
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            tmem_st32(to_a + st * kAWide, hi);
-            if constexpr (WIDE) tmem_st32(to_a + st * kAWide + 32, lo);
+            tmem_st32(to_a + st * kAWide, weights);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             /* (the codes are given back behind a store that needed them: an arrival does not wait for loads that are under way) */
-            if (lane == 0) { mbar_arrive_cluster(cluster_addr(BAR(B_A + st), leader)); mbar_arrive(BAR(B_CODES_FREE + unit)); }
+            if (lane == 0) { mbar_arrive_cluster(cluster_addr(BAR(B_STEP + st), leader)); mbar_arrive(BAR(B_CODES_FREE + unit)); }
             unit += kTeams / 2;
             if (unit >= kUnits) { unit -= kUnits; uph ^= 1u; }
             st += kTeams;
             if (st >= n_steps) { st -= n_steps; ph ^= 1u; }
             return true;
         };
-        fetch(team, sc[0]);
-        fetch(team + kTeams, sc[1]);
+        if (!WIDE) {
+            fetch(team, sc[0]);
+            fetch(team + kTeams, sc[1]);
+        }
         bool ok = true;
         for (int s = team; s < steps && ok; s += 3 * kTeams) {
             ok = step(s, sc[0], sc[2]);
@@ -304,9 +398,10 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
             if (ok && s + 2 * kTeams < steps) ok = step(s + 2 * kTeams, sc[2], sc[1]);
         }
         /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
-        if (ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 57u)) {
+        if (!WIDE && ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 57u)) {
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
             for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
                 unsigned v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
@@ -320,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
 #pragma unroll
                 for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
                 settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
-                store<T, WIDE>(a, y, n, row0 + c0, o, f.odd_out);
+                store<T, false>(a, y, n, row0 + c0, o, f.odd_out);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
@@ -329,29 +424,41 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_umma_kernel(const __
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the step that was given up are still on their way */
-    cluster_sync();
-    if (f.splits > 1) {
-        /* each CTA adds up the rows of its share, in the order of the k's */
-        if (warp < kWorkers && !*s_abort) {
-            const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
+    /* Sums in shared memory: each CTA adds up the rows of its share, in the order of the k's (WIDE: even groups and odd ones by themselves).  part(i, h, j): of row c + j, split i, set h. */
+    constexpr int kSets = WIDE ? 2 : 1, kAtOnce = 4;
+    const auto add_up = [&](const auto &part) {
+        if (warp >= 16 || *s_abort) return;
+        const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
 #pragma unroll 1
-            for (int c = first + 2 * (tid >> 7); c < last; c += 2 * kTeams) {
-                float part[kMostSplits][2], y[2] = {0.f, 0.f};
-                const int n = min(2, last - c);
+        for (int c = first + kAtOnce * (tid >> 7); c < last; c += kAtOnce * 4) {
+            float y[kAtOnce] = {};
+            const int n = min(kAtOnce, last - c);
 #pragma unroll
-                for (int i = 0; i < kMostSplits; i++)
+            for (int i = 0; i < kMostSplits; i++) {
+                if (i == f.splits) break;
+                float v[kSets][kAtOnce];
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        part[i][j] = 0.f;
-                        if (i < f.splits && j < n) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[i][j]) : "r"(cluster_addr(sbase + ((c + j) * 128 + r) * 4, 2 * i + rank)) : "memory");
-                    }
+                for (int h = 0; h < kSets; h++)
 #pragma unroll
-                for (int i = 0; i < kMostSplits; i++) { y[0] += part[i][0]; y[1] += part[i][1]; }
-                settle<T>(a, y, n, row0 + c, o, o < a.out_width);
-                store<T, WIDE>(a, y, n, row0 + c, o, f.odd_out);
+                    for (int j = 0; j < kAtOnce; j++) v[h][j] = part(i, ((h * kGroupColumns + c + j) * 128 + r) * 4);        /* (rows past the last lie in shared memory as well) */
+#pragma unroll
+                for (int h = 0; h < kSets; h++)
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; j++) y[j] += v[h][j];
             }
+            if (!WIDE) settle<T>(a, y, n, row0 + c, o, o < a.out_width);
+            store<T, WIDE>(a, y, n, row0 + c, o, f.odd_out);
         }
         __syncwarp();
+    };
+    if (WIDE && f.splits == 1) add_up([&](int, int at) { return *reinterpret_cast<const float *>(sm + at); });
+    cluster_sync();
+    if (f.splits > 1) {
+        add_up([&](int i, int at) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(sbase + at, 2 * i + rank)) : "memory");
+            return v;
+        });
         cluster_sync();
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -367,14 +474,14 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_ar
         if ((e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
-    hy3a_launch l(dim3((unsigned)tiles * 2 * f.splits), dim3(kThreads), kSmem, stream);
+    hy3a_launch l(dim3((unsigned)tiles * 2 * f.splits), dim3(warps_of<WIDE>::kThreads), kSmem, stream);
     l.cluster(2 * f.splits);
     return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_umma_kernel<T, WIDE, PER>, codes, x, f);
 }
 template <class T>
 cudaError_t launch_type(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
-    if (f.a.group == 32) return f.a.wide ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 2>(codes, x, f, tiles, device, stream);
-    return f.a.wide ? launch<T, true, 1>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
+    if (f.a.wide) return f.a.group == 32 ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : (f.a.group == 64 ? launch<T, true, 4>(codes, x, f, tiles, device, stream) : launch<T, true, 8>(codes, x, f, tiles, device, stream));
+    return f.a.group == 32 ? launch<T, false, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
 }
 
 } /* namespace */
@@ -383,21 +490,21 @@ cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int devic
     many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0};
     const int pairs = sms / 2;
     /* Row tiles: as few as there have to be, or more where their tiles then take less time: rounds of all pairs times a tile's rows. */
-    int row_tiles = (a.rows + 255) / 256;
+    const int most = a.wide ? 64 : 256;
+    int row_tiles = (a.rows + most - 1) / most;
     long long least = -1;
-    for (int n = row_tiles; n <= row_tiles + 4; n++) {
+    for (int n = row_tiles, last = row_tiles + 4; n <= last; n++) {
         const int columns = ((a.rows + n - 1) / n + 15) & ~15, need = (a.rows + columns - 1) / columns;
         const long long rounds = ((long long)need * f.m_tiles + pairs - 1) / pairs, cost = rounds * (columns + 32);
         if (least < 0 || cost < least) { least = cost; row_tiles = need; f.columns = columns; }
     }
     const long long tiles = (long long)row_tiles * f.m_tiles;
     while (f.splits < kMostSplits && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
-    const int wide = a.wide ? 64 : 32;
-    f.steps = (512 - f.columns) / wide;
+    f.steps = a.wide ? 8 : (512 - f.columns) / 32;
     const int fit = kXBytes / ((f.columns * 64 + 1023) & ~1023);
     if (f.steps > fit) f.steps = fit;
     if (f.steps > kMostSteps) f.steps = kMostSteps;
-    f.a_column = 512 - f.steps * wide;
+    f.a_column = 512 - f.steps * 32;
     *what = NULL;
     CUtensorMap codes, x;
     const encode_tiled_fn enc = encoder();
