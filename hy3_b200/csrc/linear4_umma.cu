@@ -9,11 +9,11 @@
  *   warp 18   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step.
  *
  * Results of the rows' type: a weight, of up to 15 bits (fp16) or 11 (bf16), is rounded to that type once, which leaves an error like the result's own rounding.  Results that are not finite (of weights
- * rounded beyond the type's largest) are computed again from the definition, by the warp that finds them.
+ * rounded beyond the type's largest, of an infinite x that meets the rest) are computed again from the definition, by the warp that finds them.
  *
- * Results in fp32: A is code - 8, which is exact, and a group's sum by itself; the tensor cores begin anew with each group, in one of four sums of up to 64 rows.  Warps 0-7 (every second step
- * each four) make A, and warps 8-23 (every second group each eight) add scale * sum to results in registers, in fp32.  (Weights as two numbers, the rounded one and the rest, with one sum for all k's were twice the products, and
- * the tensor cores' sums, which are cut off and not rounded, left an error of 5.6e-6 of the result over 4096 k's; 64 rows on 10240 x 4096 23.1 us.)
+ * Results in fp32: a weight enters as two numbers, the rounded one and the rest, which is exact, so that there are 8 products a step; and the tensor cores begin a new sum every 512 k's, which warps of their own
+ * add to results in registers: the tensor cores' sums are cut off and not rounded (one sum over 4096 k's left an error of 5.6e-6 of the result).  A = code - 8, with a sum for each group and its scale
+ * at the end, is half as many products, but 64 rows on 10240 x 4096 took 26.8 us: the sums are read 8 times as often.
  *
  * Where tiles are few, the CTAs of a cluster share the k's of a tile; their sums meet in shared memory, and are added in the order of the k's.
  *
@@ -33,7 +33,7 @@ using namespace hy3a_ring;
 constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
 constexpr int kMostSplits = 4;
 constexpr int kMostSteps = 12 /* of x and A: as tensor memory has room for A beside the sums, and shared memory for x */, kXBytes = 8 * kStepBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
-enum { B_CODES = 0, B_CODES_FREE = kUnits, B_STEP = 2 * kUnits /* x and A of a step are there */, B_FREE = 2 * kUnits + kMostSteps, B_SUMS = 2 * kUnits + 2 * kMostSteps, B_GROUP, B_GROUP_FREE = B_GROUP + 4, B_COUNT = B_GROUP_FREE + 4 };
+enum { B_CODES = 0, B_CODES_FREE = kUnits, B_STEP = 2 * kUnits /* x and A of a step are there */, B_FREE = 2 * kUnits + kMostSteps, B_SUMS = 2 * kUnits + 2 * kMostSteps, B_RUN, B_RUN_FREE = B_RUN + 2, B_COUNT = B_RUN_FREE + 2 };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
 static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
 
@@ -41,7 +41,7 @@ __device__ unsigned g_err[2];         /* {code, where} of the first wait that ra
 
 struct many_args {
     linear4_args a;
-    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */;
+    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */, run_columns /* fp32 results: columns of each of two sums */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -101,19 +101,14 @@ __device__ __forceinline__ unsigned peek(unsigned bar, unsigned parity) {
 __device__ __forceinline__ bool all_wait(unsigned seen, unsigned bar, unsigned parity, volatile int *abort_flag, unsigned where) {
     return __all_sync(0xffffffffu, seen) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, g_err, where));
 }
-struct f2 { float x, y; };
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 r;
-    asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 c, a, b, c;\n mov.b64 {%0, %1}, c;\n}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
 template <class T> struct pair_of;
 template <> struct pair_of<__nv_bfloat16> {
     static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 template <> struct pair_of<__half> {
     static __device__ __forceinline__ unsigned mul(unsigned a, unsigned b) { unsigned r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 
 /* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is computed again, by the whole warp (rare: one piece of code, not unrolled) */
@@ -159,15 +154,15 @@ template <class T, bool WIDE, int N> __device__ __forceinline__ void store(const
 
 /* The warps of a CTA: teams of four that make A (a warp for each 32 outputs), those that add up groups, two producers, the issuer. */
 template <bool WIDE> struct warps_of {
-    static constexpr int kTeams = WIDE ? 2 : 4, kAdders = WIDE ? 16 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
+    static constexpr int kTeams = WIDE ? 3 : 4, kAdders = WIDE ? 8 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
 };
 
-/* WIDE: the result is fp32, PER: products (of 16 k's) of a group; else PER: scales of 64 k's (groups of 32: two) */
+/* WIDE: the result is fp32.  PER: scales of 64 k's (groups of 32: two) */
 template <class T, bool WIDE, int PER>
 __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
     extern __shared__ uint8_t s_raw[];
     using W = warps_of<WIDE>;
-    constexpr int kAWide = 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kBufs = 4, kGroupColumns = 64 /* WIDE: sums of a group */;
+    constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kRun = 8 /* WIDE: steps of a sum */;
     const int n_steps = f.steps;
     const unsigned x_bytes_up = (f.columns * 64 + 1023) & ~1023u;          /* (half the rows of 64 k's, from 1024 to 1024) */
     const linear4_args &a = f.a;
@@ -187,7 +182,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), 8 /* two teams */); }
         for (int i = 0; i < n_steps; i++) { mbar_init(BAR(B_STEP + i), 9 /* a team of each CTA, and the bytes of x */); mbar_init(BAR(B_FREE + i), 1); }
         mbar_init(BAR(B_SUMS), 1);
-        for (int i = 0; i < kBufs; i++) { mbar_init(BAR(B_GROUP + i), 1); mbar_init(BAR(B_GROUP_FREE + i), 16 /* eight warps of each CTA */); }
+        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_RUN + i), 1); mbar_init(BAR(B_RUN_FREE + i), 16 /* eight warps of each CTA */); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kCodes && lane < 2) {
@@ -206,6 +201,16 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
     pdl_release();
     pdl_wait();
 
+    /* a lane's sums of output o and the n rows from c0 on: stored, or left in shared memory where other CTAs have more of them */
+    const auto put = [&](float (&y)[16], int c0, int n, int r, int o) {
+        if (f.splits > 1) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) if (j < n) *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = y[j];
+        } else {
+            settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
+            store<T, WIDE>(a, y, n, row0 + c0, o, f.odd_out);
+        }
+    };
     if (warp == kCodes) {
         /* ===================== producer of codes ===================== */
         const unsigned lead = elect_one();
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             const unsigned idesc = (1u << 4) | kType | (((unsigned)N >> 3) << 17) | ((256u >> 4) << 24);
             const unsigned short both = (unsigned short)(3u << leader);
             int st = 0, buf = 0;
-            unsigned ph = 0, gph = 0, seen = 0, group_seen = WIDE ? peek(BAR(B_GROUP_FREE), 1u) : 0;
+            unsigned ph = 0, rph = 0, seen = 0;
             bool ok = true;
             for (int s = 0; s < steps; s++) {
                 if (!(ok = all_wait(seen, BAR(B_STEP + st), ph, s_abort, 53u))) break;
@@ -255,142 +260,121 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned long long db = make_desc(sbase + kOffX + st * x_bytes_up);
                 const unsigned da = tmem + f.a_column + st * kAWide;
-                if (!WIDE) {
+                const bool begins = WIDE ? s % kRun == 0 : s == 0;
+                if (WIDE && begins) {
+                    if (!(ok = all_wait(0, BAR(B_RUN_FREE + buf), rph ^ 1u, s_abort, 59u))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                const unsigned d = tmem + (WIDE ? buf * f.run_columns : 0);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) umma_lead(tmem, da + 8 * k, db + 2 * k, idesc, s + k > 0, lead);
-                } else {
-                    constexpr int kRuns = PER == 2 ? 2 : 1, kInRun = 4 / kRuns;        /* products of a step that go to one sum */
-                    const bool begins = PER < 8 || s % 2 == 0, ends = PER < 8 || s % 2 == 1;
+                for (int k = 0; k < 4; k++) umma_lead(d, da + 8 * k, db + 2 * k, idesc, !begins || k > 0, lead);
+                if (WIDE) {
 #pragma unroll
-                    for (int run = 0; run < kRuns; run++) {
-                        if (begins && !(ok = all_wait(group_seen, BAR(B_GROUP_FREE + buf), gph ^ 1u, s_abort, 59u))) break;
-                        const unsigned d = tmem + buf * kGroupColumns, group = BAR(B_GROUP + buf);
-                        if (ends) {
-                            if (++buf == kBufs) { buf = 0; gph ^= 1u; }
-                            group_seen = peek(BAR(B_GROUP_FREE + buf), gph ^ 1u);
-                        }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                        for (int k = run * kInRun; k < (run + 1) * kInRun; k++) umma_lead(d, da + 8 * k, db + 2 * k, idesc, !begins || k > run * kInRun, lead);
-                        if (ends) umma_commit_lead(group, both, lead);
+                    for (int k = 0; k < 4; k++) umma_lead(d, da + 32 + 8 * k, db + 2 * k, idesc, 1, lead);
+                    if (s % kRun == kRun - 1 || s == steps - 1) {
+                        umma_commit_lead(BAR(B_RUN + buf), both, lead);
+                        if (++buf == 2) { buf = 0; rph ^= 1u; }
                     }
-                    if (!ok) break;
                 }
                 umma_commit_lead(BAR(B_FREE + st), both, lead);
                 st = next;
                 ph = next_ph;
             }
-            if (ok) umma_commit_lead(BAR(B_SUMS), both, lead);
+            if (!WIDE && ok) umma_commit_lead(BAR(B_SUMS), both, lead);
         }
     } else if (WIDE && warp >= 4 * kTeams) {
-        /* ===================== groups: eight warps take every other one; a lane has an output, the warp every other 16 rows ===================== */
-        const int quarter = warp & 3, half = (warp >> 2) & 1, set = (warp >> 3) - 1, r = quarter * 32 + lane, o = m0 + r;
-        const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
-        const int g0 = u0 * (kUnit / a.group), groups = (u1 - u0) * (kUnit / a.group);
-        f2 acc[2][8];
+        /* ===================== sums of 512 k's: a lane has an output, the warp every other 16 rows ===================== */
+        const int quarter = warp & 3, half = (warp >> 2) & 1, r = quarter * 32 + lane, runs = (steps + kRun - 1) / kRun;
+        float acc[4][16];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) acc[i][k] = {0.f, 0.f};
-        /* (scales are asked for three of the warp's groups before) */
-        unsigned short sc[3];
-        const auto fetch = [&](int j, unsigned short &to) { to = 0; if (j < groups && g0 + j < a.groups) to = scales[g0 + j]; };
-#pragma unroll
-        for (int q = 0; q < 3; q++) fetch(set + 2 * q, sc[q]);
+            for (int k = 0; k < 16; k++) acc[i][k] = 0.f;
         bool ok = true;
-        int buf = set;
-        unsigned ph = 0;
 #pragma unroll 1
-        for (int j = set; j < groups && ok; j += 6) {
+        for (int run = 0; run < runs; run++) {
+            const int buf = run & 1;
+            if (!(ok = mbar_wait(BAR(B_RUN + buf), (run >> 1) & 1, s_abort, g_err, 60u))) break;
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-            for (int q = 0; q < 3; q++) {
-                if (!ok || j + 2 * q >= groups) break;
-                if (!(ok = mbar_wait(BAR(B_GROUP + buf), ph, s_abort, g_err, 60u))) break;
-                __syncwarp();
-                const unsigned group_free = cluster_addr(BAR(B_GROUP_FREE + buf), leader), from = tmem + ((unsigned)(quarter * 32) << 16) + buf * kGroupColumns;
-                buf ^= 2;
-                if (buf == set) ph ^= 1u;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const float s = type<T>::up(*reinterpret_cast<const T *>(&sc[q]));
-                fetch(j + 2 * q + 6, sc[q]);
+            for (int i = 0; i < 4; i++) {
+                const int c0 = (2 * i + half) * 16;
+                if (c0 >= N) break;
+                unsigned v[16];
+                tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * f.run_columns + c0, v);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int c0 = (2 * i + half) * 16;
-                    if (c0 >= N) break;
-                    unsigned v[16];
-                    tmem_ld16(from + c0, v);
+                for (int k = 0; k < 16; k++) acc[i][k] += __uint_as_float(v[k]);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE + buf), leader));
+        }
+        if (ok) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) acc[i][k] = fma2({__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])}, {s, s}, acc[i][k]);
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(group_free);
+            for (int i = 0; i < 4; i++) {
+                const int c0 = (2 * i + half) * 16, n = min(16, rows - c0);
+                if (n <= 0) break;
+#pragma unroll
+                for (int k = 0; k < 16; k++) if (k < n) *reinterpret_cast<float *>(sm + ((c0 + k) * 128 + r) * 4) = acc[i][k];
             }
         }
-        /* (codes and x lie where the sums go: until the last product is through) */
-        if (ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 61u)) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int k = 0; k < 16; k++)
-                    if ((2 * i + half) * 16 + k < rows) *reinterpret_cast<float *>(sm + ((set * kGroupColumns + (2 * i + half) * 16 + k) * 128 + r) * 4) = k & 1 ? acc[i][k / 2].y : acc[i][k / 2].x;
-        }
     } else {
-        /* ===================== weights: a thread has an output; each team takes every second or fourth step ===================== */
-        const int quarter = warp & 3, team = warp >> 2, half = team & 1 /* of a unit */, r = quarter * 32 + lane, o = m0 + r;
+        /* ===================== weights: a thread has an output; each team takes every third or fourth step ===================== */
+        const int quarter = warp & 3, team = warp >> 2, r = quarter * 32 + lane, o = m0 + r;
         const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
         const unsigned to_a = tmem + f.a_column + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
-        constexpr int kScales = WIDE ? 1 : PER;
-        unsigned short sc[3][kScales];
-        const auto fetch = [&](int s, unsigned short (&to)[kScales]) {
+        unsigned short sc[3][PER];
+        const auto fetch = [&](int s, unsigned short (&to)[PER]) {
 #pragma unroll
-            for (int i = 0; i < kScales; i++) {
+            for (int i = 0; i < PER; i++) {
                 const int j = (u0 * kUnit + s * 64 + 32 * i) >> shift;
                 to[i] = 0;
                 if (s < steps && j < a.groups) to[i] = scales[j];
             }
         };
-        int st = team, unit = team >> 1;
-        unsigned ph = 0, uph = 0;
-        const auto step = [&](int s, const unsigned short (&now)[kScales], unsigned short (&ahead)[kScales]) {
-            if (!WIDE) fetch(s + 2 * kTeams, ahead);
-            if (!mbar_wait(BAR(B_CODES + unit), uph, s_abort, g_err, 55u)) return false;
+        int st = team;
+        unsigned ph = 0;
+        const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
+            fetch(s + 2 * kTeams, ahead);
+            const int unit = (s >> 1) % kUnits;
+            if (!mbar_wait(BAR(B_CODES + unit), (s >> 1) / kUnits & 1, s_abort, g_err, 55u)) return false;
             uint4 c[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const unsigned at = from + unit * kUnitBytes + (((unsigned)(half * 2 + i) ^ turn) << 4);
+                const unsigned at = from + unit * kUnitBytes + (((unsigned)((s & 1) * 2 + i) ^ turn) << 4);
                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(c[i].x), "=r"(c[i].y), "=r"(c[i].z), "=r"(c[i].w) : "r"(at));
             }
             const unsigned w[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
-            unsigned weights[32];
+            unsigned weights[32], rest[WIDE ? 32 : 1];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 unsigned n[4];
                 hy3a_layer::steps<T>::in_order(w[i], n);
-                const unsigned s2 = __byte_perm(now[i * kScales / 8], 0, 0x1010);
+                const unsigned s2 = __byte_perm(now[i * PER / 8], 0, 0x1010);
 #pragma unroll
-                for (int j = 0; j < 4; j++) weights[4 * i + j] = WIDE ? n[j] : pair_of<T>::mul(n[j], s2);
+                for (int j = 0; j < 4; j++) {
+                    weights[4 * i + j] = pair_of<T>::mul(n[j], s2);
+                    if (WIDE) rest[WIDE ? 4 * i + j : 0] = pair_of<T>::rest(n[j], s2, weights[4 * i + j]);
+                }
             }
             if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
             __syncwarp();              /* (lanes may leave the wait one by one; what follows is the whole warp's) */
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             tmem_st32(to_a + st * kAWide, weights);
+            if constexpr (WIDE) tmem_st32(to_a + st * kAWide + 32, rest);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             /* (the codes are given back behind a store that needed them: an arrival does not wait for loads that are under way) */
             if (lane == 0) { mbar_arrive_cluster(cluster_addr(BAR(B_STEP + st), leader)); mbar_arrive(BAR(B_CODES_FREE + unit)); }
-            unit += kTeams / 2;
-            if (unit >= kUnits) { unit -= kUnits; uph ^= 1u; }
             st += kTeams;
             if (st >= n_steps) { st -= n_steps; ph ^= 1u; }
             return true;
         };
-        if (!WIDE) {
-            fetch(team, sc[0]);
-            fetch(team + kTeams, sc[1]);
-        }
+        fetch(team, sc[0]);
+        fetch(team + kTeams, sc[1]);
         bool ok = true;
         for (int s = team; s < steps && ok; s += 3 * kTeams) {
             ok = step(s, sc[0], sc[2]);
@@ -405,17 +389,10 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
                 unsigned v[16];
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
-                const int n = min(16, rows - c0);
-                if (f.splits > 1) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++) if (j < n) *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = __uint_as_float(v[j]);
-                    continue;
-                }
                 float y[16];
 #pragma unroll
                 for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
-                settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
-                store<T, false>(a, y, n, row0 + c0, o, f.odd_out);
+                put(y, c0, min(16, rows - c0), r, o);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
@@ -424,10 +401,10 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (*s_abort) for (int i = 0; i < 10000; i++) __nanosleep(1000);      /* copies of the step that was given up are still on their way */
-    /* Sums in shared memory: each CTA adds up the rows of its share, in the order of the k's (WIDE: even groups and odd ones by themselves).  part(i, h, j): of row c + j, split i, set h. */
-    constexpr int kSets = WIDE ? 2 : 1, kAtOnce = 4;
-    const auto add_up = [&](const auto &part) {
+    /* what lies in shared memory: each CTA adds up the rows of its share, in the order of the k's */
+    const auto add_up = [&](const auto &value) {
         if (warp >= 16 || *s_abort) return;
+        constexpr int kAtOnce = 4;
         const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
 #pragma unroll 1
         for (int c = first + kAtOnce * (tid >> 7); c < last; c += kAtOnce * 4) {
@@ -436,17 +413,13 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 #pragma unroll
             for (int i = 0; i < kMostSplits; i++) {
                 if (i == f.splits) break;
-                float v[kSets][kAtOnce];
+                float v[kAtOnce];
 #pragma unroll
-                for (int h = 0; h < kSets; h++)
+                for (int j = 0; j < kAtOnce; j++) v[j] = value(i, ((c + j) * 128 + r) * 4);        /* (rows past the last lie in shared memory as well) */
 #pragma unroll
-                    for (int j = 0; j < kAtOnce; j++) v[h][j] = part(i, ((h * kGroupColumns + c + j) * 128 + r) * 4);        /* (rows past the last lie in shared memory as well) */
-#pragma unroll
-                for (int h = 0; h < kSets; h++)
-#pragma unroll
-                    for (int j = 0; j < kAtOnce; j++) y[j] += v[h][j];
+                for (int j = 0; j < kAtOnce; j++) y[j] += v[j];
             }
-            if (!WIDE) settle<T>(a, y, n, row0 + c, o, o < a.out_width);
+            settle<T>(a, y, n, row0 + c, o, o < a.out_width);
             store<T, WIDE>(a, y, n, row0 + c, o, f.odd_out);
         }
         __syncwarp();
@@ -480,17 +453,17 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_ar
 }
 template <class T>
 cudaError_t launch_type(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
-    if (f.a.wide) return f.a.group == 32 ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : (f.a.group == 64 ? launch<T, true, 4>(codes, x, f, tiles, device, stream) : launch<T, true, 8>(codes, x, f, tiles, device, stream));
-    return f.a.group == 32 ? launch<T, false, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
+    if (f.a.group == 32) return f.a.wide ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 2>(codes, x, f, tiles, device, stream);
+    return f.a.wide ? launch<T, true, 1>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
 }
 
 } /* namespace */
 
 cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, int sms, void *stream, const char **what) {
-    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0};
+    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
     const int pairs = sms / 2;
     /* Row tiles: as few as there have to be, or more where their tiles then take less time: rounds of all pairs times a tile's rows. */
-    const int most = a.wide ? 64 : 256;
+    const int most = a.wide ? 128 : 256;
     int row_tiles = (a.rows + most - 1) / most;
     long long least = -1;
     for (int n = row_tiles, last = row_tiles + 4; n <= last; n++) {
@@ -500,11 +473,13 @@ cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int devic
     }
     const long long tiles = (long long)row_tiles * f.m_tiles;
     while (f.splits < kMostSplits && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
-    f.steps = a.wide ? 8 : (512 - f.columns) / 32;
+    const int stage = a.wide ? 64 : 32;
+    f.run_columns = (f.columns + 31) & ~31;
+    f.steps = (512 - (a.wide ? 2 * f.run_columns : f.columns)) / stage;
     const int fit = kXBytes / ((f.columns * 64 + 1023) & ~1023);
     if (f.steps > fit) f.steps = fit;
     if (f.steps > kMostSteps) f.steps = kMostSteps;
-    f.a_column = 512 - f.steps * 32;
+    f.a_column = 512 - f.steps * stage;
     *what = NULL;
     CUtensorMap codes, x;
     const encode_tiled_fn enc = encoder();

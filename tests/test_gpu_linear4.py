@@ -1,8 +1,10 @@
 """hy3_b200.linear4 against the definition in 64 bits, element by element.
 
 With A = sum of |weight| |x| over an element's products, and half a step of the result's type added (fp32 2^-24, bf16 2^-8, fp16 2^-11; fp16 2^-25 where subnormal), the bound is
-  up to 8 rows, and all results in fp32:
+  up to 8 rows:
     8 steps of a group's sum on the tensor cores, 2^-22 of it each: 2^-19 A; the groups' sums in fp32, one after the other and where warps or blocks meet: (groups + 20) 2^-24 A;
+  more rows, results in fp32 (weights as two numbers that are exact together):
+    64 steps of the sum over 512 k's, 2^-22 of it each: 2^-16 A; these sums in fp32: (width / 512 + 20) 2^-24 A;
   more rows, results of the rows' type:
     a rounding of the weights, 2^-8 A (bf16) or 2^-11 A (fp16); a step of the sum for 16 products, 2^-22 of it each: (width / 16 + 20) 2^-22 A.
 """
@@ -29,8 +31,10 @@ def make(rows, width, out, group=64, dtype="bfloat16", seed=0, device="cuda"):
 
 
 def bound(y, a, x, scales, result):
-    if x.shape[0] <= 8 or result == "float32":
+    if x.shape[0] <= 8:
         sums = 2.0 ** -19 + (scales.shape[1] + 20) * 2.0 ** -24
+    elif result == "float32":
+        sums = 2.0 ** -16 + (x.shape[1] / 512 + 20) * 2.0 ** -24
     else:
         sums = V[result] + (x.shape[1] / 16 + 20) * 2.0 ** -22
     return sums * a + V[result] * y.abs() + (2.0 ** -25 if result == "float16" else 0)
