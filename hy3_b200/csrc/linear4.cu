@@ -1,13 +1,14 @@
 /*
- * linear4.cu -- rows through a matrix of 4-bit codes with a scale for each group of neighbours in a row (hy3a_linear4), up to 8 rows:
+ * linear4.cu -- rows through a matrix of 4-bit codes with a scale for each group of neighbours in a row (hy3a_linear4), up to 16 rows:
  *
  *      y[t][o] = sum over groups j of scales[o][j] * sum over k of group j of (code[o][k] - 8) x[t][k]
  *
  * The inner sums are warp-level products of 16 outputs with 8 columns; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
- *   2 to 8 rows  the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products;
- *   one row      the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
- *                below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 11, and
- *                -8 sum d comes in as the sum's first value.  (120832 x 4096: 63 us with the row as a column.)
+ *   rows     the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products.  9 to 16 rows are two blocks' (16 rows on 10240 x 4096, fp32:
+ *            15.6 us, 24.1 in linear4_umma.cu);
+ *   digits   of one row, on large matrices, the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
+ *            below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 11, and
+ *            -8 sum d comes in as the sum's first value.
  *
  * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
  * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way.  (A bulk copy
@@ -29,7 +30,7 @@ using namespace hy3a_layer;
 using namespace hy3a_ring;
 
 constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2);
-constexpr int kTile = 16 /* outputs */, kRows = 8, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24;
+constexpr int kTile = 16 /* outputs */, kRows = 8 /* of a block */, kFewRows = 16, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24;
 constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
 constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
 constexpr int kRingBytes = 184 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
@@ -98,7 +99,7 @@ template <class T> __device__ __forceinline__ void mma_first(float (&d)[4], unsi
 }
 template <class T, int W> struct row_columns {
     unsigned x[4 * W];
-    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4], float &by) const {
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4]) const {
 #pragma unroll
         for (int w = 0; w < W; w++) {
             unsigned vl[4], vh[4];
@@ -108,17 +109,17 @@ template <class T, int W> struct row_columns {
             else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], x[4 * w], x[4 * w + 1]);
             type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], x[4 * w + 2], x[4 * w + 3]);
         }
-        by = 1.f;
     }
 };
 
 /* ---- digits as columns ---- */
+constexpr unsigned kMostExponent = 127 + 100;
 constexpr int kFirstSum = 0x4B400000;        /* 3 2^22 as a float: what is added to it as an integer, up to 2^22, is added to the float */
 template <int W> struct digit_columns {
     unsigned x[2 * W];                /* the column's digits of even and odd k's of each word */
     int first[2];                     /* kFirstSum - 8 sum of digits, of columns 2 t and 2 t + 1 */
     float unit;                       /* 2^(E - 7) */
-    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4], float &by) const {
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4]) const {
         int n[4] = {first[0], first[1], first[0], first[1]};
 #pragma unroll
         for (int w = 0; w < W; w++)
@@ -126,15 +127,15 @@ template <int W> struct digit_columns {
                 : "+r"(n[0]), "+r"(n[1]), "+r"(n[2]), "+r"(n[3])
                 : "r"(wl[w] & 0x0f0f0f0fu), "r"(wh[w] & 0x0f0f0f0fu), "r"((wl[w] >> 4) & 0x0f0f0f0fu), "r"((wh[w] >> 4) & 0x0f0f0f0fu), "r"(x[2 * w]), "r"(x[2 * w + 1]));
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = __int_as_float(n[i]) - __int_as_float(kFirstSum);
-        by = unit;
+        for (int i = 0; i < 4; i++) d[i] = fmaf(__int_as_float(n[i]), unit, -__int_as_float(kFirstSum) * unit);        /* exact, in the subnormal numbers too */
     }
 };
 __device__ __forceinline__ unsigned shift_left(unsigned v, int by) { unsigned r; asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }        /* (0 by 32 and more, and by less than 0) */
 __device__ __forceinline__ unsigned shift_right(unsigned v, int by) { unsigned r; asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }
 
 /* The digits of 8 k's from k on, a thread's share of a stage's: word `word` of the stage.  Row c = group * W + word of its lane holds the digits of four lanes, 8 bytes for
- * each column and lane, column j in place j ^ (c & 7): banks.  Sets bit 0 of *odd where x is NaN, bit 1 where it is infinite. */
+ * each column and lane, column j in place j ^ (c & 7): banks.  Sets bit 0 of *odd where x is NaN, bit 1 where it is infinite, or so large that
+ * its unit times 2^24 might be. */
 template <class T, int W> __device__ __forceinline__ void store_digits(const T *row, int k, int width, int word, uint8_t *digits, float *units, int *odd) {
     uint4 raw = zero16();
     if (k < width) raw = load_row(row + k);
@@ -148,15 +149,21 @@ template <class T, int W> __device__ __forceinline__ void store_digits(const T *
         ex[i] = max((int)e, 1);
         most = max(most, ex[i]);
         sign |= (u >> 31) << i;
-        if (e == 255u) atomicOr(odd, u & 0x7fffffu ? 1 : 2);
+        if (e >= kMostExponent) atomicOr(odd, e == 255u && (u & 0x7fffffu) ? 1 : 2);
     }
 #pragma unroll
     for (int o = 1; o < 4 * W; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    /* (digits past the last bit of the warp's smallest x are 0) */
+    int low = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) if (m[i]) low = max(low, most - ex[i]);
+    const int digits_used = min(8, (__reduce_max_sync(0xffffffffu, low) + 11 + 6) / 7);
     const int c = word / (4 * W) * W + word % W, t = word / W & 3;
     if (word % (4 * W) == 0) units[word / (4 * W)] = most > 6 ? __int_as_float((most - 6) << 23) : __int_as_float(1 << (16 + most));
 #pragma unroll 1
     for (int j = 0; j < 8; j++) {
         unsigned b[2] = {0, 0};
+        if (j < digits_used)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int by = 7 * j - 4 + ex[i] - most;
@@ -181,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
     const unsigned ring = smem_u32(sm), bar0 = ring + kOffBar;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int boxes = (a.out_width + kBox - 1) / kBox, first = kBox * (int)((long long)boxes * blockIdx.x / gridDim.x), last = min(a.out_width, kBox * (int)((long long)boxes * (blockIdx.x + 1) / gridDim.x));
-    const int rows = ONE ? 1 : a.rows;
+    const int t0 = ONE ? 0 : blockIdx.y * kRows, rows = ONE ? 1 : min(kRows, a.rows - t0);
     /* outputs g and g + 8 of the products are outputs mine and mine + 8 of the tile: such that lanes that read together find their words in different banks */
     const int mine_of = W == 4 ? (g & 1) * 4 + (g >> 1) : ((g >> 1) & 1) * 4 + (g & 1) * 2 + (g >> 2);
 #define BAR(i) (bar0 + 8u * (unsigned)(i))
@@ -243,12 +250,12 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
             if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf) + (__float_as_uint(sum.x) & f.zero));
             float v[4] = {sum.x, sum.y, sum.z, sum.w};
             const auto put = [&](int r, float y) {
-                const size_t to = (size_t)r * a.out_stride + o0 + o;
+                const size_t to = (size_t)(t0 + r) * a.out_stride + o0 + o;
                 if (a.wide) reinterpret_cast<float *>(a.out)[to] = y;
                 else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
             };
             if (ONE) {
-                /* digits: column c counts 2^-7c; an x that is not finite has none */
+                /* digits: column c counts 2^-7c; an x that is not finite, or over 2^100, has none */
                 float y = (v[0] + v[1] * 0x1p-7f + (v[2] * 0x1p-14f + v[3] * 0x1p-21f)) * (r0 ? 0x1p-28f : 1.f);
                 y += __shfl_xor_sync(0xffffffffu, y, 1);
                 const int odd = *reinterpret_cast<volatile int *>(s_odd);
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
     } else {
         /* ===================== products: a warp has `per` groups of a stage, one behind the other ===================== */
         columns x[kSets][kMine];
-        const T *row = reinterpret_cast<const T *>(a.x) + (ONE ? 0 : (size_t)min(g, rows - 1) * a.x_stride);
+        const T *row = reinterpret_cast<const T *>(a.x) + (ONE ? 0 : (size_t)(t0 + min(g, rows - 1)) * a.x_stride);
         const int g0 = warp * f.per;
         const auto load_columns = [&](columns (&to)[kMine], int p) {
             if constexpr (ONE) {
@@ -343,11 +350,10 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                         unsigned wl[W], wh[W];
                         load_words<W>(at[i] + by, wl);
                         load_words<W>(at[i] + by + eight, wh);
-                        float d[4], unit;
-                        xs[i].sums(wl, wh, d, unit);
+                        float d[4];
+                        xs[i].sums(wl, wh, d);
                         const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
-                        float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
-                        if (ONE) { s0 *= unit; s1 *= unit; }
+                        const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
                         acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
                         acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
                     }
@@ -392,14 +398,16 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &scales, const fe
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
     const int boxes = (f.a.out_width + kBox - 1) / kBox;
-    hy3a_launch l(dim3(boxes < sms ? boxes : sms), dim3(kThreads), kSmem, stream);
+    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(kThreads), kSmem, stream);
     return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE>, codes, scales, f);
 }
 template <class T, int W>
 cudaError_t launch_group(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
     constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers for two stages' x) */
-    if (f.passes == 1) return f.a.rows == 1 ? launch<T, W, 1, true>(codes, scales, f, device, sms, stream) : launch<T, W, 1, false>(codes, scales, f, device, sms, stream);
-    if (f.passes == 2 && kTwo) return f.a.rows == 1 ? launch<T, W, kTwo, kTwo != 0>(codes, scales, f, device, sms, stream) : launch<T, W, kTwo, false>(codes, scales, f, device, sms, stream);
+    /* Digits save a third of a microsecond a tile and take two to make: for 6 tiles a block and more (one row on 4096 x 4096: 6.9 us with them, 5.0 without; on 120832 x 4096 50 and 63). */
+    const bool digits = f.a.rows == 1 && f.a.out_width >= 6 * kTile * sms;
+    if (f.passes == 1) return digits ? launch<T, W, 1, true>(codes, scales, f, device, sms, stream) : launch<T, W, 1, false>(codes, scales, f, device, sms, stream);
+    if (f.passes == 2 && kTwo) return digits ? launch<T, W, kTwo, kTwo != 0>(codes, scales, f, device, sms, stream) : launch<T, W, kTwo, false>(codes, scales, f, device, sms, stream);
     return launch<T, W, 0, false>(codes, scales, f, device, sms, stream);
 }
 template <class T>
@@ -462,7 +470,7 @@ extern "C" int hy3a_linear4(void *stream, int dtype, int rows, int width, int ou
     if ((rc = hy3a_layer_device("linear4", &dev, &sms))) return rc;
     const linear4_args a = {x, x_stride, (const uint8_t *)codes, scales, out, out_stride, rows, width, out_width, group, (width + group - 1) / group, out_dtype == HY3A_F32};
     const char *what = NULL;
-    const cudaError_t e = rows > kRows ? hy3a_linear4_launch_many(a, dtype, dev, sms, stream, &what)
+    const cudaError_t e = rows > kFewRows ? hy3a_linear4_launch_many(a, dtype, dev, stream, &what)
                         : (dtype == HY3A_BF16 ? launch_few<__nv_bfloat16>(a, dev, sms, stream, &what) : launch_few<__half>(a, dev, sms, stream, &what));
     if (e != cudaSuccess) return hy3a_fail(NULL, HY3A_ECUDA, "linear4: %s", what ? what : cudaGetErrorString(e));
     return HY3A_OK;

@@ -440,47 +440,55 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 }
 
 template <class T, bool WIDE, int PER>
-cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
-    static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
-    cudaError_t e;
-    if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
-        if ((e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
-        if (device < 64) ready[device].store(true, std::memory_order_release);
-    }
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, void *stream) {
     hy3a_launch l(dim3((unsigned)tiles * 2 * f.splits), dim3(warps_of<WIDE>::kThreads), kSmem, stream);
     l.cluster(2 * f.splits);
     return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_umma_kernel<T, WIDE, PER>, codes, x, f);
 }
-template <class T>
-cudaError_t launch_type(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, int device, void *stream) {
-    if (f.a.group == 32) return f.a.wide ? launch<T, true, 2>(codes, x, f, tiles, device, stream) : launch<T, false, 2>(codes, x, f, tiles, device, stream);
-    return f.a.wide ? launch<T, true, 1>(codes, x, f, tiles, device, stream) : launch<T, false, 1>(codes, x, f, tiles, device, stream);
+/* Allows the shared memory, once per device, and tells how many clusters of 2 n CTAs fit on it at once, n = 1 .. kMostSplits (74, 33, 22 or so and 15: clusters stay within a part of the GPU). */
+template <class T, bool WIDE, int PER>
+cudaError_t ready(int device, int (&fit)[kMostSplits]) {
+    static std::atomic<int> known[64][kMostSplits];
+    for (int n = 0; n < kMostSplits; n++) {
+        fit[n] = device < 64 ? known[device][n].load(std::memory_order_acquire) : 0;
+        if (fit[n]) continue;
+        cudaError_t e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return e;
+        hy3a_launch l(dim3(2 * (n + 1)), dim3(warps_of<WIDE>::kThreads), kSmem, nullptr);
+        l.cluster(2 * (n + 1));
+        if ((e = cudaOccupancyMaxActiveClusters(&fit[n], hy3a_linear4_umma_kernel<T, WIDE, PER>, &l.cfg)) != cudaSuccess) return e;
+        if (fit[n] < 1) fit[n] = 1;
+        if (device < 64) known[device][n].store(fit[n], std::memory_order_release);
+    }
+    return cudaSuccess;
 }
 
-} /* namespace */
-
-cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, int sms, void *stream, const char **what) {
-    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
-    const int pairs = sms / 2;
-    /* Row tiles: as few as there have to be, or more where their tiles then take less time: rounds of all pairs times a tile's rows. */
-    const int most = a.wide ? 128 : 256;
-    int row_tiles = (a.rows + most - 1) / most;
-    long long least = -1;
-    for (int n = row_tiles, last = row_tiles + 4; n <= last; n++) {
-        const int columns = ((a.rows + n - 1) / n + 15) & ~15, need = (a.rows + columns - 1) / columns;
-        const long long rounds = ((long long)need * f.m_tiles + pairs - 1) / pairs, cost = rounds * (columns + 32);
-        if (least < 0 || cost < least) { least = cost; row_tiles = need; f.columns = columns; }
+/* Rows of a tile and CTAs that share a tile's k's: what takes the least by rounds * (steps of a CTA * a step + what a tile costs besides), in 10 ns, measured over 9 to 2048 rows: a step takes 160 + 0.6 N ns with N
+ * rows (fp32 results 220 + 0.9 N), a tile 6.5 us besides (8.5; 1.5 more where CTAs share). */
+template <class T, bool WIDE, int PER>
+cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
+    int fit[kMostSplits];
+    cudaError_t e = ready<T, WIDE, PER>(device, fit);
+    if (e != cudaSuccess) return e;
+    const int most = WIDE ? 128 : 256, least_tiles = (a.rows + most - 1) / most;
+    double least = -1.;
+    long long tiles = 0;
+    for (int n = least_tiles; n <= least_tiles + 4; n++) {
+        const int columns = ((a.rows + n - 1) / n + 15) & ~15;
+        const long long all = (long long)((a.rows + columns - 1) / columns) * f.m_tiles;
+        for (int splits = 1; splits <= kMostSplits && splits <= f.units; splits++) {
+            const int steps = 2 * ((f.units + splits - 1) / splits);
+            const double cost = (double)((all + fit[splits - 1] - 1) / fit[splits - 1]) * (steps * (WIDE ? 22. + 0.09 * columns : 16. + 0.06 * columns) + (WIDE ? 850. : 650.) + (splits > 1 ? 150. : 0.));
+            if (least < 0. || cost < least) { least = cost; tiles = all; f.columns = columns; f.splits = splits; }
+        }
     }
-    const long long tiles = (long long)row_tiles * f.m_tiles;
-    while (f.splits < kMostSplits && tiles * f.splits * 2 <= pairs && f.units >= 4 * f.splits) f.splits *= 2;
-    const int stage = a.wide ? 64 : 32;
+    const int stage = WIDE ? 64 : 32;
     f.run_columns = (f.columns + 31) & ~31;
-    f.steps = (512 - (a.wide ? 2 * f.run_columns : f.columns)) / stage;
-    const int fit = kXBytes / ((f.columns * 64 + 1023) & ~1023);
-    if (f.steps > fit) f.steps = fit;
+    f.steps = (512 - (WIDE ? 2 * f.run_columns : f.columns)) / stage;
+    const int room = kXBytes / ((f.columns * 64 + 1023) & ~1023);
+    if (f.steps > room) f.steps = room;
     if (f.steps > kMostSteps) f.steps = kMostSteps;
     f.a_column = 512 - f.steps * stage;
-    *what = NULL;
     CUtensorMap codes, x;
     const encode_tiled_fn enc = encoder();
     const cuuint64_t dims[2] = {(cuuint64_t)(a.width / 2), (cuuint64_t)a.out_width}, strides[1] = {(cuuint64_t)(a.width / 2)};
@@ -490,7 +498,20 @@ cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int devic
                     encode(&x, 2, a.x, a.width, a.rows, 1, a.x_stride, 64, f.columns / 2);
     if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
     if (tiles * 2 * f.splits > 0x7fffffffll) { *what = "too many tiles"; return cudaErrorInvalidValue; }
-    return dtype == HY3A_BF16 ? launch_type<__nv_bfloat16>(codes, x, f, (int)tiles, device, stream) : launch_type<__half>(codes, x, f, (int)tiles, device, stream);
+    return launch<T, WIDE, PER>(codes, x, f, (int)tiles, stream);
+}
+template <class T>
+cudaError_t run_type(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
+    if (a.group == 32) return a.wide ? run<T, true, 2>(a, f, device, stream, what) : run<T, false, 2>(a, f, device, stream, what);
+    return a.wide ? run<T, true, 1>(a, f, device, stream, what) : run<T, false, 1>(a, f, device, stream, what);
+}
+
+} /* namespace */
+
+cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, void *stream, const char **what) {
+    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
+    *what = NULL;
+    return dtype == HY3A_BF16 ? run_type<__nv_bfloat16>(a, f, device, stream, what) : run_type<__half>(a, f, device, stream, what);
 }
 
 cudaError_t hy3a_linear4_many_error(unsigned *err) {

@@ -1,7 +1,7 @@
 """hy3_b200.linear4 against the definition in 64 bits, element by element.
 
 With A = sum of |weight| |x| over an element's products, and half a step of the result's type added (fp32 2^-24, bf16 2^-8, fp16 2^-11; fp16 2^-25 where subnormal), the bound is
-  up to 8 rows:
+  up to 16 rows:
     8 steps of a group's sum on the tensor cores, 2^-22 of it each: 2^-19 A; the groups' sums in fp32, one after the other and where warps or blocks meet: (groups + 20) 2^-24 A;
   more rows, results in fp32 (weights as two numbers that are exact together):
     64 steps of the sum over 512 k's, 2^-22 of it each: 2^-16 A; these sums in fp32: (width / 512 + 20) 2^-24 A;
@@ -31,13 +31,14 @@ def make(rows, width, out, group=64, dtype="bfloat16", seed=0, device="cuda"):
 
 
 def bound(y, a, x, scales, result):
-    if x.shape[0] <= 8:
+    if x.shape[0] <= 16:
         sums = 2.0 ** -19 + (scales.shape[1] + 20) * 2.0 ** -24
     elif result == "float32":
         sums = 2.0 ** -16 + (x.shape[1] / 512 + 20) * 2.0 ** -24
     else:
         sums = V[result] + (x.shape[1] / 16 + 20) * 2.0 ** -22
-    return sums * a + V[result] * y.abs() + (2.0 ** -25 if result == "float16" else 0)
+    # (fp32 sums among the subnormal numbers round to multiples of 2^-149, each of them)
+    return sums * a + V[result] * y.abs() + (2.0 ** -25 if result == "float16" else 0) + (scales.shape[1] + 40) * 2.0 ** -150
 
 
 def check(got, x, codes, scales, group):
@@ -52,7 +53,8 @@ def check(got, x, codes, scales, group):
 
 SIZES = [(1, 32, 1, 32), (1, 32, 16, 64), (1, 4096, 1024, 64), (2, 96, 17, 32), (3, 160, 300, 128), (5, 1056, 1001, 32), (7, 8192, 296, 128), (8, 4128, 333, 64), (8, 12288, 100, 32), (4, 8224, 2500, 128),
          (9, 512, 264, 64), (16, 2048, 520, 128), (17, 96, 31, 32), (33, 1056, 1001, 128), (64, 4096, 640, 64), (100, 8192, 129, 32), (128, 256, 128, 64), (257, 1056, 515, 64),
-         (300, 4096, 256, 128), (1000, 160, 24, 32), (2049, 544, 300, 64), (1, 65536, 150, 128), (130, 16384, 72, 32)]
+         (300, 4096, 256, 128), (1000, 160, 24, 32), (2049, 544, 300, 64), (1, 65536, 150, 128), (130, 16384, 72, 32),
+         (1, 256, 15000, 32), (1, 1056, 14400, 64), (1, 4096, 16001, 128), (1, 8192, 15001, 64), (1, 8192, 15000, 32), (1, 12288, 15000, 64), (64, 4096, 5000, 64), (16, 4096, 20000, 128), (15, 8192, 50, 64)]
 
 
 @pytest.mark.parametrize("dtype,result", [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16"), ("float16", "float32")])
@@ -66,7 +68,7 @@ def test_sizes(cuda, rows, width, out, group, dtype, result):
     check(got, *args)
 
 
-@pytest.mark.parametrize("rows", [1, 8, 40, 300])
+@pytest.mark.parametrize("rows", [1, 8, 13, 40, 300])
 def test_strides_and_out(cuda, rows):
     """Rows of a wider matrix, a result in a part of another, one row for all; what lies beside the result stays."""
     import torch
@@ -90,7 +92,7 @@ def test_strides_and_out(cuda, rows):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
-@pytest.mark.parametrize("rows", [1, 8, 40, 300])
+@pytest.mark.parametrize("rows", [1, 8, 13, 40, 300])
 def test_rows_and_outputs_do_not_touch_each_other(cuda, rows, dtype):
     """A NaN or an infinity in a row, or in an output's scales, stays there; an infinite x gives the infinity or NaN that the definition gives."""
     import torch
@@ -109,6 +111,32 @@ def test_rows_and_outputs_do_not_touch_each_other(cuda, rows, dtype):
     got = hy3_b200.linear4(x, codes, scales, out_dtype=torch.float32)
     want = x[:1].double() @ weights(codes, scales, group).T
     assert torch.equal(torch.isnan(got[:1]), torch.isnan(want)) and torch.equal(torch.isinf(got[:1]), torch.isinf(want)) and torch.equal(torch.sign(got[0]).nan_to_num(), torch.sign(want[0]).float().nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_one_row_on_a_large_matrix(cuda, dtype):
+    """Its digits: magnitudes far apart in a group, subnormal and largest numbers, zeros; what is not finite."""
+    import torch
+    import hy3_b200
+    x, codes, scales, group = make(1, 1024, 15000, 64, dtype)
+    top = torch.finfo(x.dtype).max / 2 if dtype == "float16" else 2.0 ** 110
+    small = torch.finfo(x.dtype).smallest_normal
+    scales.clamp_(-0.5, 0.5)
+    k = torch.arange(1024, device=cuda)
+    wide = 2.0 ** -(k % 24).double()
+    cases = [x.double() * wide, x.double() * small, torch.where(k % 64 == 5, top, x.double()), torch.where(k % 64 == 5, x.double(), 0.0), x.double() * 0, torch.where(k < 512, x.double(), small / 4)]
+    for row in cases:
+        row = row.to(x.dtype).view(1, -1)
+        check(hy3_b200.linear4(row, codes, scales, out_dtype=torch.float32), row, codes, scales, group)
+    # a large number whose code is 8: what is left is as exact as it would be without
+    codes[:, 2] = codes[:, 2] & 0xf0 | 8
+    row = torch.where(k == 4, 1000.0, x.double() * 2.0 ** -12).to(x.dtype)
+    check(hy3_b200.linear4(row, codes, scales, out_dtype=torch.float32), row, codes, scales, group)
+    for odd in (float("nan"), float("inf"), -float("inf")):
+        row = x.clone()
+        row[0, 77] = odd
+        got, want = hy3_b200.linear4(row, codes, scales, out_dtype=torch.float32), row.double() @ weights(codes, scales, group).T
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(0, 1, -1).sign()[~torch.isfinite(want)], want.nan_to_num(0, 1, -1).sign().float()[~torch.isfinite(want)])
 
 
 @pytest.mark.parametrize("rows", [2, 40])
