@@ -30,7 +30,7 @@ using namespace hy3a_layer;
 using namespace hy3a_ring;
 
 constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2);
-constexpr int kTile = 16 /* outputs */, kRows = 8 /* of a block */, kFewRows = 16, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24;
+constexpr int kTile = 16 /* outputs */, kRows = 8 /* of a block */, kFewRows = 16, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24, kMaxOut = 1 << 30 /* (numbers of outputs stay ints a tile past the last) */;
 constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
 constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
 constexpr int kRingBytes = 184 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
@@ -447,7 +447,7 @@ cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream,
 } /* namespace */
 
 int hy3a_quant4_sizes(const char *who, int out_width, int width, int group) {
-    if (out_width < 0) return hy3a_fail(NULL, HY3A_EINVAL, "%s: out_width %d < 0", who, out_width);
+    if (out_width < 0 || out_width > kMaxOut) return hy3a_fail(NULL, HY3A_EINVAL, "%s: out_width %d not in [0,%d]", who, out_width, kMaxOut);
     if (width < 32 || width > kMaxWidth || width % 32) return hy3a_fail(NULL, HY3A_EINVAL, "%s: width %d: a multiple of 32 in [32,%d]", who, width, kMaxWidth);
     if (group != 32 && group != 64 && group != 128) return hy3a_fail(NULL, HY3A_EINVAL, "%s: group %d not in {32,64,128}", who, group);
     return HY3A_OK;

@@ -4,9 +4,10 @@
  * The weights are the M side of the product and the rows its N side (up to 256).  A pair of CTAs (cta_group::2) works on 256 outputs: each has 128 of them, and half of the
  * rows of x in shared memory.  Codes become weights on their way: a thread has an output, reads its codes of 64 k's from shared memory, and stores (code - 8) * scale
  * as the A operand into tensor memory, from where the product takes it; shared memory sees 4 bits a weight, and the tensor cores read only x from there.  Per CTA:
- *   warps 0-15 weights: each four of them (a lane quarter each) every fourth step of 64 k's; afterwards the results;
- *   warps 16, 17 TMA producers: codes, 128 k's at a time, and x, 64 k's at a time;
- *   warp 18   MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step.
+ *   16 warps   weights: each four of them (a lane quarter each) every fourth step of 64 k's; afterwards the results.  fp32 results: 12, every third step, and
+ *              8 that add up sums;
+ *   2          TMA producers: codes, 128 k's at a time, and x, 64 k's at a time;
+ *   1          MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, fp32 results 8.
  *
  * Results of the rows' type: a weight, of up to 15 bits (fp16) or 11 (bf16), is rounded to that type once, which leaves an error like the result's own rounding.  Results that are not finite (of weights
  * rounded beyond the type's largest, of an infinite x that meets the rest) are computed again from the definition, by the warp that finds them.
@@ -111,25 +112,44 @@ template <> struct pair_of<__half> {
     static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 
-/* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is computed again, by the whole warp (rare: one piece of code, not unrolled) */
+template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, int t) {
+    const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride);
+    constexpr unsigned kInf = type<T>::code == HY3A_BF16 ? 0x7f80u : 0x7c00u;
+    bool is = false;
+    for (int i = threadIdx.x & 31; i < a.width / 8; i += 32) {
+        const uint4 v = x[i];
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) is |= (w[j] & 0x7fffu) > kInf || (w[j] >> 16 & 0x7fffu) > kInf;
+    }
+    return __any_sync(0xffffffffu, is);
+}
+/* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is NaN if x has one in its row (padding that nobody wrote may be such rows), and else computed again, by the whole
+ * warp (rare: one piece of code, not unrolled) */
 template <class T, int N> __device__ __forceinline__ void settle(const linear4_args &a, float (&y)[N], int n, int t, int o, bool mine) {
     bool odd = false;
 #pragma unroll
     for (int j = 0; j < N; j++) odd |= j < n && !(fabsf(y[j]) < INFINITY);
-    unsigned todo = __ballot_sync(0xffffffffu, odd && mine);
+    if (!__any_sync(0xffffffffu, odd && mine)) return;
 #pragma unroll 1
-    for (; todo; todo &= todo - 1) {
-        const int l = __ffs(todo) - 1, its = __shfl_sync(0xffffffffu, o, l);
-#pragma unroll 1
-        for (int j = 0; j < n; j++) {
-            float was = y[0];
+    for (int j = 0; j < n; j++) {
+        float now = y[0];
 #pragma unroll
-            for (int k = 1; k < N; k++) if (j == k) was = y[k];
-            if (fabsf(__shfl_sync(0xffffffffu, was, l)) < INFINITY) continue;
-            const float again = plain<T>(a, t + j, its);
-#pragma unroll
-            for (int k = 0; k < N; k++) if (j == k && (int)(threadIdx.x & 31) == l) y[k] = again;
+        for (int k = 1; k < N; k++) if (j == k) now = y[k];
+        unsigned todo = __ballot_sync(0xffffffffu, mine && !(fabsf(now) < INFINITY));
+        if (!todo) continue;
+        if (has_nan<T>(a, t + j)) {
+            if (!(fabsf(now) < INFINITY)) now = NAN;
+            todo = 0u;
         }
+#pragma unroll 1
+        for (; todo; todo &= todo - 1) {
+            const int l = __ffs(todo) - 1;
+            const float again = plain<T>(a, t + j, __shfl_sync(0xffffffffu, o, l));
+            if ((int)(threadIdx.x & 31) == l) now = again;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) if (j == k) y[k] = now;
     }
 }
 /* A lane's results of its output, row after row.  16-bit ones: neighbouring lanes exchange, so that one stores the even rows' two outputs and one the odd rows'. */

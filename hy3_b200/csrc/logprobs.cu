@@ -26,7 +26,7 @@ using namespace hy3a_layer;
  * are fewer still: 131072 fp32 logits are one round of loads for 8 of them. */
 constexpr int kAlone = 256, kShared = 512, kMaxCluster = 8;
 constexpr int kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
-constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct logprobs_args {
     const void *logits;
@@ -134,8 +134,8 @@ template <class T> __device__ __forceinline__ float largest(const uint4 &r, T t)
 
 /* order of floats as unsigned numbers, NaN below all but what is closed (0) */
 __device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned u = __float_as_uint(isnan(v) ? kLowest : v + 0.f);       /* (-0 is 0) */
-    return v == -INFINITY ? 0u : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+    const unsigned u = __float_as_uint(v + 0.f);       /* (-0 is 0) */
+    return v == -INFINITY ? 0u : isnan(v) ? 1u /* a NaN seen from value_of too */ : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ unsigned long long key_of(float v, int i) { return (unsigned long long)ordered(v) << 32 | (0xffffffffu - (unsigned)i); }
 __device__ __forceinline__ float value_of(unsigned long long key) { const unsigned u = (unsigned)(key >> 32); return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }

@@ -244,7 +244,8 @@ int hy3a_fill_random(hy3a_ctx *ctx, int layer, int seq, int t0, int n, uint64_t 
 
 /* ---- operators beside the attention -------------------------------------------------------
  * What else a layer does with rows that are chosen one by one: the experts that a row is routed to, and the low-rank adapter
- * of its request; shared projections and the output head on weights in 4 bits, and what is asked of the logits.  (The reference routes and multiplies on the CPU or with a warp per weight row, hy3.c:1266-1303, hy3_gpu.cu:75-130; it
+ * of its request; shared projections and the output head on weights in 4 bits, and what is asked of the logits.  (The reference
+ * routes and multiplies on the CPU or with a warp per weight row, hy3.c:1266-1303, hy3_gpu.cu:75-130; it
  * has no adapters.)  They need no context: the stream (a cudaStream_t) and the workspace are arguments, work is enqueued on the
  * current device, which has to be the stream's, nothing is allocated, copied to the host or kept between calls, and all of
  * them can be captured in a graph.  Messages: hy3a_last_error(NULL) of the calling thread.  A workspace may be used again by the
@@ -292,13 +293,13 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
  * apart) share a scale s of type `dtype` (HY3A_F16 or HY3A_BF16), and a weight is (q - 8) * s with 0 <= q < 16:
  *   e = the group's largest value if that is larger than minus its smallest, else its smallest;  s = -e / 8, rounded to nearest;
  *   q = min(max(rint(w / s), -8), 7) + 8, w / s in fp32; 8 where s is 0 or not finite (a NaN or an infinity in the group, or |e| too large for the type).
- * codes [out_width][width / 2] bytes, the even element in the low half; scales [out_width][ceil(width / group)], both dense.  width: a multiple of 32 up to
+ * codes [out_width][width / 2] bytes, the even element in the low half; scales [out_width][ceil(width / group)], both dense.  out_width: up to 2^30; width: a multiple of 32 up to
  * 65536; the last group may be short.  w and codes are 16-byte aligned, rows of w start on 16-byte boundaries.
  * (The reference's 4-bit weights have scales in two levels and minima, hy3_gpu.cu:75-130; it quantises none.)                 */
 int hy3a_quantize4(void *stream, int w_dtype, int out_width, int width, int group, const void *w, size_t w_stride, int dtype, void *codes, void *scales);
 
 /* Rows times a matrix in 4 bits, in hy3a_quantize4's format: out[t][o] = sum over k of (q[o][k] - 8) * s[o][k / group] * x[t][k].  x [rows][width] and
- * the scales are of dtype HY3A_F16 or HY3A_BF16, out [rows][out_width] of out_dtype: that, or HY3A_F32.  Sums are fp32.  x and codes are 16-byte aligned, and rows of x start on
+ * the scales are of dtype HY3A_F16 or HY3A_BF16, out [rows][out_width] of out_dtype: that, or HY3A_F32.  Sums are fp32; rows: at most 2^24.  x and codes are 16-byte aligned, and rows of x start on
  * 16-byte boundaries; scales and out are aligned to their types.  out must not overlap x.                                     */
 int hy3a_linear4(void *stream, int dtype, int rows, int width, int out_width, int group, const void *x, size_t x_stride, const void *codes, const void *scales,
                  int out_dtype, void *out, size_t out_stride);

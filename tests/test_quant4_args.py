@@ -17,7 +17,7 @@ def refused(lib, rc, text):
 
 
 SIZES = (({"out_width": -1}, "out_width"), ({"width": 0}, "width"), ({"width": 48}, "width"), ({"width": 65568, "stride": 65568}, "width"), ({"width": -32}, "width"),
-         ({"group": 0}, "group"), ({"group": 16}, "group"), ({"group": 256}, "group"), ({"group": -64}, "group"))
+         ({"group": 0}, "group"), ({"group": 16}, "group"), ({"group": 256}, "group"), ({"group": -64}, "group"), ({"out_width": (1 << 30) + 1}, "out_width"))
 
 
 def test_quantize4(lib):
@@ -33,7 +33,7 @@ def test_quantize4(lib):
 def test_linear4(lib):
     def call(dtype=2, rows=5, width=64, out_width=8, group=64, x=P, stride=64, codes=P, scales=P, out_dtype=2, out=P, os_=8):
         return lib.hy3a_linear4(None, dtype, rows, width, out_width, group, x, stride, codes, scales, out_dtype, out, os_)
-    for kw, text in SIZES + (({"dtype": 0}, "dtype"), ({"out_dtype": 1}, "out_dtype"), ({"dtype": 1}, "out_dtype"), ({"rows": -1}, "rows"), ({"x": None}, "NULL"), ({"codes": None}, "NULL"),
+    for kw, text in SIZES + (({"dtype": 0}, "dtype"), ({"out_dtype": 1}, "out_dtype"), ({"dtype": 1}, "out_dtype"), ({"rows": -1}, "rows"), ({"rows": (1 << 24) + 1}, "rows"), ({"x": None}, "NULL"), ({"codes": None}, "NULL"),
                              ({"scales": None}, "NULL"), ({"out": None}, "NULL"), ({"x": P + 8}, "16-byte"), ({"codes": P + 8}, "16-byte"), ({"scales": P + 1}, "aligned"),
                              ({"out": P + 1}, "aligned"), ({"out_dtype": 0, "out": P + 2}, "aligned"), ({"stride": 68}, "boundaries"), ({"os_": 7}, "overlap")):
         refused(lib, call(**kw), text)
