@@ -4,8 +4,9 @@
  *      y[t][o] = sum over groups j of scales[o][j] * sum over k of group j of (code[o][k] - 8) x[t][k]
  *
  * The inner sums are warp-level products of 16 outputs with 8 columns; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
- *   rows     the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products.  9 to 16 rows are two blocks' (16 rows on 10240 x 4096, fp32:
- *            15.6 us, 24.1 in linear4_umma.cu);
+ *   rows     the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products.  What makes numbers of codes bounds it, so a block has up to 16 rows for
+ *            them, two products for each number, where registers have room for that much x (width 4096 at most), else 8 (16 rows on 10240 x 4096 in fp32: 11.6 us, by eights 15.7, and in
+ *            linear4_umma.cu 24.4; on 120832 x 4096 80, 122 and 175.  17 rows as 16 and 1 take 21.4 and 156, but 13.3 on 4096 x 4096, where that file takes 10.8 for 16-bit results);
  *   digits   of one row, on large matrices, the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
  *            below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 11, and
  *            -8 sum d comes in as the sum's first value.
@@ -30,8 +31,8 @@ using namespace hy3a_layer;
 using namespace hy3a_ring;
 
 constexpr int kWarps = 16, kProducer = kWarps, kFinisher = kWarps + 1, kThreads = 32 * (kWarps + 2);
-constexpr int kTile = 16 /* outputs */, kRows = 8 /* of a block */, kFewRows = 16, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24, kMaxOut = 1 << 30 /* (numbers of outputs stay ints a tile past the last) */;
-constexpr int kParts = 4 /* tiles whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part */;
+constexpr int kTile = 16 /* outputs */, kRows = 8 /* columns of a product */, kFewRows = 16, kStageK = 4096, kMaxStages = 16, kMaxWidth = 1 << 16, kMaxRows = 1 << 24, kMaxOut = 1 << 30 /* (numbers of outputs stay ints a tile past the last) */;
+constexpr int kParts = 4 /* tiles of 8 rows whose parts may wait to be added up */, kPart = kTile * kRows /* values of a warp's part for 8 rows */;
 constexpr int kBox = 4 /* outputs of a copy */, kLine = 128 /* its bytes of each, times the lines of a stage */;
 constexpr int kRingBytes = 184 * 1024, kOffPart = kRingBytes, kOffBar = kOffPart + kParts * kWarps * kPart * 4, kSmem = kOffBar + 512 + 1024;
 enum { B_FULL = 0, B_EMPTY = kMaxStages, B_READY = 2 * kMaxStages, B_TAKEN = 2 * kMaxStages + kParts, B_COUNT = 2 * kMaxStages + 2 * kParts };
@@ -97,17 +98,20 @@ template <class T> __device__ __forceinline__ void mma_first(float (&d)[4], unsi
     else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
              : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-template <class T, int W> struct row_columns {
-    unsigned x[4 * W];
-    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4]) const {
+template <class T, int W, int C> struct row_columns {
+    unsigned x[C][4 * W];
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[C][4]) const {
 #pragma unroll
         for (int w = 0; w < W; w++) {
             unsigned vl[4], vh[4];
             steps<T>::of(wl[w], vl);
             steps<T>::of(wh[w], vh);
-            if (w == 0) mma_first<T>(d, vl[0], vh[0], vl[1], vh[1], x[0], x[1]);
-            else type<T>::mma(d, vl[0], vh[0], vl[1], vh[1], x[4 * w], x[4 * w + 1]);
-            type<T>::mma(d, vl[2], vh[2], vl[3], vh[3], x[4 * w + 2], x[4 * w + 3]);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                if (w == 0) mma_first<T>(d[c], vl[0], vh[0], vl[1], vh[1], x[c][0], x[c][1]);
+                else type<T>::mma(d[c], vl[0], vh[0], vl[1], vh[1], x[c][4 * w], x[c][4 * w + 1]);
+                type<T>::mma(d[c], vl[2], vh[2], vl[3], vh[3], x[c][4 * w + 2], x[c][4 * w + 3]);
+            }
         }
     }
 };
@@ -119,7 +123,7 @@ template <int W> struct digit_columns {
     unsigned x[2 * W];                /* the column's digits of even and odd k's of each word */
     int first[2];                     /* kFirstSum - 8 sum of digits, of columns 2 t and 2 t + 1 */
     float unit;                       /* 2^(E - 7) */
-    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[4]) const {
+    __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[1][4]) const {
         int n[4] = {first[0], first[1], first[0], first[1]};
 #pragma unroll
         for (int w = 0; w < W; w++)
@@ -127,7 +131,7 @@ template <int W> struct digit_columns {
                 : "+r"(n[0]), "+r"(n[1]), "+r"(n[2]), "+r"(n[3])
                 : "r"(wl[w] & 0x0f0f0f0fu), "r"(wh[w] & 0x0f0f0f0fu), "r"((wl[w] >> 4) & 0x0f0f0f0fu), "r"((wh[w] >> 4) & 0x0f0f0f0fu), "r"(x[2 * w]), "r"(x[2 * w + 1]));
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = fmaf(__int_as_float(n[i]), unit, -__int_as_float(kFirstSum) * unit);        /* exact, in the subnormal numbers too */
+        for (int i = 0; i < 4; i++) d[0][i] = fmaf(__int_as_float(n[i]), unit, -__int_as_float(kFirstSum) * unit);        /* exact, in the subnormal numbers too */
     }
 };
 __device__ __forceinline__ unsigned shift_left(unsigned v, int by) { unsigned r; asm("shl.b32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }        /* (0 by 32 and more, and by less than 0) */
@@ -174,12 +178,13 @@ template <class T, int W> __device__ __forceinline__ void store_digits(const T *
     }
 }
 
-/* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each; ONE: one row */
-template <class T, int W, int P, bool ONE>
+/* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each; ONE: one row; C: rows of a
+ * block, in eights */
+template <class T, int W, int P, bool ONE, int C>
 __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_scales, const few_args f) {
     extern __shared__ uint8_t s_raw[];
-    using columns = typename std::conditional<ONE, digit_columns<W>, row_columns<T, W>>::type;
-    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4;
+    using columns = typename std::conditional<ONE, digit_columns<W>, row_columns<T, W, C>>::type;
+    constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kBufs = kParts / C;
     __shared__ float s_units[ONE ? kStageK / kGroup : 1];
     const linear4_args &a = f.a;
     uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
     const unsigned ring = smem_u32(sm), bar0 = ring + kOffBar;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int boxes = (a.out_width + kBox - 1) / kBox, first = kBox * (int)((long long)boxes * blockIdx.x / gridDim.x), last = min(a.out_width, kBox * (int)((long long)boxes * (blockIdx.x + 1) / gridDim.x));
-    const int t0 = ONE ? 0 : blockIdx.y * kRows, rows = ONE ? 1 : min(kRows, a.rows - t0);
+    const int t0 = ONE ? 0 : blockIdx.y * (C * kRows), rows = ONE ? 1 : min(C * kRows, a.rows - t0);
     /* outputs g and g + 8 of the products are outputs mine and mine + 8 of the tile: such that lanes that read together find their words in different banks */
     const int mine_of = W == 4 ? (g & 1) * 4 + (g >> 1) : ((g >> 1) & 1) * 4 + (g & 1) * 2 + (g >> 2);
 #define BAR(i) (bar0 + 8u * (unsigned)(i))
@@ -236,19 +241,25 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
         int turn = 0;
 #pragma unroll 1
         for (int o0 = first; o0 < last; o0 += kTile, turn++) {
-            const int buf = turn % kParts;
-            if (!mbar_wait(BAR(B_READY + buf), (turn / kParts) & 1, s_abort, g_err, 42u)) break;
-            const float *part = reinterpret_cast<const float *>(sm + kOffPart) + buf * kWarps * kPart + lane * 4;
-            float4 sum = *reinterpret_cast<const float4 *>(part);
+            const int buf = turn % kBufs;
+            if (!mbar_wait(BAR(B_READY + buf), (turn / kBufs) & 1, s_abort, g_err, 42u)) break;
+            float v[4 * C];
+            unsigned taken = 0u;
 #pragma unroll
-            for (int w = 1; w < kWarps; w++) {
-                const float4 v = *reinterpret_cast<const float4 *>(part + w * kPart);
-                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            for (int c = 0; c < C; c++) {
+                const float *part = reinterpret_cast<const float *>(sm + kOffPart) + (buf * kWarps * C + c) * kPart + lane * 4;
+                float4 sum = *reinterpret_cast<const float4 *>(part);
+#pragma unroll
+                for (int w = 1; w < kWarps; w++) {
+                    const float4 v = *reinterpret_cast<const float4 *>(part + w * C * kPart);
+                    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+                }
+                v[4 * c] = sum.x; v[4 * c + 1] = sum.y; v[4 * c + 2] = sum.z; v[4 * c + 3] = sum.w;
+                taken |= __float_as_uint(sum.x);
             }
             __syncwarp();
             /* (an arrival does not wait for loads that are under way, so it takes something of the sums that they went into) */
-            if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf) + (__float_as_uint(sum.x) & f.zero));
-            float v[4] = {sum.x, sum.y, sum.z, sum.w};
+            if (lane == 0) mbar_arrive(BAR(B_TAKEN + buf) + (taken & f.zero));
             const auto put = [&](int r, float y) {
                 const size_t to = (size_t)(t0 + r) * a.out_stride + o0 + o;
                 if (a.wide) reinterpret_cast<float *>(a.out)[to] = y;
@@ -270,19 +281,22 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                 if (r0 == 0 && o0 + o < last) put(0, y);
             } else if (o0 + o < last) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) if (r0 + r < rows) put(r0 + r, v[r]);
+                for (int i = 0; i < 4 * C; i++) {
+                    const int r = i / 4 * kRows + r0 + i % 4;
+                    if (r < rows) put(r, v[i]);
+                }
             }
         }
     } else {
         /* ===================== products: a warp has `per` groups of a stage, one behind the other ===================== */
         columns x[kSets][kMine];
-        const T *row = reinterpret_cast<const T *>(a.x) + (ONE ? 0 : (size_t)(t0 + min(g, rows - 1)) * a.x_stride);
+        const T *const rows_of_x = reinterpret_cast<const T *>(a.x) + (size_t)t0 * a.x_stride;
         const int g0 = warp * f.per;
         const auto load_columns = [&](columns (&to)[kMine], int p) {
             if constexpr (ONE) {
                 uint8_t *const digits = sm + kOffPart;
                 meet_workers();
-                store_digits<T, W>(row, p * kStageK + tid * 8, a.width, tid, digits, s_units, s_odd);
+                store_digits<T, W>(rows_of_x, p * kStageK + tid * 8, a.width, tid, digits, s_units, s_odd);
                 meet_workers();
 #pragma unroll
                 for (int i = 0; i < kMine; i++) {
@@ -304,7 +318,12 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < kMine; i++) load_x<T, W>(row, g < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, to[i].x);
+                for (int i = 0; i < kMine; i++)
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        const int r = c * kRows + g;
+                        load_x<T, W>(rows_of_x + (size_t)min(r, rows - 1) * a.x_stride, r < rows && i < f.per, p * kStageK + (g0 + i) * kGroup, a.width, to[i].x[c]);
+                    }
             }
         };
         if (P) {
@@ -321,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
         }
         const unsigned eight = 2 * f.box_bytes, scales_at = ring + (kTile / kBox) * f.box_bytes + mine_of * f.scale_pitch + (g0 + t) * 2;
         int turn = 0;
-        const auto stage = [&](int o0, int p, const columns (&xs)[kMine], float (&acc)[4]) {
+        const auto stage = [&](int o0, int p, const columns (&xs)[kMine], float (&acc)[C][4]) {
             const int mine = min(f.per, a.groups - p * (kStageK / kGroup) - g0);
             /* scales of the lane's two outputs, group 4 i + t of the warp's for i = 0 .. */
             unsigned both[kPacks];
@@ -350,22 +369,25 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                         unsigned wl[W], wh[W];
                         load_words<W>(at[i] + by, wl);
                         load_words<W>(at[i] + by + eight, wh);
-                        float d[4];
+                        float d[C][4];
                         xs[i].sums(wl, wh, d);
                         const unsigned s = __shfl_sync(0xffffffffu, both[i / 4], (lane & 28) | (i & 3));
                         const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
-                        acc[0] = fmaf(s0, d[0], acc[0]); acc[1] = fmaf(s0, d[1], acc[1]);
-                        acc[2] = fmaf(s1, d[2], acc[2]); acc[3] = fmaf(s1, d[3], acc[3]);
+#pragma unroll
+                        for (int c = 0; c < C; c++) {
+                            acc[c][0] = fmaf(s0, d[c][0], acc[c][0]); acc[c][1] = fmaf(s0, d[c][1], acc[c][1]);
+                            acc[c][2] = fmaf(s1, d[c][2], acc[c][2]); acc[c][3] = fmaf(s1, d[c][3], acc[c][3]);
+                        }
                     }
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(BAR(B_EMPTY + st) + ((__float_as_uint(acc[0]) | __float_as_uint(acc[2])) & f.zero));
+            if (lane == 0) mbar_arrive(BAR(B_EMPTY + st) + ((__float_as_uint(acc[0][0]) | __float_as_uint(acc[0][2])) & f.zero));
             if (++st == f.stages) { st = 0; ph ^= 1u; }
         };
 #pragma unroll 1
         for (int o0 = first; o0 < last; o0 += kTile, turn++) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float acc[C][4] = {};
             if (P) {
 #pragma unroll
                 for (int p = 0; p < kSets; p++) stage(o0, p, x[p], acc);
@@ -376,11 +398,14 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                     stage(o0, p, x[0], acc);
                 }
             }
-            const int buf = turn % kParts;
-            if (turn >= kParts && !mbar_wait(BAR(B_TAKEN + buf), (turn / kParts - 1) & 1, s_abort, g_err, 43u)) break;
-            float *const part = reinterpret_cast<float *>(sm + kOffPart) + (buf * kWarps + warp) * kPart;       /* [output][column] */
-            *reinterpret_cast<float2 *>(part + mine_of * kRows + 2 * t) = make_float2(acc[0], acc[1]);
-            *reinterpret_cast<float2 *>(part + (mine_of + 8) * kRows + 2 * t) = make_float2(acc[2], acc[3]);
+            const int buf = turn % kBufs;
+            if (turn >= kBufs && !mbar_wait(BAR(B_TAKEN + buf), (turn / kBufs - 1) & 1, s_abort, g_err, 43u)) break;
+            float *const part = reinterpret_cast<float *>(sm + kOffPart) + (buf * kWarps + warp) * C * kPart;       /* [eight rows][output][row] */
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                *reinterpret_cast<float2 *>(part + c * kPart + mine_of * kRows + 2 * t) = make_float2(acc[c][0], acc[c][1]);
+                *reinterpret_cast<float2 *>(part + c * kPart + (mine_of + 8) * kRows + 2 * t) = make_float2(acc[c][2], acc[c][3]);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(BAR(B_READY + buf));
         }
@@ -389,23 +414,24 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
 #undef BAR
 }
 
-template <class T, int W, int P, bool ONE>
+template <class T, int W, int P, bool ONE, int C = 1>
 cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     cudaError_t e;
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
-        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(hy3a_linear4_kernel<T, W, P, ONE, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem)) != cudaSuccess) return e;
         if (device < 64) ready[device].store(true, std::memory_order_release);
     }
     const int boxes = (f.a.out_width + kBox - 1) / kBox;
-    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + kRows - 1) / kRows), dim3(kThreads), kSmem, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE>, codes, scales, f);
+    hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + C * kRows - 1) / (C * kRows)), dim3(kThreads), kSmem, stream);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE, C>, codes, scales, f);
 }
 template <class T, int W>
 cudaError_t launch_group(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
     constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers for two stages' x) */
     /* Digits save a third of a microsecond a tile and take two to make: for 6 tiles a block and more (one row on 4096 x 4096: 6.9 us with them, 5.0 without; on 120832 x 4096 50 and 63). */
     const bool digits = f.a.rows == 1 && f.a.out_width >= 6 * kTile * sms;
+    if (f.passes == 1 && f.a.rows > kRows) return launch<T, W, 1, false, 2>(codes, scales, f, device, sms, stream);
     if (f.passes == 1) return digits ? launch<T, W, 1, true>(codes, scales, f, device, sms, stream) : launch<T, W, 1, false>(codes, scales, f, device, sms, stream);
     if (f.passes == 2 && kTwo) return digits ? launch<T, W, kTwo, kTwo != 0>(codes, scales, f, device, sms, stream) : launch<T, W, kTwo, false>(codes, scales, f, device, sms, stream);
     return launch<T, W, 0, false>(codes, scales, f, device, sms, stream);
