@@ -8,7 +8,7 @@
  *            them, two products for each number, where registers have room for that much x (width 4096 at most), else 8 (16 rows on 10240 x 4096 in fp32: 11.6 us, by eights 15.7, and in
  *            linear4_umma.cu 24.4; on 120832 x 4096 80, 122 and 175.  17 rows as 16 and 1 take 21.4 and 156, but 13.3 on 4096 x 4096, where that file takes 10.8 for 16-bit results);
  *   digits   of one row, on large matrices, the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
- *            below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 11, and
+ *            below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 9, and
  *            -8 sum d comes in as the sum's first value.
  *
  * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
@@ -99,13 +99,15 @@ template <class T> __device__ __forceinline__ void mma_first(float (&d)[4], unsi
              : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 template <class T, int W, int C> struct row_columns {
+    static constexpr bool kOne = C == 1;         /* (sums of one eight are multiplied in less time than numbers cost; 8 rows on 120832 x 4096: 59.9 us and 62.2, 16 rows: 82.3 and 80.5) */
+    static constexpr float kPerStep = kOne ? steps<T>::kPerStep : 1.f;
     unsigned x[C][4 * W];
     __device__ __forceinline__ void sums(const unsigned (&wl)[W], const unsigned (&wh)[W], float (&d)[C][4]) const {
 #pragma unroll
         for (int w = 0; w < W; w++) {
             unsigned vl[4], vh[4];
-            steps<T>::of(wl[w], vl);
-            steps<T>::of(wh[w], vh);
+            if (kOne) { steps<T>::parts(wl[w], vl); steps<T>::parts(wh[w], vh); }
+            else { steps<T>::of(wl[w], vl); steps<T>::of(wh[w], vh); }
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 if (w == 0) mma_first<T>(d[c], vl[0], vh[0], vl[1], vh[1], x[c][0], x[c][1]);
@@ -120,6 +122,7 @@ template <class T, int W, int C> struct row_columns {
 constexpr unsigned kMostExponent = 127 + 100;
 constexpr int kFirstSum = 0x4B400000;        /* 3 2^22 as a float: what is added to it as an integer, up to 2^22, is added to the float */
 template <int W> struct digit_columns {
+    static constexpr float kPerStep = 1.f;
     unsigned x[2 * W];                /* the column's digits of even and odd k's of each word */
     int first[2];                     /* kFirstSum - 8 sum of digits, of columns 2 t and 2 t + 1 */
     float unit;                       /* 2^(E - 7) */
@@ -375,6 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                         const float s0 = unpack<T>(s, false), s1 = unpack<T>(s, true);
 #pragma unroll
                         for (int c = 0; c < C; c++) {
+                            /* (the sum is what may be scaled: a scale times kPerStep need not be finite) */
+#pragma unroll
+                            for (int k = 0; k < 4; k++) d[c][k] *= columns::kPerStep;
                             acc[c][0] = fmaf(s0, d[c][0], acc[c][0]); acc[c][1] = fmaf(s0, d[c][1], acc[c][1]);
                             acc[c][2] = fmaf(s1, d[c][2], acc[c][2]); acc[c][3] = fmaf(s1, d[c][3], acc[c][3]);
                         }

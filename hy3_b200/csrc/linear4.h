@@ -47,6 +47,16 @@ template <> struct steps<__nv_bfloat16> {
             asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(c), "r"(0x43084308u));
         }
     }
+    /* the same in units of 1 / kPerStep, in 9 operations a word and not 11: a nibble in bits 0-3 or 4-7 of a 16-bit number is that many 2^-133 or 2^-129 as it stands (subnormal, or of the lowest exponent) */
+    static constexpr float kPerStep = 64.f;
+    static __device__ __forceinline__ void parts(unsigned w, unsigned (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const unsigned u = i ? w >> 8 : w;
+            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[i]) : "r"(u & 0x000f000fu), "r"(0x7f007f00u) /* 2^127 */, "r"(0xbe00be00u) /* -1 / 8 */);
+            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v[i + 1]) : "r"(u & 0x00f000f0u), "r"(0x7d007d00u) /* 2^123 */, "r"(0xbe00be00u));
+        }
+    }
 };
 template <> struct steps<__half> {
     static __device__ __forceinline__ void in_order(unsigned w, unsigned (&v)[4]) {
@@ -64,8 +74,23 @@ template <> struct steps<__half> {
             asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v[i + 1]) : "r"(hi), "r"(0x2c002c00u) /* 1 / 16 */, "r"(0xd480d480u) /* -72 */);
         }
     }
+    static constexpr float kPerStep = 1.f;
+    static __device__ __forceinline__ void parts(unsigned w, unsigned (&v)[4]) { of(w, v); }
 };
 
+/* whether row t of x has a NaN, for a warp */
+template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, int t) {
+    const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride);
+    constexpr unsigned kInf = type<T>::code == HY3A_BF16 ? 0x7f80u : 0x7c00u;
+    bool is = false;
+    for (int i = threadIdx.x & 31; i < a.width / 8; i += 32) {
+        const uint4 v = x[i];
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) is |= (w[j] & 0x7fffu) > kInf || (w[j] >> 16 & 0x7fffu) > kInf;
+    }
+    return __any_sync(0xffffffffu, is);
+}
 /* out[t][o] from the definition, by a warp */
 template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {
     const int lane = threadIdx.x & 31;

@@ -112,18 +112,6 @@ template <> struct pair_of<__half> {
     static __device__ __forceinline__ unsigned rest(unsigned a, unsigned b, unsigned hi) { unsigned r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(hi ^ 0x80008000u)); return r; }
 };
 
-template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, int t) {
-    const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride);
-    constexpr unsigned kInf = type<T>::code == HY3A_BF16 ? 0x7f80u : 0x7c00u;
-    bool is = false;
-    for (int i = threadIdx.x & 31; i < a.width / 8; i += 32) {
-        const uint4 v = x[i];
-        const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) is |= (w[j] & 0x7fffu) > kInf || (w[j] >> 16 & 0x7fffu) > kInf;
-    }
-    return __any_sync(0xffffffffu, is);
-}
 /* What is not finite among a lane's results y of output o and rows t, t + 1, .. t + n - 1 is NaN if x has one in its row (padding that nobody wrote may be such rows), and else computed again, by the whole
  * warp (rare: one piece of code, not unrolled) */
 template <class T, int N> __device__ __forceinline__ void settle(const linear4_args &a, float (&y)[N], int n, int t, int o, bool mine) {
