@@ -24,7 +24,7 @@ using namespace hy3a_layer;
 
 /* Threads of a block: four blocks an SM where there are more rows than SMs, so that one's end runs beside the others' loads; else one, and the blocks of a cluster for a row where rows
  * are fewer still: 131072 fp32 logits are one round of loads for 8 of them. */
-constexpr int kAlone = 256, kShared = 512, kMaxCluster = 8;
+constexpr int kSmall = 64, kAlone = 256, kShared = 512, kMaxCluster = 8;
 constexpr int kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -34,7 +34,7 @@ struct logprobs_args {
     const int *tokens;
     float *asked_logp, *entropy, *top_logp;
     int *top_ids;
-    int rows, vocab, asked, top_k, cluster /* blocks of a row; 0: one by itself */;
+    int rows, vocab, asked, top_k, cluster /* blocks of a row; 0: one by itself; -1: a small one */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -202,12 +202,12 @@ struct running {
 };
 
 template <class T, bool TOP, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == kAlone ? 4 : 1) hy3a_logprobs_kernel(const logprobs_args a) {
+__global__ void __launch_bounds__(kThreads, kThreads == kShared ? 1 : 1024 / kThreads) hy3a_logprobs_kernel(const logprobs_args a) {
     constexpr int kWarps = kThreads / 32, kOf = row_of<T>::kOf, kAtOnce = 8;        /* vectors of a thread that are on their way together */
     constexpr bool kCluster = kThreads == kShared;
     __shared__ part s_part[kWarps], s_all[kMaxCluster];
     __shared__ float s_max, s_log;
-    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_lanes[TOP ? kMaxCluster : 1][32], s_list[TOP ? kList : 1];
+    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_lanes[TOP && kCluster ? kMaxCluster : 1][32], s_list[TOP ? kList : 1];
     __shared__ unsigned s_listed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cluster = kCluster ? a.cluster : 1, me = kCluster ? (int)cluster_rank() : 0, row = kCluster ? blockIdx.x / cluster : blockIdx.x;
     pdl_release();
@@ -230,9 +230,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAlone ? 4 : 1) hy3a_log
             const int i = i0 + u * kThreads + lane;
             raw[u] = r.load(i < last ? i : -1);
         }
+        /* vectors that there are, the same for a warp (small blocks alone look: rows of many vectors take 4 to 10% longer where each is asked for) */
+        const int here = kThreads == kSmall ? (last - i0 + kThreads - 1) / kThreads : kAtOnce;
         float most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
+            if (u >= here) break;
             const float vm = largest(raw[u], T());
             if (TOP && vm > best) { best = vm; best_at = i0 + u * kThreads + lane; }
             most = fmaxf(most, vm);
@@ -244,7 +247,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAlone ? 4 : 1) hy3a_log
             raise(q, warp_max(fmaxf(most, p.m)));
             p = {q.m, q.n, {q.s, 0.f}, {q.t, 0.f}};
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) with_m |= __any_sync(0xffffffffu, largest(raw[u], T()) >= p.m || p.m == -INFINITY) ? 1u << u : 0u;
+            for (int u = 0; u < kAtOnce; u++) {
+                if (u >= here) break;
+                with_m |= __any_sync(0xffffffffu, largest(raw[u], T()) >= p.m || p.m == -INFINITY) ? 1u << u : 0u;
+            }
             for (unsigned todo = with_m; todo; todo &= todo - 1) {
                 float v[kOf];
                 logits_of<T>(pick(raw, __ffs(todo) - 1), v);
@@ -253,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAlone ? 4 : 1) hy3a_log
         }
 #pragma unroll
         for (int u = 0; u < kAtOnce; u++) {
+            if (u >= here) break;
             if ((with_m >> u) & 1) continue;
             float v[kOf];
             logits_of<T>(raw[u], v);
@@ -387,7 +394,7 @@ cudaError_t launch(const logprobs_args &a, void *stream) {
     return a.top_k ? cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, true, kThreads>, a) : cudaLaunchKernelEx(&l.cfg, hy3a_logprobs_kernel<T, false, kThreads>, a);
 }
 template <class T>
-cudaError_t launch_type(const logprobs_args &a, void *stream) { return a.cluster ? launch<T, kShared>(a, stream) : launch<T, kAlone>(a, stream); }
+cudaError_t launch_type(const logprobs_args &a, void *stream) { return a.cluster < 0 ? launch<T, kSmall>(a, stream) : (a.cluster ? launch<T, kShared>(a, stream) : launch<T, kAlone>(a, stream)); }
 
 } /* namespace */
 
@@ -408,6 +415,9 @@ extern "C" int hy3a_logprobs(void *stream, int dtype, int rows, int vocab, const
     /* Blocks of a row: none but one where there are more rows than SMs; else as many as fit on the device at once for all rows, up to a portable cluster, and with half a round of
      * loads for each at least. */
     int cluster = rows > sms ? 0 : kMaxCluster;
+    /* Rows of one round of a small block's loads are its; of two rounds, where there are more rows than larger blocks fit at once (6171 rows of 2514 in bf16: 16.6 us and 52, 2692 of 5216 in fp16 26.7 and
+     * 40; 300 rows of 4000 in fp32 8.1 and 7.4). */
+    if ((long long)vocab * el <= (rows > sms * (1024 / kAlone) ? 2 : 1) * kSmall * 128) cluster = -1;
     while (cluster > 1 && (rows * cluster > sms || vocab < cluster * kShared * 16)) cluster >>= 1;
     const logprobs_args a = {logits, stride, tokens, asked_logp, entropy, top_logp, top_ids, rows, vocab, asked, top_k, cluster};
     const cudaError_t e = dtype == HY3A_F32 ? launch_type<float>(a, stream) : (dtype == HY3A_F16 ? launch_type<__half>(a, stream) : launch_type<__nv_bfloat16>(a, stream));
