@@ -300,29 +300,50 @@ __global__ void __launch_bounds__(kThreads, kThreads == kShared ? 1 : 1024 / kTh
         const float least = closed(key) ? -INFINITY : value_of(key);
         const int least_at = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
         const auto reaches = [&](float l, int i) { return l > least || (l == least && i <= least_at); };
-        if (reaches(best, best_at)) {
-            const unsigned count = peer(&s_listed, 0), list = peer(s_list, 0);
-            /* the last round's vectors, then those of the rounds before */
+        const bool mine = reaches(best, best_at);
+        const unsigned who = __ballot_sync(0xffffffffu, mine), count = peer(&s_listed, 0), list = peer(s_list, 0);
+        const auto take = [&](const uint4 &of, int vector) {
+            float v[kOf];
+            logits_of<T>(of, v);
+#pragma unroll
+            for (int j = 0; j < kOf; j++) {
+                if (!reaches(v[j], vector)) continue;
+                unsigned at;
+                asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
+                if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(v[j], vector * kOf + j - r.skip)) : "memory");
+            }
+        };
+        /* The last round's vectors are still there; those of the rounds before are read again: by the thread, round after round, or by eight lanes for each, 64 vectors at a time, where that is fewer loads one
+         * behind the other (403 rows of 115189 in fp32, top 1: 43.5 us, and 55.5 by threads alone). */
+        const int from = first + warp * 32, rounds = (i0 - from) / (kThreads * kAtOnce), threads = __popc(who);
+        const bool together = kThreads != kSmall && (threads + 3) / 4 * ((rounds + 7) / 8) < rounds;
+        if (mine)
             for (int i = i0 + lane;;) {
                 unsigned todo = 0u;
 #pragma unroll
                 for (int u = 0; u < kAtOnce; u++) todo |= reaches(largest(raw[u], T()), i + u * kThreads) ? 1u << u : 0u;
-                for (; todo; todo &= todo - 1) {
-                    const int u = __ffs(todo) - 1, vector = i + u * kThreads;
-                    float v[kOf];
-                    logits_of<T>(pick(raw, u), v);
-#pragma unroll
-                    for (int j = 0; j < kOf; j++) {
-                        if (!reaches(v[j], vector)) continue;
-                        unsigned at;
-                        asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count) : "memory");
-                        if (at < kList) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(key_of(v[j], vector * kOf + j - r.skip)) : "memory");
-                    }
-                }
+                for (; todo; todo &= todo - 1) take(pick(raw, __ffs(todo) - 1), i + (__ffs(todo) - 1) * kThreads);
                 i -= kThreads * kAtOnce;
-                if (i < first) break;
+                if (together || i < first) break;
 #pragma unroll
                 for (int u = 0; u < kAtOnce; u++) raw[u] = r.load(i + u * kThreads);
+            }
+        if (together) {
+            __syncwarp();
+            if (mine) s_key[warp * 32 + __popc(who & ((1u << lane) - 1u))] = lane;
+            __syncwarp();
+#pragma unroll 1
+            for (int c = lane >> 3; c < threads; c += 4) {
+                const int at = from + (int)s_key[warp * 32 + c];
+#pragma unroll 1
+                for (int n = lane & 7; n < rounds * kAtOnce; n += 8 * kAtOnce) {
+                    unsigned todo = 0u;
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; u++) raw[u] = r.load(n + 8 * u < rounds * kAtOnce ? at + (n + 8 * u) * kThreads : -1);
+#pragma unroll
+                    for (int u = 0; u < kAtOnce; u++) todo |= reaches(largest(raw[u], T()), at + (n + 8 * u) * kThreads) ? 1u << u : 0u;
+                    for (; todo; todo &= todo - 1) take(pick(raw, __ffs(todo) - 1), at + (n + 8 * (__ffs(todo) - 1)) * kThreads);
+                }
             }
         }
     }
