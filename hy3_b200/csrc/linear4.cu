@@ -45,7 +45,7 @@ struct few_args {
     linear4_args a;
     int lines /* of 128 bytes, of an output's codes in a stage */, box_bytes /* of four outputs, with a line's more where lines is even: banks */, stage_bytes, stages, passes /* stages of a tile */;
     int in_stage /* groups of a stage */, per /* of a warp */;
-    int whole;                /* rows of codes are whole lines */
+    int boxed;                /* outputs whose lines of a stage are one copy: all where rows of codes are whole lines, else all but the last, as a row's last line ends in the next row (at k's whose x is 0) */
     int scale_pitch;          /* bytes of an output's scales in a stage; 0: rows of scales do not start on 16-byte boundaries, and are read where they lie */
     unsigned zero;            /* 0, which the compiler does not know */
 };
@@ -184,7 +184,7 @@ template <class T, int W> __device__ __forceinline__ void store_digits(const T *
 /* W: words of a lane for a group; P: stages of a tile where x of all of them stays in registers, 0: x is read for each; ONE: one row; C: rows of a
  * block, in eights */
 template <class T, int W, int P, bool ONE, int C>
-__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_scales, const few_args f) {
+__global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_line, const __grid_constant__ CUtensorMap tm_scales, const few_args f) {
     extern __shared__ uint8_t s_raw[];
     using columns = typename std::conditional<ONE, digit_columns<W>, row_columns<T, W, C>>::type;
     constexpr int kGroup = 32 * W, kMine = kStageK / kGroup / kWarps /* groups of a warp in a stage */, kSets = P ? P : 1, kPacks = (kMine + 3) / 4, kBufs = kParts / C;
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
         for (int i = 0; i < kParts; i++) { mbar_init(BAR(B_READY + i), kWarps); mbar_init(BAR(B_TAKEN + i), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kProducer && lane < 2) {
-        const CUtensorMap *m = lane == 0 ? &tm_codes : &tm_scales;
+    if (warp == kProducer && lane < 3) {
+        const CUtensorMap *m = lane == 0 ? &tm_codes : lane == 1 ? &tm_scales : &tm_line;
         asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
     __syncthreads();
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                 if (lead) mbar_expect_tx(full, n * f.lines * kBox * kLine + kTile * f.scale_pitch);
 #pragma unroll 1
                 for (int q = 0; q < n; q++) {
-                    if (f.whole) copy_lines(to + q * f.box_bytes, &tm_codes, full, 0, o0 + q * kBox, p * (kStageK / 2 / kLine), policy, lead);
-                    else for (int c = 0; c < f.lines; c++) copy_lines(to + q * f.box_bytes + c * kBox * kLine, &tm_codes, full, p * (kStageK / 2) + c * kLine, o0 + q * kBox, 0, policy, lead);
+                    if (o0 + (q + 1) * kBox <= f.boxed || f.boxed == a.out_width) copy_lines(to + q * f.box_bytes, &tm_codes, full, 0, o0 + q * kBox, p * (kStageK / 2 / kLine), policy, lead);
+                    else for (int c = 0; c < f.lines; c++) copy_lines(to + q * f.box_bytes + c * kBox * kLine, &tm_line, full, p * (kStageK / 2) + c * kLine, o0 + q * kBox, 0, policy, lead);
                 }
                 if (f.scale_pitch) copy_scales(to + (kTile / kBox) * f.box_bytes, &tm_scales, full, p * (kStageK / kGroup), o0, lead);
                 if (++st == f.stages) { st = 0; ph ^= 1u; }
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
 }
 
 template <class T, int W, int P, bool ONE, int C = 1>
-cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
+cudaError_t launch(const CUtensorMap (&maps)[3], const few_args &f, int device, int sms, void *stream) {
     static std::atomic<bool> ready[64];       /* shared memory allowed, per device */
     cudaError_t e;
     if (device >= 64 || !ready[device].load(std::memory_order_acquire)) {
@@ -430,22 +430,22 @@ cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &scales, const fe
     }
     const int boxes = (f.a.out_width + kBox - 1) / kBox;
     hy3a_launch l(dim3(boxes < sms ? boxes : sms, (f.a.rows + C * kRows - 1) / (C * kRows)), dim3(kThreads), kSmem, stream);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE, C>, codes, scales, f);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_kernel<T, W, P, ONE, C>, maps[0], maps[1], maps[2], f);
 }
 template <class T, int W>
-cudaError_t launch_group(const CUtensorMap &codes, const CUtensorMap &scales, const few_args &f, int device, int sms, void *stream) {
+cudaError_t launch_group(const CUtensorMap (&maps)[3], const few_args &f, int device, int sms, void *stream) {
     constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers for two stages' x) */
     /* Digits save a third of a microsecond a tile and take two to make: for 6 tiles a block and more (one row on 4096 x 4096: 6.9 us with them, 5.0 without; on 120832 x 4096 50 and 63). */
     const bool digits = f.a.rows == 1 && f.a.out_width >= 6 * kTile * sms;
-    if (f.passes == 1 && f.a.rows > kRows) return launch<T, W, 1, false, 2>(codes, scales, f, device, sms, stream);
-    if (f.passes == 1) return digits ? launch<T, W, 1, true>(codes, scales, f, device, sms, stream) : launch<T, W, 1, false>(codes, scales, f, device, sms, stream);
-    if (f.passes == 2 && kTwo) return digits ? launch<T, W, kTwo, kTwo != 0>(codes, scales, f, device, sms, stream) : launch<T, W, kTwo, false>(codes, scales, f, device, sms, stream);
-    return launch<T, W, 0, false>(codes, scales, f, device, sms, stream);
+    if (f.passes == 1 && f.a.rows > kRows) return launch<T, W, 1, false, 2>(maps, f, device, sms, stream);
+    if (f.passes == 1) return digits ? launch<T, W, 1, true>(maps, f, device, sms, stream) : launch<T, W, 1, false>(maps, f, device, sms, stream);
+    if (f.passes == 2 && kTwo) return digits ? launch<T, W, kTwo, kTwo != 0>(maps, f, device, sms, stream) : launch<T, W, kTwo, false>(maps, f, device, sms, stream);
+    return launch<T, W, 0, false>(maps, f, device, sms, stream);
 }
 template <class T>
 cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream, const char **what) {
     const int k = a.width < kStageK ? a.width : kStageK, bytes = a.width / 2;
-    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, bytes % kLine == 0, 0, 0u};
+    few_args f = {a, (k / 2 + kLine - 1) / kLine, 0, 0, 0, (a.width + kStageK - 1) / kStageK, (k + a.group - 1) / a.group, 0, 0, 0, 0u};
     f.per = (f.in_stage + kWarps - 1) / kWarps;
     f.box_bytes = (f.lines | 1) * kBox * kLine;
     const bool boxed = a.groups % 8 == 0 && (uintptr_t)a.scales % 16 == 0;
@@ -453,27 +453,33 @@ cudaError_t launch_few(const linear4_args &a, int device, int sms, void *stream,
     f.stage_bytes = (kTile / kBox * f.box_bytes + kTile * f.scale_pitch + 1023) & ~1023;
     f.stages = kRingBytes / f.stage_bytes;
     if (f.stages > kMaxStages) f.stages = kMaxStages;
-    /* rows of whole lines: [lines][outputs][128 bytes], all lines of a stage in a copy; else [outputs][bytes], a line in a copy */
-    CUtensorMap codes, scales = {};
+    /* [lines][outputs][128 bytes], all lines of a stage in a copy; and [outputs][bytes], a line in a copy */
+    f.boxed = bytes % kLine == 0 ? a.out_width : bytes > kLine ? a.out_width - 1 : 0;
+    CUtensorMap maps[3] = {};
     const encode_tiled_fn enc = encoder();
     const cuuint32_t one[3] = {1, 1, 1};
-    const cuuint64_t dims[3] = {(cuuint64_t)(f.whole ? kLine : bytes), (cuuint64_t)a.out_width, (cuuint64_t)(f.whole ? bytes / kLine : 1)}, strides[2] = {(cuuint64_t)bytes, (cuuint64_t)(f.whole ? kLine : 16)};
-    const cuuint32_t box[3] = {kLine, kBox, (cuuint32_t)(f.whole ? f.lines : 1)};
-    bool ok = enc && enc(&codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const auto codes = [&](CUtensorMap *m, cuuint64_t inner, int outputs, int lines, cuuint64_t line_stride, int box_lines) {
+        const cuuint64_t dims[3] = {inner, (cuuint64_t)outputs, (cuuint64_t)lines}, strides[2] = {(cuuint64_t)bytes, line_stride};
+        const cuuint32_t box[3] = {kLine, kBox, (cuuint32_t)box_lines};
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    bool ok = enc && (!f.boxed || codes(&maps[0], kLine, f.boxed, (bytes + kLine - 1) / kLine, kLine, f.lines)) && codes(&maps[1], bytes, a.out_width, 1, 16, 1);
     if (boxed && ok) {
         const cuuint64_t sdims[2] = {(cuuint64_t)a.groups, (cuuint64_t)a.out_width}, sstrides[1] = {2ull * a.groups};
         const cuuint32_t sbox[2] = {(cuuint32_t)f.scale_pitch / 2, kTile};
-        ok = enc(&scales, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(a.scales), sdims, sstrides, sbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+        ok = enc(&maps[2], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(a.scales), sdims, sstrides, sbox, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     }
+    if (!f.boxed) maps[0] = maps[1];          /* (not used, but fetched) */
+    if (!boxed) maps[2] = maps[1];
     if (!ok) {
         *what = "no tensor map (cuTensorMapEncodeTiled)";
         return cudaErrorInvalidValue;
     }
-    if (a.group == 32) return launch_group<T, 1>(codes, scales, f, device, sms, stream);
-    if (a.group == 64) return launch_group<T, 2>(codes, scales, f, device, sms, stream);
-    return launch_group<T, 4>(codes, scales, f, device, sms, stream);
+    if (a.group == 32) return launch_group<T, 1>(maps, f, device, sms, stream);
+    if (a.group == 64) return launch_group<T, 2>(maps, f, device, sms, stream);
+    return launch_group<T, 4>(maps, f, device, sms, stream);
 }
 
 } /* namespace */
