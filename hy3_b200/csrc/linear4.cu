@@ -434,12 +434,12 @@ cudaError_t launch(const CUtensorMap (&maps)[3], const few_args &f, int device, 
 }
 template <class T, int W>
 cudaError_t launch_group(const CUtensorMap (&maps)[3], const few_args &f, int device, int sms, void *stream) {
-    constexpr int kTwo = W == 1 ? 0 : 2;       /* (short groups leave no registers for two stages' x) */
+    constexpr bool kDigitsOfTwo = W > 1;       /* (short groups leave no registers for two stages' digits) */
     /* Digits save a third of a microsecond a tile and take two to make: for 6 tiles a block and more (one row on 4096 x 4096: 6.9 us with them, 5.0 without; on 120832 x 4096 50 and 63). */
     const bool digits = f.a.rows == 1 && f.a.out_width >= 6 * kTile * sms;
     if (f.passes == 1 && f.a.rows > kRows) return launch<T, W, 1, false, 2>(maps, f, device, sms, stream);
     if (f.passes == 1) return digits ? launch<T, W, 1, true>(maps, f, device, sms, stream) : launch<T, W, 1, false>(maps, f, device, sms, stream);
-    if (f.passes == 2 && kTwo) return digits ? launch<T, W, kTwo, kTwo != 0>(maps, f, device, sms, stream) : launch<T, W, kTwo, false>(maps, f, device, sms, stream);
+    if (f.passes == 2) return digits && kDigitsOfTwo ? launch<T, W, 2, kDigitsOfTwo>(maps, f, device, sms, stream) : launch<T, W, 2, false>(maps, f, device, sms, stream);
     return launch<T, W, 0, false>(maps, f, device, sms, stream);
 }
 template <class T>
