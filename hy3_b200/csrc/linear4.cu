@@ -12,7 +12,7 @@
  *            -8 sum d comes in as the sum's first value.
  *
  * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
- * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way.  (A bulk copy
+ * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way (one row on 120832 x 4096: 44 us, 6 TB/s).  (A bulk copy
  * for each output keeps the issuing lane busy for longer than its bytes take.)  The 16 warps share the k's; each keeps its part of x in registers for the whole launch.  Their
  * sums meet in shared memory, where a warp of their own adds them up.  Short launches wait for instructions as much as for codes: loops that are run a few times are not unrolled.
  *
