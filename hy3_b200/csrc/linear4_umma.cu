@@ -12,10 +12,12 @@
  * Results of the rows' type: a weight, of up to 15 bits (fp16) or 11 (bf16), is rounded to that type once, which leaves an error like the result's own rounding.  Results that are not finite (of weights
  * rounded beyond the type's largest, of an infinite x that meets the rest) are computed again from the definition, by the warp that finds them.
  *
- * Results in fp32: a weight enters as two numbers, the rounded one and the rest, which is exact, so that there are 8 products a step; and the tensor cores begin a new sum every 512 k's, which warps of their own
- * add to results in registers: the tensor cores' sums are cut off and not rounded (one sum over 4096 k's left an error of 5.6e-6 of the result).  A = code - 8, with a sum for each group and its scale
+ * Results in fp32: a weight enters as two numbers, the rounded one and the rest, which is exact, so that there are 8 products a step; and the tensor cores begin a new sum every 512 k's (bf16; fp16: 256), which warps of their own
+ * add to results in registers: the tensor cores' sums are cut off and not rounded (one sum over 4096 k's left an error of 5.6e-6 of the result; sums of 512 leave 4.6e-7, of fp16 products, whose 22 bits lose more,
+ * 1.1e-6, of 256 k's 6e-7 for 2% more time).  A = code - 8, with a sum for each group and its scale
  * at the end, is half as many products, but 64 rows on 10240 x 4096 took 26.8 us: the sums are read 8 times as often.
  *
+ * Where tiles are more than pairs of CTAs fit at once, a pair has several, and its warps go on to the next one each as far as it can.
  * Where tiles are few, the CTAs of a cluster share the k's of a tile; their sums meet in shared memory, and are added in the order of the k's.
  *
  * Every wait is bounded; one that runs out raises the CTA's abort flag and a code in the error word (hy3a_layer_sync), lets all warps fall through, and TMEM is always
@@ -42,7 +44,7 @@ __device__ unsigned g_err[2];         /* {code, where} of the first wait that ra
 
 struct many_args {
     linear4_args a;
-    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */, run_columns /* fp32 results: columns of each of two sums */;
+    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */, run_columns /* fp32 results: columns of each of two sums */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -140,6 +142,17 @@ template <class T, int N> __device__ __forceinline__ void settle(const linear4_a
         for (int k = 0; k < N; k++) if (j == k) y[k] = now;
     }
 }
+/* the same of fp32 results that have been stored: rows t + c0 .. t + c0 + 15, t + c0 + 32 .. of a tile's n */
+template <class T> __device__ __noinline__ void settle_stored(const linear4_args &a, int t, int n, int c0, int o, bool mine) {
+#pragma unroll 1
+    for (int j = c0; j < n; j += j % 16 == 15 ? 17 : 1) {
+        float *const at = reinterpret_cast<float *>(a.out) + (size_t)(t + j) * a.out_stride + o;
+        float y[1] = {mine ? *reinterpret_cast<volatile float *>(at) : 0.f};
+        if (!__any_sync(0xffffffffu, !(fabsf(y[0]) < INFINITY))) continue;
+        settle<T>(a, y, 1, t + j, o, mine);
+        if (mine) *at = y[0];
+    }
+}
 /* A lane's results of its output, row after row.  16-bit ones: neighbouring lanes exchange, so that one stores the even rows' two outputs and one the odd rows'. */
 template <class T, bool WIDE, int N> __device__ __forceinline__ void store(const linear4_args &a, const float (&y)[N], int n, int t, int o, int odd_stride) {
     const bool mine = o < a.out_width;
@@ -165,12 +178,12 @@ template <bool WIDE> struct warps_of {
     static constexpr int kTeams = WIDE ? 3 : 4, kAdders = WIDE ? 8 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
 };
 
-/* WIDE: the result is fp32.  PER: scales of 64 k's (groups of 32: two) */
-template <class T, bool WIDE, int PER>
+/* WIDE: the result is fp32.  PER: scales of 64 k's (groups of 32: two).  MANY: more tiles than clusters, each cluster's one behind the other (then a cluster is a pair) */
+template <class T, bool WIDE, int PER, bool MANY>
 __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x, const many_args f) {
     extern __shared__ uint8_t s_raw[];
     using W = warps_of<WIDE>;
-    constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kRun = 8 /* WIDE: steps of a sum */;
+    constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kRun = type<T>::code == HY3A_BF16 ? 8 : 4 /* WIDE: steps of a sum */;
     const int n_steps = f.steps;
     const unsigned x_bytes_up = (f.columns * 64 + 1023) & ~1023u;          /* (half the rows of 64 k's, from 1024 to 1024) */
     const linear4_args &a = f.a;
@@ -181,16 +194,19 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 #define BAR(i) (bar0 + 8u * (unsigned)(i))
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0) /* uniform for the compiler too */, lane = tid & 31;
     const unsigned me = cluster_rank(), leader = me & ~1u, rank = me & 1u;
-    const int split = me >> 1, tile = blockIdx.x / (2 * f.splits), m_tile = tile % f.m_tiles, row0 = tile / f.m_tiles * f.columns;
+    const int split = me >> 1, clusters = gridDim.x / 2, tile0 = blockIdx.x / (2 * f.splits);        /* MANY: a pair's tiles are tile0, tile0 + clusters, .. */
     const int u0 = (int)((long long)f.units * split / f.splits), u1 = (int)((long long)f.units * (split + 1) / f.splits), steps = 2 * (u1 - u0);
-    const int m0 = m_tile * 256 + (int)rank * 128, N = f.columns, rows = min(N, a.rows - row0);
+    const int N = f.columns, end = MANY ? f.tiles : tile0 + 1;
+    const int m_first = tile0 % f.m_tiles * 256 + (int)rank * 128, row_first = tile0 / f.m_tiles * N;
+    const auto m_of = [&](int tile) { return MANY && tile != tile0 ? tile % f.m_tiles * 256 + (int)rank * 128 : m_first; };        /* the tile's first output here, and its first row */
+    const auto row_of = [&](int tile) { return MANY && tile != tile0 ? tile / f.m_tiles * N : row_first; };
 
     if (tid == 0) {
         *s_abort = 0;
         for (int i = 0; i < kUnits; i++) { mbar_init(BAR(B_CODES + i), 1); mbar_init(BAR(B_CODES_FREE + i), 8 /* two teams */); }
         for (int i = 0; i < n_steps; i++) { mbar_init(BAR(B_STEP + i), 9 /* a team of each CTA, and the bytes of x */); mbar_init(BAR(B_FREE + i), 1); }
         mbar_init(BAR(B_SUMS), 1);
-        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_RUN + i), 1); mbar_init(BAR(B_RUN_FREE + i), 16 /* eight warps of each CTA */); }
+        for (int i = 0; i < 2; i++) { mbar_init(BAR(B_RUN + i), 1); mbar_init(BAR(B_RUN_FREE + i), WIDE ? 16 : 32 /* those warps of each CTA that read sums */); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kCodes && lane < 2) {
@@ -210,8 +226,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
     pdl_wait();
 
     /* a lane's sums of output o and the n rows from c0 on: stored, or left in shared memory where other CTAs have more of them */
-    const auto put = [&](float (&y)[16], int c0, int n, int r, int o) {
-        if (f.splits > 1) {
+    const auto put = [&](float (&y)[16], int c0, int n, int r, int o, int row0) {
+        if (!MANY && f.splits > 1) {
 #pragma unroll
             for (int j = 0; j < 16; j++) if (j < n) *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = y[j];
         } else {
@@ -226,24 +242,32 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         int unit = 0;
         unsigned ph = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < end && ok; tile = MANY ? tile + clusters : end) {
+            const int m0 = m_of(tile);
 #pragma unroll 1
-        for (int u = u0; u < u1; u++) {
-            if (!mbar_wait(BAR(B_CODES_FREE + unit), ph ^ 1u, s_abort, g_err, 50u)) break;
-            if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
-            tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), u * (kUnit / 2), m0, policy, lead);
-            if (++unit == kUnits) { unit = 0; ph ^= 1u; }
+            for (int u = u0; u < u1; u++) {
+                if (!(ok = mbar_wait(BAR(B_CODES_FREE + unit), ph ^ 1u, s_abort, g_err, 50u))) break;
+                if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
+                tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), u * (kUnit / 2), m0, policy, lead);
+                if (++unit == kUnits) { unit = 0; ph ^= 1u; }
+            }
         }
     } else if (warp == kRowsOfX) {
         /* ===================== producer of x ===================== */
         const unsigned lead = elect_one();
         int st = 0;
         unsigned ph = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < end && ok; tile = MANY ? tile + clusters : end) {
+            const int first = row_of(tile) + (int)rank * (N >> 1);
 #pragma unroll 1
-        for (int s = 0; s < steps; s++) {
-            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u)) break;
-            if (lead && rank == 0) mbar_expect_tx(BAR(B_STEP + st), N * 128);
-            tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, row0 + (int)rank * (N >> 1), lead);
-            if (++st == n_steps) { st = 0; ph ^= 1u; }
+            for (int s = 0; s < steps; s++) {
+                if (!(ok = mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
+                if (lead && rank == 0) mbar_expect_tx(BAR(B_STEP + st), N * 128);
+                tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, first, lead);
+                if (++st == n_steps) { st = 0; ph ^= 1u; }
+            }
         }
         /* the last commits reach the barriers of both CTAs before either leaves */
         for (int i = 0; i < n_steps && !*s_abort; i++) {
@@ -260,6 +284,10 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             int st = 0, buf = 0;
             unsigned ph = 0, rph = 0, seen = 0;
             bool ok = true;
+            int turn = 0;
+            for (int tile = tile0; tile < end && ok; tile = MANY ? tile + clusters : end, turn++) {
+            /* (the sums of the tile before have been read) */
+            if (MANY && !WIDE && turn && !(ok = all_wait(0, BAR(B_RUN_FREE), (turn - 1) & 1, s_abort, 58u))) break;
             for (int s = 0; s < steps; s++) {
                 if (!(ok = all_wait(seen, BAR(B_STEP + st), ph, s_abort, 53u))) break;
                 const int next = st + 1 == n_steps ? 0 : st + 1;
@@ -289,48 +317,72 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 ph = next_ph;
             }
             if (!WIDE && ok) umma_commit_lead(BAR(B_SUMS), both, lead);
+            }
         }
     } else if (WIDE && warp >= 4 * kTeams) {
-        /* ===================== sums of 512 k's: a lane has an output, the warp every other 16 rows ===================== */
+        /* ===================== sums of kRun steps: a lane has an output, the warp every other 16 rows ===================== */
         const int quarter = warp & 3, half = (warp >> 2) & 1, r = quarter * 32 + lane, runs = (steps + kRun - 1) / kRun;
         float acc[4][16];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int k = 0; k < 16; k++) acc[i][k] = 0.f;
         bool ok = true;
+        int buf = 0;
+        unsigned rph = 0;
 #pragma unroll 1
-        for (int run = 0; run < runs; run++) {
-            const int buf = run & 1;
-            if (!(ok = mbar_wait(BAR(B_RUN + buf), (run >> 1) & 1, s_abort, g_err, 60u))) break;
-            __syncwarp();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int tile = tile0; tile < end && ok; tile = MANY ? tile + clusters : end) {
+            const int row0 = row_of(tile), rows = min(N, a.rows - row0), o = m_of(tile) + r;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int c0 = (2 * i + half) * 16;
-                if (c0 >= N) break;
-                unsigned v[16];
-                tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * f.run_columns + c0, v);
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int k = 0; k < 16; k++) acc[i][k] += __uint_as_float(v[k]);
+                for (int k = 0; k < 16; k++) acc[i][k] = 0.f;
+#pragma unroll 1
+            for (int run = 0; run < runs; run++) {
+                if (!(ok = mbar_wait(BAR(B_RUN + buf), rph, s_abort, g_err, 60u))) break;
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int c0 = (2 * i + half) * 16;
+                    if (c0 >= N) break;
+                    unsigned v[16];
+                    tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * f.run_columns + c0, v);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) acc[i][k] += __uint_as_float(v[k]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE + buf), leader));
+                if (++buf == 2) { buf = 0; rph ^= 1u; }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE + buf), leader));
-        }
-        if (ok) {
+            if (!ok) break;
+            if (!MANY) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int c0 = (2 * i + half) * 16, n = min(16, rows - c0);
-                if (n <= 0) break;
+                for (int i = 0; i < 4; i++) {
+                    const int c0 = (2 * i + half) * 16;
 #pragma unroll
-                for (int k = 0; k < 16; k++) if (k < n) *reinterpret_cast<float *>(sm + ((c0 + k) * 128 + r) * 4) = acc[i][k];
+                    for (int k = 0; k < 16; k++) if (c0 + k < rows) *reinterpret_cast<float *>(sm + ((c0 + k) * 128 + r) * 4) = acc[i][k];
+                }
+            } else {
+                /* (registers are few: what is not finite is settled once all is stored) */
+                float odd = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    /* (code that is run once a tile: short) */
+                    const int c0 = (2 * i + half) * 16, n = o < a.out_width ? rows - c0 : 0;
+                    if (c0 >= rows) break;
+                    float *to = reinterpret_cast<float *>(a.out) + (size_t)(row0 + c0) * a.out_stride + o;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        odd = fmaf(acc[i][k], 0.f, odd);
+                        if (k < n) *to = acc[i][k];
+                        to += a.out_stride;
+                    }
+                }
+                if (__any_sync(0xffffffffu, !(odd == 0.f))) settle_stored<T>(a, row0, rows, half * 16, o, o < a.out_width);
             }
         }
     } else {
         /* ===================== weights: a thread has an output; each team takes every third or fourth step ===================== */
-        const int quarter = warp & 3, team = warp >> 2, r = quarter * 32 + lane, o = m0 + r;
-        const unsigned short *const scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(o, a.out_width - 1) * a.groups;
+        const int quarter = warp & 3, team = warp >> 2, r = quarter * 32 + lane;
+        const unsigned short *scales = nullptr;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
         const unsigned to_a = tmem + f.a_column + ((unsigned)(quarter * 32) << 16), from = sbase + r * (kUnit / 2), turn = (unsigned)((r >> 1) & 3);
         unsigned short sc[3][PER];
@@ -342,12 +394,12 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 if (s < steps && j < a.groups) to[i] = scales[j];
             }
         };
-        int st = team;
+        int st = team, behind = 0;         /* units of the tiles before */
         unsigned ph = 0;
         const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
             fetch(s + 2 * kTeams, ahead);
-            const int unit = (s >> 1) % kUnits;
-            if (!mbar_wait(BAR(B_CODES + unit), (s >> 1) / kUnits & 1, s_abort, g_err, 55u)) return false;
+            const int unit = (behind + (s >> 1)) % kUnits;
+            if (!mbar_wait(BAR(B_CODES + unit), (behind + (s >> 1)) / kUnits & 1, s_abort, g_err, 55u)) return false;
             uint4 c[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -381,28 +433,48 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             if (st >= n_steps) { st -= n_steps; ph ^= 1u; }
             return true;
         };
-        fetch(team, sc[0]);
-        fetch(team + kTeams, sc[1]);
+        const auto begin = [&](int tile) {
+            scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(m_of(tile) + r, a.out_width - 1) * a.groups;
+            fetch(team, sc[0]);
+            fetch(team + kTeams, sc[1]);
+        };
+        begin(tile0);
         bool ok = true;
-        for (int s = team; s < steps && ok; s += 3 * kTeams) {
-            ok = step(s, sc[0], sc[2]);
-            if (ok && s + kTeams < steps) ok = step(s + kTeams, sc[1], sc[0]);
-            if (ok && s + 2 * kTeams < steps) ok = step(s + 2 * kTeams, sc[2], sc[1]);
-        }
-        /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
-        if (!WIDE && ok && mbar_wait(BAR(B_SUMS), 0u, s_abort, g_err, 57u)) {
-            __syncwarp();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        unsigned parity = 0;
 #pragma unroll 1
-            for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
-                unsigned v[16];
-                tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
-                float y[16];
-#pragma unroll
-                for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
-                put(y, c0, min(16, rows - c0), r, o);
+        for (int tile = tile0; tile < end; tile = MANY ? tile + clusters : end) {
+            for (int s = team; s < steps && ok; s += 3 * kTeams) {
+                ok = step(s, sc[0], sc[2]);
+                if (ok && s + kTeams < steps) ok = step(s + kTeams, sc[1], sc[0]);
+                if (ok && s + 2 * kTeams < steps) ok = step(s + 2 * kTeams, sc[2], sc[1]);
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (!ok) break;
+            if (MANY && tile + clusters < end) {
+                begin(tile + clusters);
+                behind += steps >> 1;
+                st = (2 * behind + team) % n_steps;
+                ph = (2 * behind + team) / n_steps & 1;
+            }
+            /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
+            if (!WIDE) {
+                const int row0 = row_of(tile), rows = min(N, a.rows - row0), o = m_of(tile) + r;
+                if (!mbar_wait(BAR(B_SUMS), parity, s_abort, g_err, 57u)) break;
+                parity ^= 1u;
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {
+                    unsigned v[16];
+                    tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
+                    float y[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
+                    put(y, c0, min(16, rows - c0), r, o, row0);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (MANY && lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE), leader));
+            }
         }
     }
     __syncwarp();
@@ -413,7 +485,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
     const auto add_up = [&](const auto &value) {
         if (warp >= 16 || *s_abort) return;
         constexpr int kAtOnce = 4;
-        const int r = tid & 127, o = m0 + r, first = rows * split / f.splits, last = rows * (split + 1) / f.splits;
+        const int r = tid & 127, o = m_of(tile0) + r, row0 = row_of(tile0), rows = min(N, a.rows - row0), first = rows * split / f.splits, last = rows * (split + 1) / f.splits;        /* (such clusters have one tile) */
 #pragma unroll 1
         for (int c = first + kAtOnce * (tid >> 7); c < last; c += kAtOnce * 4) {
             float y[kAtOnce] = {};
@@ -432,9 +504,9 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         }
         __syncwarp();
     };
-    if (WIDE && f.splits == 1) add_up([&](int, int at) { return *reinterpret_cast<const float *>(sm + at); });
+    if (!MANY && WIDE && f.splits == 1) add_up([&](int, int at) { return *reinterpret_cast<const float *>(sm + at); });
     cluster_sync();
-    if (f.splits > 1) {
+    if (!MANY && f.splits > 1) {
         add_up([&](int i, int at) {
             float v;
             asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(sbase + at, 2 * i + rank)) : "memory");
@@ -447,11 +519,11 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 #undef BAR
 }
 
-template <class T, bool WIDE, int PER>
-cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int tiles, void *stream) {
-    hy3a_launch l(dim3((unsigned)tiles * 2 * f.splits), dim3(warps_of<WIDE>::kThreads), kSmem, stream);
+template <class T, bool WIDE, int PER, bool MANY>
+cudaError_t launch(const CUtensorMap &codes, const CUtensorMap &x, const many_args &f, int clusters, void *stream) {
+    hy3a_launch l(dim3((unsigned)clusters * 2 * f.splits), dim3(warps_of<WIDE>::kThreads), kSmem, stream);
     l.cluster(2 * f.splits);
-    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_umma_kernel<T, WIDE, PER>, codes, x, f);
+    return cudaLaunchKernelEx(&l.cfg, hy3a_linear4_umma_kernel<T, WIDE, PER, MANY>, codes, x, f);
 }
 /* Allows the shared memory, once per device, and tells how many clusters of 2 n CTAs fit on it at once, n = 1 .. kMostSplits (74, 33, 22 or so and 15: clusters stay within a part of the GPU). */
 template <class T, bool WIDE, int PER>
@@ -460,19 +532,21 @@ cudaError_t ready(int device, int (&fit)[kMostSplits]) {
     for (int n = 0; n < kMostSplits; n++) {
         fit[n] = device < 64 ? known[device][n].load(std::memory_order_acquire) : 0;
         if (fit[n]) continue;
-        cudaError_t e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        cudaError_t e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(hy3a_linear4_umma_kernel<T, WIDE, PER, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return e;
         hy3a_launch l(dim3(2 * (n + 1)), dim3(warps_of<WIDE>::kThreads), kSmem, nullptr);
         l.cluster(2 * (n + 1));
-        if ((e = cudaOccupancyMaxActiveClusters(&fit[n], hy3a_linear4_umma_kernel<T, WIDE, PER>, &l.cfg)) != cudaSuccess) return e;
+        if ((e = cudaOccupancyMaxActiveClusters(&fit[n], hy3a_linear4_umma_kernel<T, WIDE, PER, false>, &l.cfg)) != cudaSuccess) return e;
         if (fit[n] < 1) fit[n] = 1;
         if (device < 64) known[device][n].store(fit[n], std::memory_order_release);
     }
     return cudaSuccess;
 }
 
-/* Rows of a tile and CTAs that share a tile's k's: what takes the least by rounds * (steps of a CTA * a step + what a tile costs besides), in 10 ns, measured over 9 to 2048 rows: a step takes 160 + 0.6 N ns with N
- * rows (fp32 results 220 + 0.9 N), a tile 6.5 us besides (8.5; 1.5 more where CTAs share). */
+/* Rows of a tile and CTAs that share a tile's k's: what takes the least, in 10 ns, measured over 9 to 2048 rows: a step takes 160 + 0.6 N ns with N rows (fp32 results 220 + 0.9 N), a launch 6.5 us besides
+ * (8.5; 1.5 more where CTAs share).  Pairs that have several tiles begin the next one's copies, and with fp32 results its products too, before the last one's results are stored: 2 us a tile (2698 rows on
+ * 16942 x 448 in fp32 98 us, and 249 with a launch's start and end for each; 2048 on 4096 x 8192 in bf16 99.7 and 102.3). */
 template <class T, bool WIDE, int PER>
 cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
     int fit[kMostSplits];
@@ -486,7 +560,8 @@ cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, c
         const long long all = (long long)((a.rows + columns - 1) / columns) * f.m_tiles;
         for (int splits = 1; splits <= kMostSplits && splits <= f.units; splits++) {
             const int steps = 2 * ((f.units + splits - 1) / splits);
-            const double cost = (double)((all + fit[splits - 1] - 1) / fit[splits - 1]) * (steps * (WIDE ? 22. + 0.09 * columns : 16. + 0.06 * columns) + (WIDE ? 850. : 650.) + (splits > 1 ? 150. : 0.));
+            const double rounds = (double)((all + fit[splits - 1] - 1) / fit[splits - 1]), once = WIDE ? 850. : 650., step = WIDE ? 22. + 0.09 * columns : 16. + 0.06 * columns;
+            const double cost = splits == 1 ? rounds * (steps * step + 200.) + once - 200. : rounds * (steps * step + once + 150.);
             if (least < 0. || cost < least) { least = cost; tiles = all; f.columns = columns; f.splits = splits; }
         }
     }
@@ -506,7 +581,8 @@ cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, c
                     encode(&x, 2, a.x, a.width, a.rows, 1, a.x_stride, 64, f.columns / 2);
     if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
     if (tiles * 2 * f.splits > 0x7fffffffll) { *what = "too many tiles"; return cudaErrorInvalidValue; }
-    return launch<T, WIDE, PER>(codes, x, f, (int)tiles, stream);
+    f.tiles = (int)tiles;
+    return f.splits == 1 && tiles > fit[0] ? launch<T, WIDE, PER, true>(codes, x, f, fit[0], stream) : launch<T, WIDE, PER, false>(codes, x, f, (int)tiles, stream);
 }
 template <class T>
 cudaError_t run_type(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
@@ -517,7 +593,7 @@ cudaError_t run_type(const linear4_args &a, many_args &f, int device, void *stre
 } /* namespace */
 
 cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, void *stream, const char **what) {
-    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
+    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, 0, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
     *what = NULL;
     return dtype == HY3A_BF16 ? run_type<__nv_bfloat16>(a, f, device, stream, what) : run_type<__half>(a, f, device, stream, what);
 }

@@ -4,7 +4,7 @@ With A = sum of |weight| |x| over an element's products, and half a step of the 
   up to 16 rows:
     8 steps of a group's sum on the tensor cores, 2^-22 of it each: 2^-19 A; the groups' sums in fp32, one after the other and where warps or blocks meet: (groups + 20) 2^-24 A;
   more rows, results in fp32 (weights as two numbers that are exact together):
-    64 steps of the sum over 512 k's, 2^-22 of it each: 2^-16 A; these sums in fp32: (width / 512 + 20) 2^-24 A;
+    64 steps of the sum over 512 k's, 2^-22 of it each (half as many of fp16's 256): 2^-16 A; these sums in fp32: (width / 512 + 20) 2^-24 A (fp16: at most 256 sums, within the first term's room);
   more rows, results of the rows' type:
     a rounding of the weights, 2^-8 A (bf16) or 2^-11 A (fp16); a step of the sum for 16 products, 2^-22 of it each: (width / 16 + 20) 2^-22 A.
 """
@@ -54,7 +54,8 @@ def check(got, x, codes, scales, group):
 SIZES = [(1, 32, 1, 32), (1, 32, 16, 64), (1, 4096, 1024, 64), (2, 96, 17, 32), (3, 160, 300, 128), (5, 1056, 1001, 32), (7, 8192, 296, 128), (8, 4128, 333, 64), (8, 12288, 100, 32), (4, 8224, 2500, 128),
          (9, 512, 264, 64), (16, 2048, 520, 128), (17, 96, 31, 32), (33, 1056, 1001, 128), (64, 4096, 640, 64), (100, 8192, 129, 32), (128, 256, 128, 64), (257, 1056, 515, 64),
          (300, 4096, 256, 128), (1000, 160, 24, 32), (2049, 544, 300, 64), (1, 65536, 150, 128), (130, 16384, 72, 32),
-         (1, 256, 15000, 32), (1, 1056, 14400, 64), (1, 4096, 16001, 128), (1, 8192, 15001, 64), (1, 8192, 15000, 32), (1, 12288, 15000, 64), (64, 4096, 5000, 64), (16, 4096, 20000, 128), (15, 8192, 50, 64)]
+         (1, 256, 15000, 32), (1, 1056, 14400, 64), (1, 4096, 16001, 128), (1, 8192, 15001, 64), (1, 8192, 15000, 32), (1, 12288, 15000, 64), (64, 4096, 5000, 64), (16, 4096, 20000, 128), (15, 8192, 50, 64),
+         (17, 96, 20001, 32), (40, 2048, 30000, 128), (600, 288, 10000, 64), (2100, 448, 3001, 32), (300, 4128, 10003, 64), (129, 1024, 19500, 32), (3, 8224, 2500, 32), (12, 4064, 3000, 64), (2, 672, 9, 32)]
 
 
 @pytest.mark.parametrize("dtype,result", [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16"), ("float16", "float32")])
