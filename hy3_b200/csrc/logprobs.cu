@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kShared ? 1 : 1024 / kTh
     constexpr bool kCluster = kThreads == kShared;
     __shared__ part s_part[kWarps], s_all[kMaxCluster];
     __shared__ float s_max, s_log;
-    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_lanes[TOP && kCluster ? kMaxCluster : 1][32], s_list[TOP ? kList : 1];
+    __shared__ unsigned long long s_key[TOP ? kThreads : 1], s_lanes[TOP && kCluster ? kMaxCluster : 1][32];
+    __shared__ __align__(16) unsigned long long s_list[TOP ? kList : 2];
     __shared__ unsigned s_listed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cluster = kCluster ? a.cluster : 1, me = kCluster ? (int)cluster_rank() : 0, row = kCluster ? blockIdx.x / cluster : blockIdx.x;
     pdl_release();
@@ -289,15 +290,21 @@ __global__ void __launch_bounds__(kThreads, kThreads == kShared ? 1 : 1024 / kTh
         unsigned long long key = s_key[lane];
 #pragma unroll
         for (int w = 1; w < kWarps; w++) { const unsigned long long other = s_key[32 * w + lane]; key = other > key ? other : key; }
-        if (!kCluster) s_lanes[0][lane] = key;
+        /* (the block's threshold, or what the cluster's blocks find it from each) */
+        if (!kCluster) {
+            key = kth_largest(key, a.top_k);
+            if (lane == 0) s_lanes[0][0] = key;
+        }
         else for (int c = 0; c < cluster; c++) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer(&s_lanes[me][lane], c)), "l"(key) : "memory");
     }
     meet(cluster);
     if (TOP) {
         /* the largest of each lane's threads, in all blocks; every warp finds the k-th of them (0: fewer are open) */
-        unsigned long long key = s_lanes[0][lane];
-        if (kCluster) for (int c = 1; c < cluster; c++) key = s_lanes[c][lane] > key ? s_lanes[c][lane] : key;
-        key = kth_largest(key, a.top_k);
+        unsigned long long key = s_lanes[0][kCluster ? lane : 0];
+        if (kCluster) {
+            for (int c = 1; c < cluster; c++) key = s_lanes[c][lane] > key ? s_lanes[c][lane] : key;
+            key = kth_largest(key, a.top_k);
+        }
         const float least = closed(key) ? -INFINITY : value_of(key);
         const int least_at = closed(key) ? -1 : (int)(0xffffffffu - (unsigned)key);
         const auto reaches = [&](float l, int i) { return l > least || (l == least && i <= least_at); };
@@ -381,7 +388,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kShared ? 1 : 1024 / kTh
         for (unsigned i = tid; i < n; i += kThreads) {
             const unsigned long long key = s_list[i];
             int rank = 0;
-            for (unsigned j = 0; j < n; j++) rank += s_list[j] > key;
+            unsigned j = 0;
+            for (; j + 4 <= n; j += 4) {
+                const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(s_list + j), q = *reinterpret_cast<const ulonglong2 *>(s_list + j + 2);
+                rank += (p.x > key) + (p.y > key) + (q.x > key) + (q.y > key);
+            }
+            for (; j < n; j++) rank += s_list[j] > key;
             if (rank < a.top_k) put(rank, key);
         }
         for (int i = (int)n + tid; i < a.top_k; i += kThreads) put(i, 0);
