@@ -77,7 +77,7 @@ def make(rows, vocab, dtype="float32", asked=1, closed=0.0, seed=0, scale=3.0, d
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("rows,vocab,top_k", [(1, 1, 1), (1, 2, 2), (3, 5, 3), (2, 33, 32), (7, 100, 0), (1, 1000, 20), (5, 4099, 5), (1, 32003, 1), (1, 120832, 20), (2, 151936, 32), (40, 32003, 5), (100, 9001, 32),
                                               (150, 16385, 1), (333, 32003, 20), (700, 129, 8), (33, 120832, 0),
-                                              (1, 2049, 3), (60, 4001, 7), (700, 4096, 20), (1500, 2051, 32), (900, 8191, 1), (160, 60001, 32), (20, 250001, 16)])
+                                              (1, 2049, 3), (60, 4001, 7), (700, 4096, 20), (1500, 2051, 32), (900, 8191, 1), (160, 60001, 32), (20, 250001, 16), (200, 9001, 32), (700, 20001, 31), (1000, 77, 30), (300, 40, 32)])
 def test_sizes(cuda, rows, vocab, top_k, dtype):
     check(*make(rows, vocab, dtype, asked=3), top_k)
 
