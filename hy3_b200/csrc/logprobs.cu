@@ -23,7 +23,7 @@ namespace {
 
 using namespace hy3a_layer;
 
-/* Threads of a block: four blocks an SM where there are more rows than SMs, so that one's end runs beside the others' loads; else one, and the blocks of a cluster for a row where rows
+/* Threads of a block: 64 where a row is a round or two of their loads, else four blocks an SM where there are more rows than SMs, so that one's end runs beside the others' loads; else one, and the blocks of a cluster for a row where rows
  * are fewer still: 131072 fp32 logits are one round of loads for 8 of them. */
 constexpr int kSmall = 64, kAlone = 256, kShared = 512, kMaxCluster = 8;
 constexpr int kMaxTopK = 32, kMaxVocab = 1 << 24, kMaxAsked = 1024, kMaxRows = 1 << 27, kList = 1024 /* logits that can be ranked */;
