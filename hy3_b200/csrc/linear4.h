@@ -93,15 +93,24 @@ template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, i
 }
 /* out[t][o] from the definition, by a warp */
 template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {
-    const int lane = threadIdx.x & 31;
-    const T *const x = reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride, *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
-    const uint8_t *const codes = a.codes + (size_t)o * (a.width / 2);
+    const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride), *const codes = reinterpret_cast<const uint4 *>(a.codes + (size_t)o * (a.width / 2));
+    const T *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
     float sum = 0.f;
-    for (int k = 2 * lane; k < a.width; k += 64) {
-        const int both = codes[k >> 1];
-        const float s = type<T>::up(scales[k / a.group]);
-        sum = fmaf((float)((both & 15) - 8) * s, type<T>::up(x[k]), sum);
-        sum = fmaf((float)((both >> 4) - 8) * s, type<T>::up(x[k + 1]), sum);
+#pragma unroll 1
+    for (int i = threadIdx.x & 31; i < a.width / 32; i += 32) {         /* 32 k's, of one group */
+        const uint4 c = codes[i];
+        const unsigned w[4] = {c.x, c.y, c.z, c.w};
+        const float s = type<T>::up(scales[i * 32 / a.group]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint4 v = x[4 * i + j];
+            const unsigned pairs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const unsigned short u = (unsigned short)(k % 2 ? pairs[k / 2] >> 16 : pairs[k / 2]);
+                sum = fmaf((float)((int)(w[j] >> (4 * k) & 15u) - 8) * s, type<T>::up(*reinterpret_cast<const T *>(&u)), sum);
+            }
+        }
     }
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);

@@ -34,6 +34,24 @@ def test_rows_that_nobody_wrote(cuda, rows, out, result):
         assert bool(((got[rest].double() - y).abs() <= bound(y, a, x, scales, result)).all())
 
 
+@pytest.mark.parametrize("result", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows", [1, 16, 40])
+def test_nothing_finite_in_long_rows(cuda, rows, result):
+    """An infinity in every row, so that every result is computed again: this ends well within the bound of what waits for it meanwhile."""
+    import torch
+    import hy3_b200
+    gen = torch.Generator(device=cuda).manual_seed(rows)
+    width, out = (4096 if rows == 1 else 65536), 20000
+    codes = torch.randint(0, 256, (out, width // 2), device=cuda, generator=gen, dtype=torch.uint8)
+    scales = torch.randn((out, width // 64), device=cuda, generator=gen).bfloat16()
+    x = torch.randn((rows, width), device=cuda, generator=gen).bfloat16()
+    x[:, 64] = float("inf")
+    got = hy3_b200.linear4(x, codes, scales, out_dtype=getattr(torch, result))
+    hy3_b200.layer_sync()
+    sign = (((codes[:, 32] & 15).double() - 8) * scales[:, 1].double()).sign()
+    assert bool((got[:, sign != 0].double() == (sign * float("inf"))[sign != 0]).all()) and bool(torch.isnan(got[:, sign == 0]).all())
+
+
 @pytest.mark.parametrize("rows", [3, 16, 40])
 def test_one_row_for_all_and_rows_far_apart(cuda, rows):
     """x expanded from one row; rows of x and of the result further apart than 2^32 bytes allow in 32 bits."""
