@@ -26,6 +26,7 @@
 #include <atomic>
 
 #include "linear4.h"
+#include "linear4_plan.h"
 #include "ring.cuh"
 
 namespace {
@@ -34,17 +35,17 @@ using namespace hy3a_layer;
 using namespace hy3a_ring;
 
 constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
-constexpr int kMostSplits = 4;
-constexpr int kMostSteps = 12 /* of x and A: as tensor memory has room for A beside the sums, and shared memory for x */, kXBytes = 8 * kStepBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
+constexpr int kMostSplits = kLinear4Splits, kMostSteps = kLinear4Steps, kXBytes = kLinear4XBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
 enum { B_CODES = 0, B_CODES_FREE = kUnits, B_STEP = 2 * kUnits /* x and A of a step are there */, B_FREE = 2 * kUnits + kMostSteps, B_SUMS = 2 * kUnits + 2 * kMostSteps, B_RUN, B_RUN_FREE = B_RUN + 2, B_COUNT = B_RUN_FREE + 2 };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
+static_assert(kXBytes == 8 * kStepBytes, "stages of 256 rows");
 static_assert(128 * 256 * 4 <= kOffBar, "sums of a tile");
 
 __device__ unsigned g_err[2];         /* {code, where} of the first wait that ran out, until hy3a_layer_sync reads it */
 
 struct many_args {
     linear4_args a;
-    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 16 */, m_tiles, tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before */, run_columns /* fp32 results: columns of each of two sums */;
+    int odd_out /* pairs of 16-bit results do not lie on 4-byte boundaries */, columns /* rows of a tile, a multiple of 32 */, m_tiles, tiles, units /* of 128 k's */, splits, steps /* stages of x and A */, a_column /* where those of A begin in tensor memory; the sums lie before, for fp32 results two of them */;
 };
 
 __device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
     using W = warps_of<WIDE>;
     constexpr int kAWide = WIDE ? 64 : 32 /* columns of a stage of A */, kTeams = W::kTeams, kCodes = W::kCodes, kRowsOfX = W::kRowsOfX, kIssuer = W::kIssuer, kRun = type<T>::code == HY3A_BF16 ? 8 : 4 /* WIDE: steps of a sum */;
     const int n_steps = f.steps;
-    const unsigned x_bytes_up = (f.columns * 64 + 1023) & ~1023u;          /* (half the rows of 64 k's, from 1024 to 1024) */
+    const unsigned x_bytes = f.columns * 64;          /* half the rows of 64 k's, a multiple of 1024 */
     const linear4_args &a = f.a;
     uint8_t *sm = s_raw + ((1024u - (smem_u32(s_raw) & 1023u)) & 1023u);
     const unsigned sbase = smem_u32(sm), bar0 = sbase + kOffBar;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             for (int s = 0; s < steps; s++) {
                 if (!(ok = mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
                 if (lead && rank == 0) mbar_expect_tx(BAR(B_STEP + st), N * 128);
-                tma_rows(sbase + kOffX + st * x_bytes_up, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, first, lead);
+                tma_rows(sbase + kOffX + st * x_bytes, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, first, lead);
                 if (++st == n_steps) { st = 0; ph ^= 1u; }
             }
         }
@@ -294,14 +295,14 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 const unsigned next_ph = next ? ph : ph ^ 1u;
                 seen = peek(BAR(B_STEP + next), next_ph);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned long long db = make_desc(sbase + kOffX + st * x_bytes_up);
+                const unsigned long long db = make_desc(sbase + kOffX + st * x_bytes);
                 const unsigned da = tmem + f.a_column + st * kAWide;
                 const bool begins = WIDE ? s % kRun == 0 : s == 0;
                 if (WIDE && begins) {
                     if (!(ok = all_wait(0, BAR(B_RUN_FREE + buf), rph ^ 1u, s_abort, 59u))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 }
-                const unsigned d = tmem + (WIDE ? buf * f.run_columns : 0);
+                const unsigned d = tmem + (WIDE ? buf * N : 0);
 #pragma unroll
                 for (int k = 0; k < 4; k++) umma_lead(d, da + 8 * k, db + 2 * k, idesc, !begins || k > 0, lead);
                 if (WIDE) {
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                     const int c0 = (2 * i + half) * 16;
                     if (c0 >= N) break;
                     unsigned v[16];
-                    tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * f.run_columns + c0, v);
+                    tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + buf * N + c0, v);
 #pragma unroll
                     for (int k = 0; k < 16; k++) acc[i][k] += __uint_as_float(v[k]);
                 }
@@ -544,34 +545,13 @@ cudaError_t ready(int device, int (&fit)[kMostSplits]) {
     return cudaSuccess;
 }
 
-/* Rows of a tile and CTAs that share a tile's k's: what takes the least, in 10 ns, measured over 9 to 2048 rows: a step takes 160 + 0.6 N ns with N rows (fp32 results 220 + 0.9 N), a launch 6.5 us besides
- * (8.5; 1.5 more where CTAs share).  Pairs that have several tiles begin the next one's copies, and with fp32 results its products too, before the last one's results are stored: 2 us a tile (2698 rows on
- * 16942 x 448 in fp32 98 us, and 249 with a launch's start and end for each; 2048 on 4096 x 8192 in bf16 99.7 and 102.3). */
 template <class T, bool WIDE, int PER>
 cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
     int fit[kMostSplits];
     cudaError_t e = ready<T, WIDE, PER>(device, fit);
     if (e != cudaSuccess) return e;
-    const int most = WIDE ? 128 : 256, least_tiles = (a.rows + most - 1) / most;
-    double least = -1.;
-    long long tiles = 0;
-    for (int n = least_tiles; n <= least_tiles + 4; n++) {
-        const int columns = ((a.rows + n - 1) / n + 15) & ~15;
-        const long long all = (long long)((a.rows + columns - 1) / columns) * f.m_tiles;
-        for (int splits = 1; splits <= kMostSplits && splits <= f.units; splits++) {
-            const int steps = 2 * ((f.units + splits - 1) / splits);
-            const double rounds = (double)((all + fit[splits - 1] - 1) / fit[splits - 1]), once = WIDE ? 850. : 650., step = WIDE ? 22. + 0.09 * columns : 16. + 0.06 * columns;
-            const double cost = splits == 1 ? rounds * (steps * step + 200.) + once - 200. : rounds * (steps * step + once + 150.);
-            if (least < 0. || cost < least) { least = cost; tiles = all; f.columns = columns; f.splits = splits; }
-        }
-    }
-    const int stage = WIDE ? 64 : 32;
-    f.run_columns = (f.columns + 31) & ~31;
-    f.steps = (512 - (WIDE ? 2 * f.run_columns : f.columns)) / stage;
-    const int room = kXBytes / ((f.columns * 64 + 1023) & ~1023);
-    if (f.steps > room) f.steps = room;
-    if (f.steps > kMostSteps) f.steps = kMostSteps;
-    f.a_column = 512 - f.steps * stage;
+    const linear4_plan p = linear4_plan_of(a.rows, f.m_tiles, f.units, WIDE, fit);
+    f.columns = p.columns; f.splits = p.splits; f.steps = p.steps; f.a_column = p.a_column;
     CUtensorMap codes, x;
     const encode_tiled_fn enc = encoder();
     const cuuint64_t dims[2] = {(cuuint64_t)(a.width / 2), (cuuint64_t)a.out_width}, strides[1] = {(cuuint64_t)(a.width / 2)};
@@ -580,9 +560,9 @@ cudaError_t run(const linear4_args &a, many_args &f, int device, void *stream, c
                                CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS &&
                     encode(&x, 2, a.x, a.width, a.rows, 1, a.x_stride, 64, f.columns / 2);
     if (!ok) { *what = "no tensor map (cuTensorMapEncodeTiled)"; return cudaErrorInvalidValue; }
-    if (tiles * 2 * f.splits > 0x7fffffffll) { *what = "too many tiles"; return cudaErrorInvalidValue; }
-    f.tiles = (int)tiles;
-    return f.splits == 1 && tiles > fit[0] ? launch<T, WIDE, PER, true>(codes, x, f, fit[0], stream) : launch<T, WIDE, PER, false>(codes, x, f, (int)tiles, stream);
+    if (p.tiles * 2 * f.splits > 0x7fffffffll) { *what = "too many tiles"; return cudaErrorInvalidValue; }
+    f.tiles = (int)p.tiles;
+    return f.splits == 1 && p.tiles > fit[0] ? launch<T, WIDE, PER, true>(codes, x, f, fit[0], stream) : launch<T, WIDE, PER, false>(codes, x, f, f.tiles, stream);
 }
 template <class T>
 cudaError_t run_type(const linear4_args &a, many_args &f, int device, void *stream, const char **what) {
@@ -593,7 +573,7 @@ cudaError_t run_type(const linear4_args &a, many_args &f, int device, void *stre
 } /* namespace */
 
 cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, void *stream, const char **what) {
-    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, 0, (a.width + kUnit - 1) / kUnit, 1, 0, 0, 0};
+    many_args f = {a, ((uintptr_t)a.out & 3) || a.out_stride % 2 || a.out_width % 2, 0, (a.out_width + 255) / 256, 0, (a.width + kUnit - 1) / kUnit, 1, 0, 0};
     *what = NULL;
     return dtype == HY3A_BF16 ? run_type<__nv_bfloat16>(a, f, device, stream, what) : run_type<__half>(a, f, device, stream, what);
 }
