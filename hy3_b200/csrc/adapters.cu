@@ -648,7 +648,7 @@ workspace layout(int rows, int width, int rank) {
 
 static __global__ void hy3a_adapters_wait_out_kernel() { wait_out(g_err, 39u); }
 cudaError_t hy3a_adapters_wait_out(void *stream) {
-    hy3a_adapters_wait_out_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
+    hy3a_adapters_wait_out_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
     return cudaGetLastError();
 }
 cudaError_t hy3a_adapters_error(unsigned *err) {

@@ -360,7 +360,7 @@ cudaError_t hy3a_experts_launch_umma(const expert_args &a, int dtype, int device
 
 static __global__ void hy3a_experts_wait_out_kernel() { wait_out(g_err, 29u); }
 cudaError_t hy3a_experts_wait_out(void *stream) {
-    hy3a_experts_wait_out_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
+    hy3a_experts_wait_out_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
     return cudaGetLastError();
 }
 cudaError_t hy3a_experts_error(unsigned *err) {

@@ -103,7 +103,7 @@ __device__ __forceinline__ unsigned peek(unsigned bar, unsigned parity) {
     return ok;
 }
 __device__ __forceinline__ bool all_wait(unsigned seen, unsigned bar, unsigned parity, volatile int *abort_flag, unsigned where) {
-    return __all_sync(0xffffffffu, seen) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, g_err, where));
+    return __all_sync(0xffffffffu, seen) || warp_wait(bar, parity, abort_flag, g_err, where);
 }
 template <class T> struct pair_of;
 template <> struct pair_of<__nv_bfloat16> {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             const int m0 = m_of(tile);
 #pragma unroll 1
             for (int u = u0; u < u1; u++) {
-                if (!(ok = mbar_wait(BAR(B_CODES_FREE + unit), ph ^ 1u, s_abort, g_err, 50u))) break;
+                if (!(ok = warp_wait(BAR(B_CODES_FREE + unit), ph ^ 1u, s_abort, g_err, 50u))) break;
                 if (lead) mbar_expect_tx(BAR(B_CODES + unit), kUnitBytes);
                 tma_codes(sbase + unit * kUnitBytes, &tm_codes, BAR(B_CODES + unit), u * (kUnit / 2), m0, policy, lead);
                 if (++unit == kUnits) { unit = 0; ph ^= 1u; }
@@ -264,15 +264,15 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             const int first = row_of(tile) + (int)rank * (N >> 1);
 #pragma unroll 1
             for (int s = 0; s < steps; s++) {
-                if (!(ok = mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
+                if (!(ok = warp_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 51u))) break;
                 if (lead && rank == 0) mbar_expect_tx(BAR(B_STEP + st), N * 128);
                 tma_rows(sbase + kOffX + st * x_bytes, &tm_x, cluster_addr(BAR(B_STEP + st), leader), u0 * kUnit + s * 64, first, lead);
                 if (++st == n_steps) { st = 0; ph ^= 1u; }
             }
         }
         /* the last commits reach the barriers of both CTAs before either leaves */
-        for (int i = 0; i < n_steps && !*s_abort; i++) {
-            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 52u)) break;
+        for (int i = 0; i < n_steps; i++) {
+            if (!warp_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 52u)) break;
             if (++st == n_steps) { st = 0; ph ^= 1u; }
         }
     } else if (warp == kIssuer) {
@@ -336,8 +336,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 for (int k = 0; k < 16; k++) acc[i][k] = 0.f;
 #pragma unroll 1
             for (int run = 0; run < runs; run++) {
-                if (!(ok = mbar_wait(BAR(B_RUN + buf), rph, s_abort, g_err, 60u))) break;
-                __syncwarp();
+                if (!(ok = warp_wait(BAR(B_RUN + buf), rph, s_abort, g_err, 60u))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -400,7 +399,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
             fetch(s + 2 * kTeams, ahead);
             const int unit = (behind + (s >> 1)) % kUnits;
-            if (!mbar_wait(BAR(B_CODES + unit), (behind + (s >> 1)) / kUnits & 1, s_abort, g_err, 55u)) return false;
+            if (!warp_wait(BAR(B_CODES + unit), (behind + (s >> 1)) / kUnits & 1, s_abort, g_err, 55u)) return false;
             uint4 c[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -420,8 +419,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                     if (WIDE) rest[WIDE ? 4 * i + j : 0] = pair_of<T>::rest(n[j], s2, weights[4 * i + j]);
                 }
             }
-            if (!mbar_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
-            __syncwarp();              /* (lanes may leave the wait one by one; what follows is the whole warp's) */
+            if (!warp_wait(BAR(B_FREE + st), ph ^ 1u, s_abort, g_err, 56u)) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             tmem_st32(to_a + st * kAWide, weights);
             if constexpr (WIDE) tmem_st32(to_a + st * kAWide + 32, rest);
@@ -459,9 +457,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
             if (!WIDE) {
                 const int row0 = row_of(tile), rows = min(N, a.rows - row0), o = m_of(tile) + r;
-                if (!mbar_wait(BAR(B_SUMS), parity, s_abort, g_err, 57u)) break;
+                if (!warp_wait(BAR(B_SUMS), parity, s_abort, g_err, 57u)) break;
                 parity ^= 1u;
-                __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                 for (int c0 = team * 16; c0 < rows; c0 += 16 * kTeams) {

@@ -37,13 +37,33 @@ __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatil
     if (atomicCAS(err, 0u, 2u) == 0u) err[1] = where;
     return false;
 }
-/* one wait that nothing ends (hy3a_layer_wait_out) */
+/* The same for a warp: its lanes leave the wait together and with one answer.  (Where lanes poll by themselves they may leave one by one, and one may give up where another is through; what follows is the
+ * whole warp's, products, shuffles, copies of one elected lane, and lanes that went different ways there would wait for each other for good.) */
+__device__ __forceinline__ bool warp_wait(unsigned bar, unsigned parity, volatile int *abort_flag, unsigned *err, unsigned where) {
+    constexpr unsigned kAll = 0xffffffffu;
+    if (__all_sync(kAll, mbar_try(bar, parity, 2000u))) return true;
+    unsigned long long t0, t1;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (unsigned i = 0; i < (1u << 22); i++) {
+        if (__all_sync(kAll, mbar_try(bar, parity, 20000u))) return true;
+        if (__any_sync(kAll, *abort_flag)) return false;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+        if (__any_sync(kAll, i >= (1u << 13) && t1 - t0 > 500000000ull)) break;
+    }
+    *abort_flag = 1;
+    if (atomicCAS(err, 0u, 2u) == 0u) err[1] = where;
+    return false;
+}
+/* one wait of a warp that nothing ends (hy3a_layer_wait_out), but for lane 0, which asks for a phase that is over; if the lanes' answers differed, another place is reported */
 __device__ __forceinline__ void wait_out(unsigned *err, unsigned where) {
     __shared__ alignas(8) unsigned long long s_bar;
     __shared__ int s_abort;
-    s_abort = 0;
-    mbar_init(smem_u32(&s_bar), 1);
-    mbar_wait(smem_u32(&s_bar), 0u, &s_abort, err, where);
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        mbar_init(smem_u32(&s_bar), 1);
+    }
+    __syncwarp();
+    if (warp_wait(smem_u32(&s_bar), threadIdx.x == 0, &s_abort, err, where)) err[1] = where + 100u;
 }
 __device__ __forceinline__ unsigned elect_one() {
     unsigned p;
