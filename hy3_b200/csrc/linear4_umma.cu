@@ -34,7 +34,7 @@ namespace {
 using namespace hy3a_layer;
 using namespace hy3a_ring;
 
-constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = 8 /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
+constexpr int kUnit = 128 /* k's of a copy of codes */, kUnits = kLinear4Units /* in the ring */, kUnitBytes = 128 * kUnit / 2, kStepBytes = 128 * 128 /* x of 64 k's, at most 128 rows a CTA */;
 constexpr int kMostSplits = kLinear4Splits, kMostSteps = kLinear4Steps, kXBytes = kLinear4XBytes, kOffX = kUnits * kUnitBytes, kOffBar = kOffX + kXBytes, kSmem = kOffBar + 512 + 1024;
 enum { B_CODES = 0, B_CODES_FREE = kUnits, B_STEP = 2 * kUnits /* x and A of a step are there */, B_FREE = 2 * kUnits + kMostSteps, B_SUMS = 2 * kUnits + 2 * kMostSteps, B_RUN, B_RUN_FREE = B_RUN + 2, B_COUNT = B_RUN_FREE + 2 };
 static_assert(8 * B_COUNT + 16 <= 512, "barriers");
@@ -176,7 +176,7 @@ template <class T, bool WIDE, int N> __device__ __forceinline__ void store(const
 
 /* The warps of a CTA: teams of four that make A (a warp for each 32 outputs), those that add up groups, two producers, the issuer. */
 template <bool WIDE> struct warps_of {
-    static constexpr int kTeams = WIDE ? 3 : 4, kAdders = WIDE ? 8 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
+    static constexpr int kTeams = linear4_teams(WIDE), kAdders = WIDE ? 8 : 0, kWorkers = 4 * kTeams + kAdders, kCodes = kWorkers, kRowsOfX = kWorkers + 1, kIssuer = kWorkers + 2, kThreads = 32 * (kWorkers + 3);
 };
 
 /* WIDE: the result is fp32.  PER: scales of 64 k's (groups of 32: two).  MANY: more tiles than clusters, each cluster's one behind the other (then a cluster is a pair) */
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             }
         }
     } else {
-        /* ===================== weights: a thread has an output; each team takes every third or fourth step ===================== */
+        /* ===================== weights: a thread has an output; each team takes every third or fourth step, from tile to tile too ===================== */
         const int quarter = warp & 3, team = warp >> 2, r = quarter * 32 + lane;
         const unsigned short *scales = nullptr;
         const int shift = a.group == 128 ? 7 : (a.group == 64 ? 6 : 5);
@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 if (s < steps && j < a.groups) to[i] = scales[j];
             }
         };
-        int st = team, behind = 0;         /* units of the tiles before */
+        static_assert(kTeams + kMostSteps <= 2 * kUnits, "phases of the codes that a team does not wait for");
+        int st = team, s0 = team /* the team's first step of the tile */, behind = 0;         /* units of the tiles before */
         unsigned ph = 0;
         const auto step = [&](int s, const unsigned short (&now)[PER], unsigned short (&ahead)[PER]) {
             fetch(s + 2 * kTeams, ahead);
@@ -434,25 +435,24 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         };
         const auto begin = [&](int tile) {
             scales = reinterpret_cast<const unsigned short *>(a.scales) + (size_t)min(m_of(tile) + r, a.out_width - 1) * a.groups;
-            fetch(team, sc[0]);
-            fetch(team + kTeams, sc[1]);
+            fetch(s0, sc[0]);
+            fetch(s0 + kTeams, sc[1]);
         };
         begin(tile0);
         bool ok = true;
         unsigned parity = 0;
 #pragma unroll 1
         for (int tile = tile0; tile < end; tile = MANY ? tile + clusters : end) {
-            for (int s = team; s < steps && ok; s += 3 * kTeams) {
+            for (int s = s0; s < steps && ok; s += 3 * kTeams) {
                 ok = step(s, sc[0], sc[2]);
                 if (ok && s + kTeams < steps) ok = step(s + kTeams, sc[1], sc[0]);
                 if (ok && s + 2 * kTeams < steps) ok = step(s + 2 * kTeams, sc[2], sc[1]);
             }
             if (!ok) break;
             if (MANY && tile + clusters < end) {
+                s0 = linear4_first_step(s0, steps, kTeams);
                 begin(tile + clusters);
                 behind += steps >> 1;
-                st = (2 * behind + team) % n_steps;
-                ph = (2 * behind + team) / n_steps & 1;
             }
             /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
             if (!WIDE) {

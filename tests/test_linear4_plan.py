@@ -1,4 +1,5 @@
-"""How linear4 cuts calls of more than 16 rows into tiles (host code, compiled here; runs without a GPU): the tensor cores' shapes, all rows taken, and what is laid into tensor and shared memory in its bounds."""
+"""How linear4 cuts calls of more than 16 rows into tiles (host code, compiled here; runs without a GPU): the tensor cores' shapes, all rows taken, what is laid into tensor and shared memory in its
+bounds, and the steps of the warps that make weights."""
 import os
 import subprocess
 
@@ -13,13 +14,32 @@ int main() {
     long n = 0;
     for (int rows = 17; rows <= 1 << 24; rows += rows < 2200 ? 1 : rows / 3)
         for (int out : outs) for (int width : widths) for (const auto &fit : fits) for (int wide = 0; wide < 2; wide++) {
-            const int m_tiles = (out + 255) / 256, units = (width + 127) / 128, teams = wide ? 3 : 4;
+            const int m_tiles = (out + 255) / 256, units = (width + 127) / 128, teams = linear4_teams(wide);
             const linear4_plan p = linear4_plan_of(rows, m_tiles, units, wide, fit);
             const int sums = (wide ? 2 : 1) * p.columns;
             const bool right = p.columns % 32 == 0 && p.columns >= 32 && p.columns <= (wide ? 128 : 256)      /* N of a product of two CTAs, M = 256, A in tensor memory */
                 && p.tiles == (long long)((rows + p.columns - 1) / p.columns) * m_tiles && p.splits >= 1 && p.splits <= kLinear4Splits && p.splits <= units
                 && p.steps >= teams && p.steps <= kLinear4Steps && p.steps * p.columns * 64 <= kLinear4XBytes
                 && p.a_column >= sums && p.a_column + p.steps * linear4_a_columns(wide) == kLinear4Tmem;
+            /* the teams' steps, through seven tiles of a pair where it has several: each step is one team's, and what a team has seen over rules out that a wait is over two phases early */
+            const int steps = 2 * ((units + p.splits - 1) / p.splits), tiles = p.splits == 1 && p.tiles > fit[0] ? 7 : 1;
+            if (rows % 7 == 0 && steps < 100) {
+                static int taken[7 * 100];
+                for (int &t : taken) t = 0;
+                for (int team = 0; team < teams; team++) {
+                    int s0 = team, last = -1;
+                    for (int tile = 0; tile < tiles; tile++) {
+                        for (int s = s0; s < steps; s += teams) {
+                            const int k = tile * steps + s, gap = k - last;
+                            if (last >= 0 && (gap > p.steps || gap + p.steps > 2 * kLinear4Units)) { printf("rows %d out %d width %d wide %d: steps %d apart, %d stages\\n", rows, out, width, wide, gap, p.steps); return 1; }
+                            last = k;
+                            taken[k]++;
+                        }
+                        s0 = linear4_first_step(s0, steps, teams);
+                    }
+                }
+                for (int k = 0; k < tiles * steps; k++) if (taken[k] != 1) { printf("step %d is %d teams'\\n", k, taken[k]); return 1; }
+            }
             if (!right) { printf("rows %d out %d width %d wide %d: columns %d tiles %lld splits %d steps %d a_column %d\\n", rows, out, width, wide, p.columns, p.tiles, p.splits, p.steps, p.a_column); return 1; }
             n++;
         }
