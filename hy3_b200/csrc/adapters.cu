@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) hy3a_adapters_expand_long_ker
                     for (int j = 0; j < 32; j++) if (in && j < count) out[s_out[r0 + j]] = held[j];
                     continue;
                 }
-                if (!mbar_wait(bar0 + 8 * (A_TFULL + buf), (c >> 1) & 1, s_abort, g_err, 33u)) break;
+                if (!warp_wait(bar0 + 8 * (A_TFULL + buf), (c >> 1) & 1, s_abort, g_err, 33u)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 constexpr int STEP = 16 / PER;
 #pragma unroll

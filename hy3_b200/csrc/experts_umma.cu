@@ -128,7 +128,7 @@ __device__ __forceinline__ bool produce(ring_state &q, const CUtensorMap *tm_w, 
     unsigned st = q.st, ph = q.ph;
     for (int s = 0; s < steps; s++) {
         /* (a stage whose weights are under way has not been used before) */
-        if (s >= ahead && !mbar_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
+        if (s >= ahead && !warp_wait(bar0 + 8u * (B_EMPTY + st), ph ^ 1u, s_abort, g_err, 20u)) return false;
         const unsigned full = cluster_addr(bar0 + 8u * (B_FULL + st), 0), sa = sbase + st * (kABytes + kBBytes), sb = sa + kABytes;
         if (bytes && lead && s >= ahead) mbar_expect_tx(bar0 + 8u * (B_FULL + st), bytes);
         if (s >= ahead) tma_box(sa + part * 2048, tm_w, full, s * 64, m, e, lead);
@@ -228,8 +228,8 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         if (DOWN && pair >= total) pdl_wait();
         unsigned st = q.st, ph = q.ph;
         /* the last commits reach the barriers of both CTAs before either leaves */
-        for (int i = 0; i < kStages && !*s_abort; i++) {
-            if (!mbar_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, g_err, 24u)) break;
+        for (int i = 0; i < kStages; i++) {
+            if (!warp_wait(BAR(B_EMPTY + st), ph ^ 1u, s_abort, g_err, 24u)) break;
             if (++st == kStages) { st = 0; ph ^= 1u; }
         }
     } else if (warp == kIssuer) {
@@ -241,11 +241,11 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
             tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
             for (where w; walk.take(w);) {
                 const unsigned idesc = (1u << 4) | kType | (((unsigned)(w.n + 15) >> 4) << 18) | ((256u >> 4) << 24);
-                if (!mbar_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, g_err, 21u)) break;
+                if (!warp_wait(BAR(B_TEMPTY + buf), tph ^ 1u, s_abort, g_err, 21u)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 bool ok = true;
                 for (int s = 0; s < steps; s++) {
-                    if (!(ok = mbar_wait(BAR(B_FULL + st), ph, s_abort, g_err, 22u))) break;
+                    if (!(ok = warp_wait(BAR(B_FULL + st), ph, s_abort, g_err, 22u))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const unsigned sa = sbase + st * (kABytes + kBBytes);
                     const unsigned long long da = make_desc(sa), db = make_desc(sa + kABytes);
@@ -268,7 +268,7 @@ hy3a_experts_umma_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid
         uint8_t *patch = sm + kOffPatch + warp * kPatch;
         tile_walk<DOWN> walk(a, pair, pairs, m_tiles, total);
         for (where w; walk.take(w);) {
-            if (!mbar_wait(BAR(B_TFULL + buf), tph, s_abort, g_err, 23u)) break;
+            if (!warp_wait(BAR(B_TFULL + buf), tph, s_abort, g_err, 23u)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int m0 = DOWN ? w.m0 + (int)rank * 128 + quarter * 32 : w.m0 + (int)rank * 64 + quarter * 16;
             for (int c0 = (warp >> 2) * 16; c0 < w.n; c0 += 32) {

@@ -7,7 +7,7 @@ import pytest
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hy3_b200", "csrc")
 
 
-@pytest.mark.parametrize("file", ["linear4.cu", "linear4_umma.cu"])
+@pytest.mark.parametrize("file", ["linear4.cu", "linear4_umma.cu", "experts_umma.cu"])
 def test_no_lane_waits_by_itself(file):
     with open(os.path.join(CSRC, file)) as f:
         text = f.read()
@@ -15,6 +15,13 @@ def test_no_lane_waits_by_itself(file):
     assert not re.findall(r"\bmbar_(?:wait|try)\(", text.replace("__all_sync(0xffffffffu, mbar_wait(", ""))
     # nor does a warp's loop end by what its lanes read of the abort flag one by one
     assert not re.findall(r"for \([^;]*;[^;]*\*s_abort", text)
+
+
+def test_adapters():
+    """Its copies and products are one lane's, which waits alone; the warps that store results wait as warps."""
+    with open(os.path.join(CSRC, "adapters.cu")) as f:
+        text = f.read()
+    assert re.findall(r"\b(mbar|warp)_wait\([^;]*A_(\w+) \+", text) == [("mbar", "EMPTY"), ("mbar", "EMPTY"), ("mbar", "TEMPTY"), ("mbar", "FULL"), ("warp", "TFULL")]
 
 
 @pytest.mark.gpu
