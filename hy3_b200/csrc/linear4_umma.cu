@@ -10,7 +10,7 @@
  *   1          MMA issuer (of the leader): 4 x tcgen05.mma (K = 16) a step, fp32 results 8.
  *
  * Results of the rows' type: a weight, of up to 15 bits (fp16) or 11 (bf16), is rounded to that type once, which leaves an error like the result's own rounding.  Results that are not finite (of weights
- * rounded beyond the type's largest, of an infinite x that meets the rest) are computed again from the definition, by the warp that finds them.
+ * rounded beyond the type's largest, of an infinite x that meets the rest) are computed again from the definition, by the warp that finds them, at a time when no bounded wait depends on it.
  *
  * Results in fp32: a weight enters as two numbers, the rounded one and the rest, which is exact, so that there are 8 products a step; and the tensor cores begin a new sum every 512 k's (bf16; fp16: 256), which warps of their own
  * add to results in registers: the tensor cores' sums are cut off and not rounded (one sum over 4096 k's left an error of 5.6e-6 of the result; sums of 512 leave 4.6e-7, of fp16 products, whose 22 bits lose more,
@@ -24,6 +24,7 @@
  * released.
  */
 #include <atomic>
+#include <type_traits>
 
 #include "linear4.h"
 #include "linear4_plan.h"
@@ -143,15 +144,16 @@ template <class T, int N> __device__ __forceinline__ void settle(const linear4_a
         for (int k = 0; k < N; k++) if (j == k) y[k] = now;
     }
 }
-/* the same of fp32 results that have been stored: rows t + c0 .. t + c0 + 15, t + c0 + 32 .. of a tile's n */
-template <class T> __device__ __noinline__ void settle_stored(const linear4_args &a, int t, int n, int c0, int o, bool mine) {
+/* the same of results of type O that the warp has stored: rows t + c0 .. t + c0 + 15 of a tile's n, and those `step` further on and so forth.  Settling takes as long as it takes (up to a tenth of a second for a
+ * tile of 256 rows of 65536): where a pair has several tiles, it comes when nothing in the pair waits for the warp any more, as waits are bounded. */
+template <class T, class O> __device__ __noinline__ void settle_stored(const linear4_args &a, int t, int n, int c0, int step, int o, bool mine) {
 #pragma unroll 1
-    for (int j = c0; j < n; j += j % 16 == 15 ? 17 : 1) {
-        float *const at = reinterpret_cast<float *>(a.out) + (size_t)(t + j) * a.out_stride + o;
-        float y[1] = {mine ? *reinterpret_cast<volatile float *>(at) : 0.f};
+    for (int j = c0; j < n; j += j % 16 == 15 ? step - 15 : 1) {
+        O *const at = reinterpret_cast<O *>(a.out) + (size_t)(t + j) * a.out_stride + o;
+        float y[1] = {mine ? type<O>::up(*at) : 0.f};
         if (!__any_sync(0xffffffffu, !(fabsf(y[0]) < INFINITY))) continue;
         settle<T>(a, y, 1, t + j, o, mine);
-        if (mine) *at = y[0];
+        if (mine) *at = type<O>::down(y[0]);
     }
 }
 /* A lane's results of its output, row after row.  16-bit ones: neighbouring lanes exchange, so that one stores the even rows' two outputs and one the odd rows'. */
@@ -232,9 +234,17 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 #pragma unroll
             for (int j = 0; j < 16; j++) if (j < n) *reinterpret_cast<float *>(sm + ((c0 + j) * 128 + r) * 4) = y[j];
         } else {
-            settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
+            if (!MANY) settle<T>(a, y, n, row0 + c0, o, o < a.out_width);
             store<T, WIDE>(a, y, n, row0 + c0, o, f.odd_out);
         }
+    };
+    /* MANY: what a warp found not finite, if anything, once it has stored all of its results */
+    const auto settle_all = [&](bool odd, int c0, int step, int r) {
+        if (!__any_sync(0xffffffffu, odd)) return;
+        __syncwarp();                /* (neighbours have stored for each other) */
+#pragma unroll 1
+        for (int tile = tile0; tile < end; tile += clusters)
+            settle_stored<T, typename std::conditional<WIDE, float, T>::type>(a, row_of(tile), min(N, a.rows - row_of(tile)), c0, step, m_of(tile) + r, m_of(tile) + r < a.out_width);
     };
     if (warp == kCodes) {
         /* ===================== producer of codes ===================== */
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         /* ===================== sums of kRun steps: a lane has an output, the warp every other 16 rows ===================== */
         const int quarter = warp & 3, half = (warp >> 2) & 1, r = quarter * 32 + lane, runs = (steps + kRun - 1) / kRun;
         float acc[4][16];
-        bool ok = true;
+        bool ok = true, odd = false;
         int buf = 0;
         unsigned rph = 0;
 #pragma unroll 1
@@ -361,8 +371,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                     for (int k = 0; k < 16; k++) if (c0 + k < rows) *reinterpret_cast<float *>(sm + ((c0 + k) * 128 + r) * 4) = acc[i][k];
                 }
             } else {
-                /* (registers are few: what is not finite is settled once all is stored) */
-                float odd = 0.f;
+                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     /* (code that is run once a tile: short) */
@@ -371,14 +380,15 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                     float *to = reinterpret_cast<float *>(a.out) + (size_t)(row0 + c0) * a.out_stride + o;
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        odd = fmaf(acc[i][k], 0.f, odd);
+                        sum = fmaf(acc[i][k], 0.f, sum);
                         if (k < n) *to = acc[i][k];
                         to += a.out_stride;
                     }
                 }
-                if (__any_sync(0xffffffffu, !(odd == 0.f))) settle_stored<T>(a, row0, rows, half * 16, o, o < a.out_width);
+                odd |= !(sum == 0.f);
             }
         }
+        if (MANY && ok) settle_all(odd, half * 16, 32, r);
     } else {
         /* ===================== weights: a thread has an output; each team takes every third or fourth step, from tile to tile too ===================== */
         const int quarter = warp & 3, team = warp >> 2, r = quarter * 32 + lane;
@@ -439,7 +449,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             fetch(s0 + kTeams, sc[1]);
         };
         begin(tile0);
-        bool ok = true;
+        bool ok = true, odd = false;
         unsigned parity = 0;
 #pragma unroll 1
         for (int tile = tile0; tile < end; tile = MANY ? tile + clusters : end) {
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             /* ===================== results: a lane has an output, the warp every fourth 16 rows ===================== */
             if (!WIDE) {
                 const int row0 = row_of(tile), rows = min(N, a.rows - row0), o = m_of(tile) + r;
-                if (!warp_wait(BAR(B_SUMS), parity, s_abort, g_err, 57u)) break;
+                if (!(ok = warp_wait(BAR(B_SUMS), parity, s_abort, g_err, 57u))) break;
                 parity ^= 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -466,7 +476,10 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                     tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + c0, v);
                     float y[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) y[j] = __uint_as_float(v[j]);
+                    for (int j = 0; j < 16; j++) {
+                        y[j] = __uint_as_float(v[j]);
+                        if (MANY) odd |= !(fabsf(y[j]) < INFINITY);
+                    }
                     put(y, c0, min(16, rows - c0), r, o, row0);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -474,6 +487,7 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                 if (MANY && lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE), leader));
             }
         }
+        if (MANY && !WIDE && ok) settle_all(odd, team * 16, 16 * kTeams, r);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
