@@ -363,9 +363,4 @@ cudaError_t hy3a_experts_wait_out(void *stream) {
     hy3a_experts_wait_out_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
     return cudaGetLastError();
 }
-cudaError_t hy3a_experts_error(unsigned *err) {
-    const unsigned none[2] = {0, 0};
-    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
-    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
-    return e;
-}
+cudaError_t hy3a_experts_words(unsigned **words) { return cudaGetSymbolAddress((void **)words, g_err); }

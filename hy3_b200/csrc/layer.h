@@ -24,14 +24,16 @@ int hy3a_layer_device(const char *who, int *device, int *sms);
 /* Whether sizes of a matrix in 4 bits are in their limits: 0 or HY3A_EINVAL. */
 int hy3a_quant4_sizes(const char *who, int out_width, int width, int group);
 
-/* The files' error words {code, where} of the first wait that ran out on the current device; read and cleared. */
-cudaError_t hy3a_experts_error(unsigned *err);
-cudaError_t hy3a_adapters_error(unsigned *err);
-cudaError_t hy3a_linear4_error(unsigned *err);
+/* Where the files' error words {code, where} of the first wait that ran out lie on the current device (hy3a_layer_sync reads and clears them) */
+cudaError_t hy3a_experts_words(unsigned **words);
+cudaError_t hy3a_adapters_words(unsigned **words);
+cudaError_t hy3a_linear4_words(unsigned **words);
+cudaError_t hy3a_linear4_many_words(unsigned **words);
 /* a launch of the file's with one wait that runs out */
 cudaError_t hy3a_experts_wait_out(void *stream);
 cudaError_t hy3a_adapters_wait_out(void *stream);
 cudaError_t hy3a_linear4_wait_out(void *stream);
+cudaError_t hy3a_linear4_many_wait_out(void *stream);
 
 /* launch configuration with programmatic stream serialisation: the kernels wait (pdl_wait) before they touch memory */
 struct hy3a_launch {

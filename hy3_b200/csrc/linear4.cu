@@ -520,9 +520,4 @@ cudaError_t hy3a_linear4_wait_out(void *stream) {
     hy3a_linear4_wait_out_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
     return cudaGetLastError();
 }
-cudaError_t hy3a_linear4_error(unsigned *err) {
-    const unsigned none[2] = {0, 0};
-    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
-    if (e == cudaSuccess && err[0]) return cudaMemcpyToSymbol(g_err, none, sizeof(none));
-    return e == cudaSuccess ? hy3a_linear4_many_error(err) : e;
-}
+cudaError_t hy3a_linear4_words(unsigned **words) { return cudaGetSymbolAddress((void **)words, g_err); }

@@ -17,7 +17,6 @@ struct linear4_args {
 
 /* linear4_umma.cu: any number of rows; *what: why, where it is not CUDA's error */
 cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int device, void *stream, const char **what);
-cudaError_t hy3a_linear4_many_error(unsigned *err);
 
 namespace hy3a_layer {
 

@@ -589,9 +589,9 @@ cudaError_t hy3a_linear4_launch_many(const linear4_args &a, int dtype, int devic
     return dtype == HY3A_BF16 ? run_type<__nv_bfloat16>(a, f, device, stream, what) : run_type<__half>(a, f, device, stream, what);
 }
 
-cudaError_t hy3a_linear4_many_error(unsigned *err) {
-    const unsigned none[2] = {0, 0};
-    cudaError_t e = cudaMemcpyFromSymbol(err, g_err, sizeof(none));
-    if (e == cudaSuccess && err[0]) e = cudaMemcpyToSymbol(g_err, none, sizeof(none));
-    return e;
+static __global__ void hy3a_linear4_many_wait_out_kernel() { wait_out(g_err, 69u); }
+cudaError_t hy3a_linear4_many_wait_out(void *stream) {
+    hy3a_linear4_many_wait_out_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
+    return cudaGetLastError();
 }
+cudaError_t hy3a_linear4_many_words(unsigned **words) { return cudaGetSymbolAddress((void **)words, g_err); }

@@ -318,7 +318,7 @@ int hy3a_logprobs(void *stream, int dtype, int rows, int vocab, const void *logi
  * hy3a_experts, hy3a_adapters or hy3a_linear4 ran out on the current device since the last call (it then returned early, and outputs since are
  * not valid).  */
 int hy3a_layer_sync(void *stream);
-/* For checks of that report: a launch with one bounded wait of hy3a_experts (which 0), hy3a_adapters (1) or hy3a_linear4 (4) that nothing ends; it returns after half a second. */
+/* For checks of that report: a launch with one bounded wait of hy3a_experts (which 0), hy3a_adapters (1) or hy3a_linear4 (4; of its calls of more than 16 rows: 5) that nothing ends; it returns after half a second. */
 int hy3a_layer_wait_out(void *stream, int which);
 
 /* ---- introspection ------------------------------------------------------------------*/
