@@ -81,14 +81,21 @@ template <> struct steps<__half> {
 template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, int t) {
     const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride);
     constexpr unsigned kInf = type<T>::code == HY3A_BF16 ? 0x7f80u : 0x7c00u;
-    bool is = false;
-    for (int i = threadIdx.x & 31; i < a.width / 8; i += 32) {
-        const uint4 v = x[i];
-        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+    /* (rows that nobody wrote have theirs early) */
+#pragma unroll 1
+    for (int i0 = threadIdx.x & 31, n = a.width / 8; __any_sync(0xffffffffu, i0 < n); i0 += 128) {
+        bool is = false;
 #pragma unroll
-        for (int j = 0; j < 4; j++) is |= (w[j] & 0x7fffu) > kInf || (w[j] >> 16 & 0x7fffu) > kInf;
+        for (int u = 0; u < 4; u++) {
+            if (i0 + 32 * u >= n) continue;
+            const uint4 v = x[i0 + 32 * u];
+            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) is |= (w[j] & 0x7fffu) > kInf || (w[j] >> 16 & 0x7fffu) > kInf;
+        }
+        if (__any_sync(0xffffffffu, is)) return true;
     }
-    return __any_sync(0xffffffffu, is);
+    return false;
 }
 /* out[t][o] from the definition, by a warp */
 template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {

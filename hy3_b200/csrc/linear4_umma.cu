@@ -148,12 +148,17 @@ template <class T, int N> __device__ __forceinline__ void settle(const linear4_a
  * tile of 256 rows of 65536): where a pair has several tiles, it comes when nothing in the pair waits for the warp any more, as waits are bounded. */
 template <class T, class O> __device__ __noinline__ void settle_stored(const linear4_args &a, int t, int n, int c0, int step, int o, bool mine) {
 #pragma unroll 1
-    for (int j = c0; j < n; j += j % 16 == 15 ? step - 15 : 1) {
-        O *const at = reinterpret_cast<O *>(a.out) + (size_t)(t + j) * a.out_stride + o;
-        float y[1] = {mine ? type<O>::up(*at) : 0.f};
-        if (!__any_sync(0xffffffffu, !(fabsf(y[0]) < INFINITY))) continue;
-        settle<T>(a, y, 1, t + j, o, mine);
-        if (mine) *at = type<O>::down(y[0]);
+    for (int c = c0; c < n; c += step) {
+        O *const at = reinterpret_cast<O *>(a.out) + (size_t)(t + c) * a.out_stride + o;
+        float y[16];
+        unsigned odd = 0u;
+#pragma unroll
+        for (int j = 0; j < 16; j++) y[j] = mine && c + j < n ? type<O>::up(at[j * a.out_stride]) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) odd |= fabsf(y[j]) < INFINITY ? 0u : 1u << j;
+        settle<T>(a, y, min(16, n - c), t + c, o, mine);
+#pragma unroll
+        for (int j = 0; j < 16; j++) if (odd >> j & 1) at[j * a.out_stride] = type<O>::down(y[j]);
     }
 }
 /* A lane's results of its output, row after row.  16-bit ones: neighbouring lanes exchange, so that one stores the even rows' two outputs and one the odd rows'. */
@@ -238,13 +243,14 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             store<T, WIDE>(a, y, n, row0 + c0, o, f.odd_out);
         }
     };
-    /* MANY: what a warp found not finite, if anything, once it has stored all of its results */
-    const auto settle_all = [&](bool odd, int c0, int step, int r) {
-        if (!__any_sync(0xffffffffu, odd)) return;
+    /* MANY: what a warp found not finite, if anything, once it has stored all of its results; odd: a bit for each tile that has some, the last one for all from the 32nd on */
+    const auto settle_all = [&](unsigned odd, int c0, int step, int r) {
+        odd = __reduce_or_sync(0xffffffffu, odd);
+        if (!odd) return;
         __syncwarp();                /* (neighbours have stored for each other) */
 #pragma unroll 1
-        for (int tile = tile0; tile < end; tile += clusters)
-            settle_stored<T, typename std::conditional<WIDE, float, T>::type>(a, row_of(tile), min(N, a.rows - row_of(tile)), c0, step, m_of(tile) + r, m_of(tile) + r < a.out_width);
+        for (int tile = tile0, turn = 0; tile < end; tile += clusters, turn++)
+            if (odd >> min(turn, 31) & 1) settle_stored<T, typename std::conditional<WIDE, float, T>::type>(a, row_of(tile), min(N, a.rows - row_of(tile)), c0, step, m_of(tile) + r, m_of(tile) + r < a.out_width);
     };
     if (warp == kCodes) {
         /* ===================== producer of codes ===================== */
@@ -334,7 +340,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
         /* ===================== sums of kRun steps: a lane has an output, the warp every other 16 rows ===================== */
         const int quarter = warp & 3, half = (warp >> 2) & 1, r = quarter * 32 + lane, runs = (steps + kRun - 1) / kRun;
         float acc[4][16];
-        bool ok = true, odd = false;
+        bool ok = true;
+        unsigned odd = 0u, now = 1u;         /* bits of the tiles that have results that are not finite, and of this one */
         int buf = 0;
         unsigned rph = 0;
 #pragma unroll 1
@@ -385,7 +392,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
                         to += a.out_stride;
                     }
                 }
-                odd |= !(sum == 0.f);
+                odd |= sum == 0.f ? 0u : now;
+                now = now << 1 ? now << 1 : now;
             }
         }
         if (MANY && ok) settle_all(odd, half * 16, 32, r);
@@ -449,8 +457,8 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
             fetch(s0 + kTeams, sc[1]);
         };
         begin(tile0);
-        bool ok = true, odd = false;
-        unsigned parity = 0;
+        bool ok = true;
+        unsigned parity = 0, odd = 0u, now = 1u;         /* (bits of tiles) */
 #pragma unroll 1
         for (int tile = tile0; tile < end; tile = MANY ? tile + clusters : end) {
             for (int s = s0; s < steps && ok; s += 3 * kTeams) {
@@ -478,13 +486,14 @@ __global__ void __launch_bounds__(warps_of<WIDE>::kThreads, 1) hy3a_linear4_umma
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         y[j] = __uint_as_float(v[j]);
-                        if (MANY) odd |= !(fabsf(y[j]) < INFINITY);
+                        if (MANY) odd |= fabsf(y[j]) < INFINITY ? 0u : now;
                     }
                     put(y, c0, min(16, rows - c0), r, o, row0);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (MANY && lane == 0) mbar_arrive_cluster(cluster_addr(BAR(B_RUN_FREE), leader));
+                now = now << 1 ? now << 1 : now;
             }
         }
         if (MANY && !WIDE && ok) settle_all(odd, team * 16, 16 * kTeams, r);
