@@ -81,10 +81,11 @@ template <int W> __device__ __forceinline__ void load_words(unsigned addr, unsig
 /* ---- rows as columns: x of a lane for a group from k0 on, in the pairs' order; zeros past the width, and where the row is none ---- */
 template <class T, int W> __device__ __forceinline__ void load_x(const T *row, bool there, int k0, int width, unsigned (&x)[4 * W]) {
     const int k = k0 + (threadIdx.x & 3) * 8 * W;
+    there = there && k < width;        /* (all of the lane's or none: widths are multiples of 32) */
 #pragma unroll
     for (int w = 0; w < W; w++) {
         uint4 v = zero16();
-        if (there && k + 8 * w < width) v = load_row(row + k + 8 * w);
+        if (there) v = load_row(row + k + 8 * w);
         x[4 * w + 0] = __byte_perm(v.x, v.z, 0x5410);
         x[4 * w + 1] = __byte_perm(v.x, v.z, 0x7632);
         x[4 * w + 2] = __byte_perm(v.y, v.w, 0x5410);
@@ -141,8 +142,8 @@ __device__ __forceinline__ unsigned shift_left(unsigned v, int by) { unsigned r;
 __device__ __forceinline__ unsigned shift_right(unsigned v, int by) { unsigned r; asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by)); return r; }
 
 /* The digits of 8 k's from k on, a thread's share of a stage's: word `word` of the stage.  Row c = group * W + word of its lane holds the digits of four lanes, 8 bytes for
- * each column and lane, column j in place j ^ (c & 7): banks.  Sets bit 0 of *odd where x is NaN, bit 1 where it is infinite, or so large that
- * its unit times 2^24 might be. */
+ * each column and lane, column j in place j ^ (c & 7): banks.  Sets *odd where x is not finite, or so large that its
+ * unit times 2^24 might be infinite. */
 template <class T, int W> __device__ __forceinline__ void store_digits(const T *row, int k, int width, int word, uint8_t *digits, float *units, int *odd) {
     uint4 raw = zero16();
     if (k < width) raw = load_row(row + k);
@@ -156,7 +157,7 @@ template <class T, int W> __device__ __forceinline__ void store_digits(const T *
         ex[i] = max((int)e, 1);
         most = max(most, ex[i]);
         sign |= (u >> 31) << i;
-        if (e >= kMostExponent) atomicOr(odd, e == 255u && (u & 0x7fffffu) ? 1 : 2);
+        if (e >= kMostExponent) *odd = 1;
     }
 #pragma unroll
     for (int o = 1; o < 4 * W; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
         /* ===================== the warps' parts, added up in the warps' order; a lane has an output and four columns ===================== */
         const int o = lane >> 1, r0 = (lane & 1) * 4;
         int turn = 0;
+        unsigned skip = 0u;      /* rows with a NaN, whose results all are */
 #pragma unroll 1
         for (int o0 = first; o0 < last; o0 += kTile, turn++) {
             const int buf = turn % kBufs;
@@ -268,25 +270,48 @@ __global__ void __launch_bounds__(kThreads, 1) hy3a_linear4_kernel(const __grid_
                 if (a.wide) reinterpret_cast<float *>(a.out)[to] = y;
                 else reinterpret_cast<T *>(a.out)[to] = type<T>::down(y);
             };
+            unsigned most = 0u;
             if (ONE) {
-                /* digits: column c counts 2^-7c; an x that is not finite, or over 2^100, has none */
+                /* digits: column c counts 2^-7c; an x that is not finite, or over 2^100, has none, and all results come from the definition */
                 float y = (v[0] + v[1] * 0x1p-7f + (v[2] * 0x1p-14f + v[3] * 0x1p-21f)) * (r0 ? 0x1p-28f : 1.f);
                 y += __shfl_xor_sync(0xffffffffu, y, 1);
-                const int odd = *reinterpret_cast<volatile int *>(s_odd);
-                if (odd & 1) y = NAN;
-                else if (odd) {
-#pragma unroll 1
-                    for (int i = 0; i < kTile && o0 + i < last; i++) {
-                        const float again = plain<T>(a, 0, o0 + i);
-                        if (o == i) y = again;
-                    }
+                v[0] = *reinterpret_cast<volatile int *>(s_odd) ? NAN : y;
+                if (r0 == 0 && o0 + o < last) {
+                    put(0, v[0]);
+                    most = skip ? 0u : __float_as_uint(v[0]) & 0x7fffffffu;
                 }
-                if (r0 == 0 && o0 + o < last) put(0, y);
             } else if (o0 + o < last) {
 #pragma unroll
                 for (int i = 0; i < 4 * C; i++) {
                     const int r = i / 4 * kRows + r0 + i % 4;
-                    if (r < rows) put(r, v[i]);
+                    if (r < rows) {
+                        put(r, v[i]);
+                        most = max(most, skip >> r & 1 ? 0u : __float_as_uint(v[i]) & 0x7fffffffu);
+                    }
+                }
+            }
+            /* What is not finite (an infinite x or scale, a group's sum beyond fp32 whose product with its scale is not, digits that there are not) comes from the definition.  (256 results of 65536 products,
+             * the most a tile has, take a small part of the half second that others wait for it.  Called functions cost each launch 0.4 to 2 us, also where they are not reached: these are in line.) */
+            if (__any_sync(0xffffffffu, most >= 0x7f800000u)) {
+#pragma unroll 1
+                for (int r = 0; r < rows; r++) {
+                    const int i = r / kRows * 4 + r % 4;
+                    float y = v[0];
+#pragma unroll
+                    for (int k = 1; k < 4 * C; k++) if (i == k) y = v[k];
+                    const bool mine = o0 + o < last && r0 == r % kRows / 4 * 4;
+                    unsigned todo = __ballot_sync(0xffffffffu, mine && !(skip >> r & 1) && !(fabsf(y) < INFINITY));
+                    if (!todo) continue;
+                    if (has_nan<T>(a, t0 + r)) {
+                        skip |= 1u << r;
+                        continue;
+                    }
+#pragma unroll 1
+                    for (; todo; todo &= todo - 1) {
+                        const int l = __ffs(todo) - 1;
+                        const float again = plain<T>(a, t0 + r, o0 + (l >> 1));
+                        if (lane == l) put(r, again);
+                    }
                 }
             }
         }

@@ -78,7 +78,7 @@ template <> struct steps<__half> {
 };
 
 /* whether row t of x has a NaN, for a warp */
-template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, int t) {
+template <class T> __device__ __forceinline__ bool has_nan(const linear4_args &a, int t) {
     const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride);
     constexpr unsigned kInf = type<T>::code == HY3A_BF16 ? 0x7f80u : 0x7c00u;
     /* (rows that nobody wrote have theirs early) */
@@ -98,7 +98,7 @@ template <class T> __device__ __noinline__ bool has_nan(const linear4_args &a, i
     return false;
 }
 /* out[t][o] from the definition, by a warp */
-template <class T> __device__ __noinline__ float plain(const linear4_args &a, int t, int o) {
+template <class T> __device__ __forceinline__ float plain(const linear4_args &a, int t, int o) {
     const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride), *const codes = reinterpret_cast<const uint4 *>(a.codes + (size_t)o * (a.width / 2));
     const T *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
     float sum = 0.f;
