@@ -97,7 +97,7 @@ template <class T> __device__ __forceinline__ bool has_nan(const linear4_args &a
     }
     return false;
 }
-/* out[t][o] from the definition, by a warp */
+/* out[t][o] from the definition, by a warp; weights in eighths, which are exact: 8 steps of a scale from 2^125 on are beyond fp32 where their products with x need not be */
 template <class T> __device__ __forceinline__ float plain(const linear4_args &a, int t, int o) {
     const uint4 *const x = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.x) + (size_t)t * a.x_stride), *const codes = reinterpret_cast<const uint4 *>(a.codes + (size_t)o * (a.width / 2));
     const T *const scales = reinterpret_cast<const T *>(a.scales) + (size_t)o * a.groups;
@@ -106,7 +106,7 @@ template <class T> __device__ __forceinline__ float plain(const linear4_args &a,
     for (int i = threadIdx.x & 31; i < a.width / 32; i += 32) {         /* 32 k's, of one group */
         const uint4 c = codes[i];
         const unsigned w[4] = {c.x, c.y, c.z, c.w};
-        const float s = type<T>::up(scales[i * 32 / a.group]);
+        const float s = 0.125f * type<T>::up(scales[i * 32 / a.group]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint4 v = x[4 * i + j];
@@ -120,7 +120,7 @@ template <class T> __device__ __forceinline__ float plain(const linear4_args &a,
     }
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
-    return sum;
+    return 8.f * sum;
 }
 } /* namespace hy3a_layer */
 #endif

@@ -1,4 +1,4 @@
-"""linear4's results do not turn infinite, or NaN, with the number of rows: a group's sum of steps beyond fp32 whose product with its scale is not, infinite scales.  (Tolerances: test_gpu_linear4.py.)"""
+"""linear4's results do not turn infinite, or NaN, with the number of rows: a group's sum of steps beyond fp32 whose product with its scale is not, weights beyond fp32, infinite scales.  (Tolerances: test_gpu_linear4.py.)"""
 import pytest
 
 from test_gpu_linear4 import check, make, weights
@@ -27,6 +27,25 @@ def test_large_rows_with_small_scales(cuda, rows, out, width, group, result):
         mixed[rows // 2] = x[0]
         args = mixed, codes, scales, group
         check(hy3_b200.linear4(*args[:3], out_dtype=getattr(torch, result)), *args)
+
+
+@pytest.mark.parametrize("result", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,out", CALLS)
+def test_large_scales_with_small_rows(cuda, rows, out, result):
+    """Scales of 2^125 to 2^127, with which up to 8 steps are beyond fp32 (and beyond bf16), and rows of 2^-30; what quantize4 makes of the largest fp32 numbers is of that kind."""
+    import torch
+    import hy3_b200
+    x, codes, scales, group = make(rows, 544, out, 32)
+    x = (x * 2.0 ** -30).to(x.dtype)
+    scales[:, ::3] = ((1 + scales[:, ::3].abs() % 1) * 2.0 ** 126).to(scales.dtype)
+    args = x, codes, scales, group
+    check(hy3_b200.linear4(*args[:3], out_dtype=getattr(torch, result)), *args)
+    w = torch.randn((64, 512), device=cuda)
+    w[::2, 5::32] = torch.finfo(torch.float32).max
+    codes, scales = hy3_b200.quantize4(w, 32, torch.bfloat16)
+    assert bool((scales.float()[::2] == -2.0 ** 125).all())
+    args = x[:, :512], codes, scales, 32
+    check(hy3_b200.linear4(*args[:3], out_dtype=getattr(torch, result)), *args)
 
 
 @pytest.mark.parametrize("dtype,result", [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16")])
