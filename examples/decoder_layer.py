@@ -45,6 +45,8 @@ class DecoderLayer:
         self.shared_gate, self.shared_up, self.shared_down = weight(inter, hidden), weight(inter, hidden), weight(hidden, inter)
         shared = {"qkv": self.qkv, "o": self.o, "gate": self.shared_gate, "up": self.shared_up, "down": self.shared_down}
         self.bits4 = {name: hy3_b200.quantize4(w) for name, w in shared.items()} if bits4 else None
+        if bits4:           # (what they were made of is not kept)
+            self.qkv = self.o = self.shared_gate = self.shared_up = self.shared_down = None
         self.ctx = Hy3Attn(kv_dtype=kv_dtype, n_layers=1, max_seqs=requests, max_batch=max(chunk, requests), max_tokens=requests * max_tokens_per_seq,
                            max_tokens_per_seq=max_tokens_per_seq)
         self.q16 = torch.empty((chunk, H, D), dtype=torch.float16, device=device)
