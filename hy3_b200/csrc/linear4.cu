@@ -5,14 +5,15 @@
  *
  * The inner sums are warp-level products of 16 outputs with 8 columns; the scale of a group multiplies its sum in fp32.  Nothing is rounded to fewer bits before the result.
  *   rows     the columns are rows: mma.m16n8k16 with fp32 sums; code - 8 is exact in the rows' type, and so are the products.  What makes numbers of codes bounds it, so a block has up to 16 rows for
- *            them, two products for each number, where registers have room for that much x (width 4096 at most), else 8 (16 rows on 10240 x 4096 in fp32: 11.6 us, by eights 15.7, and in
- *            linear4_umma.cu 24.4; on 120832 x 4096 80, 122 and 175.  17 rows as 16 and 1 take 21.4 and 156, but 13.3 on 4096 x 4096, where that file takes 10.8 for 16-bit results);
+ *            them, two products for each number, where registers have room for that much x (width 4096 at most), else 8 (16 rows on 10240 x 4096 in fp32: 12.0 us, by eights 15.7; on 120832 x 4096 85 and
+ *            122).  More go to linear4_umma.cu, where 17 rows take 24.8 and 142 there (16-bit results 18 and 97, 10.6 on 4096 x 4096): 16 and 1 in calls of their own would take 21 and 130 for fp32 results, less,
+ *            and more for 16-bit ones;
  *   digits   of one row, on large matrices, the columns are its digits: x = 2^E (d0 2^-7 + d1 2^-14 + .. + d7 2^-56), |d| < 128, with E from the largest |x| of the group, so that what is lost lies 2^-56
  *            below that (of 16-bit numbers: nothing, down to 2^-45 of it); mma.m16n8k32 of bytes with integer sums takes the codes as they are, two operations a word instead of 9, and
  *            -8 sum d comes in as the sum's first value.
  *
  * A block takes a contiguous part of the outputs (parts differ by four outputs at most), in tiles of 16, and streams their codes through a ring of shared memory: a
- * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way (one row on 120832 x 4096: 44 us, 6 TB/s).  (A bulk copy
+ * stage is a tile's codes for 4096 k's (or all, where there are fewer), copied as a box for each four outputs, and its scales, so that all blocks have 170 KB under way (one row on 120832 x 4096: 44 to 49 us, 5.4 to 6 TB/s).  (A bulk copy
  * for each output keeps the issuing lane busy for longer than its bytes take.)  The 16 warps share the k's; each keeps its part of x in registers for the whole launch.  Their
  * sums meet in shared memory, where a warp of their own adds them up.  Short launches wait for instructions as much as for codes: loops that are run a few times are not unrolled.
  *

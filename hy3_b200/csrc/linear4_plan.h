@@ -37,7 +37,7 @@ HY3A_ANYWHERE constexpr int linear4_first_step(int before, int steps, int teams)
 
 /* Rows of a tile and CTAs that share a tile's k's: what takes the least, in 10 ns, measured over 9 to 2048 rows: a step takes 160 + 0.6 N ns with N rows (fp32 results 220 + 0.9 N), a launch 6.5 us besides
  * (8.5; 1.5 more where CTAs share).  Pairs that have several tiles begin the next one's copies, and with fp32 results its products too, before the last one's results are stored: 2 us a tile (2698 rows on
- * 16942 x 448 in fp32 98 us, and 249 with a launch's start and end for each; 2048 on 4096 x 8192 in bf16 99.7 and 102.3).  units: of 128 k's; fit: clusters of 1 .. kLinear4Splits pairs at once. */
+ * 16942 x 448 in fp32 98 to 117 us, and 249 with a launch's start and end for each; 2048 on 4096 x 8192 in bf16 100 and 102).  units: of 128 k's; fit: clusters of 1 .. kLinear4Splits pairs at once. */
 static inline linear4_plan linear4_plan_of(int rows, int m_tiles, int units, bool wide, const int (&fit)[kLinear4Splits]) {
     linear4_plan p = {};
     const int most = wide ? 128 : 256, least_tiles = (rows + most - 1) / most;

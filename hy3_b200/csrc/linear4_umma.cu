@@ -15,7 +15,7 @@
  * Results in fp32: a weight enters as two numbers, the rounded one and the rest, which is exact, so that there are 8 products a step; and the tensor cores begin a new sum every 512 k's (bf16; fp16: 256), which warps of their own
  * add to results in registers: the tensor cores' sums are cut off and not rounded (one sum over 4096 k's left an error of 5.6e-6 of the result; sums of 512 leave 4.6e-7, of fp16 products, whose 22 bits lose more,
  * 1.1e-6, of 256 k's 6e-7 for 2% more time).  A = code - 8, with a sum for each group and its scale
- * at the end, is half as many products, but 64 rows on 10240 x 4096 took 26.8 us: the sums are read 8 times as often.
+ * at the end, is half as many products and rounds nothing, but reads sums 8 times as often: 64 rows on 10240 x 4096 took 26.8 us in an early form of this file, which had one tile a pair, and 26.4 as it is now; it has not been tried since.
  *
  * Where tiles are more than pairs of CTAs fit at once, a pair has several, and its warps go on to the next one each as far as it can.
  * Where tiles are few, the CTAs of a cluster share the k's of a tile; their sums meet in shared memory, and are added in the order of the k's.

@@ -6,8 +6,8 @@
  * in one pass, with running m.  The logits that equal m are counted (n) and the others' exponentials added up (S), so that log Z = log1p(S) where the largest stands
  * alone: a token that is nearly certain keeps the digits of its log probability.  The terms of H are all positive.
  *
- * Memory bounds it where rows are many and long (2048 x 120832 fp32: 147 us, 6.7 TB/s; bf16 rows are bound by the exponentials and 10 instructions a pair of logits), the chain of loads, meetings and
- * ranking where they are few (1 x 120832, top 20: 6.7 us).  A row is a block's, or the blocks' of a cluster where rows are few.  A warp shares m, so that it seldom rises: past the first vectors nearly all take the
+ * Memory bounds it where rows are many and long (2048 x 120832 fp32: 151 to 160 us, 6.2 to 6.5 TB/s; bf16 rows, 106 us, are bound by the exponentials and 10 instructions a pair of logits), the chain of loads, meetings and
+ * ranking where they are few (1 x 120832, top 20: 7.3 to 7.8 us).  A row is a block's, or the blocks' of a cluster where rows are few.  A warp shares m, so that it seldom rises: past the first vectors nearly all take the
  * branch without it, and of those that raise it only the vectors that have the new m are looked at logit by logit.
  *
  * The top k are found without a second pass over the row: a thread keeps its largest logit and the vector of 16 bytes that had it; the k-th largest of 32

@@ -1,6 +1,6 @@
 /*
  * ring.cuh -- barriers, bounded waits and tensor copies of the kernels with shared-memory rings beside the attention (experts_umma.cu,
- * adapters.cu).
+ * adapters.cu, linear4.cu, linear4_umma.cu).
  *
  * Every wait is bounded: one that runs out raises the block's abort flag and leaves a code in the file's error words (hy3a_layer_sync).
  */

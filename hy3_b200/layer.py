@@ -73,7 +73,8 @@ def linear4(x, codes, scales, out_dtype=None, out=None):
     """Rows times a matrix in 4 bits: out[t, o] = sum_k (q[o, k] - 8) * s[o, k / group] * x[t, k], codes and scales as `quantize4` gives them.
 
     x [rows, width] fp16 or bf16 (row stride free), scales of x's type; the group's size follows from their number.  The result [rows, out_width] is of x's type,
-    or fp32 (`out_dtype`, or out's).  Sums are fp32.  Returns out."""
+    or fp32 (`out_dtype`, or out's).  Sums are fp32.  In calls of more than 16 rows with a result of x's type each weight is rounded to that type once (an error like that of
+    the result's own rounding; an fp32 result has none of it).  out must not overlap x, codes or scales.  Returns out."""
     return _out(load_native().linear4(_stream(x), x, codes, scales, out_dtype, out))
 
 

@@ -299,8 +299,13 @@ int hy3a_adapters(void *stream, int dtype, int rows, int width, int out_width, i
 int hy3a_quantize4(void *stream, int w_dtype, int out_width, int width, int group, const void *w, size_t w_stride, int dtype, void *codes, void *scales);
 
 /* Rows times a matrix in 4 bits, in hy3a_quantize4's format: out[t][o] = sum over k of (q[o][k] - 8) * s[o][k / group] * x[t][k].  x [rows][width] and
- * the scales are of dtype HY3A_F16 or HY3A_BF16, out [rows][out_width] of out_dtype: that, or HY3A_F32.  Sums are fp32; rows: at most 2^24.  x and codes are 16-byte aligned, and rows of x start on
- * 16-byte boundaries; scales and out are aligned to their types.  out must not overlap x.                                     */
+ * the scales are of dtype HY3A_F16 or HY3A_BF16, out [rows][out_width] of out_dtype: that, or HY3A_F32; rows: at most 2^24.
+ * Sums are fp32 and weights are taken as they are, but for calls of more than 16 rows:
+ *   - with a result of the rows' type a weight is rounded to that type once, an error like that of the result's own rounding (2.2e-3 of the result's norm in bf16, 1.7e-3 without; fp16 2.7e-4 and 2.1e-4): ask for
+ *     an fp32 result where that matters, and round it;
+ *   - with an fp32 result partial sums of 512 k's (fp16 rows: 256) are cut off and not rounded: 5e-7 of the result's norm (up to 16 rows: 1e-7).
+ * A row's last bits may so differ between calls of 1, 2 to 8, 9 to 16 and more rows; whether it is finite does not.  Rows of one call do not change each other's results.
+ * x and codes are 16-byte aligned, and rows of x start on 16-byte boundaries; scales and out are aligned to their types.  out must not overlap x, codes or scales.  */
 int hy3a_linear4(void *stream, int dtype, int rows, int width, int out_width, int group, const void *x, size_t x_stride, const void *codes, const void *scales,
                  int out_dtype, void *out, size_t out_stride);
 
